@@ -292,7 +292,8 @@ int focr_linear_upload(focr_ctx *handle, int bits, size_t n, size_t k, size_t gr
                        const float *exc_vals, size_t n_exc, focr_linear **out) {
   Ctx *ctx = reinterpret_cast<Ctx *>(handle);
   FOCR_REQUIRE(ctx && out && codes, FOCR_E_ARG, "focr_linear_upload: null argument");
-  FOCR_REQUIRE(bits == 8 || bits == 16 || bits == 32, FOCR_E_ARG, "focr_linear_upload: bits must be 8, 16 or 32");
+  FOCR_REQUIRE(bits == 4 || bits == 8 || bits == 16 || bits == 32, FOCR_E_ARG,
+               "focr_linear_upload: bits must be 4, 8, 16 or 32");
   FOCR_REQUIRE(n > 0 && k > 0, FOCR_E_SHAPE, "focr_linear_upload: empty matrix");
   FOCR_REQUIRE(n <= (size_t(1) << 31) / 1 && k <= (size_t(1) << 24), FOCR_E_SHAPE,
                "focr_linear_upload: matrix too large");
@@ -319,9 +320,14 @@ int focr_linear_upload(focr_ctx *handle, int bits, size_t n, size_t k, size_t gr
           for (size_t i = g * group; i < std::min(k, (g + 1) * group); i++)
             FOCR_REQUIRE(c8[row * k + i] == 0, FOCR_E_VALUE, "nonzero code in zero-scale group");
   }
+  // The same rules for 4 bits (the codes are checked as they are packed). The
+  // GEMV multiplies group sums of up to 2^20 by the scale.
+  if (bits == 4)
+    for (size_t i = 0; i < n * groups; i++)
+      FOCR_REQUIRE(scales[i] >= 0.0f && scales[i] <= 0x1p96f, FOCR_E_VALUE, "invalid W4 scale");
   // with_exceptions' rules (src/quant/linear.rs:366-390,437-452).
   if (n_exc) {
-    FOCR_REQUIRE(bits != 32, FOCR_E_ARG, "exception columns need 8- or 16-bit codes");
+    FOCR_REQUIRE(bits != 32, FOCR_E_ARG, "exception columns need 4-, 8- or 16-bit codes");
     // The kernels find a column's exception through a 16-bit index per input.
     FOCR_REQUIRE(n_exc <= size_t(INT16_MAX), FOCR_E_UNSUPPORTED, "at most 32767 exception columns");
     FOCR_REQUIRE(exc_cols && exc_vals, FOCR_E_ARG, "focr_linear_upload: null exception arrays");
@@ -334,7 +340,7 @@ int focr_linear_upload(focr_ctx *handle, int bits, size_t n, size_t k, size_t gr
     for (size_t e = 0; e < n_exc; e++)
       for (size_t row = 0; row < n; row++) {
         const size_t at = row * k + size_t(exc_cols[e]);
-        const bool zero = bits == 8 ? static_cast<const int8_t *>(codes)[at] == 0
+        const bool zero = bits <= 8 ? static_cast<const int8_t *>(codes)[at] == 0
                                     : static_cast<const int16_t *>(codes)[at] == 0;
         FOCR_REQUIRE(zero, FOCR_E_VALUE, "nonzero code in an exception column");
       }
@@ -357,7 +363,7 @@ int focr_linear_upload(focr_ctx *handle, int bits, size_t n, size_t k, size_t gr
   };
   const size_t cb = code_bytes(bits);
   size_t total = 0;
-  {
+  if (bits != 4) {
     std::vector<uint8_t> raw(static_cast<const uint8_t *>(codes), static_cast<const uint8_t *>(codes) + n * k * cb);
     uint8_t *dev = nullptr;
     if ((rc = upload_vector(raw, &dev, &total)) != FOCR_OK) return fail(rc);
@@ -377,7 +383,9 @@ int focr_linear_upload(focr_ctx *handle, int bits, size_t n, size_t k, size_t gr
     if ((rc = upload_vector(index, &lin->exc_index, &total)) != FOCR_OK) return fail(rc);
   }
   // Decode GEMV tiles.
-  {
+  if (bits == 4) {
+    if ((rc = pack_linear4(ctx, lin, static_cast<const int8_t *>(codes), &total)) != FOCR_OK) return fail(rc);
+  } else {
     const size_t S = 16 / (2 * cb);
     const size_t nb = k / 32;
     lin->gemv_blocks = nb;
@@ -512,8 +520,8 @@ int focr_linear_prefill(focr_ctx *handle, const focr_linear *lh, const float *x,
     case FOCR_PROJ_F32_SPLIT:
       return launch_prefill_split(ctx, lin, x, rows, row_scale, epilogue, out);
     case FOCR_PROJ_I16:
-      FOCR_REQUIRE(lin->i16_b, FOCR_E_UNSUPPORTED,
-                   "the INT16 panels take 8-bit codes in groups of 64 with out % 32 == 0 and in % 64 == 0 "
+      FOCR_REQUIRE(lin->i16_wsum, FOCR_E_UNSUPPORTED,
+                   "the INT16 panels take 4- or 8-bit codes in groups of 64 with out % 32 == 0 and in % 64 == 0 "
                    "(fits_i16_panels); plan the FP32 panels for this matrix");
       return launch_prefill_i16(ctx, lin, x, rows, row_scale, epilogue, out);
     default:

@@ -74,19 +74,20 @@ int noalloc_scratch_init(int device);
 constexpr int kGemvChannels = 4;  // per wave tile (2 per lane half)
 
 struct Linear {
-  int bits = 8;  // 8, 16 or 32
+  int bits = 8;  // 4, 8, 16 or 32
   size_t n = 0, k = 0, group = 64, groups = 0, n_exc = 0;
   // Row-major copies (dequantization, GEMM operands, GEMV tails).
-  void *codes = nullptr;   // [n][k] int8 / int16 / float
-  float *scales = nullptr; // [n][groups] (bits 8/16)
+  void *codes = nullptr;   // [n][k] int8 / int16 / float (bits 4: only the tiles below)
+  float *scales = nullptr; // [n][groups] (bits 4/8/16)
   int32_t *exc_cols = nullptr;  // [n_exc]
   float *exc_vals = nullptr;    // [n][n_exc]
   int16_t *exc_index = nullptr; // [k]: exception number of a column, or -1
-  // GEMV tiles.
+  // GEMV tiles (bits 4: tiles of 16 channels x 128 columns, linear4.hpp).
   void *gemv_codes = nullptr;    // [tiles][steps][64 lanes][16 B]
   float *gemv_scales = nullptr;  // [tiles][steps][2 halves][2 ch][sps]
   size_t gemv_tiles = 0, gemv_steps = 0, gemv_sps = 0, gemv_blocks = 0;
-  // INT16-panel operands (bits 8, group 64): B tiles in MFMA lane order and
+  // INT16-panel operands (bits 4 and 8, group 64): B tiles in MFMA lane order
+  // (bits 8; those of 4-bit codes are unpacked for each call) and
   // per-(group, column) weight sums times 128.
   int8_t *i16_b = nullptr;      // [groups][n/16][64 lanes][16 B]
   int32_t *i16_wsum = nullptr;  // [groups][n]  (128 * sum of the group's codes)
@@ -105,6 +106,14 @@ inline const float *const kRmsInKernel = reinterpret_cast<const float *>(uintptr
 int launch_gemv(Ctx *ctx, const Linear *lin, const float *x, size_t rows, const float *row_scale, int epilogue,
                 float *out, bool rms_norm = false);
 int launch_dequantize(Ctx *ctx, const Linear *lin, float *out);
+// 4-bit codes (gemv_i4.hip): the tiles of row-major codes, a byte each (host
+// memory; lin->scales is there already; synchronous), the GEMV, the weights in FP32,
+// and the codes as bytes, row-major or as the INT16 panels' B tiles.
+int pack_linear4(Ctx *ctx, Linear *lin, const int8_t *codes, size_t *total);
+int launch_gemv4(Ctx *ctx, const Linear *lin, const float *x, size_t rows, const float *row_scale, int epilogue,
+                 float *out, bool rms_norm);
+int launch_dequantize4(Ctx *ctx, const Linear *lin, float *out);
+int launch_unpack4(Ctx *ctx, const Linear *lin, bool panel, int8_t *out);
 int launch_row_scales(Ctx *ctx, const float *h, size_t rows, size_t width, float eps, float *out);
 int launch_prefill_f32(Ctx *ctx, const Linear *lin, const float *x, size_t rows,
                        const float *row_scale, int epilogue, float *out);

@@ -1478,6 +1478,19 @@ int launch_f32_common(bool chain, Ctx *ctx, const Linear *lin, const float *x, s
   // Codes stay codes: every kernel forms fl(code * scale) (exception columns
   // in place) in registers from the uploaded matrix; no FP32 copy of the
   // weights is written.
+  Linear bytes;
+  if (lin->bits == 4) {
+    // 4-bit codes are unpacked to bytes in the scratch first; then they are an
+    // 8-bit matrix.
+    int rc = ensure_scratch(ctx, lin->n * lin->k);
+    if (rc != FOCR_OK) return rc;
+    rc = launch_unpack4(ctx, lin, false, static_cast<int8_t *>(ctx->scratch));
+    if (rc != FOCR_OK) return rc;
+    bytes = *lin;
+    bytes.bits = 8;
+    bytes.codes = ctx->scratch;
+    lin = &bytes;
+  }
   const GemmArgs a = make_args(lin, x, rows, row_scale, out);
   if (chain && launch_chain_mfma(a, lin->bits, epilogue, ctx->stream)) {
     FOCR_HIP_CHECK(hipGetLastError());

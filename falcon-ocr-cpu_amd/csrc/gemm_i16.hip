@@ -447,8 +447,16 @@ int launch_prefill_i16(Ctx *ctx, const Linear *lin, const float *x, size_t rows,
   const size_t a_bytes = m_pad * k * 2;
   const size_t s_bytes = groups * m_pad * sizeof(float);
   const size_t e_bytes = m_pad * (lin->n_exc ? lin->n_exc : 1) * sizeof(float);
-  int rc = ensure_scratch(ctx, a_bytes + s_bytes + e_bytes + 256);
+  const size_t b_at = (a_bytes + s_bytes + e_bytes + 511) / 256 * 256;  // 4-bit codes: their B tiles
+  int rc = ensure_scratch(ctx, b_at + (lin->bits == 4 ? n * k : 0));
   if (rc != FOCR_OK) return rc;
+  const int8_t *b_tiles = lin->i16_b;
+  if (lin->bits == 4) {
+    int8_t *unpacked = static_cast<int8_t *>(ctx->scratch) + b_at;
+    rc = launch_unpack4(ctx, lin, true, unpacked);
+    if (rc != FOCR_OK) return rc;
+    b_tiles = unpacked;
+  }
   int8_t *a_tiles = static_cast<int8_t *>(ctx->scratch);
   float *steps = reinterpret_cast<float *>(static_cast<char *>(ctx->scratch) + a_bytes);
   float *exc_inputs = reinterpret_cast<float *>(static_cast<char *>(ctx->scratch) + a_bytes + s_bytes);
@@ -480,7 +488,7 @@ int launch_prefill_i16(Ctx *ctx, const Linear *lin, const float *x, size_t rows,
       const int rt = static_cast<int>((m + 16 * RB - 1) / (16 * RB));
       const int ct = static_cast<int>((n / 16 + CB * WV - 1) / (CB * WV));
       hipLaunchKernelGGL((gemm_small_kernel<E, RB, CB, WV, D>), dim3(static_cast<unsigned>(rt * ct)), dim3(64 * WV), 0,
-                         ctx->stream, a_tiles, steps, exc_inputs, lin->i16_b, lin->i16_wsum, lin->i16_sw, lin->exc_vals,
+                         ctx->stream, a_tiles, steps, exc_inputs, b_tiles, lin->i16_wsum, lin->i16_sw, lin->exc_vals,
                          static_cast<int>(lin->n_exc), static_cast<int>(m), static_cast<int>(n),
                          static_cast<int>(groups), static_cast<int>(row_blocks), static_cast<int>(m_pad), rt, ct, out);
     };
@@ -511,7 +519,7 @@ int launch_prefill_i16(Ctx *ctx, const Linear *lin, const float *x, size_t rows,
   const int row_tiles = static_cast<int>(m_pad / kBM);
 #define FOCR_LAUNCH_I16(E, BN)                                                                                    \
   hipLaunchKernelGGL((gemm_kernel<E, BN>), dim3(static_cast<unsigned>(row_tiles * ((n + BN - 1) / BN))), dim3(BN * 4), \
-                     0, ctx->stream, a_tiles, steps, exc_inputs, lin->i16_b, lin->i16_wsum, lin->i16_sw,             \
+                     0, ctx->stream, a_tiles, steps, exc_inputs, b_tiles, lin->i16_wsum, lin->i16_sw,             \
                      lin->exc_vals, static_cast<int>(lin->n_exc), static_cast<int>(m), static_cast<int>(n),          \
                      static_cast<int>(groups), static_cast<int>(row_blocks), static_cast<int>(m_pad), row_tiles,     \
                      static_cast<int>((n + BN - 1) / BN), out)

@@ -1,5 +1,6 @@
 // Decode GEMV dispatch (kernel: gemv_kernel.hpp; one instantiation file per
-// code type: gemv_i8.hip, gemv_i16.hip, gemv_f32.hip).
+// code type: gemv_i8.hip, gemv_i16.hip, gemv_f32.hip; 4-bit codes have a kernel
+// of their own, gemv_i4.hip).
 #include "gemv_kernel.hpp"
 
 namespace focr {
@@ -14,6 +15,7 @@ static size_t rows_per_launch(const Linear *lin) {
 
 int launch_gemv(Ctx *ctx, const Linear *lin, const float *x, size_t rows, const float *row_scale, int epilogue,
                 float *out, bool rms_norm) {
+  if (lin->bits == 4) return launch_gemv4(ctx, lin, x, rows, row_scale, epilogue, out, rms_norm);
   FOCR_HIP_CHECK(hipSetDevice(ctx->device));
   const size_t chunk = rows_per_launch(lin);
   FOCR_REQUIRE(chunk >= 1, FOCR_E_SHAPE, "GEMV: in_dim too large for one row of x in LDS");

@@ -261,6 +261,7 @@ __global__ __launch_bounds__(256) void argmax_kernel(const float *__restrict__ l
 
 int launch_dequantize(Ctx *ctx, const Linear *lin, float *out) {
   FOCR_HIP_CHECK(hipSetDevice(ctx->device));
+  if (lin->bits == 4) return launch_dequantize4(ctx, lin, out);
   const size_t total = lin->n * lin->k;
   if (lin->bits == 32) {
     FOCR_HIP_CHECK(hipMemcpyAsync(out, lin->codes, total * sizeof(float), hipMemcpyDeviceToDevice, ctx->stream));

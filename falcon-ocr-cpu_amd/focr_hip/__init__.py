@@ -224,13 +224,15 @@ class PrefillProjection(enum.IntEnum):
 
 
 class Linear:
-    """A device-resident matrix (focr_linear): 8/16-bit codes or FP32 weights."""
+    """A device-resident matrix (focr_linear): 4/8/16-bit codes or FP32 weights.
+
+    4-bit codes come as int8 in -8..7, one an element; the device holds two a byte."""
 
     def __init__(self, bits, codes, scales, group, exc_cols=None, exc_vals=None, ctx: Optional[Context] = None):
         self.ctx = ctx or default_context()
         codes = np.ascontiguousarray(codes)
         n, k = codes.shape
-        dtype = {8: np.int8, 16: np.int16, 32: np.float32}[bits]
+        dtype = {4: np.int8, 8: np.int8, 16: np.int16, 32: np.float32}[bits]
         codes = codes.astype(dtype, copy=False)
         sc = None if scales is None else np.ascontiguousarray(scales, dtype=np.float32)
         cols = vals = None
@@ -341,12 +343,20 @@ class Linear:
 
 
 class QuantLinear(Linear):
-    """A quantized matrix with 8- or 16-bit codes (src/quant/linear.rs:123-130)."""
+    """A quantized matrix with 8- or 16-bit codes (src/quant/linear.rs:123-130),
+    or 4-bit ones (`bits=4`, a `hip` format with no reference counterpart)."""
 
     @classmethod
-    def from_parts(cls, out_dim, in_dim, group_size, codes, scales, ctx: Optional[Context] = None) -> "QuantLinear":
+    def from_parts(cls, out_dim, in_dim, group_size, codes, scales, ctx: Optional[Context] = None,
+                   bits: Optional[int] = None) -> "QuantLinear":
+        """`bits` None takes 8 or 16 from the codes' type; 4 takes int8 codes in -8..7."""
         codes = np.asarray(codes).reshape(out_dim, in_dim)
-        bits = 8 if codes.dtype == np.int8 else 16
+        if bits is None:
+            bits = 8 if codes.dtype == np.int8 else 16
+        elif bits not in (4, 8, 16):
+            raise FocrError(-1, "quantized codes have 4, 8 or 16 bits")
+        elif codes.dtype != (np.int16 if bits == 16 else np.int8):
+            raise FocrError(-1, "4- and 8-bit codes are int8, 16-bit ones int16")
         return cls(bits, codes, np.asarray(scales, dtype=np.float32).reshape(out_dim, -1), group_size, ctx=ctx)
 
     def with_exceptions(self, columns, values) -> "QuantLinear":

@@ -104,8 +104,9 @@ int focr_ctx_sync(focr_ctx *ctx);
  * captured graph can hold: the scratch (above) and an 8-float row-scale
  * array allocated at creation (focr_argmax's result words are read back to
  * the host within the call, which therefore cannot be captured). No
- * context buffer holds weights: prefill on INT8/INT16 codes reads the codes
- * and forms fl(code * scale) in registers. */
+ * context buffer holds weights past the call that unpacked them (4-bit codes):
+ * prefill on INT8/INT16 codes reads the codes and forms fl(code * scale) in
+ * registers. */
 int focr_ctx_reserve_scratch(focr_ctx *ctx, size_t bytes);
 int focr_ctx_scratch_bytes(const focr_ctx *ctx, size_t *bytes);
 /* Message of the calling thread's last failure ("" if none). */
@@ -125,6 +126,9 @@ int focr_memcpy_d2h(focr_ctx *ctx, void *dst, const void *src_dev, size_t bytes)
  *           no -128, finite non-negative scales, zero codes in zero-scale
  *           groups); bits 16: codes int16 [out][in]; bits 32: FP32 weights
  *           [out][in], scales NULL, group ignored.
+ *   bits 4 (no reference counterpart): codes int8 [out][in], each in -8..7
+ *           (FOCR_E_VALUE otherwise), held on the device as two a byte; scales
+ *           0 .. 2^96 under the W8 rules.
  *   scales: FP32 [out][ceil(in/group)], group 32, 64 or 128.
  *   exc_cols/exc_vals: optional exception columns (sorted, unique, < in)
  *           and their FP32 weights [out][n_exc]; codes there must be zero.
@@ -144,7 +148,11 @@ int focr_linear_dequantize(focr_ctx *ctx, const focr_linear *lin, float *out_dev
 /* QuantLinear::linear for 1..=8 rows (src/quant/linear.rs:497-549,783-817),
  * and kernels::linear_with_simd rows <= 8 for bits 32
  * (src/kernels/mod.rs:407-432). x_dev [rows][in], out_dev [rows][out].
- * Bitwise equal to the reference's AVX2/NEON/portable dot_q / dot order. */
+ * Bitwise equal to the reference's AVX2/NEON/portable dot_q / dot order.
+ * Bits 4: the inputs of each 64 columns are taken to 2^-23 of their largest
+ * magnitude, the products with the codes of a group are summed exactly, and
+ * the groups' sums times their scales are added in FP32 (the same for the two
+ * calls below); rows that hold an infinity or NaN by FP32 multiply-adds. */
 int focr_linear_decode(focr_ctx *ctx, const focr_linear *lin, const float *x_dev, size_t rows,
                        float *out_dev);
 /* QuantLinear::linear_glu / kernels::linear_glu_with_simd for 1..=8 rows
@@ -164,7 +172,8 @@ int focr_linear_decode_glu(focr_ctx *ctx, const focr_linear *lin, const float *x
  *   epilogue FOCR_EPI_STORE (linear), FOCR_EPI_GLU (linear_glu, out
  *     [rows][out/2]) or FOCR_EPI_ADD (add_residual, src/model/rope.rs:155-169:
  *     out += projection).
- * Bitwise equal to the separate reference passes. */
+ * Bitwise equal to the separate reference passes (bits 4: within FP32
+ * rounding, as focr_linear_decode). */
 int focr_linear_decode_ex(focr_ctx *ctx, const focr_linear *lin, const float *x_dev, size_t rows,
                           const float *row_scale_dev, int rms_norm, int epilogue, float *out_dev);
 
@@ -174,9 +183,10 @@ int focr_linear_decode_ex(focr_ctx *ctx, const focr_linear *lin, const float *x_
  *   x_dev [rows][in]; row_scale_dev optional [rows] (an RMS norm folded
  *   into packing); epilogue FOCR_EPI_*; kernel FOCR_PROJ_*.
  *   out_dev [rows][out] (STORE, ADD) or [rows][out/2] (GLU).
- * FOCR_PROJ_I16 needs 8-bit codes, group 64, out % 32 == 0, in % 64 == 0
+ * FOCR_PROJ_I16 needs 4- or 8-bit codes, group 64, out % 32 == 0, in % 64 == 0
  * (fits_i16_panels, src/quant/linear.rs:29-31); it uses a scratch buffer the
- * context owns and grows. FOCR_PROJ_F32_SPLIT needs FP32 weights
+ * context owns and grows. 4-bit codes are unpacked to a byte each in that
+ * buffer by every call; from there on they are an 8-bit matrix. FOCR_PROJ_F32_SPLIT needs FP32 weights
  * (FOCR_E_UNSUPPORTED for codes) and keeps the FP16 pairs, 4 bytes per
  * element of x and of the weights (rows and out rounded up to 128, in to 32),
  * and a row exponent each, in the same scratch buffer. */
