@@ -6,17 +6,16 @@
 //
 // with x' the input row, times a row scale or RMS-normalized if asked.
 //
-// Mathematics. Each 64 columns of a row of x' are written as integers
-// x' = i 2^(e - 22), |i| <= 2^22, 2^e above their largest magnitude, and i as
-// three signed bytes, i = d0 + 256 d1 + 65536 d2. The INT8 matrix instruction
-// then forms the exact sums of 16 channels' codes times the three bytes of up to
-// five rows (eight in two instructions) over the 64 columns: operands are
-// the codes as the tile holds them (no conversion) and the bytes, one
+// Mathematics. Each block of 128 W columns of a row of x' (W steps of a wave, 1 to
+// 4) is written as integers, x' = i 2^(e - 22), |i| <= 2^22, 2^e above its
+// largest magnitude, and i as three signed bytes, i = d0 + 256 d1 + 65536 d2. The
+// INT8 matrix instruction then forms the exact sums of 16 channels' codes times
+// the bytes of up to five rows (eight in two instructions) over 64 columns: operands
+// are the codes as the tile holds them (no conversion) and the bytes, one
 // column of the product per (row, byte). A sum is at most 64 * 128 * 128 = 2^20, so
-// its FP32 value is exact, and the only roundings are x' to 2^-23 of its
-// group's largest magnitude (FP32's own half step there), and the FP32 products
-// and sums of the group results. A row that holds an infinity or NaN is computed
-// by FP32 multiply-adds instead, column after column.
+// its FP32 value is exact, and the only roundings are x' to 2^(e - 23) and the
+// FP32 multiply-adds of the groups' sums by their scales. A row that holds an infinity or NaN is
+// computed by FP32 multiply-adds instead, column after column.
 #include <type_traits>
 
 #include "linear4.hpp"
@@ -27,6 +26,8 @@ namespace {
 using namespace linear4;
 
 typedef int v4i __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 8;
 constexpr size_t kLdsBytes = 160 * 1024;
@@ -40,6 +41,12 @@ struct Args {
   const float *x, *row_scale;
   float *out;
   int m, n, k, group, steps, tiles_total, rms, epilogue;
+  // The rows as bytes, written by rows4_kernel (PRE): blocks and their weights as
+  // they stand in the GEMV's LDS, row factors, non-finite marks of `parts` parts.
+  char *digits;
+  float *weights, *row_factors;
+  uint32_t *marks;
+  int parts;
 };
 
 // The largest of the 16 lanes of a DPP row, in every one of them.
@@ -64,131 +71,310 @@ __device__ __forceinline__ float row_up(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + 16 - N, 0xf, 0xf, false));
 }
 
-// NB: 16-column blocks of the product: one for up to 5 rows (column 5 d + r holds
-// byte d of row r), two for up to 8 (column 8 d + r). SK: waves that share a tile's
-// steps. G: columns per scale.
-template <int NB, int SK, int G>
-__global__ __launch_bounds__(64 * kWaves) void gemv4_kernel(Args a) {
-  constexpr int CW = 16 * NB, RS = NB == 1 ? 5 : 8;
-  constexpr int NS = kStep / G;      // scales of a channel per step
-  constexpr int SLOTS = kWaves / SK;  // tiles a workgroup has at once
-  constexpr int WINDOW = 4;          // steps of a wave in flight
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int groups = 2 * a.steps;
-  char *digits = lds;                                                    // [groups][4][CW][16 B]
-  float *factors = reinterpret_cast<float *>(lds + static_cast<size_t>(groups) * 64 * CW);  // [groups][CW]
-  float *red = factors + groups * CW;                                    // [kWaves][8][16]
-  float *row_factor = red + kWaves * 8 * 16;                             // [8]
-  uint32_t *bad = reinterpret_cast<uint32_t *>(row_factor + 8);          // [8]
-  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int slot = wave / SK, part = wave % SK;
-  const int M = a.m, k = a.k, steps = a.steps;
+// The largest of a wave, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = row_max16(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = a[0] > a[1] ? a[0] : a[1];
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return b[0] > b[1] ? b[0] : b[1];
+}
 
-  // The wave's work: steps part, part + SK, ... (J of them, past the last one
-  // masked) of tiles first, first + stride, ...
-  const int J = (steps + SK - 1) / SK;
-  const int stride = gridDim.x * SLOTS;
-  const int rounds = (a.tiles_total + stride - 1) / stride;
-  const int total = rounds * J;
-  uint4 codes[WINDOW];
-  float4 scales[WINDOW][NS];
-  int load_round = 0, load_j = 0;
-  auto load = [&](uint4 &c, float4(&s)[NS]) {
-    int tile = slot + SLOTS * blockIdx.x + load_round * stride;
-    tile = tile < a.tiles_total ? tile : a.tiles_total - 1;
-    int step = part + SK * load_j;
-    step = step < steps ? step : steps - 1;
-    const size_t at = static_cast<size_t>(tile) * steps + step;
-    c = a.tiles[at * 64 + lane];
+// The sum over a wave, in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+  v = v + row_up<8>(v);
+  v = v + row_up<4>(v);
+  v = v + row_up<2>(v);
+  v = v + row_up<1>(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Four columns of a row, zeros past its end.
+__device__ __forceinline__ float4 load_x(const Args &a, bool vec, int r, int col) {
+  const float *row = a.x + static_cast<size_t>(r) * a.k;
+  if (vec) return col < a.k ? *reinterpret_cast<const float4 *>(row + col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  return make_float4(col < a.k ? row[col] : 0.0f, col + 1 < a.k ? row[col + 1] : 0.0f,
+                     col + 2 < a.k ? row[col + 2] : 0.0f, col + 3 < a.k ? row[col + 3] : 0.0f);
+}
+__device__ __forceinline__ bool rows_vec(const Args &a) {
+  return a.k % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+}
+
+// 1 / sqrt(mean of squares + eps) from the sum of squares.
+__device__ __forceinline__ float rms_factor(float sum, int k) {
+  return __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(sum, static_cast<float>(k)) + 1.1920929e-7f));
+}
+__device__ __forceinline__ float square_sum(float4 v, float sum) {
+  sum = fmaf_(v.x, v.x, sum);
+  sum = fmaf_(v.y, v.y, sum);
+  sum = fmaf_(v.z, v.z, sum);
+  return fmaf_(v.w, v.w, sum);
+}
+
+// The product's columns: with one 16-column block column 5 d + r holds byte d of
+// row r (5 rows), with two column 8 d + r (8 rows).
+template <int NB>
+struct Columns {
+  static constexpr int kWide = 16 * NB, kRows = NB == 1 ? 5 : 8;
+  // A 64-column group: [4 lane chunks][columns][16 bytes].
+  static constexpr int kGroup = 64 * kWide;
+  __device__ static __forceinline__ int at(int kg, int col) { return (kg * kWide + col) * 16; }
+};
+
+// A block of 128 W columns of a row in a wave's registers, 256 columns at a time.
+template <int W>
+struct Block {
+  static constexpr int kParts = (W + 1) / 2;
+  float4 v[kParts];
+  __device__ static __forceinline__ bool holds(int p) { return 2 * p + (threadIdx.x & 63) / 32 < W; }
+  __device__ __forceinline__ void load(const Args &a, bool vec, int r, int col0) {
 #pragma unroll
-    for (int i = 0; i < NS; i++) s[i] = *reinterpret_cast<const float4 *>(a.scales + (at * NS + i) * kTile + 4 * kg);
-    if (++load_j == J) {
-      load_j = 0;
-      load_round++;
+    for (int p = 0; p < kParts; p++)
+      v[p] = holds(p) ? load_x(a, vec, r, col0 + 256 * p + 4 * (threadIdx.x & 63)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+};
+
+// A wave writes block v of row r, times `factor` if scaled: bytes to `digits`
+// [2 W groups], their weights to `weights` [columns]. True (in every lane) if a
+// value is not finite.
+template <int NB, int W>
+__device__ __forceinline__ bool stage_block(Block<W> x, int r, bool scaled, float factor, char *digits, float *weights) {
+  using C = Columns<NB>;
+  constexpr int P = Block<W>::kParts;
+  const int lane = threadIdx.x & 63, l16 = lane & 15;
+  float4(&v)[P] = x.v;
+  uint32_t big = 0;
+#pragma unroll
+  for (int p = 0; p < P; p++) {
+    if (scaled) v[p] = make_float4(v[p].x * factor, v[p].y * factor, v[p].z * factor, v[p].w * factor);
+    const float u[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t bits = __float_as_uint(u[i]) & 0x7fffffffu;
+      big = bits > big ? bits : big;
     }
+  }
+  big = wave_max(big);
+  const bool bad = big >= 0x7f800000u;
+  int e = bad || big == 0 ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(big));
+  e = e < -96 ? -96 : e;
+  // 1.5 2^23 + i holds the integer i in its low bits; adding 128 to each byte of
+  // i and inverting their top bits leaves signed bytes whose weighted sum is i.
+  auto bytes = [&](float f) {
+    const float t = __builtin_ldexpf(f, 22 - e) + 12582912.0f;
+    return (__float_as_uint(t) + (0x00808080u - 0x4b400000u)) ^ 0x00808080u;
   };
 #pragma unroll
-  for (int i = 0; i < WINDOW; i++) load(codes[i], scales[i]);
-
-  // x' as bytes, in the order the matrix instruction reads them.
-  const bool vec = k % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
-  auto load_x = [&](int r, int col) {
-    const float *row = a.x + static_cast<size_t>(r) * k;
-    if (vec) return col < k ? *reinterpret_cast<const float4 *>(row + col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    return make_float4(col < k ? row[col] : 0.0f, col + 1 < k ? row[col + 1] : 0.0f, col + 2 < k ? row[col + 2] : 0.0f,
-                       col + 3 < k ? row[col + 3] : 0.0f);
-  };
-  if (tid < 8) {
-    bad[tid] = 0;
-    row_factor[tid] = a.row_scale && tid < M ? a.row_scale[tid] : 1.0f;
-  }
-  if (a.rms) {
-    for (int r = wave; r < M; r += kWaves) {
-      float sum = 0.0f;
-      for (int col = 4 * lane; col < k; col += 256) {
-        const float4 v = load_x(r, col);
-        sum = fmaf_(v.x, v.x, sum);
-        sum = fmaf_(v.y, v.y, sum);
-        sum = fmaf_(v.z, v.z, sum);
-        sum = fmaf_(v.w, v.w, sum);
-      }
-#pragma unroll
-      for (int mask = 32; mask >= 1; mask /= 2) sum = sum + __shfl_xor(sum, mask);
-      if (lane == 0)
-        red[r] = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(sum, static_cast<float>(k)) + 1.1920929e-7f));
-    }
-  }
-  __syncthreads();
-  if (a.rms && tid < M) row_factor[tid] = red[tid];
-  __syncthreads();
-  const bool scaled = a.rms || a.row_scale;
-  for (int u = wave * 4 + kg; u < M * groups; u += kWaves * 4) {
-    const int r = u / groups, g = u - r * groups;
-    float4 v = load_x(r, 64 * g + 4 * l16);
-    if (scaled) {
-      const float f = row_factor[r];
-      v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-    }
-    uint32_t big = __float_as_uint(v.x) & 0x7fffffffu;
-    const uint32_t by = __float_as_uint(v.y) & 0x7fffffffu, bz = __float_as_uint(v.z) & 0x7fffffffu,
-                   bw = __float_as_uint(v.w) & 0x7fffffffu;
-    big = by > big ? by : big;
-    big = bz > big ? bz : big;
-    big = bw > big ? bw : big;
-    big = row_max16(big);
-    if (big >= 0x7f800000u) bad[r] = 1;
-    int e = big >= 0x7f800000u || big == 0 ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(big));
-    e = e < -96 ? -96 : e;
-    // 1.5 2^23 + i holds the integer i in its low bits; adding 128 to each
-    // byte of i and inverting their top bits leaves signed bytes whose weighted
-    // sum is i.
-    auto bytes = [&](float f) {
-      const float t = __builtin_ldexpf(f, 22 - e) + 12582912.0f;
-      return (__float_as_uint(t) + (0x00808080u - 0x4b400000u)) ^ 0x00808080u;
-    };
-    const uint32_t w0 = bytes(v.x), w1 = bytes(v.y), w2 = bytes(v.z), w3 = bytes(v.w);
+  for (int p = 0; p < P; p++) {
+    const uint32_t w0 = bytes(v[p].x), w1 = bytes(v[p].y), w2 = bytes(v[p].z), w3 = bytes(v[p].w);
     const uint32_t a01 = __builtin_amdgcn_perm(w1, w0, 0x05010400u), a23 = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
     const uint32_t b01 = __builtin_amdgcn_perm(w1, w0, 0x0c0c0602u), b23 = __builtin_amdgcn_perm(w3, w2, 0x0c0c0602u);
     const uint32_t d[3] = {__builtin_amdgcn_perm(a23, a01, 0x05040100u), __builtin_amdgcn_perm(a23, a01, 0x07060302u),
                            __builtin_amdgcn_perm(b23, b01, 0x05040100u)};
-    char *to = digits + (static_cast<size_t>(g * 4 + l16 / 4) * CW + r) * 16 + 4 * (l16 % 4);
+    if (x.holds(p)) {
+      char *to = digits + (4 * p + lane / 16) * C::kGroup + C::at(l16 / 4, r) + 4 * (l16 % 4);
 #pragma unroll
-    for (int i = 0; i < 3; i++) *reinterpret_cast<uint32_t *>(to + i * RS * 16) = d[i];
-    if (l16 < 3) factors[g * CW + l16 * RS + r] = __builtin_ldexpf(1.0f, e - 26 + 8 * l16);
+      for (int i = 0; i < 3; i++) *reinterpret_cast<uint32_t *>(to + i * C::kRows * 16) = d[i];
+    }
+  }
+  if (lane < 3) weights[lane * C::kRows + r] = __builtin_ldexpf(1.0f, e - 26 + 8 * lane);
+  return bad;
+}
+
+// Steps of a wave's turn where the rows come as bytes.
+constexpr int kPreSteps = 4;
+
+// The rows as bytes in memory, for large calls: a wave for each block (blockIdx.x,
+// wave) of row blockIdx.y, after the sum of squares of the whole row if it is
+// normalized.
+template <int NB>
+__global__ __launch_bounds__(256) void rows4_kernel(Args a, int blocks) {
+  using C = Columns<NB>;
+  __shared__ float s_sum[4];
+  __shared__ uint32_t s_bad;
+  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool vec = rows_vec(a);
+  const int block = 4 * blockIdx.x + wave;
+  Block<kPreSteps> x;
+  x.load(a, vec, r, block * kPreSteps * kStep);
+  if (tid == 0) s_bad = 0;
+  float factor = a.row_scale ? a.row_scale[r] : 1.0f;
+  if (a.rms) {
+    float sum = 0.0f;
+    for (int col = 4 * tid; col < a.k; col += 8192) {
+      float4 v[8];  // in flight together
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = load_x(a, vec, r, col + 1024 * i);
+#pragma unroll
+      for (int i = 0; i < 8; i++) sum = square_sum(v[i], sum);
+    }
+    sum = wave_sum(sum);
+    if (lane == 0) s_sum[wave] = sum;
   }
   __syncthreads();
+  if (a.rms) factor = rms_factor((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), a.k);
+  if (block < blocks &&
+      stage_block<NB, kPreSteps>(x, r, a.rms || a.row_scale, factor,
+                                 a.digits + static_cast<size_t>(block) * 2 * kPreSteps * C::kGroup,
+                                 a.weights + block * C::kWide))
+    s_bad = 1;
+  __syncthreads();
+  if (tid == 0) {
+    a.marks[blockIdx.x * 8 + r] = s_bad;
+    a.row_factors[r] = factor;
+  }
+}
+
+// The workgroup's LDS accesses so far, and no load from memory, are waited for.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// NB: 16-column blocks of the product (Columns). SK: waves that share a tile's
+// columns, each W steps of a turn. G: columns per scale. PRE: the rows come as bytes
+// from rows4_kernel and pass through LDS turn by turn; otherwise the workgroup
+// writes all of them to LDS itself.
+template <int NB, int SK, int W, int G, bool PRE>
+__global__ __launch_bounds__(64 * kWaves, G == 32 && W > 2 ? 2 : 4) void gemv4_kernel(Args a) {
+  using C = Columns<NB>;
+  constexpr int NS = kStep / G;             // scales of a channel per step
+  constexpr int SLOTS = kWaves / SK;        // tiles a workgroup has at once
+  constexpr int BLOCK = 2 * W * C::kGroup;  // bytes of a block
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int steps = a.steps, M = a.m, k = a.k;
+  const int turns = (steps + W * SK - 1) / (W * SK);
+  const int held = PRE ? 2 * SK : turns * SK;                    // blocks in LDS (PRE: two turns)
+  float *weights = reinterpret_cast<float *>(lds + held * BLOCK);  // [held][columns]
+  float *red = weights + held * C::kWide;                        // [kWaves][8][16]
+  float *row_factor = red + kWaves * 8 * 16;                     // [8]
+  uint32_t *bad = reinterpret_cast<uint32_t *>(row_factor + 8);  // [8]
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int slot = wave / SK, part = wave % SK;
+  const bool scaled = a.rms || a.row_scale;
+
+  // The wave's work: of tiles first, first + stride, ... block part of every
+  // turn: W steps, whose bytes are zeros past the last one.
+  const int stride = gridDim.x * SLOTS;
+  const int rounds = (a.tiles_total + stride - 1) / stride;
+  v4u codes[W];
+  v4f scales[W][NS];
+  auto load = [&](int i, int round, int turn) {
+    int tile = slot + SLOTS * blockIdx.x + round * stride;
+    tile = tile < a.tiles_total ? tile : a.tiles_total - 1;
+    int step = (turn * SK + part) * W + i;
+    step = step < steps ? step : steps - 1;
+    const size_t at = static_cast<size_t>(tile) * steps + step;
+    codes[i] = reinterpret_cast<const v4u *>(a.tiles)[at * 64 + lane];
+#pragma unroll
+    for (int q = 0; q < NS; q++) scales[i][q] = *reinterpret_cast<const v4f *>(a.scales + (at * NS + q) * kTile + 4 * kg);
+  };
+
+  // PRE: a turn's bytes from memory to registers and on to LDS, and its weights to
+  // registers.
+  constexpr int PER = PRE ? SK * BLOCK / 16 / (64 * kWaves) : 1;  // 16-byte pieces of a thread
+  static_assert(!PRE || SK * BLOCK % (16 * 64 * kWaves) == 0, "whole pieces");
+  v4u moved[PER];
+  float weight[NB];
+  auto fetch = [&](int turn) {
+#pragma unroll
+    for (int p = 0; p < PER; p++)
+      moved[p] = reinterpret_cast<const v4u *>(a.digits)[turn * (SK * BLOCK / 16) + tid + 64 * kWaves * p];
+  };
+  auto fetch_weight = [&](int turn) {
+#pragma unroll
+    for (int b = 0; b < NB; b++) weight[b] = a.weights[(turn * SK + part) * C::kWide + 16 * b + l16];
+  };
+  auto place = [&](int buffer) {
+#pragma unroll
+    for (int p = 0; p < PER; p++) reinterpret_cast<v4u *>(lds)[buffer * (SK * BLOCK / 16) + tid + 64 * kWaves * p] = moved[p];
+  };
+  if constexpr (PRE) {
+    fetch(0);
+    fetch_weight(0);
+#pragma unroll
+    for (int i = 0; i < W; i++) load(i, 0, 0);
+    if (tid < 8) {
+      uint32_t any = 0;
+      for (int p = 0; p < a.parts; p++) any |= tid < M ? a.marks[p * 8 + tid] : 0;
+      bad[tid] = any;
+      row_factor[tid] = tid < M ? a.row_factors[tid] : 1.0f;
+    }
+    place(0);
+  } else {
+    // The rows' loads go before the codes': loads arrive in order, and so the rows
+    // are written while the codes are on their way. This wave writes block
+    // turn * SK + part of rows slot, slot + SLOTS, ...: a turn's at a time, the
+    // first one's from registers.
+    constexpr int ROWS = (C::kRows + SLOTS - 1) / SLOTS;
+    const bool vec = rows_vec(a);
+    float row_scale = 1.0f;
+    if (tid < 8 && a.row_scale) row_scale = a.row_scale[tid < M ? tid : 0];
+    Block<W> x[ROWS];
+    auto load_rows = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < ROWS; i++)
+        if (slot + SLOTS * i < M) x[i].load(a, vec, slot + SLOTS * i, (t * SK + part) * W * kStep);
+    };
+    load_rows(0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < W; i++) load(i, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (tid < 8) {
+      bad[tid] = 0;
+      row_factor[tid] = row_scale;
+    }
+    if (a.rms) {
+      float sum[ROWS];
+#pragma unroll
+      for (int i = 0; i < ROWS; i++) sum[i] = 0.0f;
+      for (int t = 0; t < turns; t++) {
+        if (t > 0) load_rows(t);
+#pragma unroll
+        for (int i = 0; i < ROWS; i++)
+          if (slot + SLOTS * i < M)
+#pragma unroll
+            for (int p = 0; p < Block<W>::kParts; p++) sum[i] = square_sum(x[i].v[p], sum[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < ROWS; i++) {
+        const float total = wave_sum(sum[i]);
+        if (lane == 0 && slot + SLOTS * i < M) red[(slot + SLOTS * i) * SK + part] = total;
+      }
+      lds_barrier();
+      if (tid < M) {
+        float total = red[tid * SK];
+        for (int q = 1; q < SK; q++) total += red[tid * SK + q];
+        row_factor[tid] = rms_factor(total, k);
+      }
+      if (turns > 1) load_rows(0);
+    }
+    lds_barrier();
+    for (int t = 0; t < turns; t++) {
+      if (t > 0) load_rows(t);
+      const int block = t * SK + part;
+#pragma unroll
+      for (int i = 0; i < ROWS; i++) {
+        const int r = slot + SLOTS * i;
+        if (r < M &&
+            stage_block<NB, W>(x[i], r, scaled, row_factor[r], lds + block * BLOCK, weights + block * C::kWide))
+          bad[r] = 1;
+      }
+    }
+  }
+  lds_barrier();
 
   float acc[NB][4];
 #pragma unroll
   for (int b = 0; b < NB; b++)
 #pragma unroll
     for (int i = 0; i < 4; i++) acc[b][i] = 0.0f;
-  auto consume = [&](const uint4 &c, const float4(&s)[NS], int step) {
-    const uint32_t word[4] = {c.x, c.y, c.z, c.w};
+  // Step i of the block at `digits`, added to the block's sums.
+  auto consume = [&](const v4u &word, const v4f(&s)[NS], const char *digits, float(&sum)[NB][4]) {
 #pragma unroll
     for (int half = 0; half < 2; half++) {
-      const int g = 2 * step + half;
       v4i A;
 #pragma unroll
       for (int w = 0; w < 2; w++) {
@@ -197,13 +383,11 @@ __global__ __launch_bounds__(64 * kWaves) void gemv4_kernel(Args a) {
       }
 #pragma unroll
       for (int b = 0; b < NB; b++) {
-        const v4i B = *reinterpret_cast<const v4i *>(digits + (static_cast<size_t>(g * 4 + kg) * CW + 16 * b + l16) * 16);
-        const float f = factors[g * CW + 16 * b + l16];
+        const v4i B = *reinterpret_cast<const v4i *>(digits + half * C::kGroup + C::at(kg, 16 * b + l16));
         const v4i zero = {0, 0, 0, 0};
-        auto add = [&](const v4i &sum, const float4 &sc) {
-          const float q[4] = {sc.x, sc.y, sc.z, sc.w};
+        auto add = [&](const v4i &c, const v4f &q) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) acc[b][i] = fmaf_(static_cast<float>(sum[i]) * q[i], f, acc[b][i]);
+          for (int i = 0; i < 4; i++) sum[b][i] = fmaf_(static_cast<float>(c[i]), q[i], sum[b][i]);
         };
         if constexpr (G >= 64) {
           add(__builtin_amdgcn_mfma_i32_16x16x64_i8(A, B, zero, 0, 0, 0), s[G == 64 ? half : 0]);
@@ -214,6 +398,21 @@ __global__ __launch_bounds__(64 * kWaves) void gemv4_kernel(Args a) {
           add(__builtin_amdgcn_mfma_i32_16x16x64_i8(A, hi, zero, 0, 0, 0), s[2 * half + 1]);
         }
       }
+    }
+  };
+
+  // What an ADD call adds to: loaded ahead of a tile's last turn.
+  const bool quads = a.n % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  v4f residual = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto load_residual = [&](int round) {
+    const int ch = (slot + SLOTS * blockIdx.x + round * stride) * kTile + 4 * kg;
+    if (l16 >= M || part > 0 || ch >= a.n) return;
+    const float *out = a.out + static_cast<size_t>(l16) * a.n + ch;
+    if (quads) {
+      residual = *reinterpret_cast<const v4f *>(out);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i++) residual[i] = out[ch + i < a.n ? i : 0];
     }
   };
 
@@ -233,7 +432,7 @@ __global__ __launch_bounds__(64 * kWaves) void gemv4_kernel(Args a) {
     if constexpr (SK > 1) {
       if (part > 0 && l16 < 8)
         *reinterpret_cast<float4 *>(red + (wave * 8 + l16) * 16 + 4 * kg) = make_float4(total[0], total[1], total[2], total[3]);
-      __syncthreads();
+      lds_barrier();
       if (part == 0 && l16 < 8) {
 #pragma unroll
         for (int p = 1; p < SK; p++) {
@@ -244,7 +443,7 @@ __global__ __launch_bounds__(64 * kWaves) void gemv4_kernel(Args a) {
           total[3] += v.w;
         }
       }
-      __syncthreads();
+      lds_barrier();
       if (part > 0) return;
     }
     const int r = l16, ch = tile * kTile + 4 * kg;
@@ -276,70 +475,129 @@ __global__ __launch_bounds__(64 * kWaves) void gemv4_kernel(Args a) {
       if (ch + 2 < a.n) out[1] = squared_relu_glu(total[2], total[3]);
       return;
     }
+    if (a.epilogue == FOCR_EPI_ADD)
+#pragma unroll
+      for (int i = 0; i < 4; i++) total[i] = residual[i] + total[i];
     float *out = a.out + static_cast<size_t>(r) * a.n + ch;
+    if (quads) {
+      *reinterpret_cast<v4f *>(out) = v4f{total[0], total[1], total[2], total[3]};
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++)
-      if (ch + i < a.n) out[i] = a.epilogue == FOCR_EPI_ADD ? out[i] + total[i] : total[i];
+      if (ch + i < a.n) out[i] = total[i];
   };
 
-  int round = 0, j = 0;
-  for (int base = 0; base < total; base += WINDOW) {
+  // Turn after turn: every load is one that the next turn consumes, and none is
+  // under a branch, so a step waits for its own codes only. A turn with nothing
+  // after it loads nothing.
+  int round = 0, turn = 0, buffer = 0;
+  auto take = [&](auto more) {
+    constexpr bool kMore = decltype(more)::value;
+    const bool ends = turn + 1 == turns;
+    const int next_round = ends ? round + 1 : round, next_turn = ends ? 0 : turn + 1;
+    if (ends && a.epilogue == FOCR_EPI_ADD) load_residual(round);
+    if constexpr (PRE && kMore) fetch(next_turn);
+    const int block = PRE ? buffer * SK + part : turn * SK + part;
+    float sum[NB][4], f[NB];
 #pragma unroll
-    for (int i = 0; i < WINDOW; i++) {
-      if (base + i < total) {
-        const int step = part + SK * j;
-        if (step < steps) consume(codes[i], scales[i], step);
-        if (++j == J) {
-          finish(round);
-          j = 0;
-          round++;
-        }
-        if (base + i + WINDOW < total) load(codes[i], scales[i]);
-      }
+    for (int b = 0; b < NB; b++) {
+      f[b] = PRE ? weight[b] : weights[block * C::kWide + 16 * b + l16];
+#pragma unroll
+      for (int i = 0; i < 4; i++) sum[b][i] = 0.0f;
     }
-  }
+    if constexpr (PRE && kMore) fetch_weight(next_turn);
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+      consume(codes[i], scales[i], lds + block * BLOCK + 2 * i * C::kGroup, sum);
+      if constexpr (kMore) load(i, next_round, next_turn);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[b][i] = fmaf_(sum[b][i], f[b], acc[b][i]);
+    if constexpr (PRE && kMore) {
+      buffer ^= 1;
+      place(buffer);
+      lds_barrier();
+    }
+    if (ends) finish(round);
+    round = next_round;
+    turn = next_turn;
+  };
+  for (int t = 1; t < rounds * turns; t++) take(std::true_type());
+  take(std::false_type());
 }
 
-size_t lds_bytes(int nb, size_t steps) {
-  const size_t cw = 16 * nb;
-  return 2 * steps * (64 * cw + 4 * cw) + kWaves * 8 * 16 * 4 + 8 * 4 + 8 * 4;
-}
-
-template <int NB, int SK, int G>
-int launch_one(Ctx *ctx, const Args &a, int blocks, size_t lds) {
-  // Above 64 KB the attribute has to allow it; once per device and kernel.
-  static bool allowed[64] = {};
-  if (lds > 64 * 1024 && !(ctx->device < 64 && allowed[ctx->device])) {
-    FOCR_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(gemv4_kernel<NB, SK, G>),
+template <int NB, int SK, int W, int G, bool PRE>
+int launch_one(Ctx *ctx, const Args &a) {
+  using C = Columns<NB>;
+  const size_t turns = (static_cast<size_t>(a.steps) + W * SK - 1) / (W * SK), held = PRE ? 2 * SK : turns * SK;
+  const size_t lds = held * (2 * W * C::kGroup + C::kWide * 4) + kWaves * 8 * 16 * 4 + 8 * 4 + 8 * 4;
+  FOCR_REQUIRE(lds <= kLdsBytes, FOCR_E_SHAPE, "GEMV: in_dim too large for the rows of x in LDS");
+  // Above 64 KB the kernel has to be allowed it, on each device.
+  if (lds > 64 * 1024)
+    FOCR_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(gemv4_kernel<NB, SK, W, G, PRE>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLdsBytes)));
-    if (ctx->device < 64) allowed[ctx->device] = true;
-  }
-  hipLaunchKernelGGL((gemv4_kernel<NB, SK, G>), dim3(blocks), dim3(64 * kWaves), lds, ctx->stream, a);
+  constexpr int slots = kWaves / SK;
+  const int want = (a.tiles_total + slots - 1) / slots;
+  const int blocks = want < 512 ? want : 512;
+  hipLaunchKernelGGL((gemv4_kernel<NB, SK, W, G, PRE>), dim3(blocks), dim3(64 * kWaves), lds, ctx->stream, a);
   FOCR_HIP_CHECK(hipGetLastError());
   return FOCR_OK;
 }
 
-template <int NB, int G>
-int launch_parts(Ctx *ctx, const Args &a, size_t lds) {
-  // Waves per tile: enough to give each SIMD two.
-  const int sk = a.tiles_total >= 2048 ? 1 : a.tiles_total >= 512 ? 4 : 8;
-  const int slots = kWaves / sk;
-  const int want = (a.tiles_total + slots - 1) / slots;
-  const int blocks = want < 512 ? want : 512;
-  switch (sk) {
-    case 1: return launch_one<NB, 1, G>(ctx, a, blocks, lds);
-    case 4: return launch_one<NB, 4, G>(ctx, a, blocks, lds);
-    default: return launch_one<NB, 8, G>(ctx, a, blocks, lds);
+// The fewest steps of a turn that take all of a row, at most 4.
+template <int NB, int SK, int G>
+int launch_steps(Ctx *ctx, const Args &a) {
+  switch ((a.steps + SK - 1) / SK) {
+    case 1: return launch_one<NB, SK, 1, G, false>(ctx, a);
+    case 2: return launch_one<NB, SK, 2, G, false>(ctx, a);
+    case 3: return launch_one<NB, SK, 3, G, false>(ctx, a);
+    default: return launch_one<NB, SK, 4, G, false>(ctx, a);
   }
 }
 
-template <int NB>
-int launch_group(Ctx *ctx, const Args &a, size_t lds) {
-  switch (a.group) {
-    case 32: return launch_parts<NB, 32>(ctx, a, lds);
-    case 64: return launch_parts<NB, 64>(ctx, a, lds);
-    default: return launch_parts<NB, 128>(ctx, a, lds);
+template <int NB, int G>
+int launch_parts(Ctx *ctx, const Args &a, bool pre) {
+  // Waves per tile: enough to give each SIMD two.
+  if (pre) {
+    if (a.tiles_total >= 2048) return launch_one<NB, 1, kPreSteps, G, true>(ctx, a);
+    if (a.tiles_total >= 512) return launch_one<NB, 2, kPreSteps, G, true>(ctx, a);
+    return launch_one<NB, 4, kPreSteps, G, true>(ctx, a);
   }
+  if (a.tiles_total >= 2048) return launch_steps<NB, 2, G>(ctx, a);
+  if (a.tiles_total >= 512) return launch_steps<NB, 4, G>(ctx, a);
+  return launch_steps<NB, 8, G>(ctx, a);
+}
+
+// Blocks of the rows' bytes: whole turns of up to four waves.
+size_t pre_blocks(size_t steps) { return (steps + 4 * kPreSteps - 1) / (4 * kPreSteps) * 4; }
+
+template <int NB>
+int launch_group(Ctx *ctx, Args a, bool pre) {
+  using C = Columns<NB>;
+  if (pre) {
+    const size_t blocks = pre_blocks(a.steps);
+    a.parts = static_cast<int>(blocks / 4);
+    a.digits = static_cast<char *>(ctx->scratch);
+    a.weights = reinterpret_cast<float *>(a.digits + blocks * 2 * kPreSteps * C::kGroup);
+    a.row_factors = a.weights + blocks * C::kWide;
+    a.marks = reinterpret_cast<uint32_t *>(a.row_factors + 8);
+    hipLaunchKernelGGL(rows4_kernel<NB>, dim3(a.parts, a.m), dim3(256), 0, ctx->stream, a, static_cast<int>(blocks));
+    FOCR_HIP_CHECK(hipGetLastError());
+  }
+  switch (a.group) {
+    case 32: return launch_parts<NB, 32>(ctx, a, pre);
+    case 64: return launch_parts<NB, 64>(ctx, a, pre);
+    default: return launch_parts<NB, 128>(ctx, a, pre);
+  }
+}
+
+// Scratch of a call whose rows are written as bytes first.
+size_t rows_bytes(size_t m, size_t steps) {
+  const size_t blocks = pre_blocks(steps), wide = m <= 5 ? Columns<1>::kWide : Columns<2>::kWide;
+  return blocks * (2 * kPreSteps * 64 * wide + wide * 4) + 8 * 4 + blocks / 4 * 8 * 4;
 }
 
 // ---- storage -------------------------------------------------------------------
@@ -435,33 +693,30 @@ unsigned blocks_for(size_t count) {
 int launch_gemv4(Ctx *ctx, const Linear *lin, const float *x, size_t rows, const float *row_scale, int epilogue,
                  float *out, bool rms_norm) {
   FOCR_HIP_CHECK(hipSetDevice(ctx->device));
-  const size_t steps = steps_of(lin->k), width = epilogue == FOCR_EPI_GLU ? lin->n / 2 : lin->n;
-  FOCR_REQUIRE(lds_bytes(1, steps) <= kLdsBytes, FOCR_E_SHAPE, "GEMV: in_dim too large for the rows of x in LDS");
-  const size_t chunk = lds_bytes(2, steps) <= kLdsBytes ? 8 : 5;
-  for (size_t r0 = 0; r0 < rows; r0 += chunk) {
-    const size_t m = rows - r0 < chunk ? rows - r0 : chunk;
-    Args a = {};
-    a.tiles = static_cast<const uint4 *>(lin->gemv_codes);
-    a.scales = lin->gemv_scales;
-    a.exc_cols = lin->exc_cols;
-    a.exc_vals = lin->exc_vals;
-    a.n_exc = static_cast<int>(lin->n_exc);
-    a.x = x + r0 * lin->k;
-    a.row_scale = row_scale ? row_scale + r0 : nullptr;
-    a.out = out + r0 * width;
-    a.m = static_cast<int>(m);
-    a.n = static_cast<int>(lin->n);
-    a.k = static_cast<int>(lin->k);
-    a.group = static_cast<int>(lin->group);
-    a.steps = static_cast<int>(steps);
-    a.tiles_total = static_cast<int>(lin->gemv_tiles);
-    a.rms = rms_norm ? 1 : 0;
-    a.epilogue = epilogue;
-    const int nb = m <= 5 ? 1 : 2;
-    const int rc = nb == 1 ? launch_group<1>(ctx, a, lds_bytes(1, steps)) : launch_group<2>(ctx, a, lds_bytes(2, steps));
+  const size_t steps = steps_of(lin->k);
+  Args a = {};
+  a.tiles = static_cast<const uint4 *>(lin->gemv_codes);
+  a.scales = lin->gemv_scales;
+  a.exc_cols = lin->exc_cols;
+  a.exc_vals = lin->exc_vals;
+  a.n_exc = static_cast<int>(lin->n_exc);
+  a.x = x;
+  a.row_scale = row_scale;
+  a.out = out;
+  a.m = static_cast<int>(rows);
+  a.n = static_cast<int>(lin->n);
+  a.k = static_cast<int>(lin->k);
+  a.group = static_cast<int>(lin->group);
+  a.steps = static_cast<int>(steps);
+  a.tiles_total = static_cast<int>(lin->gemv_tiles);
+  a.rms = rms_norm ? 1 : 0;
+  a.epilogue = epilogue;
+  const bool pre = rows * lin->k > 16384 || lin->k > 8192;
+  if (pre) {
+    const int rc = ensure_scratch(ctx, rows_bytes(rows, steps));
     if (rc != FOCR_OK) return rc;
   }
-  return FOCR_OK;
+  return rows <= 5 ? launch_group<1>(ctx, a, pre) : launch_group<2>(ctx, a, pre);
 }
 
 int pack_linear4(Ctx *ctx, Linear *lin, const int8_t *codes, size_t *total) {

@@ -37,16 +37,20 @@ def weights64(codes, scales, group, columns=(), vals=None):
 
 
 def product(x, w):
-    """x w^T in 64 bits, and how far FP32's may be from it: the inputs of each 64
-    columns to 2^-23 of the largest of them, and one rounding for each of the
-    products, sums and scales of the groups' results, of terms whose magnitudes
-    add up to `size`."""
+    """x w^T in 64 bits, and how far FP32's may be from it. Inputs are integers of
+    2^(e - 22), 2^e up to twice the largest of their block of 128, 256, 384 or 512
+    columns, so off by 2^-22 of that; and sums of terms whose magnitudes add up to
+    `size` (1.02 of it with the bytes' own magnitudes) round once for every 32
+    columns, for every block, and a few times for the bytes' and waves' parts."""
     rows, k = x.shape
-    pad = -k % 64
-    big = np.abs(np.pad(x, ((0, 0), (0, pad)))).reshape(rows, -1, 64).max(axis=2)
-    size = np.repeat(big, 64, axis=1)[:, :k] @ np.abs(w).T
+    big = np.zeros_like(x)
+    for wide in (128, 256, 384, 512):
+        pad = -k % wide
+        most = np.abs(np.pad(x, ((0, 0), (0, pad)))).reshape(rows, -1, wide).max(axis=2)
+        big = np.maximum(big, np.repeat(most, wide, axis=1)[:, :k])
+    size = 1.02 * big @ np.abs(w).T
     groups = -(-k // 32)
-    return x @ w.T, size * (2 * EPS + (3 * groups + 16) * EPS)
+    return x @ w.T, size * (4 * EPS + (1.25 * groups + 16) * EPS)
 
 
 def normed(x):
@@ -85,7 +89,21 @@ def test_decode_against_64_bits(fh, n, k, group):
         check(got, *product(x.astype(np.float64), w), f"n {n} k {k} group {group} rows {rows}")
 
 
-@pytest.mark.parametrize("n,k,group", [(64, 96, 32), (2048, 768, 64), (1030, 1300, 128), (4608, 768, 64)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,k", [(20, 20000), (300, 8200), (1000, 4100), (9000, 2304), (33000, 2200)])
+def test_decode_of_large_calls(fh, n, k, group):
+    # Rows written as bytes by a kernel of their own, and passed through LDS in turns.
+    codes, scales, _ = matrix(n, k, group, n + k)
+    lin = fh.QuantLinear.from_parts(n, k, group, codes, scales, bits=4)
+    w = weights64(codes, scales, group)
+    for rows in (1, 5, 8) if k > 8192 else (5, 8):
+        x = gen.normal((rows, k), 2.0, rows)
+        x[:, k // 3] *= 50.0
+        got = host(lin.linear(to_dev(x), rows))
+        check(got, *product(x.astype(np.float64), w), f"n {n} k {k} group {group} rows {rows}")
+
+
+@pytest.mark.parametrize("n,k,group", [(64, 96, 32), (2048, 768, 64), (1030, 1300, 128), (4608, 768, 64), (70, 4500, 64)])
 @pytest.mark.parametrize("rows", [1, 4, 5, 8])
 def test_decode_with_its_neighbours(fh, n, k, group, rows):
     codes, scales, _ = matrix(n, k, group, n + k)
@@ -135,7 +153,7 @@ def test_dequantize_is_bit_exact(fh, n, k, group):
 
 
 def test_inputs_of_every_magnitude(fh):
-    # Each 64 columns have an exponent of their own; tiny and huge rows too.
+    # Rows and blocks of columns have exponents of their own.
     n, k, group = 64, 512, 64
     codes, scales, _ = matrix(n, k, group, 13)
     lin = fh.QuantLinear.from_parts(n, k, group, codes, scales, bits=4)
@@ -151,10 +169,11 @@ def test_inputs_of_every_magnitude(fh):
     check(host(lin.linear(to_dev(x), 8)), *product(x.astype(np.float64), w))
 
 
-def test_rows_with_infinities_and_nans(fh):
+@pytest.mark.parametrize("k", [200, 4200])
+def test_rows_with_infinities_and_nans(fh, k):
     # Such a row is the FP32 sum of its products: an infinity times a code of zero
     # is NaN, and so are two infinities of different sign; the other rows keep their values.
-    n, k, group = 300, 200, 32
+    n, group = 300, 32
     codes, scales, _ = matrix(n, k, group, 19)
     codes[:, 7] = np.where(codes[:, 7] == 0, 1, codes[:, 7])
     codes[5, 7] = 0
@@ -218,6 +237,39 @@ def test_captured_steps_replay(fh):
         torch.cuda.synchronize()
         got = host(out)
         assert_bitwise(got, host(lin.linear_ex(x, 5, rms_norm=True)), f"replay {seed}")
+
+
+def test_capture_needs_the_scratch_of_a_large_call(fh):
+    import torch
+
+    n, k = 64, 9000
+    codes, scales, _ = matrix(n, k, 64, 71)
+    ctx = fh.Context(0)
+    lin = fh.QuantLinear.from_parts(n, k, 64, codes, scales, ctx=ctx, bits=4)
+    x = torch.zeros(3, k, device="cuda:0")
+    out = torch.zeros(3, n, device="cuda:0")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ctx.use_stream(torch.cuda.current_stream())
+        with pytest.raises(fh.FocrError) as e:
+            lin.linear(x, 3, output=out)
+        out.add_(1.0)
+    ctx.use_stream(torch.cuda.current_stream())
+    assert e.value.code == -3
+    lin.linear(x, 3, output=out)  # uncaptured: the scratch grows
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ctx.use_stream(torch.cuda.current_stream())
+        lin.linear(x, 3, output=out)
+    ctx.use_stream(torch.cuda.current_stream())
+    for seed in range(3):
+        x.copy_(to_dev(gen.normal((3, k), 1.0, seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = host(out)
+        assert_bitwise(got, host(lin.linear(x, 3)), f"replay {seed}")
 
 
 @pytest.mark.parametrize("rows", [9, 40, 200])
