@@ -1,0 +1,811 @@
+// A cache of pages that sequences share, in 8 bits: appending a step's keys and
+// values (ready, or split, normalized and rotated from the QKV rows on the way),
+// attention of 1..=8 rows of every sequence of a batch, and reading rows back.
+//
+// A block is 16 positions of one head: 1 KB of codes and one FP32 scale,
+//
+//   scale = fl(m / 127), m the largest magnitude of the block's stored positions
+//   code = rint(fl(x fl(1 / scale))), and the block holds fl(code scale)
+//
+// (zeros where m / 127 is below 2^-126; NaN where a value is not finite). Pages hold
+// `page` positions, a power of two from 16 on: for each head its blocks in order.
+// Key codes stand as [position][64], signed; value codes as [dim][16 positions],
+// plus 128: both what the attention's matrix instructions take 16 bytes at a time.
+//
+// A block that is not full is written again by the next append, with the scale that
+// its positions then need. So that this rounds every value once, the last two
+// blocks of a sequence are also kept in FP32 beside the pages (two, so that a step
+// that takes back up to 16 positions finds them too): what the cache holds depends
+// on the rows appended, and not on how many at a time. Where a block is not
+// there (a sequence that goes on from pages it was given, or goes back further),
+// its earlier positions are taken from its codes.
+#include <type_traits>
+
+#include "decode_common.hpp"
+#include "rms_tree.hpp"
+
+namespace focr {
+namespace {
+
+constexpr int kBlock = 16, kBlockBytes = kBlock * 64;
+
+struct Pages {
+  int device = 0, shift = 0;  // log2 of the blocks of a page
+  size_t n_pages = 0, page = 0, n_seqs = 0, seq_pages = 0, n_heads = 0, key_heads = 0, kv_heads = 0;
+  int8_t *k_codes = nullptr;   // [page][key head][block][1 KB]
+  uint8_t *v_codes = nullptr;  // [page][KV head][block][1 KB]
+  float *k_scales = nullptr, *v_scales = nullptr;  // [page][head][block]
+  int32_t *table = nullptr;    // [sequence][seq_pages], -1: no page
+  float *open = nullptr;       // [sequence][key heads, then KV heads][block % 2][16][64]
+  int32_t *tags = nullptr;     // [sequence][heads][2]: the block that `open` holds, or -1
+  int32_t *refused = nullptr;  // [sequence]
+  size_t device_bytes = 0;
+};
+
+// What the kernels read of a cache, and a call's rows.
+struct Cache {
+  int8_t *k_codes;
+  uint8_t *v_codes;
+  float *k_scales, *v_scales;
+  const int32_t *table;
+  float *open;
+  int32_t *tags, *refused;
+  int shift, seq_pages, n_pages, n_heads, key_heads, kv_heads;
+  const int32_t *row_start, *lens;  // row_start null: row r is sequence r's
+  int rows, n_seqs;
+
+  // Positions `len` .. `len + n - 1` of a sequence are rows `first` .. of the call;
+  // false if it is refused (n and len are 0 then, as for one that takes no part).
+  __device__ __forceinline__ bool span(int seq, int &len, int &first, int &n) const {
+    first = row_start ? row_start[seq] : seq;
+    const int end = row_start ? row_start[seq + 1] : seq + 1;
+    len = lens[seq];
+    n = end - first;
+    if (len < 0) {
+      n = len = 0;
+      return true;
+    }
+    const long capacity = static_cast<long>(seq_pages) << (shift + 4);
+    if (first < 0 || end < first || end > rows || static_cast<long>(len) + n > capacity) {
+      n = len = 0;
+      return false;
+    }
+    return true;
+  }
+  // The block's number in the pages of one head, or -1 if it has no page.
+  __device__ __forceinline__ long block_at(int seq, int block, int heads, int head) const {
+    const int page = table[static_cast<size_t>(seq) * seq_pages + (block >> shift)];
+    return page < 0 ? -1 : (((static_cast<long>(page) * heads + head) << shift) + (block & ((1 << shift) - 1)));
+  }
+};
+
+// One unit of a call's work that is dealt over the sequences: `of` gives the units of
+// n rows from position len on. A wave finds unit u; false past the last one. Rows
+// have to begin where the sequences before end, or later, so that all units together
+// are bounded by the call's rows.
+struct Unit {
+  int seq, len, first, n, index;
+};
+template <typename Of>
+__device__ __forceinline__ bool find_unit(const Cache &c, int u, const Of &of, Unit &unit) {
+  const int lane = threadIdx.x & 63;
+  if (!c.row_start) {
+    if (u >= c.n_seqs) return false;
+    unit.seq = u;
+    unit.index = 0;
+    if (!c.span(u, unit.len, unit.first, unit.n)) c.refused[u] = 1;
+    return unit.n > 0;
+  }
+  int before = 0, most = 0;
+  for (int base = 0; base < c.n_seqs; base += 64) {
+    const int seq = base + lane;
+    int len = 0, first = 0, n = 0, units = 0, reach = 0;
+    bool fine = true;
+    if (seq < c.n_seqs) {
+      fine = c.span(seq, len, first, n);
+      reach = n > 0 ? first + n : 0;
+    }
+    // The furthest end of the sequences before this one.
+    int top = reach;
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(top, d);
+      if (lane >= d) top = o > top ? o : top;
+    }
+    int prior = __shfl_up(top, 1);
+    prior = lane == 0 ? most : (prior > most ? prior : most);
+    if (n > 0 && first < prior) {
+      fine = false;
+      n = 0;
+    }
+    if (!fine) c.refused[seq] = 1;
+    units = n > 0 ? of(len, n) : 0;
+    int sum = units;
+    for (int d = 1; d < 64; d *= 2) {
+      const int o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
+    }
+    const bool here = units > 0 && u >= before + sum - units && u < before + sum;
+    const unsigned long long found = __ballot(here);
+    if (found) {
+      const int src = __ffsll(found) - 1;
+      unit.seq = base + src;
+      unit.len = __shfl(len, src);
+      unit.first = __shfl(first, src);
+      unit.n = __shfl(n, src);
+      unit.index = u - before - __shfl(sum - units, src);
+      return true;
+    }
+    before += __shfl(sum, 63);
+    const int last = __shfl(top, 63);
+    most = last > most ? last : most;
+  }
+  return false;
+}
+
+// ---- append ------------------------------------------------------------------
+struct AppendArgs {
+  Cache c;
+  const float *qkv, *rope;  // QKV rows and factors, or
+  const float *k, *v;       // ready keys [rows][key heads][64] and values [rows][KV heads][64]
+  float *q;
+};
+
+// The largest magnitude's bits in a wave, in every lane.
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+  auto other = [&](auto ctrl) {
+    const uint32_t o = static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, 0xf, 0xf, false));
+    v = o > v ? o : v;
+  };
+  other(std::integral_constant<int, 0x128>());
+  other(std::integral_constant<int, 0x124>());
+  other(std::integral_constant<int, 0x122>());
+  other(std::integral_constant<int, 0x121>());
+  const auto a = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = a[0] > a[1] ? a[0] : a[1];
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return b[0] > b[1] ? b[0] : b[1];
+}
+
+// decode::norm_rope, bit for bit, without LDS: lane = element.
+__device__ __forceinline__ float norm_rotate(float x, float2 factor, int lane) {
+  const float leaf = fold_leaf_pair(x * x);
+  const float leaf0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(leaf), 0));
+  const float leaf1 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(leaf), 32));
+  const float scale = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(leaf0 + leaf1, 64.0f) + 1.1920929e-7f));
+  const float y = x * scale;
+  const float partner = rms_dpp<0xB1>(y);
+  const bool even = (lane & 1) == 0;
+  const float a = even ? y : partner, b = even ? partner : y;
+  return even ? a * factor.x - b * factor.y : a * factor.y + b * factor.x;
+}
+
+// Units of an append: the blocks of a sequence's rows, the first and the last two
+// together (they read and write the FP32 blocks), the others one by one.
+__device__ __forceinline__ int touched(int len, int n) { return (len + n - 1) / kBlock - len / kBlock + 1; }
+
+// A wave takes one unit and one head: a stored head (keys, then values), or with QKV
+// a query head. Lane = element; a block's 16 positions are 16 registers.
+template <bool QKV>
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+  const Cache &c = a.c;
+  __shared__ __attribute__((aligned(16))) int8_t turn[4][kBlockBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.y * 4 + wave, stored = c.key_heads + c.kv_heads;
+  const auto of = [](int len, int n) {
+    const int blocks = touched(len, n);
+    return blocks <= 3 ? 1 : blocks - 2;
+  };
+  Unit unit;
+  const bool found = find_unit(c, blockIdx.x, of, unit);
+  if (blockIdx.x == 0 && head == 0 && c.row_start) {
+    // Marks every refused sequence.
+    Unit none;
+    find_unit(c, 0x7fffffff, of, none);
+  }
+  if (!found || head >= stored + (QKV ? c.n_heads : 0)) return;
+  const bool is_key = head < c.key_heads, is_query = head >= stored;
+  const int qkv_width = (c.n_heads + 2 * c.kv_heads) * 64;
+  // The head's element in a row, and its pair's factors.
+  int from, pair = 0;
+  const float *source;
+  size_t width;
+  if constexpr (QKV) {
+    source = a.qkv;
+    width = qkv_width;
+    if (is_query) {
+      from = (head - stored) * 64;
+      pair = head - stored;
+    } else if (is_key) {
+      from = (c.n_heads + head * c.kv_heads / c.key_heads) * 64;
+      pair = head * (c.n_heads / c.key_heads);
+    } else {
+      from = (c.n_heads + c.kv_heads + head - c.key_heads) * 64;
+    }
+  } else {
+    source = is_key ? a.k : a.v;
+    width = static_cast<size_t>(is_key ? c.key_heads : c.kv_heads) * 64;
+    from = (is_key ? head : head - c.key_heads) * 64;
+  }
+  const int first_block = unit.len / kBlock, blocks = touched(unit.len, unit.n), last_block = first_block + blocks - 1;
+  const int held = is_key ? c.key_heads : c.kv_heads, at_head = is_key ? head : head - c.key_heads;
+  const size_t slot = (static_cast<size_t>(unit.seq) * stored + head) * 2;
+
+  auto process = [&](int block) {
+    const int row0 = block * kBlock - unit.len;  // the row of its first position
+    const bool saved = block >= last_block - 1;
+    if (is_query) {
+      float x[kBlock];
+      float2 f[kBlock];
+#pragma unroll
+      for (int t = 0; t < kBlock; t++) {
+        const int row = row0 + t, at = unit.first + (row >= 0 && row < unit.n ? row : 0);
+        x[t] = source[at * width + from + lane];
+        f[t] = reinterpret_cast<const float2 *>(a.rope)[(static_cast<size_t>(at) * c.n_heads + pair) * 32 + lane / 2];
+      }
+#pragma unroll
+      for (int t = 0; t < kBlock; t++) {
+        const int row = row0 + t;
+        if (row >= 0 && row < unit.n)
+          a.q[(static_cast<size_t>(unit.first + row) * c.n_heads + pair) * 64 + lane] = norm_rotate(x[t], f[t], lane);
+      }
+      return;
+    }
+    const long number = c.block_at(unit.seq, block, held, at_head);
+    if (number < 0) {
+      c.refused[unit.seq] = 1;
+      return;
+    }
+    float *const open = c.open + (slot + block % 2) * kBlock * 64;
+    const bool kept = row0 < 0 && c.tags[slot + block % 2] == block;
+    float *scale_at = (is_key ? c.k_scales : c.v_scales) + number;
+    // Earlier positions from the FP32 block, new ones from the rows.
+    float x[kBlock];
+    float2 f[kBlock];
+#pragma unroll
+    for (int t = 0; t < kBlock; t++) {
+      const int row = row0 + t, at = unit.first + (row >= 0 && row < unit.n ? row : 0);
+      x[t] = *(row < 0 ? open + t * 64 + lane : source + at * width + from + lane);
+      if (QKV && is_key)
+        f[t] = reinterpret_cast<const float2 *>(a.rope)[(static_cast<size_t>(at) * c.n_heads + pair) * 32 + lane / 2];
+    }
+    if (row0 < 0 && !kept) {
+      // From the codes.
+      const float scale = *scale_at;
+#pragma unroll
+      for (int t = 0; t < kBlock; t++)
+        if (row0 + t < 0) {
+          const int code = is_key ? c.k_codes[number * kBlockBytes + t * 64 + lane]
+                                  : c.v_codes[number * kBlockBytes + lane * kBlock + t] - 128;
+          x[t] = static_cast<float>(code) * scale;
+        }
+    }
+    uint32_t big = 0;
+#pragma unroll
+    for (int t = 0; t < kBlock; t++) {
+      const int row = row0 + t;
+      if (row >= unit.n) x[t] = 0.0f;
+      if (QKV && is_key && row >= 0 && row < unit.n) x[t] = norm_rotate(x[t], f[t], lane);
+      const uint32_t bits = __float_as_uint(x[t]) & 0x7fffffffu;
+      big = bits > big ? bits : big;
+    }
+    big = wave_max_bits(big);
+    float scale = __fdiv_rn(__uint_as_float(big), 127.0f);
+    if (scale < 1.17549435e-38f) scale = 0.0f;
+    const float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+    const bool finite = big < 0x7f800000u;
+    int code[kBlock];
+#pragma unroll
+    for (int t = 0; t < kBlock; t++) code[t] = finite ? static_cast<int>(__builtin_rintf(x[t] * inverse)) : 0;
+    if (is_key) {
+      // [position][64]: through LDS, 16 bytes a lane.
+#pragma unroll
+      for (int t = 0; t < kBlock; t++) turn[wave][t * 64 + lane] = static_cast<int8_t>(code[t]);
+      __builtin_amdgcn_wave_barrier();
+      const uint4 bytes = *reinterpret_cast<const uint4 *>(&turn[wave][lane * 16]);
+      __builtin_amdgcn_wave_barrier();
+      *reinterpret_cast<uint4 *>(c.k_codes + number * kBlockBytes + lane * 16) = bytes;
+    } else {
+      uint32_t word[4];
+#pragma unroll
+      for (int w = 0; w < 4; w++)
+        word[w] = static_cast<uint32_t>(code[4 * w] + 128) | static_cast<uint32_t>(code[4 * w + 1] + 128) << 8 |
+                  static_cast<uint32_t>(code[4 * w + 2] + 128) << 16 | static_cast<uint32_t>(code[4 * w + 3] + 128) << 24;
+      *reinterpret_cast<uint4 *>(c.v_codes + number * kBlockBytes + lane * kBlock) = make_uint4(word[0], word[1], word[2], word[3]);
+    }
+    if (lane == 0) *scale_at = finite ? scale : __builtin_nanf("");
+    if (saved) {
+#pragma unroll
+      for (int t = 0; t < kBlock; t++)
+        if (row0 + t < unit.n && (row0 + t >= 0 || !kept)) open[t * 64 + lane] = x[t];
+      if (lane == 0) c.tags[slot + block % 2] = block;
+    }
+  };
+  if (unit.index > 0) {
+    process(first_block + unit.index);
+    return;
+  }
+  process(first_block);
+  // The last two, which may be written where the first was read.
+  for (int block = last_block - 1 > first_block ? last_block - 1 : first_block + 1; block <= last_block; block++)
+    process(block);
+}
+
+// ---- reading back --------------------------------------------------------------
+// A wave takes one block of a sequence's rows and one stored head.
+__global__ __launch_bounds__(256) void read_kernel(Cache c, float *__restrict__ k, float *__restrict__ v) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int head = blockIdx.y * 4 + wave, stored = c.key_heads + c.kv_heads;
+  const auto of = [](int len, int n) { return touched(len, n); };
+  Unit unit;
+  const bool found = find_unit(c, blockIdx.x, of, unit);
+  if (blockIdx.x == 0 && head == 0 && c.row_start) {
+    Unit none;
+    find_unit(c, 0x7fffffff, of, none);
+  }
+  if (!found || head >= stored) return;
+  const bool is_key = head < c.key_heads;
+  const int held = is_key ? c.key_heads : c.kv_heads, at_head = is_key ? head : head - c.key_heads;
+  const int block = unit.len / kBlock + unit.index, row0 = block * kBlock - unit.len;
+  const long number = c.block_at(unit.seq, block, held, at_head);
+  if (number < 0) c.refused[unit.seq] = 1;
+  const size_t at = number < 0 ? 0 : number;
+  const float scale = number < 0 ? __builtin_nanf("") : (is_key ? c.k_scales : c.v_scales)[at];
+  if (is_key) {
+    // Lane: 16 elements of position lane / 4.
+    const uint4 bytes = *reinterpret_cast<const uint4 *>(c.k_codes + at * kBlockBytes + lane * 16);
+    const int row = row0 + lane / 4;
+    if (row < 0 || row >= unit.n) return;
+    float *to = k + (static_cast<size_t>(unit.first + row) * held + at_head) * 64 + lane % 4 * 16;
+    const uint32_t word[4] = {bytes.x, bytes.y, bytes.z, bytes.w};
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+      reinterpret_cast<float4 *>(to)[w] = make_float4(sdwa_cvt<0>(word[w]) * scale, sdwa_cvt<1>(word[w]) * scale,
+                                                      sdwa_cvt<2>(word[w]) * scale, sdwa_cvt<3>(word[w]) * scale);
+    return;
+  }
+  // Lane: element `lane` of all 16 positions.
+  const uint4 bytes = *reinterpret_cast<const uint4 *>(c.v_codes + at * kBlockBytes + lane * kBlock);
+  const uint32_t word[4] = {bytes.x, bytes.y, bytes.z, bytes.w};
+#pragma unroll
+  for (int t = 0; t < kBlock; t++) {
+    const int row = row0 + t;
+    if (row >= 0 && row < unit.n)
+      v[(static_cast<size_t>(unit.first + row) * held + at_head) * 64 + lane] =
+          static_cast<float>(static_cast<int>((word[t / 4] >> (8 * (t % 4))) & 255) - 128) * scale;
+  }
+}
+
+// ---- attention -----------------------------------------------------------------
+struct AttendArgs {
+  Cache c;
+  const float *q, *sinks;
+  float *out;
+  float *part_o, *part_md;  // [row][head][part][64], [..][2]
+  int max_len, chunk, parts, tiles, most;  // most: rows of a sequence at most
+};
+
+// A sequence's rows for attention; false where there is nothing to do (n = 0) or it
+// is refused (bad).
+__device__ __forceinline__ bool attend_span(const AttendArgs &a, int seq, int &len, int &first, int &n, bool &bad) {
+  bad = !a.c.span(seq, len, first, n);
+  if (n > 8 || (n > 0 && len + n > a.max_len)) bad = true;
+  return n > 0 && !bad;
+}
+
+// out = o / den / (1 + exp(sink - lse)), lse = (m + log2(den)) ln 2.
+__device__ __forceinline__ float sink_factor(const float *sinks, int head, float m, float den) {
+  if (!sinks) return 1.0f;
+  const float lse = (m + log2f(den)) * 0.693147180559945f;
+  return __fdiv_rn(1.0f, 1.0f + expf_acc(sinks[head] - lse));
+}
+
+// Simple form: a wave takes one query row and head and one part of its keys, lane =
+// element for the values and key for the scores.
+__global__ __launch_bounds__(64) void attend_kernel(AttendArgs a) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x, part = blockIdx.x % a.parts, r = blockIdx.x / a.parts, head = blockIdx.y, seq = blockIdx.z;
+  int len, first, n;
+  bool bad;
+  if (!attend_span(a, seq, len, first, n, bad) || r >= n) return;
+  const int group = c.n_heads / c.key_heads, key_head = head / group, value_head = head / (c.n_heads / c.kv_heads);
+  const int visible = len + r + 1, begin = part * a.chunk;
+  int end = begin + a.chunk;
+  end = end < visible ? end : visible;
+  __shared__ float s_q[64], s_p[64];
+  s_q[lane] = a.q[(static_cast<size_t>(first + r) * c.n_heads + head) * 64 + lane] * 0.180336880111120426f;  // log2(e) / 8
+  __syncthreads();
+  float m = -__builtin_inff(), den = 0.0f, o = 0.0f;
+  for (int base = begin; base < end; base += 64) {
+    const int key = base + lane;
+    float s = -__builtin_inff();
+    if (key < end) {
+      const long number = c.block_at(seq, key / kBlock, c.key_heads, key_head);
+      if (number < 0) {
+        c.refused[seq] = 1;
+        s = __builtin_nanf("");
+      } else {
+        const int8_t *codes = c.k_codes + number * kBlockBytes + key % kBlock * 64;
+        float dot = 0.0f;
+        for (int d = 0; d < 64; d++) dot = fmaf_(s_q[d], static_cast<float>(codes[d]), dot);
+        s = dot * c.k_scales[number];
+      }
+    }
+    float top = s;
+    bool nan = s != s;
+    for (int mask = 1; mask < 64; mask *= 2) top = fmaxf(top, __shfl_xor(top, mask));
+    nan = __any(nan);
+    const float next = nan ? __builtin_nanf("") : fmaxf(top, m);
+    const float p = s == -__builtin_inff() ? 0.0f : exp2f(s - next);
+    const float keep = m == -__builtin_inff() ? 0.0f : exp2f(m - next);
+    float sum = p;
+    for (int mask = 1; mask < 64; mask *= 2) sum += __shfl_xor(sum, mask);
+    den = den * keep + sum;
+    o = o * keep;
+    m = next;
+    s_p[lane] = p;
+    __syncthreads();
+    const int count = end - base < 64 ? end - base : 64;
+    for (int j = 0; j < count; j++) {
+      const long number = c.block_at(seq, (base + j) / kBlock, c.kv_heads, value_head);
+      const size_t at = number < 0 ? 0 : number;
+      const float code = static_cast<float>(static_cast<int>(c.v_codes[at * kBlockBytes + lane * kBlock + (base + j) % kBlock]) - 128);
+      o = fmaf_(s_p[j], code * c.v_scales[at], o);
+    }
+    __syncthreads();
+  }
+  const size_t at = (static_cast<size_t>(first + r) * c.n_heads + head) * a.parts + part;
+  if (begin >= visible) return;
+  a.part_o[at * 64 + lane] = o;
+  if (lane == 0) *reinterpret_cast<float2 *>(a.part_md + at * 2) = make_float2(m, den);
+}
+
+// The parts of one row and head. Workgroup (sequence, row, head): 4 waves, lane =
+// element.
+__global__ __launch_bounds__(256) void merge_kernel(AttendArgs a) {
+  const Cache &c = a.c;
+  const int head = blockIdx.x, r = blockIdx.y, seq = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ float s_m[4], s_den[4], s_o[4][64];
+  int len, first, n;
+  bool bad;
+  const bool live = attend_span(a, seq, len, first, n, bad);
+  if (bad) {
+    if (tid == 0) c.refused[seq] = 1;
+    // Its rows, where they are rows of the call.
+    const int begin = c.row_start ? c.row_start[seq] : seq, end = c.row_start ? c.row_start[seq + 1] : seq + 1;
+    if (r == 0 && begin >= 0 && end <= c.rows && tid < 64)
+      for (int row = begin; row < end; row++)
+        a.out[(static_cast<size_t>(row) * c.n_heads + head) * 64 + lane] = __builtin_nanf("");
+    return;
+  }
+  if (!live || r >= n) return;
+  const int parts = (len + r) / a.chunk + 1;
+  const size_t at = (static_cast<size_t>(first + r) * c.n_heads + head) * a.parts;
+  const float2 *md = reinterpret_cast<const float2 *>(a.part_md) + at;
+  float m = -__builtin_inff(), den = 0.0f, o = 0.0f;
+  for (int p = wave; p < parts; p += 4) {
+    const float2 v = md[p];
+    const float x = a.part_o[(at + p) * 64 + lane];
+    const float next = v.x != v.x ? v.x : fmaxf(v.x, m);
+    const float keep = m == -__builtin_inff() ? 0.0f : exp2f(m - next), gain = exp2f(v.x - next);
+    den = den * keep + v.y * gain;
+    o = o * keep + x * gain;
+    m = next;
+  }
+  if (lane == 0) {
+    s_m[wave] = m;
+    s_den[wave] = den;
+  }
+  s_o[wave][lane] = o;
+  __syncthreads();
+  if (wave > 0) return;
+  float top = s_m[0];
+  for (int w = 1; w < 4; w++) top = s_m[w] != s_m[w] || top != top ? __builtin_nanf("") : fmaxf(top, s_m[w]);
+  den = o = 0.0f;
+  for (int w = 0; w < 4; w++) {
+    const float gain = s_m[w] == -__builtin_inff() ? 0.0f : exp2f(s_m[w] - top);
+    den += s_den[w] * gain;
+    o += s_o[w][lane] * gain;
+  }
+  a.out[(static_cast<size_t>(first + r) * c.n_heads + head) * 64 + lane] = __fdiv_rn(o, den) * sink_factor(a.sinks, head, top, den);
+}
+
+// ---- pages of a sequence ---------------------------------------------------------
+constexpr int kMapped = 240;
+struct MapArgs {
+  int32_t *table, *tags;  // of the sequence
+  int first, count, shift, heads;
+  int32_t pages[kMapped];
+};
+
+// Writes table entries, and forgets the FP32 blocks that stood in those pages.
+__global__ __launch_bounds__(256) void map_kernel(MapArgs a) {
+  for (int i = threadIdx.x; i < a.count; i += 256) a.table[a.first + i] = a.pages[i];
+  for (int i = threadIdx.x; i < 2 * a.heads; i += 256) {
+    const int block = a.tags[i], at = block >> a.shift;
+    if (block >= 0 && at >= a.first && at < a.first + a.count) a.tags[i] = -1;
+  }
+}
+
+__global__ __launch_bounds__(256) void fill_kernel(int32_t *to, size_t count, int32_t value) {
+  for (size_t i = blockIdx.x * static_cast<size_t>(256) + threadIdx.x; i < count; i += static_cast<size_t>(gridDim.x) * 256)
+    to[i] = value;
+}
+
+void free_pages(Pages *kv) {
+  void *buffers[] = {kv->k_codes, kv->v_codes, kv->k_scales, kv->v_scales, kv->table, kv->open, kv->tags, kv->refused};
+  for (void *p : buffers)
+    if (p) (void)hipFree(p);
+}
+
+Cache cache_of(const Pages *kv, size_t rows, const int32_t *row_start, const int32_t *lens, size_t n_seqs) {
+  Cache c = {};
+  c.k_codes = kv->k_codes;
+  c.v_codes = kv->v_codes;
+  c.k_scales = kv->k_scales;
+  c.v_scales = kv->v_scales;
+  c.table = kv->table;
+  c.open = kv->open;
+  c.tags = kv->tags;
+  c.refused = kv->refused;
+  c.shift = kv->shift;
+  c.seq_pages = static_cast<int>(kv->seq_pages);
+  c.n_pages = static_cast<int>(kv->n_pages);
+  c.n_heads = static_cast<int>(kv->n_heads);
+  c.key_heads = static_cast<int>(kv->key_heads);
+  c.kv_heads = static_cast<int>(kv->kv_heads);
+  c.row_start = row_start;
+  c.lens = lens;
+  c.rows = static_cast<int>(rows);
+  c.n_seqs = static_cast<int>(n_seqs);
+  return c;
+}
+
+// What every call over a batch checks.
+int check_batch(const char *name, const Ctx *ctx, const Pages *kv, size_t rows, const int32_t *row_start,
+                const int32_t *lens, size_t n_seqs) {
+  const std::string at = std::string(name) + ": ";
+  FOCR_REQUIRE(ctx && kv, FOCR_E_ARG, at + "null argument");
+  FOCR_REQUIRE(kv->device == ctx->device, FOCR_E_ARG, at + "the cache is on another device than the context");
+  FOCR_REQUIRE(n_seqs <= kv->n_seqs, FOCR_E_SHAPE, at + "more sequences than the cache has");
+  FOCR_REQUIRE(rows < (size_t(1) << 24), FOCR_E_SHAPE, at + "too many rows");
+  FOCR_REQUIRE(row_start || rows == n_seqs, FOCR_E_SHAPE, at + "without row_start every sequence has one row");
+  FOCR_REQUIRE(rows == 0 || n_seqs == 0 || lens, FOCR_E_ARG, at + "null lengths");
+  return FOCR_OK;
+}
+
+int launch_append(Ctx *ctx, const AppendArgs &a, bool qkv) {
+  const Cache &c = a.c;
+  // Units: n rows touch at most (n + 14) / 16 + 1 blocks, three of which are one
+  // unit, so at most n / 16 units, or one.
+  const int units = c.row_start ? c.rows / kBlock + (c.rows < c.n_seqs ? c.rows : c.n_seqs) : c.n_seqs;
+  const int heads = c.key_heads + c.kv_heads + (qkv ? c.n_heads : 0);
+  FOCR_HIP_CHECK(hipSetDevice(ctx->device));
+  const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>((heads + 3) / 4));
+  if (qkv)
+    hipLaunchKernelGGL(append_kernel<true>, grid, dim3(256), 0, ctx->stream, a);
+  else
+    hipLaunchKernelGGL(append_kernel<false>, grid, dim3(256), 0, ctx->stream, a);
+  FOCR_HIP_CHECK(hipGetLastError());
+  return FOCR_OK;
+}
+
+}  // namespace
+}  // namespace focr
+
+using namespace focr;
+
+extern "C" {
+
+int focr_kv_pages_create(focr_ctx *handle, size_t n_pages, size_t page_size, size_t n_seqs, size_t seq_pages,
+                         size_t n_heads, size_t n_key_heads, size_t n_kv_heads, size_t head_dim, focr_kv_pages **out) {
+  Ctx *ctx = reinterpret_cast<Ctx *>(handle);
+  FOCR_REQUIRE(ctx && out, FOCR_E_ARG, "focr_kv_pages_create: null argument");
+  FOCR_REQUIRE(head_dim == 64, FOCR_E_UNSUPPORTED, "the paged cache takes head_dim 64");
+  FOCR_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && n_heads <= 1024, FOCR_E_SHAPE,
+               "focr_kv_pages_create: GQA grouping");
+  FOCR_REQUIRE(n_key_heads == n_kv_heads || n_key_heads == n_heads, FOCR_E_SHAPE,
+               "focr_kv_pages_create: keys are held for each KV head or for each query head");
+  FOCR_REQUIRE(page_size >= kBlock && page_size <= 4096 && (page_size & (page_size - 1)) == 0, FOCR_E_SHAPE,
+               "focr_kv_pages_create: page_size is a power of two from 16 to 4096");
+  FOCR_REQUIRE(n_pages > 0 && n_pages < (size_t(1) << 31) && n_seqs > 0 && n_seqs <= 65535 && seq_pages > 0 &&
+                   seq_pages * page_size < (size_t(1) << 30) && seq_pages < (size_t(1) << 30),
+               FOCR_E_SHAPE, "focr_kv_pages_create: sizes");
+  FOCR_HIP_CHECK(hipSetDevice(ctx->device));
+  Pages *kv = new (std::nothrow) Pages();
+  FOCR_REQUIRE(kv, FOCR_E_ARG, "focr_kv_pages_create: out of host memory");
+  kv->device = ctx->device;
+  kv->n_pages = n_pages;
+  kv->page = page_size;
+  kv->n_seqs = n_seqs;
+  kv->seq_pages = seq_pages;
+  kv->n_heads = n_heads;
+  kv->key_heads = n_key_heads;
+  kv->kv_heads = n_kv_heads;
+  for (size_t b = page_size / kBlock; b > 1; b /= 2) kv->shift++;
+  const size_t blocks = n_pages * (page_size / kBlock), heads = n_key_heads + n_kv_heads;
+  struct {
+    void **at;
+    size_t bytes;
+    int32_t value;
+  } buffers[] = {{reinterpret_cast<void **>(&kv->k_codes), blocks * n_key_heads * kBlockBytes, 0},
+                 {reinterpret_cast<void **>(&kv->v_codes), blocks * n_kv_heads * kBlockBytes, 0},
+                 {reinterpret_cast<void **>(&kv->k_scales), blocks * n_key_heads * sizeof(float), 0},
+                 {reinterpret_cast<void **>(&kv->v_scales), blocks * n_kv_heads * sizeof(float), 0},
+                 {reinterpret_cast<void **>(&kv->table), n_seqs * seq_pages * sizeof(int32_t), -1},
+                 {reinterpret_cast<void **>(&kv->open), n_seqs * heads * 2 * kBlock * 64 * sizeof(float), 0},
+                 {reinterpret_cast<void **>(&kv->tags), n_seqs * heads * 2 * sizeof(int32_t), -1},
+                 {reinterpret_cast<void **>(&kv->refused), n_seqs * sizeof(int32_t), 0}};
+  for (auto &b : buffers) {
+    hipError_t err = hipMalloc(b.at, b.bytes);
+    if (err == hipSuccess) {
+      kv->device_bytes += b.bytes;
+      hipLaunchKernelGGL(fill_kernel, dim3(1024), dim3(256), 0, ctx->stream, static_cast<int32_t *>(*b.at),
+                         b.bytes / sizeof(int32_t), b.value);
+      err = hipGetLastError();
+    }
+    if (err != hipSuccess) {
+      (void)hipStreamSynchronize(ctx->stream);
+      free_pages(kv);
+      delete kv;
+      return set_error(FOCR_E_HIP, std::string("focr_kv_pages_create: ") + hipGetErrorString(err));
+    }
+  }
+  // The cache may be used on another stream next.
+  const hipError_t err = hipStreamSynchronize(ctx->stream);
+  if (err != hipSuccess) {
+    free_pages(kv);
+    delete kv;
+    return set_error(FOCR_E_HIP, std::string("focr_kv_pages_create: ") + hipGetErrorString(err));
+  }
+  *out = reinterpret_cast<focr_kv_pages *>(kv);
+  return FOCR_OK;
+}
+
+int focr_kv_pages_free(focr_kv_pages *handle) {
+  Pages *kv = reinterpret_cast<Pages *>(handle);
+  if (!kv) return FOCR_OK;
+  free_pages(kv);
+  delete kv;
+  return FOCR_OK;
+}
+
+int focr_kv_pages_info(const focr_kv_pages *handle, size_t *n_pages, size_t *page_size, size_t *n_seqs,
+                       size_t *seq_pages, size_t *device_bytes) {
+  const Pages *kv = reinterpret_cast<const Pages *>(handle);
+  FOCR_REQUIRE(kv, FOCR_E_ARG, "focr_kv_pages_info: null cache");
+  if (n_pages) *n_pages = kv->n_pages;
+  if (page_size) *page_size = kv->page;
+  if (n_seqs) *n_seqs = kv->n_seqs;
+  if (seq_pages) *seq_pages = kv->seq_pages;
+  if (device_bytes) *device_bytes = kv->device_bytes;
+  return FOCR_OK;
+}
+
+int focr_kv_pages_map(focr_ctx *handle, focr_kv_pages *pages, size_t seq, size_t first, size_t count,
+                      const int32_t *ids) {
+  Ctx *ctx = reinterpret_cast<Ctx *>(handle);
+  Pages *kv = reinterpret_cast<Pages *>(pages);
+  FOCR_REQUIRE(ctx && kv, FOCR_E_ARG, "focr_kv_pages_map: null argument");
+  FOCR_REQUIRE(kv->device == ctx->device, FOCR_E_ARG, "focr_kv_pages_map: the cache is on another device than the context");
+  FOCR_REQUIRE(seq < kv->n_seqs && first <= kv->seq_pages && count <= kv->seq_pages - first, FOCR_E_SHAPE,
+               "focr_kv_pages_map: outside the sequence's pages");
+  if (count == 0) return FOCR_OK;
+  FOCR_REQUIRE(ids, FOCR_E_ARG, "focr_kv_pages_map: null pages");
+  for (size_t i = 0; i < count; i++)
+    FOCR_REQUIRE(ids[i] >= -1 && ids[i] < static_cast<int64_t>(kv->n_pages), FOCR_E_VALUE, "focr_kv_pages_map: no such page");
+  FOCR_HIP_CHECK(hipSetDevice(ctx->device));
+  const size_t heads = kv->key_heads + kv->kv_heads;
+  for (size_t at = 0; at < count; at += kMapped) {
+    MapArgs a = {};
+    a.table = kv->table + seq * kv->seq_pages;
+    a.tags = kv->tags + seq * heads * 2;
+    a.first = static_cast<int>(first + at);
+    a.count = static_cast<int>(count - at < kMapped ? count - at : kMapped);
+    a.shift = kv->shift;
+    a.heads = static_cast<int>(heads);
+    for (int i = 0; i < a.count; i++) a.pages[i] = ids[at + i];
+    hipLaunchKernelGGL(map_kernel, dim3(1), dim3(256), 0, ctx->stream, a);
+    FOCR_HIP_CHECK(hipGetLastError());
+  }
+  return FOCR_OK;
+}
+
+int focr_kv_pages_append(focr_ctx *handle, focr_kv_pages *pages, const float *k, const float *v, size_t rows,
+                         const int32_t *row_start, const int32_t *lens, size_t n_seqs) {
+  Ctx *ctx = reinterpret_cast<Ctx *>(handle);
+  Pages *kv = reinterpret_cast<Pages *>(pages);
+  const int rc = check_batch("focr_kv_pages_append", ctx, kv, rows, row_start, lens, n_seqs);
+  if (rc != FOCR_OK || rows == 0 || n_seqs == 0) return rc;
+  FOCR_REQUIRE(k && v, FOCR_E_ARG, "focr_kv_pages_append: null buffer");
+  AppendArgs a = {};
+  a.c = cache_of(kv, rows, row_start, lens, n_seqs);
+  a.k = k;
+  a.v = v;
+  return launch_append(ctx, a, false);
+}
+
+int focr_kv_pages_qkv_rows(focr_ctx *handle, focr_kv_pages *pages, const float *qkv, size_t rows, const float *rope,
+                           const int32_t *row_start, const int32_t *lens, size_t n_seqs, float *q) {
+  Ctx *ctx = reinterpret_cast<Ctx *>(handle);
+  Pages *kv = reinterpret_cast<Pages *>(pages);
+  const int rc = check_batch("focr_kv_pages_qkv_rows", ctx, kv, rows, row_start, lens, n_seqs);
+  if (rc != FOCR_OK || rows == 0 || n_seqs == 0) return rc;
+  FOCR_REQUIRE(qkv && rope && q, FOCR_E_ARG, "focr_kv_pages_qkv_rows: null buffer");
+  AppendArgs a = {};
+  a.c = cache_of(kv, rows, row_start, lens, n_seqs);
+  a.qkv = qkv;
+  a.rope = rope;
+  a.q = q;
+  return launch_append(ctx, a, true);
+}
+
+int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const float *q, size_t rows,
+                            const int32_t *row_start, const int32_t *lens, size_t n_seqs, size_t max_len,
+                            const float *sinks, float *out) {
+  Ctx *ctx = reinterpret_cast<Ctx *>(handle);
+  const Pages *kv = reinterpret_cast<const Pages *>(pages);
+  int rc = check_batch("focr_kv_pages_attention", ctx, kv, rows, row_start, lens, n_seqs);
+  if (rc != FOCR_OK || rows == 0 || n_seqs == 0) return rc;
+  FOCR_REQUIRE(q && out, FOCR_E_ARG, "focr_kv_pages_attention: null buffer");
+  FOCR_REQUIRE(max_len > 0 && max_len <= kv->seq_pages * kv->page, FOCR_E_SHAPE,
+               "focr_kv_pages_attention: max_len is 1 .. what a sequence's pages hold");
+  AttendArgs a = {};
+  a.c = cache_of(kv, rows, row_start, lens, n_seqs);
+  a.q = q;
+  a.sinks = sinks;
+  a.out = out;
+  a.max_len = static_cast<int>(max_len);
+  a.most = row_start ? static_cast<int>(rows < 8 ? rows : 8) : 1;
+  const size_t waves = n_seqs * kv->n_heads * a.most;
+  size_t chunk = (max_len * waves / 4096 + 63) / 64 * 64;
+  const size_t least = ((max_len + 255) / 256 + 63) / 64 * 64;
+  if (chunk < least) chunk = least;
+  a.chunk = static_cast<int>(chunk);
+  a.parts = static_cast<int>((max_len + chunk - 1) / chunk);
+  const size_t slots = rows * kv->n_heads * a.parts;
+  FOCR_HIP_CHECK(hipSetDevice(ctx->device));
+  rc = ensure_scratch(ctx, slots * 66 * sizeof(float));
+  if (rc != FOCR_OK) return rc;
+  a.part_o = static_cast<float *>(ctx->scratch);
+  a.part_md = a.part_o + slots * 64;
+  const unsigned heads = static_cast<unsigned>(kv->n_heads), seqs = static_cast<unsigned>(n_seqs);
+  hipLaunchKernelGGL(attend_kernel, dim3(static_cast<unsigned>(a.parts * a.most), heads, seqs), dim3(64), 0, ctx->stream, a);
+  FOCR_HIP_CHECK(hipGetLastError());
+  hipLaunchKernelGGL(merge_kernel, dim3(heads, static_cast<unsigned>(a.most), seqs), dim3(256), 0, ctx->stream, a);
+  FOCR_HIP_CHECK(hipGetLastError());
+  return FOCR_OK;
+}
+
+int focr_kv_pages_dequantize(focr_ctx *handle, const focr_kv_pages *pages, size_t rows, const int32_t *row_start,
+                             const int32_t *lens, size_t n_seqs, float *k, float *v) {
+  Ctx *ctx = reinterpret_cast<Ctx *>(handle);
+  const Pages *kv = reinterpret_cast<const Pages *>(pages);
+  const int rc = check_batch("focr_kv_pages_dequantize", ctx, kv, rows, row_start, lens, n_seqs);
+  if (rc != FOCR_OK || rows == 0 || n_seqs == 0) return rc;
+  FOCR_REQUIRE(k && v, FOCR_E_ARG, "focr_kv_pages_dequantize: null buffer");
+  const Cache c = cache_of(kv, rows, row_start, lens, n_seqs);
+  // n rows touch at most (n + 14) / 16 + 1 blocks.
+  const size_t units = row_start ? rows / kBlock + 2 * (rows < n_seqs ? rows : n_seqs) : n_seqs;
+  FOCR_HIP_CHECK(hipSetDevice(ctx->device));
+  hipLaunchKernelGGL(read_kernel, dim3(static_cast<unsigned>(units), static_cast<unsigned>((c.key_heads + c.kv_heads + 3) / 4)),
+                     dim3(256), 0, ctx->stream, c, k, v);
+  FOCR_HIP_CHECK(hipGetLastError());
+  return FOCR_OK;
+}
+
+int focr_kv_pages_refused(focr_ctx *handle, focr_kv_pages *pages, int32_t *seqs) {
+  Ctx *ctx = reinterpret_cast<Ctx *>(handle);
+  Pages *kv = reinterpret_cast<Pages *>(pages);
+  FOCR_REQUIRE(ctx && kv && seqs, FOCR_E_ARG, "focr_kv_pages_refused: null argument");
+  FOCR_REQUIRE(kv->device == ctx->device, FOCR_E_ARG, "focr_kv_pages_refused: the cache is on another device than the context");
+  FOCR_HIP_CHECK(hipSetDevice(ctx->device));
+  FOCR_HIP_CHECK(hipMemcpyAsync(seqs, kv->refused, kv->n_seqs * sizeof(int32_t), hipMemcpyDeviceToHost, ctx->stream));
+  hipLaunchKernelGGL(fill_kernel, dim3(1), dim3(256), 0, ctx->stream, kv->refused, kv->n_seqs, 0);
+  FOCR_HIP_CHECK(hipGetLastError());
+  FOCR_HIP_CHECK(hipStreamSynchronize(ctx->stream));
+  return FOCR_OK;
+}
+
+}  // extern "C"

@@ -31,6 +31,10 @@ pub struct focr_screen {
 pub struct focr_kv_split {
     _private: [u8; 0],
 }
+#[repr(C)]
+pub struct focr_kv_pages {
+    _private: [u8; 0],
+}
 
 // Status codes.
 pub const FOCR_OK: c_int = 0;
@@ -348,6 +352,81 @@ extern "C" {
         device_bytes: *mut usize,
     ) -> c_int;
     pub fn focr_kv_free(kv: *mut focr_kv_split) -> c_int;
+
+    // ---- 8-bit cache of pages for a batch of sequences -------------------------
+    pub fn focr_kv_pages_create(
+        ctx: *mut focr_ctx,
+        n_pages: usize,
+        page_size: usize,
+        n_seqs: usize,
+        seq_pages: usize,
+        n_heads: usize,
+        n_key_heads: usize,
+        n_kv_heads: usize,
+        head_dim: usize,
+        out: *mut *mut focr_kv_pages,
+    ) -> c_int;
+    pub fn focr_kv_pages_free(kv: *mut focr_kv_pages) -> c_int;
+    pub fn focr_kv_pages_info(
+        kv: *const focr_kv_pages,
+        n_pages: *mut usize,
+        page_size: *mut usize,
+        n_seqs: *mut usize,
+        seq_pages: *mut usize,
+        device_bytes: *mut usize,
+    ) -> c_int;
+    pub fn focr_kv_pages_map(
+        ctx: *mut focr_ctx,
+        kv: *mut focr_kv_pages,
+        seq: usize,
+        first: usize,
+        count: usize,
+        pages: *const i32,
+    ) -> c_int;
+    pub fn focr_kv_pages_append(
+        ctx: *mut focr_ctx,
+        kv: *mut focr_kv_pages,
+        k_dev: *const f32,
+        v_dev: *const f32,
+        rows: usize,
+        row_start_dev: *const i32,
+        lens_dev: *const i32,
+        n_seqs: usize,
+    ) -> c_int;
+    pub fn focr_kv_pages_qkv_rows(
+        ctx: *mut focr_ctx,
+        kv: *mut focr_kv_pages,
+        qkv_dev: *const f32,
+        rows: usize,
+        rope_dev: *const f32,
+        row_start_dev: *const i32,
+        lens_dev: *const i32,
+        n_seqs: usize,
+        q_dev: *mut f32,
+    ) -> c_int;
+    pub fn focr_kv_pages_attention(
+        ctx: *mut focr_ctx,
+        kv: *const focr_kv_pages,
+        q_dev: *const f32,
+        rows: usize,
+        row_start_dev: *const i32,
+        lens_dev: *const i32,
+        n_seqs: usize,
+        max_len: usize,
+        sinks_dev: *const f32,
+        out_dev: *mut f32,
+    ) -> c_int;
+    pub fn focr_kv_pages_dequantize(
+        ctx: *mut focr_ctx,
+        kv: *const focr_kv_pages,
+        rows: usize,
+        row_start_dev: *const i32,
+        lens_dev: *const i32,
+        n_seqs: usize,
+        k_dev: *mut f32,
+        v_dev: *mut f32,
+    ) -> c_int;
+    pub fn focr_kv_pages_refused(ctx: *mut focr_ctx, kv: *mut focr_kv_pages, seqs: *mut i32) -> c_int;
 
     // ---- INT8 screened vocabulary head (src/head_screen.rs)
     pub fn focr_screen_build(

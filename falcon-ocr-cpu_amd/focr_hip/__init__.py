@@ -90,6 +90,15 @@ SIGNATURES = {
     "focr_kv_decode_row": (_I, [_P, _P, _P, _P, _P, _P, _P]),
     "focr_kv_info": (_I, [_P, _P, _P, _P, _P, _P]),
     "focr_kv_free": (_I, [_P]),
+    "focr_kv_pages_create": (_I, [_P] + [_Z] * 8 + [ctypes.POINTER(_P)]),
+    "focr_kv_pages_free": (_I, [_P]),
+    "focr_kv_pages_info": (_I, [_P] * 6),
+    "focr_kv_pages_map": (_I, [_P, _P, _Z, _Z, _Z, _P]),
+    "focr_kv_pages_append": (_I, [_P, _P, _P, _P, _Z, _P, _P, _Z]),
+    "focr_kv_pages_qkv_rows": (_I, [_P, _P, _P, _Z, _P, _P, _P, _Z, _P]),
+    "focr_kv_pages_attention": (_I, [_P, _P, _P, _Z, _P, _P, _Z, _Z, _P, _P]),
+    "focr_kv_pages_dequantize": (_I, [_P, _P, _Z, _P, _P, _Z, _P, _P]),
+    "focr_kv_pages_refused": (_I, [_P, _P, _P]),
     "focr_screen_build": (_I, [_P, _P, _Z, _Z, ctypes.POINTER(_P)]),
     "focr_screen_upload": (_I, [_P, _P, _P, _Z, _Z, ctypes.c_float, ctypes.c_float, ctypes.POINTER(_P)]),
     "focr_screen_free": (_I, [_P]),
@@ -640,6 +649,121 @@ class KvSplit:
     def free(self) -> None:
         if getattr(self, "handle", None):
             _check(lib().focr_kv_free(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
+def _int32(t, count: int, what: str):
+    """Device pointer of an int32 CUDA tensor of `count` values."""
+    if t is None:
+        return None
+    if t.dtype != _torch().int32 or t.numel() != count:
+        raise FocrError(-2, f"{what}: {count} int32 values")
+    return _dev(t)
+
+
+class KvPages:
+    """An 8-bit cache of pages for a batch of sequences (no reference
+    counterpart): blocks of 16 positions and one head share a scale.
+
+    A call's batch: sequence i has the rows row_start[i] .. row_start[i + 1] - 1
+    (None: one row each), at the positions lens[i], lens[i] + 1, ... (below 0: it
+    takes no part). `lens` [n] and `row_start` [n + 1] are int32 CUDA tensors
+    that the caller advances; n is at most the cache's n_seqs. Which page holds
+    which positions is the caller's to say (`map`)."""
+
+    def __init__(self, n_pages: int, page_size: int, n_seqs: int, seq_pages: int, n_heads: int = 16,
+                 n_kv_heads: int = 8, key_heads: Optional[int] = None, ctx: Optional[Context] = None):
+        self.handle = None
+        self.ctx = ctx or default_context()
+        self.n_pages, self.page_size, self.n_seqs, self.seq_pages = n_pages, page_size, n_seqs, seq_pages
+        self.n_heads, self.n_kv_heads = n_heads, n_kv_heads
+        self.key_heads = n_kv_heads if key_heads is None else key_heads
+        handle = ctypes.c_void_p()
+        _check(lib().focr_kv_pages_create(self.ctx.handle, n_pages, page_size, n_seqs, seq_pages, n_heads,
+                                          self.key_heads, n_kv_heads, 64, ctypes.byref(handle)))
+        self.handle = handle
+
+    def map(self, seq: int, first: int, pages) -> None:
+        """Pages (numbers, -1: none) of the sequence from its page `first` on."""
+        ids = np.ascontiguousarray(pages, dtype=np.int32)
+        if ids.ndim != 1 or seq < 0 or first < 0:
+            raise FocrError(-2, "pages of a sequence: a list from page `first` on")
+        _check(lib().focr_kv_pages_map(self.ctx.handle, self.handle, seq, first, len(ids),
+                                       ids.ctypes.data_as(ctypes.c_void_p)))
+
+    def _batch(self, rows: int, lens, row_start):
+        seqs = lens.numel()
+        return _int32(row_start, seqs + 1, "row_start"), _int32(lens, seqs, "lens"), seqs
+
+    def append(self, k, v, lens, row_start=None) -> None:
+        """Keys [rows][key_heads][64] and values [rows][n_kv_heads][64] at the batch's positions."""
+        rows = v.numel() // (self.n_kv_heads * 64)
+        if k.numel() != rows * self.key_heads * 64 or v.numel() != rows * self.n_kv_heads * 64:
+            raise FocrError(-2, "keys [rows][key_heads][64] and values [rows][n_kv_heads][64]")
+        _check(lib().focr_kv_pages_append(self.ctx.handle, self.handle, _dev(k), _dev(v), rows,
+                                          *self._batch(rows, lens, row_start)))
+
+    def qkv_rows(self, qkv, rope, lens, row_start=None, q=None):
+        """`qkv_rows` with its keys and values appended: queries [rows][n_heads][64]."""
+        torch = _torch()
+        rows, width = qkv.numel() // ((self.n_heads + 2 * self.n_kv_heads) * 64), self.n_heads * 64
+        if qkv.numel() != rows * (width + 2 * self.n_kv_heads * 64) or rope.numel() != rows * width:
+            raise FocrError(-2, "QKV rows [rows][qdim + 2 kdim] and factors [rows][n_heads][32][2]")
+        if q is None:
+            q = torch.empty((rows, self.n_heads, 64), dtype=torch.float32, device=qkv.device)
+        elif q.numel() != rows * width:
+            raise FocrError(-2, "queries [rows][n_heads][64]")
+        _check(lib().focr_kv_pages_qkv_rows(self.ctx.handle, self.handle, _dev(qkv), rows, _dev(rope),
+                                            *self._batch(rows, lens, row_start), _dev(q)))
+        return q
+
+    def attention(self, q, lens, max_len: int, row_start=None, sinks=None, out=None):
+        """Attention of the batch's rows (1..8 of a sequence), appended before:
+        [rows][n_heads][64]. No sequence has more than `max_len` positions, these included."""
+        torch = _torch()
+        rows = q.numel() // (self.n_heads * 64)
+        if q.numel() != rows * self.n_heads * 64 or (sinks is not None and sinks.numel() != self.n_heads):
+            raise FocrError(-2, "queries [rows][n_heads][64] and sinks [n_heads]")
+        if max_len < 1:
+            raise FocrError(-2, "max_len is positive")
+        if out is None:
+            out = torch.empty((rows, self.n_heads, 64), dtype=torch.float32, device=q.device)
+        elif out.numel() != q.numel():
+            raise FocrError(-2, "outputs [rows][n_heads][64]")
+        _check(lib().focr_kv_pages_attention(self.ctx.handle, self.handle, _dev(q), rows,
+                                             *self._batch(rows, lens, row_start), max_len, _dev(sinks), _dev(out)))
+        return out
+
+    def dequantize(self, rows: int, lens, row_start=None):
+        """What the cache holds at the batch's positions: keys [rows][key_heads][64], values [rows][n_kv_heads][64]."""
+        torch = _torch()
+        dev = f"cuda:{self.ctx.device}"
+        k = torch.empty((rows, self.key_heads, 64), dtype=torch.float32, device=dev)
+        v = torch.empty((rows, self.n_kv_heads, 64), dtype=torch.float32, device=dev)
+        _check(lib().focr_kv_pages_dequantize(self.ctx.handle, self.handle, rows, *self._batch(rows, lens, row_start),
+                                              _dev(k), _dev(v)))
+        return k, v
+
+    def refused(self):
+        """The sequences that calls refused, wholly or in part, since this was last asked."""
+        seqs = (ctypes.c_int32 * self.n_seqs)()
+        _check(lib().focr_kv_pages_refused(self.ctx.handle, self.handle, ctypes.cast(seqs, ctypes.c_void_p)))
+        return [i for i, s in enumerate(seqs) if s]
+
+    def device_bytes(self) -> int:
+        n = ctypes.c_size_t()
+        _check(lib().focr_kv_pages_info(self.handle, None, None, None, None, ctypes.byref(n)))
+        return n.value
+
+    def free(self) -> None:
+        if getattr(self, "handle", None):
+            _check(lib().focr_kv_pages_free(self.handle))
             self.handle = None
 
     def __del__(self):

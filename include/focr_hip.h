@@ -73,6 +73,7 @@ typedef struct focr_ctx focr_ctx;
 typedef struct focr_linear focr_linear;
 typedef struct focr_screen focr_screen;
 typedef struct focr_kv_split focr_kv_split;
+typedef struct focr_kv_pages focr_kv_pages;
 
 /* ---- context ------------------------------------------------------------ */
 /* No reference counterpart (the CPU runner needs no device state); the
@@ -429,6 +430,78 @@ int focr_kv_fast_exp(const focr_kv_split *kv, int *fast);
 int focr_kv_info(const focr_kv_split *kv, int *bits, size_t *prefix_len, size_t *tail_len,
                  size_t *capacity, size_t *device_bytes);
 int focr_kv_free(focr_kv_split *kv);
+
+/* ---- 8-bit cache of pages for a batch of sequences ------------------------ */
+/* No reference counterpart (the CPU runner decodes one session): the state of
+ * up to n_seqs sequences that are decoded together, in n_pages pages of
+ * page_size positions (a power of two, 16 .. 4096). A block of 16 positions of
+ * one head holds INT8 codes and one FP32 scale: scale = fl(m / 127), m the
+ * largest magnitude of its stored positions, code = rint(fl(x * fl(1 /
+ * scale))), value fl(code * scale). A block whose scale is below 2^-126 holds
+ * zeros; one with a non-finite value decodes to NaN until that position is
+ * written again. Keys are held for each KV head (n_key_heads = n_kv_heads: the
+ * factors of query head g * (n_heads / n_kv_heads), as generated keys) or for
+ * each query head (n_key_heads = n_heads, as prefix keys). seq_pages: pages of
+ * a sequence at most. FOCR_E_UNSUPPORTED unless head_dim is 64. Synchronous.
+ *
+ * The batch of a call: sequence i (i < n_seqs) has the rows row_start_dev[i] ..
+ * row_start_dev[i + 1] - 1 of its rows (row_start_dev [n_seqs + 1], not
+ * decreasing; NULL: rows == n_seqs, one row each), which stand at positions
+ * lens_dev[i], lens_dev[i] + 1, ... (lens_dev [n_seqs]: positions before the
+ * call; below 0: the sequence takes no part). Both are device arrays that the
+ * kernels read and the caller advances, so a captured step replays with new
+ * lengths. Rows of sequences that take no part, and rows before the first or
+ * behind the last sequence, are neither read nor written. A sequence whose
+ * entries do not fit (rows out of range, positions past seq_pages pages or
+ * without a page) is refused alone: focr_kv_pages_refused names it. */
+int focr_kv_pages_create(focr_ctx *ctx, size_t n_pages, size_t page_size, size_t n_seqs, size_t seq_pages,
+                         size_t n_heads, size_t n_key_heads, size_t n_kv_heads, size_t head_dim,
+                         focr_kv_pages **out);
+int focr_kv_pages_free(focr_kv_pages *kv);
+int focr_kv_pages_info(const focr_kv_pages *kv, size_t *n_pages, size_t *page_size, size_t *n_seqs,
+                       size_t *seq_pages, size_t *device_bytes);
+/* Pages (host, -1: none) of positions [first, first + count) * page_size of a
+ * sequence, in stream order, without waiting. Which pages are free is the
+ * caller's to know. Sequences may share pages that none of them writes: full
+ * pages of a common prompt. FOCR_E_VALUE for a page the cache does not have. */
+int focr_kv_pages_map(focr_ctx *ctx, focr_kv_pages *kv, size_t seq, size_t first, size_t count,
+                      const int32_t *pages);
+/* Appends rows: keys k_dev [rows][n_key_heads][64] as they are to be attended
+ * to, values v_dev [rows][n_kv_heads][64]. Positions from lens_dev[i] on are
+ * written, and what the last touched block held behind them is gone. The
+ * values that a block held before are coded again from FP32 (the last two
+ * blocks of a sequence are kept in it), so the cache depends on the rows and
+ * not on the calls they came in, also after up to 16 positions were taken back
+ * (lens_dev lowered); further back, or in pages that the sequence was mapped
+ * and did not write, the block's codes are coded again. Positions without a
+ * page are left out. */
+int focr_kv_pages_append(focr_ctx *ctx, focr_kv_pages *kv, const float *k_dev, const float *v_dev, size_t rows,
+                         const int32_t *row_start_dev, const int32_t *lens_dev, size_t n_seqs);
+/* The row step over such a cache: focr_qkv_rows (qkv_dev [rows][qdim + 2 kdim],
+ * rope_dev [rows][n_heads][32][2], queries to q_dev [rows][n_heads][64]) with
+ * focr_kv_pages_append of its keys and values, in one launch, bitwise the two
+ * calls. */
+int focr_kv_pages_qkv_rows(focr_ctx *ctx, focr_kv_pages *kv, const float *qkv_dev, size_t rows,
+                           const float *rope_dev, const int32_t *row_start_dev, const int32_t *lens_dev,
+                           size_t n_seqs, float *q_dev);
+/* Attention of 1..8 rows of each sequence, appended before: row r of a sequence
+ * (at position lens_dev[i] + r) attends to the positions up to its own, with
+ * the per-head sink (sinks_dev [n_heads], NULL: none), scale 1/8. q_dev, out_dev
+ * [rows][n_heads][64]. max_len: no sequence has more positions, the call's rows
+ * included; the call's work is dealt out by it. A refused sequence (also one
+ * with more than 8 rows or max_len positions) gets NaN rows, as does a
+ * non-finite query. Within FP32 rounding of the decoded values' attention.
+ * Uses the context scratch. */
+int focr_kv_pages_attention(focr_ctx *ctx, const focr_kv_pages *kv, const float *q_dev, size_t rows,
+                            const int32_t *row_start_dev, const int32_t *lens_dev, size_t n_seqs, size_t max_len,
+                            const float *sinks_dev, float *out_dev);
+/* What the cache holds of the batch's rows: k_dev [rows][n_key_heads][64],
+ * v_dev [rows][n_kv_heads][64] (NaN without a page). */
+int focr_kv_pages_dequantize(focr_ctx *ctx, const focr_kv_pages *kv, size_t rows, const int32_t *row_start_dev,
+                             const int32_t *lens_dev, size_t n_seqs, float *k_dev, float *v_dev);
+/* seqs (host) [n_seqs of the cache]: 1 for each sequence that a call refused,
+ * wholly or in part, since the last time this was asked. Synchronous. */
+int focr_kv_pages_refused(focr_ctx *ctx, focr_kv_pages *kv, int32_t *seqs);
 
 /* ---- INT8 screened vocabulary head (src/head_screen.rs) ------------------ */
 /* ScreenedHead::build (src/head_screen.rs:84-118): quantizes the FP32 head
