@@ -19,6 +19,8 @@
 // on the rows appended, and not on how many at a time. Where a block is not
 // there (a sequence that goes on from pages it was given, or goes back further),
 // its earlier positions are taken from its codes.
+#include <algorithm>
+#include <new>
 #include <type_traits>
 
 #include "decode_common.hpp"
@@ -28,6 +30,12 @@ namespace focr {
 namespace {
 
 constexpr int kBlock = 16, kBlockBytes = kBlock * 64;
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 struct Pages {
   int device = 0, shift = 0;  // log2 of the blocks of a page
@@ -400,64 +408,291 @@ __device__ __forceinline__ float sink_factor(const float *sinks, int head, float
   return __fdiv_rn(1.0f, 1.0f + expf_acc(sinks[head] - lse));
 }
 
-// Simple form: a wave takes one query row and head and one part of its keys, lane =
-// element for the values and key for the scores.
-__global__ __launch_bounds__(64) void attend_kernel(AttendArgs a) {
+// The rows of a refused sequence, where they are rows of the call: NaN.
+__device__ __forceinline__ void refuse_rows(const AttendArgs &a, int seq, int head0, int heads) {
   const Cache &c = a.c;
-  const int lane = threadIdx.x, part = blockIdx.x % a.parts, r = blockIdx.x / a.parts, head = blockIdx.y, seq = blockIdx.z;
+  const int lane = threadIdx.x & 63;
+  const int begin = c.row_start ? c.row_start[seq] : seq, end = c.row_start ? c.row_start[seq + 1] : seq + 1;
+  if (lane == 0) c.refused[seq] = 1;
+  if (begin < 0 || end > c.rows) return;
+  for (int row = begin; row < end; row++)
+    for (int h = head0; h < head0 + heads; h++)
+      a.out[(static_cast<size_t>(row) * c.n_heads + h) * 64 + lane] = __builtin_nanf("");
+}
+
+// The largest (sum) of lanes l, l + 16, l + 32, l + 48, in each of them.
+__device__ __forceinline__ float across_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __builtin_fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __builtin_fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float across_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// A wave takes one sequence, one key head's queries (its query heads times the
+// sequence's rows, 16 at a time: the columns of both products) and one part of the
+// keys, 64 at a time: four blocks, block g the business of lanes 16 g .. + 15.
+//
+// Scores: the query row is written as integers i 2^(e - 22) of three signed bytes
+// (2^e above its largest element, so to 2^-22 of it), and the INT8 matrix instruction
+// forms 16 keys' exact sums with each byte from the codes as they stand. Row
+// 4 g + i of key tile t is key 16 g + 4 t + i, so that the scores of lane group g are
+// those of block g, in the order in which the second product takes its keys.
+// Values: codes become FP16 integers exactly (byte b under the exponent of 1024 is
+// 1024 + b), and a weight times its block's scale, to a common power of two, an FP16
+// pair hi + lo, together to 2^-21 of it: two FP32-accumulating products. The running
+// maximum and sum are per column; the power of two is the largest block scale's so far.
+struct Stage {
+  v4i k[4];
+  v4u v[4];
+  float k_scale, v_scale;
+};
+__global__ __launch_bounds__(256, 2) void attend_kernel(AttendArgs a) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int task = blockIdx.x * 4 + wave;
+  const int key_head = task % c.key_heads;
+  task /= c.key_heads;
+  const int tile = task % a.tiles;
+  task /= a.tiles;
+  const int part = task % a.parts, seq = task / a.parts;
+  if (seq >= c.n_seqs) return;
+  const int group = c.n_heads / c.key_heads, value_head = key_head * c.kv_heads / c.key_heads;
   int len, first, n;
   bool bad;
-  if (!attend_span(a, seq, len, first, n, bad) || r >= n) return;
-  const int group = c.n_heads / c.key_heads, key_head = head / group, value_head = head / (c.n_heads / c.kv_heads);
-  const int visible = len + r + 1, begin = part * a.chunk;
-  int end = begin + a.chunk;
-  end = end < visible ? end : visible;
-  __shared__ float s_q[64], s_p[64];
-  s_q[lane] = a.q[(static_cast<size_t>(first + r) * c.n_heads + head) * 64 + lane] * 0.180336880111120426f;  // log2(e) / 8
-  __syncthreads();
-  float m = -__builtin_inff(), den = 0.0f, o = 0.0f;
-  for (int base = begin; base < end; base += 64) {
-    const int key = base + lane;
-    float s = -__builtin_inff();
-    if (key < end) {
-      const long number = c.block_at(seq, key / kBlock, c.key_heads, key_head);
-      if (number < 0) {
-        c.refused[seq] = 1;
-        s = __builtin_nanf("");
-      } else {
-        const int8_t *codes = c.k_codes + number * kBlockBytes + key % kBlock * 64;
-        float dot = 0.0f;
-        for (int d = 0; d < 64; d++) dot = fmaf_(s_q[d], static_cast<float>(codes[d]), dot);
-        s = dot * c.k_scales[number];
+  if (!attend_span(a, seq, len, first, n, bad)) {
+    if (bad && a.parts == 1 && tile == 0) refuse_rows(a, seq, key_head * group, group);
+    return;
+  }
+  const int limit = len + n, begin = part * a.chunk;
+  if (16 * tile >= group * n || begin >= limit) return;
+  const int end = begin + a.chunk < limit ? begin + a.chunk : limit;
+
+  // Pages and blocks of 64 keys: lane's key block and value block (past the last
+  // block, that one again: masked).
+  const int last_block = (limit - 1) / kBlock, blocks_mask = (1 << c.shift) - 1;
+  const int32_t *table = c.table + static_cast<size_t>(seq) * c.seq_pages;
+  struct Pages64 {
+    int k_block, v_block, k_page, v_page;
+  };
+  auto find = [&](int key0) {
+    Pages64 p;
+    const int b = key0 / kBlock;
+    p.k_block = b + l16 / 4 < last_block ? b + l16 / 4 : last_block;
+    p.v_block = b + g < last_block ? b + g : last_block;
+    p.k_page = table[p.k_block >> c.shift];
+    p.v_page = table[p.v_block >> c.shift];
+    return p;
+  };
+  bool missing = false;
+  auto load = [&](const Pages64 &p, Stage &s) {
+    // A block without a page is NaN.
+    missing |= p.v_page < 0;
+    const long kp = p.k_page < 0 ? 0 : p.k_page, vp = p.v_page < 0 ? 0 : p.v_page;
+    const long kn = ((kp * c.key_heads + key_head) << c.shift) + (p.k_block & blocks_mask);
+    const long sn = ((vp * c.key_heads + key_head) << c.shift) + (p.v_block & blocks_mask);
+    const long vn = ((vp * c.kv_heads + value_head) << c.shift) + (p.v_block & blocks_mask);
+    const int8_t *k = c.k_codes + kn * kBlockBytes + l16 % 4 * 64 + g * 16;
+    const uint8_t *v = c.v_codes + vn * kBlockBytes + l16 * 16;
+#pragma unroll
+    for (int t = 0; t < 4; t++) s.k[t] = *reinterpret_cast<const v4i *>(k + t * 256);
+#pragma unroll
+    for (int d = 0; d < 4; d++) s.v[d] = *reinterpret_cast<const v4u *>(v + d * 256);
+    s.k_scale = c.k_scales[sn];
+    s.v_scale = c.v_scales[vn];
+    if (p.v_page < 0) s.k_scale = s.v_scale = __builtin_nanf("");
+  };
+
+  // This lane's column: query row first + r, head key_head * group + column / n.
+  int column = 16 * tile + l16;
+  const bool mine = column < group * n;
+  column = mine ? column : group * n - 1;
+  const int r = column % n, head = key_head * group + column / n;
+  const int visible = len + r + 1;
+  const size_t row = (static_cast<size_t>(first + r) * c.n_heads + head) * 64;
+  float4 qv[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) qv[i] = reinterpret_cast<const float4 *>(a.q + row + 16 * g)[i];
+
+  Pages64 next = find(begin);
+  Stage stage[2];
+  load(next, stage[0]);
+  next = find(begin + 64);
+
+  // The query as bytes: the columns of the first product.
+  v4i digit[3];
+  float q_factor;
+  {
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float x[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint32_t bits = __float_as_uint(x[j]) & 0x7fffffffu;
+        big = bits > big ? bits : big;
       }
     }
-    float top = s;
-    bool nan = s != s;
-    for (int mask = 1; mask < 64; mask *= 2) top = fmaxf(top, __shfl_xor(top, mask));
-    nan = __any(nan);
-    const float next = nan ? __builtin_nanf("") : fmaxf(top, m);
-    const float p = s == -__builtin_inff() ? 0.0f : exp2f(s - next);
-    const float keep = m == -__builtin_inff() ? 0.0f : exp2f(m - next);
-    float sum = p;
-    for (int mask = 1; mask < 64; mask *= 2) sum += __shfl_xor(sum, mask);
-    den = den * keep + sum;
-    o = o * keep;
-    m = next;
-    s_p[lane] = p;
-    __syncthreads();
-    const int count = end - base < 64 ? end - base : 64;
-    for (int j = 0; j < count; j++) {
-      const long number = c.block_at(seq, (base + j) / kBlock, c.kv_heads, value_head);
-      const size_t at = number < 0 ? 0 : number;
-      const float code = static_cast<float>(static_cast<int>(c.v_codes[at * kBlockBytes + lane * kBlock + (base + j) % kBlock]) - 128);
-      o = fmaf_(s_p[j], code * c.v_scales[at], o);
+    auto p = __builtin_amdgcn_permlane16_swap(big, big, false, false);
+    big = p[0] > p[1] ? p[0] : p[1];
+    p = __builtin_amdgcn_permlane32_swap(big, big, false, false);
+    big = p[0] > p[1] ? p[0] : p[1];
+    const bool finite = big < 0x7f800000u;
+    int e = !finite || big == 0 ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(big));
+    e = e < -96 ? -96 : e;
+    // log2(e) / 8: scores in powers of two.
+    q_factor = finite ? __builtin_ldexpf(0.180336880111120426f, e - 22) : __builtin_nanf("");
+    // 1.5 2^23 + i holds the integer i in its low bits; adding 128 to each byte of
+    // i and inverting their top bits leaves signed bytes whose weighted sum is i.
+    auto bytes = [&](float f) {
+      const float t = __builtin_ldexpf(f, 22 - e) + 12582912.0f;
+      return (__float_as_uint(t) + (0x00808080u - 0x4b400000u)) ^ 0x00808080u;
+    };
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t w0 = bytes(qv[i].x), w1 = bytes(qv[i].y), w2 = bytes(qv[i].z), w3 = bytes(qv[i].w);
+      const uint32_t a01 = __builtin_amdgcn_perm(w1, w0, 0x05010400u), a23 = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
+      const uint32_t b01 = __builtin_amdgcn_perm(w1, w0, 0x0c0c0602u), b23 = __builtin_amdgcn_perm(w3, w2, 0x0c0c0602u);
+      digit[0][i] = static_cast<int>(__builtin_amdgcn_perm(a23, a01, 0x05040100u));
+      digit[1][i] = static_cast<int>(__builtin_amdgcn_perm(a23, a01, 0x07060302u));
+      digit[2][i] = static_cast<int>(__builtin_amdgcn_perm(b23, b01, 0x05040100u));
     }
-    __syncthreads();
   }
-  const size_t at = (static_cast<size_t>(first + r) * c.n_heads + head) * a.parts + part;
-  if (begin >= visible) return;
-  a.part_o[at * 64 + lane] = o;
-  if (lane == 0) *reinterpret_cast<float2 *>(a.part_md + at * 2) = make_float2(m, den);
+
+  const float ninf = -__builtin_inff();
+  float m = ninf, den = 0.0f;
+  int power = -300;  // 2^power above every block scale of the values so far
+  v4f acc[4];
+#pragma unroll
+  for (int d = 0; d < 4; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+  auto consume = [&](const Stage &s, int key0, auto masked) {
+    constexpr bool kMasked = decltype(masked)::value;
+    float p[16];
+    const float factor = q_factor * s.k_scale;
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      const v4i zero = {0, 0, 0, 0};
+      const v4i c0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.k[t], digit[0], zero, 0, 0, 0);
+      const v4i c1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.k[t], digit[1], zero, 0, 0, 0);
+      const v4i c2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.k[t], digit[2], zero, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float sum = fmaf_(static_cast<float>(c2[i]), 65536.0f, static_cast<float>((c1[i] << 8) + c0[i]));
+        p[4 * t + i] = sum * factor;
+        if (kMasked && key0 + 16 * g + 4 * t + i >= visible) p[4 * t + i] = ninf;
+      }
+    }
+    float top = p[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) top = __builtin_fmaxf(top, p[i]);
+    top = __builtin_fmaxf(m, across_max(top));
+    const float from = top == ninf ? 0.0f : top;
+    const float widest = across_max(s.v_scale);
+    int above = widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -300;
+    above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
+    if (__any(top > m) || above > power) {
+      const float keep = __builtin_amdgcn_exp2f(m - from);
+      den = den * keep;
+      const float scaled = __builtin_ldexpf(keep, power - above);
+#pragma unroll
+      for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[d][i] = acc[d][i] * scaled;
+      m = top;
+      power = above;
+    }
+    const float weight = __builtin_ldexpf(s.v_scale, 15 - power);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      p[i] = __builtin_amdgcn_exp2f(p[i] - from);
+      sum = sum + p[i];
+      p[i] = p[i] * weight;
+      // A masked position's block may hold NaN.
+      if (kMasked && key0 + 16 * g + i >= visible) p[i] = 0.0f;
+    }
+    den = den + sum;
+#pragma unroll
+    for (int step = 0; step < 2; step++) {
+      // hi cut off, lo rounded to nearest: both conversions of hi (into the
+      // product and into lo) are this one instruction's result.
+      v8h hi, lo;
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float x = p[8 * step + j], y = p[8 * step + j + 1];
+        const v2h pair = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x, y));
+        hi[j] = pair[0];
+        hi[j + 1] = pair[1];
+        lo[j] = static_cast<_Float16>(x - static_cast<float>(pair[0]));
+        lo[j + 1] = static_cast<_Float16>(y - static_cast<float>(pair[1]));
+      }
+#pragma unroll
+      for (int d = 0; d < 4; d++) {
+        v8h v;
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          const uint32_t word = s.v[d][2 * step + w];
+          const v2h bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+          const v2h even = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, word, 0x04010400u)) - bias;
+          const v2h odd = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, word, 0x04030402u)) - bias;
+          v[4 * w] = even[0];
+          v[4 * w + 1] = even[1];
+          v[4 * w + 2] = odd[0];
+          v[4 * w + 3] = odd[1];
+        }
+        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, acc[d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, acc[d], 0, 0, 0);
+      }
+    }
+  };
+  // While one 64 keys are worked on, the next are on their way, and the pages of
+  // those after them.
+  auto turn = [&](const Stage &now, Stage &then, int key0) {
+    if (key0 + 64 < end) {
+      load(next, then);
+      next = find(key0 + 128);
+    }
+    if (key0 + 64 <= len)
+      consume(now, key0, std::false_type());
+    else
+      consume(now, key0, std::true_type());
+  };
+  for (int key0 = begin; key0 < end; key0 += 128) {
+    turn(stage[0], stage[1], key0);
+    if (key0 + 64 < end) turn(stage[1], stage[0], key0 + 64);
+  }
+
+  den = across_sum(den);
+  if (__any(missing) && lane == 0) c.refused[seq] = 1;
+  if (!mine) return;
+  const float back = __builtin_ldexpf(1.0f, power - 15);
+  if (a.parts == 1) {
+    const float factor = sink_factor(a.sinks, head, m, den);
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+      v4f o;
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] = __fdiv_rn(acc[d][i] * back, den) * factor;
+      *reinterpret_cast<v4f *>(a.out + row + 16 * d + 4 * g) = o;
+    }
+    return;
+  }
+  const size_t at = row / 64 * a.parts + part;
+#pragma unroll
+  for (int d = 0; d < 4; d++) {
+    v4f o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = acc[d][i] * back;
+    *reinterpret_cast<v4f *>(a.part_o + at * 64 + 16 * d + 4 * g) = o;
+  }
+  if (g == 0) *reinterpret_cast<float2 *>(a.part_md + at * 2) = make_float2(m, den);
 }
 
 // The parts of one row and head. Workgroup (sequence, row, head): 4 waves, lane =
@@ -470,28 +705,23 @@ __global__ __launch_bounds__(256) void merge_kernel(AttendArgs a) {
   int len, first, n;
   bool bad;
   const bool live = attend_span(a, seq, len, first, n, bad);
-  if (bad) {
-    if (tid == 0) c.refused[seq] = 1;
-    // Its rows, where they are rows of the call.
-    const int begin = c.row_start ? c.row_start[seq] : seq, end = c.row_start ? c.row_start[seq + 1] : seq + 1;
-    if (r == 0 && begin >= 0 && end <= c.rows && tid < 64)
-      for (int row = begin; row < end; row++)
-        a.out[(static_cast<size_t>(row) * c.n_heads + head) * 64 + lane] = __builtin_nanf("");
-    return;
-  }
+  if (bad && r == 0 && wave == 0) refuse_rows(a, seq, head, 1);
   if (!live || r >= n) return;
-  const int parts = (len + r) / a.chunk + 1;
+  // A part that this row does not reach, or holds only NaN, has m = -infinity: the
+  // first adds nothing, the second its NaN sum.
+  const int parts = (len + n - 1) / a.chunk + 1;
   const size_t at = (static_cast<size_t>(first + r) * c.n_heads + head) * a.parts;
   const float2 *md = reinterpret_cast<const float2 *>(a.part_md) + at;
-  float m = -__builtin_inff(), den = 0.0f, o = 0.0f;
+  const float ninf = -__builtin_inff();
+  float m = ninf, den = 0.0f, o = 0.0f;
   for (int p = wave; p < parts; p += 4) {
     const float2 v = md[p];
     const float x = a.part_o[(at + p) * 64 + lane];
-    const float next = v.x != v.x ? v.x : fmaxf(v.x, m);
-    const float keep = m == -__builtin_inff() ? 0.0f : exp2f(m - next), gain = exp2f(v.x - next);
+    const float top = __builtin_fmaxf(v.x, m), from = top == ninf ? 0.0f : top;
+    const float keep = exp2f(m - from), gain = v.x == ninf && v.y != v.y ? 1.0f : exp2f(v.x - from);
     den = den * keep + v.y * gain;
     o = o * keep + x * gain;
-    m = next;
+    m = top;
   }
   if (lane == 0) {
     s_m[wave] = m;
@@ -500,11 +730,11 @@ __global__ __launch_bounds__(256) void merge_kernel(AttendArgs a) {
   s_o[wave][lane] = o;
   __syncthreads();
   if (wave > 0) return;
-  float top = s_m[0];
-  for (int w = 1; w < 4; w++) top = s_m[w] != s_m[w] || top != top ? __builtin_nanf("") : fmaxf(top, s_m[w]);
+  const float top = __builtin_fmaxf(__builtin_fmaxf(s_m[0], s_m[1]), __builtin_fmaxf(s_m[2], s_m[3]));
+  const float from = top == ninf ? 0.0f : top;
   den = o = 0.0f;
   for (int w = 0; w < 4; w++) {
-    const float gain = s_m[w] == -__builtin_inff() ? 0.0f : exp2f(s_m[w] - top);
+    const float gain = s_m[w] == ninf && s_den[w] != s_den[w] ? 1.0f : exp2f(s_m[w] - from);
     den += s_den[w] * gain;
     o += s_o[w][lane] * gain;
   }
@@ -758,23 +988,31 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
   a.out = out;
   a.max_len = static_cast<int>(max_len);
   a.most = row_start ? static_cast<int>(rows < 8 ? rows : 8) : 1;
-  const size_t waves = n_seqs * kv->n_heads * a.most;
-  size_t chunk = (max_len * waves / 4096 + 63) / 64 * 64;
-  const size_t least = ((max_len + 255) / 256 + 63) / 64 * 64;
-  if (chunk < least) chunk = least;
-  a.chunk = static_cast<int>(chunk);
-  a.parts = static_cast<int>((max_len + chunk - 1) / chunk);
+  const size_t group = kv->n_heads / kv->key_heads;
+  a.tiles = static_cast<int>((group * a.most + 15) / 16);
+  // Parts of whole 64 keys: about 4,096 waves (16 for each compute unit) where
+  // all sequences are as long as the longest may be, and at most 256 of a sequence.
+  const size_t heads = n_seqs * kv->key_heads * a.tiles;
+  const size_t want = heads >= 4096 ? 1 : 4096 / heads;
+  const size_t chunk = std::max((max_len + want - 1) / want, (max_len + 255) / 256);
+  a.chunk = static_cast<int>((chunk + 63) / 64 * 64);
+  a.parts = static_cast<int>((max_len + a.chunk - 1) / a.chunk);
+  FOCR_REQUIRE(heads * a.parts < (size_t(1) << 32), FOCR_E_SHAPE, "focr_kv_pages_attention: too many sequences and heads");
   const size_t slots = rows * kv->n_heads * a.parts;
   FOCR_HIP_CHECK(hipSetDevice(ctx->device));
-  rc = ensure_scratch(ctx, slots * 66 * sizeof(float));
-  if (rc != FOCR_OK) return rc;
-  a.part_o = static_cast<float *>(ctx->scratch);
-  a.part_md = a.part_o + slots * 64;
-  const unsigned heads = static_cast<unsigned>(kv->n_heads), seqs = static_cast<unsigned>(n_seqs);
-  hipLaunchKernelGGL(attend_kernel, dim3(static_cast<unsigned>(a.parts * a.most), heads, seqs), dim3(64), 0, ctx->stream, a);
+  if (a.parts > 1) {
+    rc = ensure_scratch(ctx, slots * 66 * sizeof(float));
+    if (rc != FOCR_OK) return rc;
+    a.part_o = static_cast<float *>(ctx->scratch);
+    a.part_md = a.part_o + slots * 64;
+  }
+  hipLaunchKernelGGL(attend_kernel, dim3(static_cast<unsigned>((heads * a.parts + 3) / 4)), dim3(256), 0, ctx->stream, a);
   FOCR_HIP_CHECK(hipGetLastError());
-  hipLaunchKernelGGL(merge_kernel, dim3(heads, static_cast<unsigned>(a.most), seqs), dim3(256), 0, ctx->stream, a);
-  FOCR_HIP_CHECK(hipGetLastError());
+  if (a.parts > 1) {
+    hipLaunchKernelGGL(merge_kernel, dim3(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(a.most),
+                                          static_cast<unsigned>(n_seqs)), dim3(256), 0, ctx->stream, a);
+    FOCR_HIP_CHECK(hipGetLastError());
+  }
   return FOCR_OK;
 }
 
