@@ -408,6 +408,15 @@ __device__ __forceinline__ float sink_factor(const float *sinks, int head, float
   return __fdiv_rn(1.0f, 1.0f + expf_acc(sinks[head] - lse));
 }
 
+constexpr int kMaxParts = 256;
+
+// The weight of a softmax state among states whose largest maximum is `top`. A state
+// without a maximum holds no key that its row sees (weight 0), or only NaN (its sum).
+__device__ __forceinline__ float state_weight(float m, float den, float top) {
+  if (m == -__builtin_inff()) return den != den ? den : 0.0f;
+  return __builtin_amdgcn_exp2f(m - top);
+}
+
 // The rows of a refused sequence, where they are rows of the call: NaN.
 __device__ __forceinline__ void refuse_rows(const AttendArgs &a, int seq, int head0, int heads) {
   const Cache &c = a.c;
@@ -452,11 +461,14 @@ struct Stage {
   v4u v[4];
   float k_scale, v_scale;
 };
-__global__ __launch_bounds__(256, 2) void attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int task = blockIdx.x * 4 + wave;
+  // Workgroups go to the 8 XCDs in turn: those of the key heads of one value head
+  // follow one another on the same one, whose L2 then holds the values for all.
+  const int share = c.key_heads / c.kv_heads, turn_of = blockIdx.x / 8;
+  int task = (turn_of / share * 8 + blockIdx.x % 8) * share + turn_of % share;
   const int key_head = task % c.key_heads;
   task /= c.key_heads;
   const int tile = task % a.tiles;
@@ -467,12 +479,15 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(AttendArgs a) {
   int len, first, n;
   bool bad;
   if (!attend_span(a, seq, len, first, n, bad)) {
-    if (bad && a.parts == 1 && tile == 0) refuse_rows(a, seq, key_head * group, group);
+    if (bad && a.parts == 1 && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
     return;
   }
-  const int limit = len + n, begin = part * a.chunk;
-  if (16 * tile >= group * n || begin >= limit) return;
-  const int end = begin + a.chunk < limit ? begin + a.chunk : limit;
+  const int limit = len + n, from_key = part * a.chunk;
+  if (16 * tile >= group * n || from_key >= limit) return;
+  // The part's keys, in whole 64s, over the four waves.
+  const int to_key = from_key + a.chunk < limit ? from_key + a.chunk : limit;
+  const int each = (to_key - from_key + 255) / 256 * 64;
+  const int begin = from_key + wave * each, end = begin + each < to_key ? begin + each : to_key;
 
   // Pages and blocks of 64 keys: lane's key block and value block (past the last
   // block, that one again: masked).
@@ -671,74 +686,90 @@ __global__ __launch_bounds__(256, 2) void attend_kernel(AttendArgs a) {
 
   den = across_sum(den);
   if (__any(missing) && lane == 0) c.refused[seq] = 1;
-  if (!mine) return;
+  // The four waves' states meet in LDS; thread: column tid / 16, dims 4 (tid % 16) .. + 3.
+  __shared__ float s_m[4][16], s_den[4][16];
+  __shared__ __attribute__((aligned(16))) float s_o[4][16][68];
   const float back = __builtin_ldexpf(1.0f, power - 15);
-  if (a.parts == 1) {
-    const float factor = sink_factor(a.sinks, head, m, den);
-#pragma unroll
-    for (int d = 0; d < 4; d++) {
-      v4f o;
-#pragma unroll
-      for (int i = 0; i < 4; i++) o[i] = __fdiv_rn(acc[d][i] * back, den) * factor;
-      *reinterpret_cast<v4f *>(a.out + row + 16 * d + 4 * g) = o;
-    }
-    return;
-  }
-  const size_t at = row / 64 * a.parts + part;
 #pragma unroll
   for (int d = 0; d < 4; d++) {
     v4f o;
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = acc[d][i] * back;
-    *reinterpret_cast<v4f *>(a.part_o + at * 64 + 16 * d + 4 * g) = o;
+    *reinterpret_cast<v4f *>(&s_o[wave][l16][16 * d + 4 * g]) = o;
   }
-  if (g == 0) *reinterpret_cast<float2 *>(a.part_md + at * 2) = make_float2(m, den);
+  if (g == 0) {
+    s_m[wave][l16] = m;
+    s_den[wave][l16] = den;
+  }
+  __syncthreads();
+  const int col = threadIdx.x / 16, dim = threadIdx.x % 16 * 4;
+  const int out_column = 16 * tile + col;
+  if (out_column >= group * n) return;
+  const float top = __builtin_fmaxf(__builtin_fmaxf(s_m[0][col], s_m[1][col]), __builtin_fmaxf(s_m[2][col], s_m[3][col]));
+  float total = 0.0f;
+  v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    const float f = state_weight(s_m[w][col], s_den[w][col], top);
+    total = fmaf_(s_den[w][col], f, total);
+    const v4f x = *reinterpret_cast<const v4f *>(&s_o[w][col][dim]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = fmaf_(x[i], f, o[i]);
+  }
+  const int out_head = key_head * group + out_column / n;
+  const size_t out_row = static_cast<size_t>(first + out_column % n) * c.n_heads + out_head;
+  if (a.parts == 1) {
+    const float factor = sink_factor(a.sinks, out_head, top, total);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = __fdiv_rn(o[i], total) * factor;
+    *reinterpret_cast<v4f *>(a.out + out_row * 64 + dim) = o;
+    return;
+  }
+  const size_t at = out_row * a.parts + part;
+  *reinterpret_cast<v4f *>(a.part_o + at * 64 + dim) = o;
+  if (dim == 0) *reinterpret_cast<float2 *>(a.part_md + at * 2) = make_float2(top, total);
 }
 
-// The parts of one row and head. Workgroup (sequence, row, head): 4 waves, lane =
-// element.
+// The parts of one row and head. Workgroup (head, row, sequence): thread = part
+// for the weights, then 4 waves, lane = element, 8 parts of a wave in flight.
 __global__ __launch_bounds__(256) void merge_kernel(AttendArgs a) {
   const Cache &c = a.c;
   const int head = blockIdx.x, r = blockIdx.y, seq = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __shared__ float s_m[4], s_den[4], s_o[4][64];
+  __shared__ float s_f[kMaxParts], s_top[4], s_den[4], s_o[4][64];
   int len, first, n;
   bool bad;
   const bool live = attend_span(a, seq, len, first, n, bad);
   if (bad && r == 0 && wave == 0) refuse_rows(a, seq, head, 1);
   if (!live || r >= n) return;
-  // A part that this row does not reach, or holds only NaN, has m = -infinity: the
-  // first adds nothing, the second its NaN sum.
   const int parts = (len + n - 1) / a.chunk + 1;
-  const size_t at = (static_cast<size_t>(first + r) * c.n_heads + head) * a.parts;
-  const float2 *md = reinterpret_cast<const float2 *>(a.part_md) + at;
-  const float ninf = -__builtin_inff();
-  float m = ninf, den = 0.0f, o = 0.0f;
-  for (int p = wave; p < parts; p += 4) {
-    const float2 v = md[p];
-    const float x = a.part_o[(at + p) * 64 + lane];
-    const float top = __builtin_fmaxf(v.x, m), from = top == ninf ? 0.0f : top;
-    const float keep = exp2f(m - from), gain = v.x == ninf && v.y != v.y ? 1.0f : exp2f(v.x - from);
-    den = den * keep + v.y * gain;
-    o = o * keep + x * gain;
-    m = top;
-  }
-  if (lane == 0) {
-    s_m[wave] = m;
-    s_den[wave] = den;
+  const size_t row = static_cast<size_t>(first + r) * c.n_heads + head, at = row * a.parts;
+  float2 md = make_float2(-__builtin_inff(), 0.0f);
+  if (tid < parts) md = reinterpret_cast<const float2 *>(a.part_md)[at + tid];
+  float top = decode::wave_max(md.x);
+  if (lane == 0) s_top[wave] = top;
+  __syncthreads();
+  top = __builtin_fmaxf(__builtin_fmaxf(s_top[0], s_top[1]), __builtin_fmaxf(s_top[2], s_top[3]));
+  const float f = state_weight(md.x, md.y, top);
+  s_f[tid] = f;
+  const float den = decode::wave_sum(md.y * f);
+  if (lane == 0) s_den[wave] = den;
+  __syncthreads();
+  float o = 0.0f;
+  for (int p = wave; p < parts; p += 32) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = a.part_o[(at + (p + 4 * i < parts ? p + 4 * i : p)) * 64 + lane];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      if (p + 4 * i < parts) o = fmaf_(x[i], s_f[p + 4 * i], o);
   }
   s_o[wave][lane] = o;
   __syncthreads();
   if (wave > 0) return;
-  const float top = __builtin_fmaxf(__builtin_fmaxf(s_m[0], s_m[1]), __builtin_fmaxf(s_m[2], s_m[3]));
-  const float from = top == ninf ? 0.0f : top;
-  den = o = 0.0f;
-  for (int w = 0; w < 4; w++) {
-    const float gain = s_m[w] == ninf && s_den[w] != s_den[w] ? 1.0f : exp2f(s_m[w] - from);
-    den += s_den[w] * gain;
-    o += s_o[w][lane] * gain;
-  }
-  a.out[(static_cast<size_t>(first + r) * c.n_heads + head) * 64 + lane] = __fdiv_rn(o, den) * sink_factor(a.sinks, head, top, den);
+  const float total = (s_den[0] + s_den[1]) + (s_den[2] + s_den[3]);
+  o = (s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane]);
+  a.out[row * 64 + lane] = __fdiv_rn(o, total) * sink_factor(a.sinks, head, top, total);
 }
 
 // ---- pages of a sequence ---------------------------------------------------------
@@ -990,14 +1021,16 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
   a.most = row_start ? static_cast<int>(rows < 8 ? rows : 8) : 1;
   const size_t group = kv->n_heads / kv->key_heads;
   a.tiles = static_cast<int>((group * a.most + 15) / 16);
-  // Parts of whole 64 keys: about 4,096 waves (16 for each compute unit) where
-  // all sequences are as long as the longest may be, and at most 256 of a sequence.
+  // Parts of whole 256 keys: about 2,048 workgroups (8 for each compute unit) where
+  // all sequences are as long as the longest may be.
   const size_t heads = n_seqs * kv->key_heads * a.tiles;
-  const size_t want = heads >= 4096 ? 1 : 4096 / heads;
-  const size_t chunk = std::max((max_len + want - 1) / want, (max_len + 255) / 256);
-  a.chunk = static_cast<int>((chunk + 63) / 64 * 64);
+  const size_t want = heads >= 2048 ? 1 : 2048 / heads;
+  const size_t chunk = std::max((max_len + want - 1) / want, (max_len + kMaxParts - 1) / kMaxParts);
+  a.chunk = static_cast<int>((chunk + 255) / 256 * 256);
   a.parts = static_cast<int>((max_len + a.chunk - 1) / a.chunk);
-  FOCR_REQUIRE(heads * a.parts < (size_t(1) << 32), FOCR_E_SHAPE, "focr_kv_pages_attention: too many sequences and heads");
+  const size_t share = kv->key_heads / kv->kv_heads;
+  const size_t grid = (heads * a.parts + 8 * share - 1) / (8 * share) * (8 * share);
+  FOCR_REQUIRE(grid < (size_t(1) << 31), FOCR_E_SHAPE, "focr_kv_pages_attention: too many sequences and heads");
   const size_t slots = rows * kv->n_heads * a.parts;
   FOCR_HIP_CHECK(hipSetDevice(ctx->device));
   if (a.parts > 1) {
@@ -1006,7 +1039,7 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
     a.part_o = static_cast<float *>(ctx->scratch);
     a.part_md = a.part_o + slots * 64;
   }
-  hipLaunchKernelGGL(attend_kernel, dim3(static_cast<unsigned>((heads * a.parts + 3) / 4)), dim3(256), 0, ctx->stream, a);
+  hipLaunchKernelGGL(attend_kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
   FOCR_HIP_CHECK(hipGetLastError());
   if (a.parts > 1) {
     hipLaunchKernelGGL(merge_kernel, dim3(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(a.most),
