@@ -9,8 +9,9 @@
 //
 // (zeros where m / 127 is below 2^-126; NaN where a value is not finite). Pages hold
 // `page` positions, a power of two from 16 on: for each head its blocks in order.
-// Key codes stand as [position][64], signed; value codes as [dim][16 positions],
-// plus 128: both what the attention's matrix instructions take 16 bytes at a time.
+// Key codes stand as [position % 4][position / 4][64], value codes as
+// [dim][16 positions]: what the attention's matrix instructions take 16 bytes at a
+// time, in runs of 256 bytes for a load of a wave.
 //
 // A block that is not full is written again by the next append, with the scale that
 // its positions then need. So that this rounds every value once, the last two
@@ -32,16 +33,13 @@ namespace {
 constexpr int kBlock = 16, kBlockBytes = kBlock * 64;
 
 typedef int v4i __attribute__((ext_vector_type(4)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 struct Pages {
   int device = 0, shift = 0;  // log2 of the blocks of a page
   size_t n_pages = 0, page = 0, n_seqs = 0, seq_pages = 0, n_heads = 0, key_heads = 0, kv_heads = 0;
   int8_t *k_codes = nullptr;   // [page][key head][block][1 KB]
-  uint8_t *v_codes = nullptr;  // [page][KV head][block][1 KB]
+  int8_t *v_codes = nullptr;   // [page][KV head][block][1 KB]
   float *k_scales = nullptr, *v_scales = nullptr;  // [page][head][block]
   int32_t *table = nullptr;    // [sequence][seq_pages], -1: no page
   float *open = nullptr;       // [sequence][key heads, then KV heads][block % 2][16][64]
@@ -52,8 +50,7 @@ struct Pages {
 
 // What the kernels read of a cache, and a call's rows.
 struct Cache {
-  int8_t *k_codes;
-  uint8_t *v_codes;
+  int8_t *k_codes, *v_codes;
   float *k_scales, *v_scales;
   const int32_t *table;
   float *open;
@@ -149,6 +146,9 @@ __device__ __forceinline__ bool find_unit(const Cache &c, int u, const Of &of, U
   }
   return false;
 }
+
+// Where position t's key codes begin in their block.
+__device__ __forceinline__ constexpr int key_at(int t) { return t % 4 * 256 + t / 4 * 64; }
 
 // ---- append ------------------------------------------------------------------
 struct AppendArgs {
@@ -283,8 +283,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 #pragma unroll
       for (int t = 0; t < kBlock; t++)
         if (row0 + t < 0) {
-          const int code = is_key ? c.k_codes[number * kBlockBytes + t * 64 + lane]
-                                  : c.v_codes[number * kBlockBytes + lane * kBlock + t] - 128;
+          const int code = is_key ? c.k_codes[number * kBlockBytes + key_at(t) + lane]
+                                  : c.v_codes[number * kBlockBytes + lane * kBlock + t];
           x[t] = static_cast<float>(code) * scale;
         }
     }
@@ -306,9 +306,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 #pragma unroll
     for (int t = 0; t < kBlock; t++) code[t] = finite ? static_cast<int>(__builtin_rintf(x[t] * inverse)) : 0;
     if (is_key) {
-      // [position][64]: through LDS, 16 bytes a lane.
+      // Through LDS, 16 bytes a lane.
 #pragma unroll
-      for (int t = 0; t < kBlock; t++) turn[wave][t * 64 + lane] = static_cast<int8_t>(code[t]);
+      for (int t = 0; t < kBlock; t++) turn[wave][key_at(t) + lane] = static_cast<int8_t>(code[t]);
       __builtin_amdgcn_wave_barrier();
       const uint4 bytes = *reinterpret_cast<const uint4 *>(&turn[wave][lane * 16]);
       __builtin_amdgcn_wave_barrier();
@@ -317,8 +317,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       uint32_t word[4];
 #pragma unroll
       for (int w = 0; w < 4; w++)
-        word[w] = static_cast<uint32_t>(code[4 * w] + 128) | static_cast<uint32_t>(code[4 * w + 1] + 128) << 8 |
-                  static_cast<uint32_t>(code[4 * w + 2] + 128) << 16 | static_cast<uint32_t>(code[4 * w + 3] + 128) << 24;
+        word[w] = static_cast<uint32_t>(code[4 * w] & 255) | static_cast<uint32_t>(code[4 * w + 1] & 255) << 8 |
+                  static_cast<uint32_t>(code[4 * w + 2] & 255) << 16 | static_cast<uint32_t>(code[4 * w + 3]) << 24;
       *reinterpret_cast<uint4 *>(c.v_codes + number * kBlockBytes + lane * kBlock) = make_uint4(word[0], word[1], word[2], word[3]);
     }
     if (lane == 0) *scale_at = finite ? scale : __builtin_nanf("");
@@ -360,9 +360,9 @@ __global__ __launch_bounds__(256) void read_kernel(Cache c, float *__restrict__ 
   const size_t at = number < 0 ? 0 : number;
   const float scale = number < 0 ? __builtin_nanf("") : (is_key ? c.k_scales : c.v_scales)[at];
   if (is_key) {
-    // Lane: 16 elements of position lane / 4.
+    // Lane: 16 elements of position 4 (lane / 4 % 4) + lane / 16.
     const uint4 bytes = *reinterpret_cast<const uint4 *>(c.k_codes + at * kBlockBytes + lane * 16);
-    const int row = row0 + lane / 4;
+    const int row = row0 + 4 * (lane / 4 % 4) + lane / 16;
     if (row < 0 || row >= unit.n) return;
     float *to = k + (static_cast<size_t>(unit.first + row) * held + at_head) * 64 + lane % 4 * 16;
     const uint32_t word[4] = {bytes.x, bytes.y, bytes.z, bytes.w};
@@ -380,7 +380,7 @@ __global__ __launch_bounds__(256) void read_kernel(Cache c, float *__restrict__ 
     const int row = row0 + t;
     if (row >= 0 && row < unit.n)
       v[(static_cast<size_t>(unit.first + row) * held + at_head) * 64 + lane] =
-          static_cast<float>(static_cast<int>((word[t / 4] >> (8 * (t % 4))) & 255) - 128) * scale;
+          static_cast<float>(static_cast<int8_t>(word[t / 4] >> (8 * (t % 4)))) * scale;
   }
 }
 
@@ -429,38 +429,41 @@ __device__ __forceinline__ void refuse_rows(const AttendArgs &a, int seq, int he
       a.out[(static_cast<size_t>(row) * c.n_heads + h) * 64 + lane] = __builtin_nanf("");
 }
 
-// The largest (sum) of lanes l, l + 16, l + 32, l + 48, in each of them.
-__device__ __forceinline__ float across_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __builtin_fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __builtin_fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+// Largest and sum of the 16 lanes of a DPP row, in each of them.
+template <int N>
+__device__ __forceinline__ float row_ror(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, false));
 }
-__device__ __forceinline__ float across_sum(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+__device__ __forceinline__ float row_max(float v) {
+  v = __builtin_fmaxf(v, row_ror<8>(v));
+  v = __builtin_fmaxf(v, row_ror<4>(v));
+  v = __builtin_fmaxf(v, row_ror<2>(v));
+  return __builtin_fmaxf(v, row_ror<1>(v));
 }
 
-// A wave takes one sequence, one key head's queries (its query heads times the
-// sequence's rows, 16 at a time: the columns of both products) and one part of the
-// keys, 64 at a time: four blocks, block g the business of lanes 16 g .. + 15.
+// A workgroup takes one sequence, one key head's queries (its query heads times the
+// sequence's rows: columns, up to 16 of them) and one part of the keys. A wave takes
+// four columns and one run of the part's keys, 64 (four blocks) at a time: up to four
+// columns leave each wave a run of its own, up to eight two waves, more all four.
 //
-// Scores: the query row is written as integers i 2^(e - 22) of three signed bytes
-// (2^e above its largest element, so to 2^-22 of it), and the INT8 matrix instruction
-// forms 16 keys' exact sums with each byte from the codes as they stand. Row
-// 4 g + i of key tile t is key 16 g + 4 t + i, so that the scores of lane group g are
-// those of block g, in the order in which the second product takes its keys.
-// Values: codes become FP16 integers exactly (byte b under the exponent of 1024 is
-// 1024 + b), and a weight times its block's scale, to a common power of two, an FP16
-// pair hi + lo, together to 2^-21 of it: two FP32-accumulating products. The running
-// maximum and sum are per column; the power of two is the largest block scale's so far.
+// Scores. A query row is integers i 2^(e - 22) of three signed bytes (2^e above
+// its largest element, so to 2^-22 of it). Row 4 q + d of the INT8 matrix
+// product holds byte d of query q, column j of key tile t is key 4 j + t as its codes
+// stand: lane (j, q) gets the three exact sums of its four keys with its query,
+// and nothing is computed twice. Weights. exp2(s - m) times the block's value scale,
+// over the power of two above the largest such scale so far, rounded to 2^-30, as four
+// signed bytes (half a step a key: of its run's largest value, and a run is 4,096
+// keys at most, so together at most 2^-18, usually some 2^-25, of that): byte d of query q is column 4 d + q of the second product, whose
+// operands are the value codes as they stand (lane group g: block g) and these
+// bytes, turned through 1 KB of LDS. Its sums are exact integers too, and stay in
+// the accumulators while m and the power of two do; when one of them changes
+// they are added to FP32 ones, which are scaled.
 struct Stage {
-  v4i k[4];
-  v4u v[4];
+  v4i k[4], v[4];
   float k_scale, v_scale;
+  bool none;
 };
+template <bool WIDE>
 __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
@@ -484,73 +487,96 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   }
   const int limit = len + n, from_key = part * a.chunk;
   if (16 * tile >= group * n || from_key >= limit) return;
-  // The part's keys, in whole 64s, over the four waves.
+  // Waves: runs of the part's keys, in whole 64s, times quads of columns.
+  const int columns = group * n, left = columns - 16 * tile;
+  const int quads = left <= 4 ? 1 : left <= 8 ? 2 : 4, runs = 4 / quads, run = wave / quads, quad = wave % quads;
   const int to_key = from_key + a.chunk < limit ? from_key + a.chunk : limit;
-  const int each = (to_key - from_key + 255) / 256 * 64;
-  const int begin = from_key + wave * each, end = begin + each < to_key ? begin + each : to_key;
+  const int each = (to_key - from_key + 64 * runs - 1) / (64 * runs) * 64;
+  const int begin = from_key + run * each, end = begin + each < to_key ? begin + each : to_key;
+  const int column0 = 16 * tile + 4 * quad;
 
-  // Pages and blocks of 64 keys: lane's key block and value block (past the last
-  // block, that one again: masked).
+  // 64 keys: lane's key block is l16 / 4 of four, its value block g. In a page of 64
+  // positions or more (WIDE) they follow one another, and their addresses are scalar
+  // but for the lane's share; otherwise each lane looks its blocks' pages up (past the
+  // last block, that one again). A block without a page is NaN.
   const int last_block = (limit - 1) / kBlock, blocks_mask = (1 << c.shift) - 1;
   const int32_t *table = c.table + static_cast<size_t>(seq) * c.seq_pages;
-  struct Pages64 {
-    int k_block, v_block, k_page, v_page;
+  typedef __attribute__((address_space(4))) const int32_t scalar_table;  // read by scalar loads
+  bool missing = false;
+  struct Found {
+    int k_page, v_page;
   };
   auto find = [&](int key0) {
-    Pages64 p;
+    Found f;
     const int b = key0 / kBlock;
-    p.k_block = b + l16 / 4 < last_block ? b + l16 / 4 : last_block;
-    p.v_block = b + g < last_block ? b + g : last_block;
-    p.k_page = table[p.k_block >> c.shift];
-    p.v_page = table[p.v_block >> c.shift];
-    return p;
+    if constexpr (WIDE) {
+      const int at = b < last_block ? b : last_block;
+      f.k_page = f.v_page = reinterpret_cast<scalar_table *>(reinterpret_cast<uintptr_t>(table))[at >> c.shift];
+    } else {
+      f.k_page = table[(b + l16 / 4 < last_block ? b + l16 / 4 : last_block) >> c.shift];
+      f.v_page = table[(b + g < last_block ? b + g : last_block) >> c.shift];
+    }
+    return f;
   };
-  bool missing = false;
-  auto load = [&](const Pages64 &p, Stage &s) {
-    // A block without a page is NaN.
-    missing |= p.v_page < 0;
-    const long kp = p.k_page < 0 ? 0 : p.k_page, vp = p.v_page < 0 ? 0 : p.v_page;
-    const long kn = ((kp * c.key_heads + key_head) << c.shift) + (p.k_block & blocks_mask);
-    const long sn = ((vp * c.key_heads + key_head) << c.shift) + (p.v_block & blocks_mask);
-    const long vn = ((vp * c.kv_heads + value_head) << c.shift) + (p.v_block & blocks_mask);
-    const int8_t *k = c.k_codes + kn * kBlockBytes + l16 % 4 * 64 + g * 16;
-    const uint8_t *v = c.v_codes + vn * kBlockBytes + l16 * 16;
+  const int k_lane = l16 % 4 * 64 + g * 16, v_lane = l16 * 16;
+  auto load = [&](const Found &f, int key0, Stage &s) {
+    const int b = key0 / kBlock;
+    const bool none = f.k_page < 0;
+    missing |= none;
+    const long kp = none ? 0 : f.k_page, vp = f.v_page < 0 ? 0 : f.v_page;
+    if constexpr (WIDE) {
+      const long kn = ((kp * c.key_heads + key_head) << c.shift) + (b & blocks_mask);
+      const long vn = ((kp * c.kv_heads + value_head) << c.shift) + (b & blocks_mask);
+      const int8_t *k = c.k_codes + kn * kBlockBytes, *v = c.v_codes + vn * kBlockBytes;
+      s.k_scale = (c.k_scales + kn)[l16 / 4];
+      s.v_scale = (c.v_scales + vn)[l16 / 4];
+      s.none = none;
 #pragma unroll
-    for (int t = 0; t < 4; t++) s.k[t] = *reinterpret_cast<const v4i *>(k + t * 256);
+      for (int t = 0; t < 4; t++) s.k[t] = *reinterpret_cast<const v4i *>(k + t * 256 + (l16 / 4 * kBlockBytes + k_lane));
 #pragma unroll
-    for (int d = 0; d < 4; d++) s.v[d] = *reinterpret_cast<const v4u *>(v + d * 256);
-    s.k_scale = c.k_scales[sn];
-    s.v_scale = c.v_scales[vn];
-    if (p.v_page < 0) s.k_scale = s.v_scale = __builtin_nanf("");
+      for (int d = 0; d < 4; d++) s.v[d] = *reinterpret_cast<const v4i *>(v + d * 256 + (g * kBlockBytes + v_lane));
+    } else {
+      const int k_in = (b + l16 / 4 < last_block ? b + l16 / 4 : last_block) & blocks_mask;
+      const int v_in = (b + g < last_block ? b + g : last_block) & blocks_mask;
+      const long kn = ((kp * c.key_heads + key_head) << c.shift) + k_in;
+      const long sn = ((kp * c.kv_heads + value_head) << c.shift) + k_in;
+      const long vn = ((vp * c.kv_heads + value_head) << c.shift) + v_in;
+      s.k_scale = c.k_scales[kn];
+      s.v_scale = c.v_scales[sn];
+      s.none = none;
+      const int8_t *k = c.k_codes + kn * kBlockBytes + k_lane, *v = c.v_codes + vn * kBlockBytes + v_lane;
+#pragma unroll
+      for (int t = 0; t < 4; t++) s.k[t] = *reinterpret_cast<const v4i *>(k + t * 256);
+#pragma unroll
+      for (int d = 0; d < 4; d++) s.v[d] = *reinterpret_cast<const v4i *>(v + d * 256);
+    }
   };
-
-  // This lane's column: query row first + r, head key_head * group + column / n.
-  int column = 16 * tile + l16;
-  const bool mine = column < group * n;
-  column = mine ? column : group * n - 1;
-  const int r = column % n, head = key_head * group + column / n;
-  const int visible = len + r + 1;
-  const size_t row = (static_cast<size_t>(first + r) * c.n_heads + head) * 64;
-  float4 qv[4];
-#pragma unroll
-  for (int i = 0; i < 4; i++) qv[i] = reinterpret_cast<const float4 *>(a.q + row + 16 * g)[i];
-
-  Pages64 next = find(begin);
+  Found next;
   Stage stage[2];
-  load(next, stage[0]);
-  next = find(begin + 64);
+  const bool works = begin < end && column0 < columns;
+  if (works) next = find(begin);
 
-  // The query as bytes: the columns of the first product.
-  v4i digit[3];
+  // Column column0 + q: query row first + column % n, head key_head * group +
+  // column / n. Lane l16 brings row l16 of the first product (query l16 / 4, byte
+  // l16 % 4), lane (l16, g) works on query g.
+  v4i digit;
   float q_factor;
-  {
+  int visible;
+  if (works) {
+    float4 x[4];
+    const int wanted = column0 + l16 / 4, column = wanted < columns ? wanted : columns - 1;
+    const float *q = a.q + (static_cast<size_t>(first + column % n) * c.n_heads + key_head * group + column / n) * 64 + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = reinterpret_cast<const float4 *>(q)[i];
+    load(next, begin, stage[0]);
+    next = find(begin + 64);
     uint32_t big = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const float x[4] = {qv[i].x, qv[i].y, qv[i].z, qv[i].w};
+      const float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const uint32_t bits = __float_as_uint(x[j]) & 0x7fffffffu;
+        const uint32_t bits = __float_as_uint(y[j]) & 0x7fffffffu;
         big = bits > big ? bits : big;
       }
     }
@@ -561,158 +587,179 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     const bool finite = big < 0x7f800000u;
     int e = !finite || big == 0 ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(big));
     e = e < -96 ? -96 : e;
-    // log2(e) / 8: scores in powers of two.
-    q_factor = finite ? __builtin_ldexpf(0.180336880111120426f, e - 22) : __builtin_nanf("");
+    // log2(e) / 8: scores in powers of two. From query l16 / 4 to query g.
+    const float factor = finite ? __builtin_ldexpf(0.180336880111120426f, e - 22) : __builtin_nanf("");
+    q_factor = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (4 * g), __float_as_int(factor)));
     // 1.5 2^23 + i holds the integer i in its low bits; adding 128 to each byte of
     // i and inverting their top bits leaves signed bytes whose weighted sum is i.
     auto bytes = [&](float f) {
       const float t = __builtin_ldexpf(f, 22 - e) + 12582912.0f;
       return (__float_as_uint(t) + (0x00808080u - 0x4b400000u)) ^ 0x00808080u;
     };
+    // Byte l16 % 4 of four values; the fourth is none.
+    const uint32_t pick = l16 % 4 == 3 ? 0x0c0c0c0cu : 0x0c0c0400u + 0x0101u * (l16 % 4);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const uint32_t w0 = bytes(qv[i].x), w1 = bytes(qv[i].y), w2 = bytes(qv[i].z), w3 = bytes(qv[i].w);
-      const uint32_t a01 = __builtin_amdgcn_perm(w1, w0, 0x05010400u), a23 = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
-      const uint32_t b01 = __builtin_amdgcn_perm(w1, w0, 0x0c0c0602u), b23 = __builtin_amdgcn_perm(w3, w2, 0x0c0c0602u);
-      digit[0][i] = static_cast<int>(__builtin_amdgcn_perm(a23, a01, 0x05040100u));
-      digit[1][i] = static_cast<int>(__builtin_amdgcn_perm(a23, a01, 0x07060302u));
-      digit[2][i] = static_cast<int>(__builtin_amdgcn_perm(b23, b01, 0x05040100u));
+      const uint32_t lo = __builtin_amdgcn_perm(bytes(x[i].y), bytes(x[i].x), pick);
+      const uint32_t hi = __builtin_amdgcn_perm(bytes(x[i].w), bytes(x[i].z), pick);
+      digit[i] = static_cast<int>(lo | hi << 16);
     }
+    const int mine = column0 + g;
+    visible = len + (mine < columns ? mine : columns - 1) % n + 1;
   }
 
   const float ninf = -__builtin_inff();
   float m = ninf, den = 0.0f;
   int power = -300;  // 2^power above every block scale of the values so far
+  v4i sums[4];
   v4f acc[4];
 #pragma unroll
-  for (int d = 0; d < 4; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int d = 0; d < 4; d++) {
+    sums[d] = v4i{0, 0, 0, 0};
+    acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  // The bytes of the weights: [column 4 d + q][64 keys], a wave's own.
+  __shared__ __attribute__((aligned(16))) char turned[4][16 * 64];
+  char *const turn_to = turned[wave] + g * 64 + 4 * l16;
+  const char *const turn_from = turned[wave] + l16 * 64 + 16 * g;
 
-  auto consume = [&](const Stage &s, int key0, auto masked) {
-    constexpr bool kMasked = decltype(masked)::value;
-    float p[16];
-    const float factor = q_factor * s.k_scale;
+  // The integer sums to the FP32 ones, times `scaled` of query g: column 4 d + q's
+  // lanes take that of query q.
+  auto flush = [&](float scaled) {
+    const float s0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 0));
+    const float s1 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 16));
+    const float s2 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 32));
+    const float s3 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 48));
+    const float f = l16 & 2 ? (l16 & 1 ? s3 : s2) : (l16 & 1 ? s1 : s0);
+#pragma unroll
+    for (int d = 0; d < 4; d++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        acc[d][i] = (acc[d][i] + static_cast<float>(sums[d][i])) * f;
+        sums[d][i] = 0;
+      }
+  };
+
+  auto consume = [&](const Stage &s, int key0, bool overflow) {
+    // Blocks that hold none of the sequence's positions do not count; NaN reaches a
+    // row by its scores, as integers have none for the weights.
+    const float v_scale = key0 / kBlock + l16 / 4 <= last_block ? s.v_scale : 0.0f;
+    const float k_scale = s.none || v_scale != v_scale ? __builtin_nanf("") : s.k_scale;
+    // The largest value scale of the four blocks (lanes 4 b .. + 3 of a row).
+    float widest = __builtin_fmaxf(v_scale, row_ror<4>(v_scale));
+    widest = __builtin_fmaxf(widest, row_ror<8>(widest));
+    int above = widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -300;
+    above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
+    const int lower = power - above;
+    power = above;
+    const float weight = __builtin_ldexpf(v_scale, 30 - power);
+    float p[4];
+    const float factor = q_factor * k_scale;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       const v4i zero = {0, 0, 0, 0};
-      const v4i c0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.k[t], digit[0], zero, 0, 0, 0);
-      const v4i c1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.k[t], digit[1], zero, 0, 0, 0);
-      const v4i c2 = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.k[t], digit[2], zero, 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float sum = fmaf_(static_cast<float>(c2[i]), 65536.0f, static_cast<float>((c1[i] << 8) + c0[i]));
-        p[4 * t + i] = sum * factor;
-        if (kMasked && key0 + 16 * g + 4 * t + i >= visible) p[4 * t + i] = ninf;
-      }
+      const v4i dots = __builtin_amdgcn_mfma_i32_16x16x64_i8(digit, s.k[t], zero, 0, 0, 0);
+      const float sum = fmaf_(static_cast<float>(dots[2]), 65536.0f, static_cast<float>((dots[1] << 8) + dots[0]));
+      p[t] = sum * factor;
+      if (key0 + 4 * l16 + t >= visible) p[t] = ninf;
     }
-    float top = p[0];
-#pragma unroll
-    for (int i = 1; i < 16; i++) top = __builtin_fmaxf(top, p[i]);
-    top = __builtin_fmaxf(m, across_max(top));
+    float top = __builtin_fmaxf(__builtin_fmaxf(p[0], p[1]), __builtin_fmaxf(p[2], p[3]));
+    top = __builtin_fmaxf(m, row_max(top));
     const float from = top == ninf ? 0.0f : top;
-    const float widest = across_max(s.v_scale);
-    int above = widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -300;
-    above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
-    if (__any(top > m) || above > power) {
+    if (__any(top > m) || lower < 0 || overflow) {
       const float keep = __builtin_amdgcn_exp2f(m - from);
       den = den * keep;
-      const float scaled = __builtin_ldexpf(keep, power - above);
-#pragma unroll
-      for (int d = 0; d < 4; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[d][i] = acc[d][i] * scaled;
+      flush(__builtin_ldexpf(keep, lower));
       m = top;
-      power = above;
     }
-    const float weight = __builtin_ldexpf(s.v_scale, 15 - power);
-    float sum = 0.0f;
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      p[i] = __builtin_amdgcn_exp2f(p[i] - from);
-      sum = sum + p[i];
-      p[i] = p[i] * weight;
-      // A masked position's block may hold NaN.
-      if (kMasked && key0 + 16 * g + i >= visible) p[i] = 0.0f;
+    for (int t = 0; t < 4; t++) {
+      const float e = __builtin_amdgcn_exp2f(p[t] - from);
+      den = den + e;
+      w[t] = (static_cast<uint32_t>(static_cast<int>(fmaf_(e, weight, 0.5f))) + 0x80808080u) ^ 0x80808080u;
     }
-    den = den + sum;
+    // Bytes of four values to values of four bytes.
+    const uint32_t a01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), a23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+    const uint32_t b01 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), b23 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    asm volatile("" ::: "memory");
+    *reinterpret_cast<uint32_t *>(turn_to) = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+    *reinterpret_cast<uint32_t *>(turn_to + 4 * 64) = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
+    *reinterpret_cast<uint32_t *>(turn_to + 8 * 64) = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
+    *reinterpret_cast<uint32_t *>(turn_to + 12 * 64) = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const v4i weights = *reinterpret_cast<const v4i *>(turn_from);
+    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int step = 0; step < 2; step++) {
-      // hi cut off, lo rounded to nearest: both conversions of hi (into the
-      // product and into lo) are this one instruction's result.
-      v8h hi, lo;
-#pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float x = p[8 * step + j], y = p[8 * step + j + 1];
-        const v2h pair = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x, y));
-        hi[j] = pair[0];
-        hi[j + 1] = pair[1];
-        lo[j] = static_cast<_Float16>(x - static_cast<float>(pair[0]));
-        lo[j + 1] = static_cast<_Float16>(y - static_cast<float>(pair[1]));
-      }
-#pragma unroll
-      for (int d = 0; d < 4; d++) {
-        v8h v;
-#pragma unroll
-        for (int w = 0; w < 2; w++) {
-          const uint32_t word = s.v[d][2 * step + w];
-          const v2h bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
-          const v2h even = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, word, 0x04010400u)) - bias;
-          const v2h odd = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, word, 0x04030402u)) - bias;
-          v[4 * w] = even[0];
-          v[4 * w + 1] = even[1];
-          v[4 * w + 2] = odd[0];
-          v[4 * w + 3] = odd[1];
-        }
-        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, acc[d], 0, 0, 0);
-        acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, acc[d], 0, 0, 0);
-      }
-    }
+    for (int d = 0; d < 4; d++) sums[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.v[d], weights, sums[d], 0, 0, 0);
   };
-  // While one 64 keys are worked on, the next are on their way, and the pages of
-  // those after them.
-  auto turn = [&](const Stage &now, Stage &then, int key0) {
+  // While one 64 keys are worked on, the next are on their way, and before them the
+  // pages of those after: no load is under a branch, so the waits count what is
+  // still out. A sum grows by at most 2^20 with 64 keys: it is flushed every 1,024
+  // times.
+  auto turn = [&](const Stage &now, Stage &then, int key0, auto more) {
+    if constexpr (decltype(more)::value) {
+      const Found after = find(key0 + 128);
+      load(next, key0 + 64, then);
+      next = after;
+    }
+    consume(now, key0, ((key0 - begin) & 0xffff) == 0xffc0);
+  };
+  if (works) {
+    const std::true_type more;
+    const std::false_type no_more;
+    int key0 = begin;
+    for (; key0 + 128 < end; key0 += 128) {
+      turn(stage[0], stage[1], key0, more);
+      turn(stage[1], stage[0], key0 + 64, more);
+    }
     if (key0 + 64 < end) {
-      load(next, then);
-      next = find(key0 + 128);
+      turn(stage[0], stage[1], key0, more);
+      turn(stage[1], stage[0], key0 + 64, no_more);
+    } else {
+      turn(stage[0], stage[1], key0, no_more);
     }
-    if (key0 + 64 <= len)
-      consume(now, key0, std::false_type());
-    else
-      consume(now, key0, std::true_type());
-  };
-  for (int key0 = begin; key0 < end; key0 += 128) {
-    turn(stage[0], stage[1], key0);
-    if (key0 + 64 < end) turn(stage[1], stage[0], key0 + 64);
   }
-
-  den = across_sum(den);
   if (__any(missing) && lane == 0) c.refused[seq] = 1;
-  // The four waves' states meet in LDS; thread: column tid / 16, dims 4 (tid % 16) .. + 3.
-  __shared__ float s_m[4][16], s_den[4][16];
-  __shared__ __attribute__((aligned(16))) float s_o[4][16][68];
-  const float back = __builtin_ldexpf(1.0f, power - 15);
+
+  // The waves' states meet in LDS: [run][column], 16 in all.
+  __shared__ float s_m[16], s_den[16];
+  __shared__ __attribute__((aligned(16))) float s_o[16][68];
+  const float back = __builtin_ldexpf(1.0f, power - 30);
+  flush(1.0f);
+  den = den + row_ror<8>(den);
+  den = den + row_ror<4>(den);
+  den = den + row_ror<2>(den);
+  den = den + row_ror<1>(den);
+  if (l16 == 0) {
+    s_m[4 * wave + g] = m;
+    s_den[4 * wave + g] = den;
+  }
 #pragma unroll
   for (int d = 0; d < 4; d++) {
     v4f o;
 #pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = acc[d][i] * back;
-    *reinterpret_cast<v4f *>(&s_o[wave][l16][16 * d + 4 * g]) = o;
-  }
-  if (g == 0) {
-    s_m[wave][l16] = m;
-    s_den[wave][l16] = den;
+    for (int i = 0; i < 4; i++) {
+      // Lane l16 < 4: byte sums of lanes l16, + 4, + 8, + 12.
+      const float x = acc[d][i];
+      const float sum = fmaf_(row_ror<4>(x), 16777216.0f, fmaf_(row_ror<8>(x), 65536.0f, fmaf_(row_ror<12>(x), 256.0f, x)));
+      o[i] = sum * back;
+    }
+    if (l16 < 4) *reinterpret_cast<v4f *>(&s_o[4 * wave + l16][16 * d + 4 * g]) = o;
   }
   __syncthreads();
-  const int col = threadIdx.x / 16, dim = threadIdx.x % 16 * 4;
+  // Thread: a column and four dims.
+  const int col = threadIdx.x / 16, dim = threadIdx.x % 16 * 4, wide = 4 * quads;
   const int out_column = 16 * tile + col;
-  if (out_column >= group * n) return;
-  const float top = __builtin_fmaxf(__builtin_fmaxf(s_m[0][col], s_m[1][col]), __builtin_fmaxf(s_m[2][col], s_m[3][col]));
-  float total = 0.0f;
+  if (col >= wide || out_column >= columns) return;
+  float top = s_m[col], total = 0.0f;
+  for (int w = 1; w < runs; w++) top = __builtin_fmaxf(top, s_m[w * wide + col]);
   v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int w = 0; w < 4; w++) {
-    const float f = state_weight(s_m[w][col], s_den[w][col], top);
-    total = fmaf_(s_den[w][col], f, total);
-    const v4f x = *reinterpret_cast<const v4f *>(&s_o[w][col][dim]);
+  for (int w = 0; w < runs; w++) {
+    const int at = w * wide + col;
+    const float f = state_weight(s_m[at], s_den[at], top);
+    total = fmaf_(s_den[at], f, total);
+    const v4f x = *reinterpret_cast<const v4f *>(&s_o[at][dim]);
 #pragma unroll
     for (int i = 0; i < 4; i++) o[i] = fmaf_(x[i], f, o[i]);
   }
@@ -730,45 +777,66 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   if (dim == 0) *reinterpret_cast<float2 *>(a.part_md + at * 2) = make_float2(top, total);
 }
 
-// The parts of one row and head. Workgroup (head, row, sequence): thread = part
-// for the weights, then 4 waves, lane = element, 8 parts of a wave in flight.
-__global__ __launch_bounds__(256) void merge_kernel(AttendArgs a) {
+// The parts of a sequence's rows of one head: 8 waves, as many for each row as there
+// are, lane = element, eight parts of a wave in flight.
+__global__ __launch_bounds__(512) void merge_kernel(AttendArgs a) {
   const Cache &c = a.c;
-  const int head = blockIdx.x, r = blockIdx.y, seq = blockIdx.z;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __shared__ float s_f[kMaxParts], s_top[4], s_den[4], s_o[4][64];
+  constexpr int WAVES = 8, BATCH = 8;
+  const int head = blockIdx.x, seq = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ float s_m[WAVES], s_den[WAVES], s_o[WAVES][64];
   int len, first, n;
   bool bad;
   const bool live = attend_span(a, seq, len, first, n, bad);
-  if (bad && r == 0 && wave == 0) refuse_rows(a, seq, head, 1);
-  if (!live || r >= n) return;
+  if (bad && wave == 0) refuse_rows(a, seq, head, 1);
+  if (!live) return;
+  const int waves = n == 1 ? 8 : n == 2 ? 4 : n <= 4 ? 2 : 1, r = wave / waves, own = wave % waves;
   const int parts = (len + n - 1) / a.chunk + 1;
-  const size_t row = static_cast<size_t>(first + r) * c.n_heads + head, at = row * a.parts;
-  float2 md = make_float2(-__builtin_inff(), 0.0f);
-  if (tid < parts) md = reinterpret_cast<const float2 *>(a.part_md)[at + tid];
-  float top = decode::wave_max(md.x);
-  if (lane == 0) s_top[wave] = top;
-  __syncthreads();
-  top = __builtin_fmaxf(__builtin_fmaxf(s_top[0], s_top[1]), __builtin_fmaxf(s_top[2], s_top[3]));
-  const float f = state_weight(md.x, md.y, top);
-  s_f[tid] = f;
-  const float den = decode::wave_sum(md.y * f);
-  if (lane == 0) s_den[wave] = den;
-  __syncthreads();
-  float o = 0.0f;
-  for (int p = wave; p < parts; p += 32) {
-    float x[8];
+  const size_t row = static_cast<size_t>(first + (r < n ? r : 0)) * c.n_heads + head, at = row * a.parts;
+  const float2 *md = reinterpret_cast<const float2 *>(a.part_md) + at;
+  const float *part_o = a.part_o + at * 64 + lane;
+  float m = -__builtin_inff(), den = 0.0f, o = 0.0f;
+  if (r < n)
+    for (int p = own; p < parts; p += waves * BATCH) {
+      float2 v[BATCH];
+      float x[BATCH];
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = a.part_o[(at + (p + 4 * i < parts ? p + 4 * i : p)) * 64 + lane];
+      for (int i = 0; i < BATCH; i++) {
+        const int q = p + waves * i;
+        v[i] = md[q < parts ? q : p];
+        x[i] = part_o[static_cast<size_t>(q < parts ? q : p) * 64];
+      }
+      float top = m;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (p + 4 * i < parts) o = fmaf_(x[i], s_f[p + 4 * i], o);
+      for (int i = 0; i < BATCH; i++) top = __builtin_fmaxf(top, v[i].x);
+      const float keep = state_weight(m, den, top);
+      den = den * keep;
+      o = o * keep;
+#pragma unroll
+      for (int i = 0; i < BATCH; i++)
+        if (p + waves * i < parts) {
+          const float f = state_weight(v[i].x, v[i].y, top);
+          den = fmaf_(v[i].y, f, den);
+          o = fmaf_(x[i], f, o);
+        }
+      m = top;
+    }
+  if (lane == 0) {
+    s_m[wave] = m;
+    s_den[wave] = den;
   }
   s_o[wave][lane] = o;
   __syncthreads();
-  if (wave > 0) return;
-  const float total = (s_den[0] + s_den[1]) + (s_den[2] + s_den[3]);
-  o = (s_o[0][lane] + s_o[1][lane]) + (s_o[2][lane] + s_o[3][lane]);
+  if (own > 0 || r >= n) return;
+  float top = m;
+  for (int w = 1; w < waves; w++) top = __builtin_fmaxf(top, s_m[wave + w]);
+  float total = 0.0f;
+  o = 0.0f;
+  for (int w = 0; w < waves; w++) {
+    const float f = state_weight(s_m[wave + w], s_den[wave + w], top);
+    total = fmaf_(s_den[wave + w], f, total);
+    o = fmaf_(s_o[wave + w][lane], f, o);
+  }
   a.out[row * 64 + lane] = __fdiv_rn(o, total) * sink_factor(a.sinks, head, top, total);
 }
 
@@ -1022,10 +1090,11 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
   const size_t group = kv->n_heads / kv->key_heads;
   a.tiles = static_cast<int>((group * a.most + 15) / 16);
   // Parts of whole 256 keys: about 2,048 workgroups (8 for each compute unit) where
-  // all sequences are as long as the longest may be.
+  // all sequences are as long as the longest may be, and at most 4,096 keys (the
+  // longest run) up to a million positions.
   const size_t heads = n_seqs * kv->key_heads * a.tiles;
   const size_t want = heads >= 2048 ? 1 : 2048 / heads;
-  const size_t chunk = std::max((max_len + want - 1) / want, (max_len + kMaxParts - 1) / kMaxParts);
+  const size_t chunk = std::max(std::min<size_t>((max_len + want - 1) / want, 4096), (max_len + kMaxParts - 1) / kMaxParts);
   a.chunk = static_cast<int>((chunk + 255) / 256 * 256);
   a.parts = static_cast<int>((max_len + a.chunk - 1) / a.chunk);
   const size_t share = kv->key_heads / kv->kv_heads;
@@ -1039,11 +1108,14 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
     a.part_o = static_cast<float *>(ctx->scratch);
     a.part_md = a.part_o + slots * 64;
   }
-  hipLaunchKernelGGL(attend_kernel, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
+  if (kv->page >= 64)
+    hipLaunchKernelGGL(attend_kernel<true>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
+  else
+    hipLaunchKernelGGL(attend_kernel<false>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
   FOCR_HIP_CHECK(hipGetLastError());
   if (a.parts > 1) {
-    hipLaunchKernelGGL(merge_kernel, dim3(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(a.most),
-                                          static_cast<unsigned>(n_seqs)), dim3(256), 0, ctx->stream, a);
+    hipLaunchKernelGGL(merge_kernel, dim3(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(n_seqs)), dim3(512), 0,
+                       ctx->stream, a);
     FOCR_HIP_CHECK(hipGetLastError());
   }
   return FOCR_OK;

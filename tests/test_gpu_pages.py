@@ -192,9 +192,11 @@ def attention64(q, k, v, first, sinks):
     key, and a few roundings of itself and of its exponent; a weight by the
     exponential of twice that (its own and the maximum's). A weighted value passes up
     to 32 roundings in its matrix product, one for each 32 keys and each 64 keys of
-    its part, and some 80 where parts meet. It enters its product as an FP16 pair
-    whose low half ends at 2^-24, in units of 2^-15 of a power of two that is at most
-    twice the largest block scale: 2^-38 of the largest value, for each key."""
+    its part, and some 80 where parts meet. It enters its product as an integer of
+    2^-30 of a power of two that is at most twice the largest block scale of its
+    run: off by half of that, 2^-30 of the largest value, for each key of a run (4,096
+    at most), relative to the run's largest weight, which is part of its sum: so over
+    all runs 2^-30 of the largest value for each key of the longest."""
     n, heads, _ = q.shape
     out, bound = np.empty(q.shape), np.empty(q.shape)
     q, k, v = (x.astype(np.float64) for x in (q, k, v))
@@ -209,7 +211,7 @@ def attention64(q, k, v, first, sinks):
             out[r, h] = w @ vh[:seen] / total * sink
             off = 4 * EPS * np.abs(q[r, h]).max() * np.abs(kh[:seen]).sum(axis=1).max() / 8 + EPS * (8 * np.abs(s).max() + 16)
             size = w @ np.abs(vh[:seen]) / total * sink
-            least = seen * 2.0 ** -38 * np.abs(vh[:seen]).max() / total * sink
+            least = min(seen, 4096) * 2.0 ** -30 * np.abs(vh[:seen]).max() * sink
             bound[r, h] = size * (2.2 * off + EPS * (seen / 20 + 112)) + least + 1e-40
     return out, bound
 
