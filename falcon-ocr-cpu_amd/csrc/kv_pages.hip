@@ -777,11 +777,12 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   if (dim == 0) *reinterpret_cast<float2 *>(a.part_md + at * 2) = make_float2(top, total);
 }
 
-// The parts of a sequence's rows of one head: 8 waves, as many for each row as there
-// are, lane = element, eight parts of a wave in flight.
-__global__ __launch_bounds__(512) void merge_kernel(AttendArgs a) {
+// The parts of a sequence's rows of one head: as many of the waves for each row as
+// there are, lane = element, eight parts of a wave in flight.
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttendArgs a) {
   const Cache &c = a.c;
-  constexpr int WAVES = 8, BATCH = 8;
+  constexpr int BATCH = 8;
   const int head = blockIdx.x, seq = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   __shared__ float s_m[WAVES], s_den[WAVES], s_o[WAVES][64];
@@ -790,54 +791,60 @@ __global__ __launch_bounds__(512) void merge_kernel(AttendArgs a) {
   const bool live = attend_span(a, seq, len, first, n, bad);
   if (bad && wave == 0) refuse_rows(a, seq, head, 1);
   if (!live) return;
-  const int waves = n == 1 ? 8 : n == 2 ? 4 : n <= 4 ? 2 : 1, r = wave / waves, own = wave % waves;
+  const int spread = n == 1 ? 1 : n == 2 ? 2 : n <= 4 ? 4 : 8;
+  const int waves = spread < WAVES ? WAVES / spread : 1, own = wave % waves;
   const int parts = (len + n - 1) / a.chunk + 1;
-  const size_t row = static_cast<size_t>(first + (r < n ? r : 0)) * c.n_heads + head, at = row * a.parts;
-  const float2 *md = reinterpret_cast<const float2 *>(a.part_md) + at;
-  const float *part_o = a.part_o + at * 64 + lane;
-  float m = -__builtin_inff(), den = 0.0f, o = 0.0f;
-  if (r < n)
-    for (int p = own; p < parts; p += waves * BATCH) {
-      float2 v[BATCH];
-      float x[BATCH];
+  for (int r0 = 0; r0 < n; r0 += WAVES / waves) {
+    const int r = r0 + wave / waves;
+    const size_t row = static_cast<size_t>(first + (r < n ? r : 0)) * c.n_heads + head, at = row * a.parts;
+    const float2 *md = reinterpret_cast<const float2 *>(a.part_md) + at;
+    const float *part_o = a.part_o + at * 64 + lane;
+    float m = -__builtin_inff(), den = 0.0f, o = 0.0f;
+    if (r < n)
+      for (int p = own; p < parts; p += waves * BATCH) {
+        float2 v[BATCH];
+        float x[BATCH];
 #pragma unroll
-      for (int i = 0; i < BATCH; i++) {
-        const int q = p + waves * i;
-        v[i] = md[q < parts ? q : p];
-        x[i] = part_o[static_cast<size_t>(q < parts ? q : p) * 64];
-      }
-      float top = m;
-#pragma unroll
-      for (int i = 0; i < BATCH; i++) top = __builtin_fmaxf(top, v[i].x);
-      const float keep = state_weight(m, den, top);
-      den = den * keep;
-      o = o * keep;
-#pragma unroll
-      for (int i = 0; i < BATCH; i++)
-        if (p + waves * i < parts) {
-          const float f = state_weight(v[i].x, v[i].y, top);
-          den = fmaf_(v[i].y, f, den);
-          o = fmaf_(x[i], f, o);
+        for (int i = 0; i < BATCH; i++) {
+          const int q = p + waves * i;
+          v[i] = md[q < parts ? q : p];
+          x[i] = part_o[static_cast<size_t>(q < parts ? q : p) * 64];
         }
-      m = top;
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) top = __builtin_fmaxf(top, v[i].x);
+        const float keep = state_weight(m, den, top);
+        den = den * keep;
+        o = o * keep;
+#pragma unroll
+        for (int i = 0; i < BATCH; i++)
+          if (p + waves * i < parts) {
+            const float f = state_weight(v[i].x, v[i].y, top);
+            den = fmaf_(v[i].y, f, den);
+            o = fmaf_(x[i], f, o);
+          }
+        m = top;
+      }
+    if (lane == 0) {
+      s_m[wave] = m;
+      s_den[wave] = den;
     }
-  if (lane == 0) {
-    s_m[wave] = m;
-    s_den[wave] = den;
+    s_o[wave][lane] = o;
+    __syncthreads();
+    if (own == 0 && r < n) {
+      float top = m;
+      for (int w = 1; w < waves; w++) top = __builtin_fmaxf(top, s_m[wave + w]);
+      float total = 0.0f;
+      o = 0.0f;
+      for (int w = 0; w < waves; w++) {
+        const float f = state_weight(s_m[wave + w], s_den[wave + w], top);
+        total = fmaf_(s_den[wave + w], f, total);
+        o = fmaf_(s_o[wave + w][lane], f, o);
+      }
+      a.out[row * 64 + lane] = __fdiv_rn(o, total) * sink_factor(a.sinks, head, top, total);
+    }
+    __syncthreads();
   }
-  s_o[wave][lane] = o;
-  __syncthreads();
-  if (own > 0 || r >= n) return;
-  float top = m;
-  for (int w = 1; w < waves; w++) top = __builtin_fmaxf(top, s_m[wave + w]);
-  float total = 0.0f;
-  o = 0.0f;
-  for (int w = 0; w < waves; w++) {
-    const float f = state_weight(s_m[wave + w], s_den[wave + w], top);
-    total = fmaf_(s_den[wave + w], f, total);
-    o = fmaf_(s_o[wave + w][lane], f, o);
-  }
-  a.out[row * 64 + lane] = __fdiv_rn(o, total) * sink_factor(a.sinks, head, top, total);
 }
 
 // ---- pages of a sequence ---------------------------------------------------------
@@ -1089,11 +1096,15 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
   a.most = row_start ? static_cast<int>(rows < 8 ? rows : 8) : 1;
   const size_t group = kv->n_heads / kv->key_heads;
   a.tiles = static_cast<int>((group * a.most + 15) / 16);
-  // Parts of whole 256 keys: about 2,048 workgroups (8 for each compute unit) where
-  // all sequences are as long as the longest may be, and at most 4,096 keys (the
-  // longest run) up to a million positions.
+  // Parts of whole 256 keys, at most 4,096 (the longest run) up to a million
+  // positions. Few sequences need only fill the chip (us a call with 512 / 1,024 /
+  // 2,048 workgroups: one of 131,072 positions 33.1 / 36.2 / 37.3, four of up to
+  // 16,000 16.8 / 16.7 / 19.2); more, of different lengths, want parts to spare
+  // (20 of up to 9,000 49.4 / 44.9 / 45.0, 40 of up to 5,000 with up to 8 rows 88.9 /
+  // 59.7 / 54.0).
   const size_t heads = n_seqs * kv->key_heads * a.tiles;
-  const size_t want = heads >= 2048 ? 1 : 2048 / heads;
+  const size_t enough = n_seqs <= 2 ? 512 : n_seqs <= 8 ? 1024 : 2048;
+  const size_t want = heads >= enough ? 1 : enough / heads;
   const size_t chunk = std::max(std::min<size_t>((max_len + want - 1) / want, 4096), (max_len + kMaxParts - 1) / kMaxParts);
   a.chunk = static_cast<int>((chunk + 255) / 256 * 256);
   a.parts = static_cast<int>((max_len + a.chunk - 1) / a.chunk);
@@ -1114,8 +1125,11 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
     hipLaunchKernelGGL(attend_kernel<false>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
   FOCR_HIP_CHECK(hipGetLastError());
   if (a.parts > 1) {
-    hipLaunchKernelGGL(merge_kernel, dim3(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(n_seqs)), dim3(512), 0,
-                       ctx->stream, a);
+    const dim3 each(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(n_seqs));
+    if (a.parts <= 16)
+      hipLaunchKernelGGL(merge_kernel<4>, each, dim3(256), 0, ctx->stream, a);
+    else
+      hipLaunchKernelGGL(merge_kernel<16>, each, dim3(1024), 0, ctx->stream, a);
     FOCR_HIP_CHECK(hipGetLastError());
   }
   return FOCR_OK;
