@@ -147,9 +147,6 @@ __device__ __forceinline__ bool find_unit(const Cache &c, int u, const Of &of, U
   return false;
 }
 
-// Where position t's key codes begin in their block.
-__device__ __forceinline__ constexpr int key_at(int t) { return t % 4 * 256 + t / 4 * 64; }
-
 // ---- append ------------------------------------------------------------------
 struct AppendArgs {
   Cache c;
@@ -175,30 +172,75 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
   return b[0] > b[1] ? b[0] : b[1];
 }
 
-// decode::norm_rope, bit for bit, without LDS: lane = element.
-__device__ __forceinline__ float norm_rotate(float x, float2 factor, int lane) {
-  const float leaf = fold_leaf_pair(x * x);
-  const float leaf0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(leaf), 0));
-  const float leaf1 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(leaf), 32));
-  const float scale = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(leaf0 + leaf1, 64.0f) + 1.1920929e-7f));
-  const float y = x * scale;
-  const float partner = rms_dpp<0xB1>(y);
-  const bool even = (lane & 1) == 0;
-  const float a = even ? y : partner, b = even ? partner : y;
-  return even ? a * factor.x - b * factor.y : a * factor.y + b * factor.x;
+// The value N lanes up in the 16 lanes of a DPP row (cyclically), and lane N's.
+template <int N>
+__device__ __forceinline__ float row_up(float v) {
+  return rms_dpp<0x120 + 16 - N>(v);
+}
+template <int N>
+__device__ __forceinline__ float row_lane(float v) {
+  return rms_dpp<0x150 + N>(v);
+}
+
+// decode::norm_rope, bit for bit, of four times four rows: lane (r, c) of the wave
+// holds elements 4 c .. + 3 of row 4 r + s in x[s]. The pairwise sum of squares folds
+// lanes 4, 2 and 1 apart (elements 16, 8 and 4), then the lane's own (2 and 1), of both
+// halves of 32; the four sums of a row's 16 lanes meet in four of them, so that the
+// divisions and the root are done once for all 16 rows. A rotated pair is the lane's own.
+__device__ __forceinline__ void norm_rotate(v4f (&x)[4], const v4f (&f)[4]) {
+  float sums = 0.0f;
+  const int l16 = threadIdx.x & 15;
+  auto total = [&](const v4f &v) {
+    float p[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = v[i] * v[i];
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = p[i] + row_up<4>(p[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = p[i] + row_up<2>(p[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = p[i] + row_up<1>(p[i]);
+    const float leaf = (p[0] + p[2]) + (p[1] + p[3]);
+    return row_lane<0>(leaf) + row_lane<8>(leaf);
+  };
+#pragma unroll
+  for (int s = 0; s < 4; s++) {
+    const float t = total(x[s]);
+    sums = l16 == s ? t : sums;
+  }
+  const float scales = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(sums, 64.0f) + 1.1920929e-7f));
+  const float scale[4] = {row_lane<0>(scales), row_lane<1>(scales), row_lane<2>(scales), row_lane<3>(scales)};
+#pragma unroll
+  for (int s = 0; s < 4; s++) {
+    const v4f y = {x[s][0] * scale[s], x[s][1] * scale[s], x[s][2] * scale[s], x[s][3] * scale[s]};
+    x[s] = v4f{y[0] * f[s][0] - y[1] * f[s][1], y[0] * f[s][1] + y[1] * f[s][0], y[2] * f[s][2] - y[3] * f[s][3],
+               y[2] * f[s][3] + y[3] * f[s][2]};
+  }
 }
 
 // Units of an append: the blocks of a sequence's rows, the first and the last two
 // together (they read and write the FP32 blocks), the others one by one.
 __device__ __forceinline__ int touched(int len, int n) { return (len + n - 1) / kBlock - len / kBlock + 1; }
 
+// Four bytes of four words to four words of four bytes.
+__device__ __forceinline__ void turn_bytes(uint32_t (&w)[4]) {
+  const uint32_t a01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), a23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t b01 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), b23 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
+}
+
 // A wave takes one unit and one head: a stored head (keys, then values), or with QKV
-// a query head. Lane = element; a block's 16 positions are 16 registers.
+// a query head. Lane (r, c): elements 4 c .. + 3 of the block's positions 4 r + s, s =
+// 0 .. 3, so that a load or store of FP32 rows is 1 KB, key codes go to memory as
+// they stand (256 bytes for each s) and a dim's codes of four positions are one word.
 template <bool QKV>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const Cache &c = a.c;
-  __shared__ __attribute__((aligned(16))) int8_t turn[4][kBlockBytes];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r4 = lane / 16 * 4, e4 = lane % 16 * 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = blockIdx.y * 4 + wave, stored = c.key_heads + c.kv_heads;
   const auto of = [](int len, int n) {
     const int blocks = touched(len, n);
@@ -213,119 +255,121 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   }
   if (!found || head >= stored + (QKV ? c.n_heads : 0)) return;
   const bool is_key = head < c.key_heads, is_query = head >= stored;
-  const int qkv_width = (c.n_heads + 2 * c.kv_heads) * 64;
-  // The head's element in a row, and its pair's factors.
-  int from, pair = 0;
+  // Where the head stands in a row, and whose factors its pairs take.
   const float *source;
   size_t width;
+  int pair = 0;
   if constexpr (QKV) {
-    source = a.qkv;
-    width = qkv_width;
+    width = static_cast<size_t>(c.n_heads + 2 * c.kv_heads) * 64;
+    int from;
     if (is_query) {
-      from = (head - stored) * 64;
-      pair = head - stored;
+      from = pair = head - stored;
     } else if (is_key) {
-      from = (c.n_heads + head * c.kv_heads / c.key_heads) * 64;
+      from = c.n_heads + head * c.kv_heads / c.key_heads;
       pair = head * (c.n_heads / c.key_heads);
     } else {
-      from = (c.n_heads + c.kv_heads + head - c.key_heads) * 64;
+      from = c.n_heads + c.kv_heads + head - c.key_heads;
     }
+    source = a.qkv + from * 64;
   } else {
-    source = is_key ? a.k : a.v;
     width = static_cast<size_t>(is_key ? c.key_heads : c.kv_heads) * 64;
-    from = (is_key ? head : head - c.key_heads) * 64;
+    source = (is_key ? a.k : a.v) + (is_key ? head : head - c.key_heads) * 64;
   }
+  const bool turned = QKV && (is_key || is_query);
   const int first_block = unit.len / kBlock, blocks = touched(unit.len, unit.n), last_block = first_block + blocks - 1;
   const int held = is_key ? c.key_heads : c.kv_heads, at_head = is_key ? head : head - c.key_heads;
   const size_t slot = (static_cast<size_t>(unit.seq) * stored + head) * 2;
 
   auto process = [&](int block) {
     const int row0 = block * kBlock - unit.len;  // the row of its first position
-    const bool saved = block >= last_block - 1;
-    if (is_query) {
-      float x[kBlock];
-      float2 f[kBlock];
+    float *const open = is_query ? nullptr : c.open + (slot + block % 2) * kBlock * 64;
+    const bool earlier = !is_query && row0 < 0;
+    // Earlier positions from the FP32 block, new ones from the rows.
+    v4f x[4], f[4];
 #pragma unroll
-      for (int t = 0; t < kBlock; t++) {
-        const int row = row0 + t, at = unit.first + (row >= 0 && row < unit.n ? row : 0);
-        x[t] = source[at * width + from + lane];
-        f[t] = reinterpret_cast<const float2 *>(a.rope)[(static_cast<size_t>(at) * c.n_heads + pair) * 32 + lane / 2];
+    for (int s = 0; s < 4; s++) {
+      const int row = row0 + r4 + s;
+      const size_t at = unit.first + (row < 0 ? 0 : row < unit.n ? row : unit.n - 1);
+      const float *from = earlier && row < 0 ? open + (r4 + s) * 64 : source + at * width;
+      x[s] = *reinterpret_cast<const v4f *>(from + e4);
+      if (turned) f[s] = *reinterpret_cast<const v4f *>(a.rope + (at * c.n_heads + pair) * 64 + e4);
+    }
+    if (turned) {
+      v4f y[4] = {x[0], x[1], x[2], x[3]};
+      norm_rotate(y, f);
+      if (is_query) {
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+          const int row = row0 + r4 + s;
+          if (row >= 0 && row < unit.n)
+            *reinterpret_cast<v4f *>(a.q + (static_cast<size_t>(unit.first + row) * c.n_heads + pair) * 64 + e4) = y[s];
+        }
+        return;
       }
 #pragma unroll
-      for (int t = 0; t < kBlock; t++) {
-        const int row = row0 + t;
-        if (row >= 0 && row < unit.n)
-          a.q[(static_cast<size_t>(unit.first + row) * c.n_heads + pair) * 64 + lane] = norm_rotate(x[t], f[t], lane);
-      }
-      return;
+      for (int s = 0; s < 4; s++)
+        if (row0 + r4 + s >= 0) x[s] = y[s];
     }
     const long number = c.block_at(unit.seq, block, held, at_head);
     if (number < 0) {
       c.refused[unit.seq] = 1;
       return;
     }
-    float *const open = c.open + (slot + block % 2) * kBlock * 64;
-    const bool kept = row0 < 0 && c.tags[slot + block % 2] == block;
-    float *scale_at = (is_key ? c.k_scales : c.v_scales) + number;
-    // Earlier positions from the FP32 block, new ones from the rows.
-    float x[kBlock];
-    float2 f[kBlock];
-#pragma unroll
-    for (int t = 0; t < kBlock; t++) {
-      const int row = row0 + t, at = unit.first + (row >= 0 && row < unit.n ? row : 0);
-      x[t] = *(row < 0 ? open + t * 64 + lane : source + at * width + from + lane);
-      if (QKV && is_key)
-        f[t] = reinterpret_cast<const float2 *>(a.rope)[(static_cast<size_t>(at) * c.n_heads + pair) * 32 + lane / 2];
-    }
-    if (row0 < 0 && !kept) {
+    int8_t *const codes = (is_key ? c.k_codes : c.v_codes) + number * kBlockBytes;
+    float *const scale_at = (is_key ? c.k_scales : c.v_scales) + number;
+    const bool kept = earlier && c.tags[slot + block % 2] == block;
+    if (earlier && !kept) {
       // From the codes.
       const float scale = *scale_at;
+      uint32_t w[4];
 #pragma unroll
-      for (int t = 0; t < kBlock; t++)
-        if (row0 + t < 0) {
-          const int code = is_key ? c.k_codes[number * kBlockBytes + key_at(t) + lane]
-                                  : c.v_codes[number * kBlockBytes + lane * kBlock + t];
-          x[t] = static_cast<float>(code) * scale;
-        }
+      for (int s = 0; s < 4; s++)
+        w[s] = *reinterpret_cast<const uint32_t *>(is_key ? codes + s * 256 + lane * 4 : codes + (e4 + s) * kBlock + r4);
+      if (!is_key) turn_bytes(w);
+#pragma unroll
+      for (int s = 0; s < 4; s++)
+        if (row0 + r4 + s < 0)
+          x[s] = v4f{sdwa_cvt<0>(w[s]) * scale, sdwa_cvt<1>(w[s]) * scale, sdwa_cvt<2>(w[s]) * scale, sdwa_cvt<3>(w[s]) * scale};
     }
     uint32_t big = 0;
 #pragma unroll
-    for (int t = 0; t < kBlock; t++) {
-      const int row = row0 + t;
-      if (row >= unit.n) x[t] = 0.0f;
-      if (QKV && is_key && row >= 0 && row < unit.n) x[t] = norm_rotate(x[t], f[t], lane);
-      const uint32_t bits = __float_as_uint(x[t]) & 0x7fffffffu;
-      big = bits > big ? bits : big;
+    for (int s = 0; s < 4; s++) {
+      if (row0 + r4 + s >= unit.n) x[s] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint32_t bits = __float_as_uint(x[s][i]) & 0x7fffffffu;
+        big = bits > big ? bits : big;
+      }
     }
     big = wave_max_bits(big);
     float scale = __fdiv_rn(__uint_as_float(big), 127.0f);
     if (scale < 1.17549435e-38f) scale = 0.0f;
-    const float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
-    const bool finite = big < 0x7f800000u;
-    int code[kBlock];
-#pragma unroll
-    for (int t = 0; t < kBlock; t++) code[t] = finite ? static_cast<int>(__builtin_rintf(x[t] * inverse)) : 0;
-    if (is_key) {
-      // Through LDS, 16 bytes a lane.
-#pragma unroll
-      for (int t = 0; t < kBlock; t++) turn[wave][key_at(t) + lane] = static_cast<int8_t>(code[t]);
-      __builtin_amdgcn_wave_barrier();
-      const uint4 bytes = *reinterpret_cast<const uint4 *>(&turn[wave][lane * 16]);
-      __builtin_amdgcn_wave_barrier();
-      *reinterpret_cast<uint4 *>(c.k_codes + number * kBlockBytes + lane * 16) = bytes;
-    } else {
-      uint32_t word[4];
-#pragma unroll
-      for (int w = 0; w < 4; w++)
-        word[w] = static_cast<uint32_t>(code[4 * w] & 255) | static_cast<uint32_t>(code[4 * w + 1] & 255) << 8 |
-                  static_cast<uint32_t>(code[4 * w + 2] & 255) << 16 | static_cast<uint32_t>(code[4 * w + 3]) << 24;
-      *reinterpret_cast<uint4 *>(c.v_codes + number * kBlockBytes + lane * kBlock) = make_uint4(word[0], word[1], word[2], word[3]);
+    float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+    if (big >= 0x7f800000u) {
+      scale = __builtin_nanf("");
+      inverse = 0.0f;
     }
-    if (lane == 0) *scale_at = finite ? scale : __builtin_nanf("");
-    if (saved) {
+    uint32_t w[4];
 #pragma unroll
-      for (int t = 0; t < kBlock; t++)
-        if (row0 + t < unit.n && (row0 + t >= 0 || !kept)) open[t * 64 + lane] = x[t];
+    for (int s = 0; s < 4; s++) {
+      // 1.5 2^23 + code, rounded to nearest even, holds the code in its low byte.
+      uint32_t bits[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) bits[i] = __float_as_uint(x[s][i] * inverse + 12582912.0f);
+      const uint32_t lo = __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400u);
+      w[s] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[3], bits[2], 0x0c0c0400u), lo, 0x05040100u);
+    }
+    if (!is_key) turn_bytes(w);
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+      *reinterpret_cast<uint32_t *>(is_key ? codes + s * 256 + lane * 4 : codes + (e4 + s) * kBlock + r4) = w[s];
+    if (lane == 0) *scale_at = scale;
+    if (block >= last_block - 1) {
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        const int row = row0 + r4 + s;
+        if (row < unit.n && (row >= 0 || !kept)) *reinterpret_cast<v4f *>(open + (r4 + s) * 64 + e4) = x[s];
+      }
       if (lane == 0) c.tags[slot + block % 2] = block;
     }
   };
@@ -359,28 +403,21 @@ __global__ __launch_bounds__(256) void read_kernel(Cache c, float *__restrict__ 
   if (number < 0) c.refused[unit.seq] = 1;
   const size_t at = number < 0 ? 0 : number;
   const float scale = number < 0 ? __builtin_nanf("") : (is_key ? c.k_scales : c.v_scales)[at];
-  if (is_key) {
-    // Lane: 16 elements of position 4 (lane / 4 % 4) + lane / 16.
-    const uint4 bytes = *reinterpret_cast<const uint4 *>(c.k_codes + at * kBlockBytes + lane * 16);
-    const int row = row0 + 4 * (lane / 4 % 4) + lane / 16;
-    if (row < 0 || row >= unit.n) return;
-    float *to = k + (static_cast<size_t>(unit.first + row) * held + at_head) * 64 + lane % 4 * 16;
-    const uint32_t word[4] = {bytes.x, bytes.y, bytes.z, bytes.w};
+  // Lane (r, c): elements 4 c .. + 3 of positions 4 r + s, as they were appended.
+  const int r4 = lane / 16 * 4, e4 = lane % 16 * 4;
+  const int8_t *const codes = (is_key ? c.k_codes : c.v_codes) + at * kBlockBytes;
+  float *const to = (is_key ? k : v) + at_head * 64 + e4;
+  uint32_t w[4];
 #pragma unroll
-    for (int w = 0; w < 4; w++)
-      reinterpret_cast<float4 *>(to)[w] = make_float4(sdwa_cvt<0>(word[w]) * scale, sdwa_cvt<1>(word[w]) * scale,
-                                                      sdwa_cvt<2>(word[w]) * scale, sdwa_cvt<3>(word[w]) * scale);
-    return;
-  }
-  // Lane: element `lane` of all 16 positions.
-  const uint4 bytes = *reinterpret_cast<const uint4 *>(c.v_codes + at * kBlockBytes + lane * kBlock);
-  const uint32_t word[4] = {bytes.x, bytes.y, bytes.z, bytes.w};
+  for (int s = 0; s < 4; s++)
+    w[s] = *reinterpret_cast<const uint32_t *>(is_key ? codes + s * 256 + lane * 4 : codes + (e4 + s) * kBlock + r4);
+  if (!is_key) turn_bytes(w);
 #pragma unroll
-  for (int t = 0; t < kBlock; t++) {
-    const int row = row0 + t;
+  for (int s = 0; s < 4; s++) {
+    const int row = row0 + r4 + s;
     if (row >= 0 && row < unit.n)
-      v[(static_cast<size_t>(unit.first + row) * held + at_head) * 64 + lane] =
-          static_cast<float>(static_cast<int8_t>(word[t / 4] >> (8 * (t % 4)))) * scale;
+      *reinterpret_cast<v4f *>(to + static_cast<size_t>(unit.first + row) * held * 64) =
+          v4f{sdwa_cvt<0>(w[s]) * scale, sdwa_cvt<1>(w[s]) * scale, sdwa_cvt<2>(w[s]) * scale, sdwa_cvt<3>(w[s]) * scale};
   }
 }
 

@@ -662,7 +662,7 @@ def _int32(t, count: int, what: str):
     """Device pointer of an int32 CUDA tensor of `count` values."""
     if t is None:
         return None
-    if t.dtype != _torch().int32 or t.numel() != count:
+    if t.numel() != count or t.dtype != _torch().int32:
         raise FocrError(-2, f"{what}: {count} int32 values")
     return _dev(t)
 
@@ -711,12 +711,12 @@ class KvPages:
 
     def qkv_rows(self, qkv, rope, lens, row_start=None, q=None):
         """`qkv_rows` with its keys and values appended: queries [rows][n_heads][64]."""
-        torch = _torch()
-        rows, width = qkv.numel() // ((self.n_heads + 2 * self.n_kv_heads) * 64), self.n_heads * 64
-        if qkv.numel() != rows * (width + 2 * self.n_kv_heads * 64) or rope.numel() != rows * width:
+        width = self.n_heads * 64
+        rows, rest = divmod(qkv.numel(), width + 2 * self.n_kv_heads * 64)
+        if rest or rope.numel() != rows * width:
             raise FocrError(-2, "QKV rows [rows][qdim + 2 kdim] and factors [rows][n_heads][32][2]")
         if q is None:
-            q = torch.empty((rows, self.n_heads, 64), dtype=torch.float32, device=qkv.device)
+            q = qkv.new_empty((rows, self.n_heads, 64))
         elif q.numel() != rows * width:
             raise FocrError(-2, "queries [rows][n_heads][64]")
         _check(lib().focr_kv_pages_qkv_rows(self.ctx.handle, self.handle, _dev(qkv), rows, _dev(rope),
@@ -726,14 +726,13 @@ class KvPages:
     def attention(self, q, lens, max_len: int, row_start=None, sinks=None, out=None):
         """Attention of the batch's rows (1..8 of a sequence), appended before:
         [rows][n_heads][64]. No sequence has more than `max_len` positions, these included."""
-        torch = _torch()
-        rows = q.numel() // (self.n_heads * 64)
-        if q.numel() != rows * self.n_heads * 64 or (sinks is not None and sinks.numel() != self.n_heads):
+        rows, rest = divmod(q.numel(), self.n_heads * 64)
+        if rest or (sinks is not None and sinks.numel() != self.n_heads):
             raise FocrError(-2, "queries [rows][n_heads][64] and sinks [n_heads]")
         if max_len < 1:
             raise FocrError(-2, "max_len is positive")
         if out is None:
-            out = torch.empty((rows, self.n_heads, 64), dtype=torch.float32, device=q.device)
+            out = q.new_empty((rows, self.n_heads, 64))
         elif out.numel() != q.numel():
             raise FocrError(-2, "outputs [rows][n_heads][64]")
         _check(lib().focr_kv_pages_attention(self.ctx.handle, self.handle, _dev(q), rows,
@@ -743,9 +742,8 @@ class KvPages:
     def dequantize(self, rows: int, lens, row_start=None):
         """What the cache holds at the batch's positions: keys [rows][key_heads][64], values [rows][n_kv_heads][64]."""
         torch = _torch()
-        dev = f"cuda:{self.ctx.device}"
-        k = torch.empty((rows, self.key_heads, 64), dtype=torch.float32, device=dev)
-        v = torch.empty((rows, self.n_kv_heads, 64), dtype=torch.float32, device=dev)
+        k = lens.new_empty((rows, self.key_heads, 64), dtype=torch.float32)
+        v = lens.new_empty((rows, self.n_kv_heads, 64), dtype=torch.float32)
         _check(lib().focr_kv_pages_dequantize(self.ctx.handle, self.handle, rows, *self._batch(rows, lens, row_start),
                                               _dev(k), _dev(v)))
         return k, v
