@@ -42,6 +42,15 @@ fast mode's plan does (``PrefillAttention::Bf16`` / ``Bf16Static`` by
 come from the caller ([rows][n_heads][32][2] cos/sin pairs), as
 ``rotary_factors`` provides them to the reference's row kernels.
 
+Sessions that are decoded together keep their positions in a `KvPages` cache
+(one for each layer): `enter_pages` appends a prefilled prompt as one of its
+sequences, and `decode_pages` runs one step of the whole batch::
+
+    rms_norm(h) . qkv -> qkv                 the decode GEMV up to 8 rows in all, else the panels
+    KvPages.qkv_rows -> q, codes             split, norm, rotation, append
+    KvPages.attention                        each sequence's rows over its pages
+    wo, w13, w2                              as in `decode` or `prefill`
+
 `clock`, if given, is called with a stage name after each stage is
 enqueued, as the reference's PhaseClock marks phases (model/profile.rs:40-60).
 """
@@ -49,7 +58,7 @@ from __future__ import annotations
 
 from typing import Optional
 
-from . import (CompactKv, Context, Epilogue, ExpMode, FocrError, Geometry, KvSplit, PrefillOptions, PrefillProjection,
+from . import (CompactKv, Context, Epilogue, ExpMode, FocrError, Geometry, KvPages, KvSplit, PrefillOptions, PrefillProjection,
                Softmax, attention_decode_row, attention_prefill_bf16, attention_with, default_context,
                default_fast_exp, qkv_rows,
                row_scales)
@@ -220,6 +229,74 @@ class DecoderLayer:
         self.w2.linear_ex(gated, rows, epilogue=Epilogue.ADD, out=h)
         mark("w2")
         self.len = total
+        return h
+
+    def _pages(self, pages: KvPages) -> None:
+        if (pages.n_heads, pages.n_kv_heads) != (self.n_heads, self.n_kv_heads):
+            raise FocrError(-2, "the pages' heads are not the layer's")
+
+    def enter_pages(self, pages: KvPages, seq: int) -> None:
+        """Appends this layer's prefilled prompt to `pages` as sequence `seq`
+        from position 0 on (its pages mapped before). A prompt's keys are
+        those of every query head: pages with key_heads = n_heads."""
+        import torch
+
+        self._pages(pages)
+        if self.len == 0 or self.len != self.prefix_len:
+            raise FocrError(-2, "a prefilled prompt enters the pages before it is decoded")
+        if pages.key_heads != self.n_heads:
+            raise FocrError(-2, "a prompt's keys are held for each query head")
+        if not 0 <= seq < pages.n_seqs:
+            raise FocrError(-2, "no such sequence")
+        if self.prefix_len > pages.seq_pages * pages.page_size:
+            raise FocrError(-2, "KV context exhausted")
+        n = self.prefix_len
+        batch = torch.full((2, seq + 2), -1, dtype=torch.int32)
+        batch[0, seq] = 0
+        batch[1, :seq + 1] = 0
+        batch[1, seq + 1] = n
+        lens, row_start = batch[0, :seq + 1].to(self.v.device), batch[1].to(self.v.device)
+        pages.append(self.prefix_k[:n], self.v[:n], lens, row_start=row_start)
+
+    def decode_pages(self, h, rope, pages: KvPages, lens, max_len: int, row_start=None, clock=None):
+        """One step of a batch of sequences: updates `h` [rows][dim] in place
+        and appends to `pages` at the positions `lens` (see `KvPages`; no
+        sequence has more than `max_len`, these rows included)."""
+        self._pages(pages)
+        rows = h.shape[0]
+        if rows == 0:
+            return h
+        ctx, panel = self.ctx, rows > 8
+        if pages.ctx is not ctx:
+            raise FocrError(-1, "the pages belong to another context")
+        mark = clock or (lambda stage: None)
+        qkv = self._buf("pqkv", (rows, self.qkv.out_dim))
+        if panel:
+            rs = row_scales(h, self.dim, out=self._buf("prs", (rows,)), ctx=ctx)
+            self.qkv.prefill(h, rows, row_scale=rs, kernel=self.projection, out=qkv)
+        else:
+            self.qkv.linear_ex(h, rows, rms_norm=True, out=qkv)
+        mark("qkv")
+        q = pages.qkv_rows(qkv, rope, lens, row_start=row_start, q=self._buf("pq", (rows, self.n_heads, 64)))
+        mark("qkv_rows")
+        attn = pages.attention(q, lens, max_len, row_start=row_start, sinks=self.sinks,
+                               out=self._buf("pattn", (rows, self.n_heads, 64)))
+        mark("attention")
+        gated = self._buf("pgated", (rows, self.w13.out_dim // 2))
+        if panel:
+            self.wo.prefill(attn, rows, epilogue=Epilogue.ADD, out=h, kernel=self.projection)
+            mark("wo")
+            rs = row_scales(h, self.dim, out=rs, ctx=ctx)
+            self.w13.prefill(h, rows, row_scale=rs, epilogue=Epilogue.GLU, kernel=self.projection, out=gated)
+            mark("w13")
+            self.w2.prefill(gated, rows, epilogue=Epilogue.ADD, out=h, kernel=self.projection)
+        else:
+            self.wo.linear_ex(attn, rows, epilogue=Epilogue.ADD, out=h)
+            mark("wo")
+            self.w13.linear_ex(h, rows, rms_norm=True, epilogue=Epilogue.GLU, out=gated)
+            mark("w13")
+            self.w2.linear_ex(gated, rows, epilogue=Epilogue.ADD, out=h)
+        mark("w2")
         return h
 
     def truncate(self, length: int) -> None:
