@@ -6,16 +6,18 @@
 //
 // with x' the input row, times a row scale or RMS-normalized if asked.
 //
-// Mathematics. Each block of 128 W columns of a row of x' (W steps of a wave, 1 to
-// 4) is written as integers, x' = i 2^(e - 22), |i| <= 2^22, 2^e above its
-// largest magnitude, and i as three signed bytes, i = d0 + 256 d1 + 65536 d2. The
-// INT8 matrix instruction then forms the exact sums of 16 channels' codes times
-// the bytes of up to five rows (eight in two instructions) over 64 columns: operands
-// are the codes as the tile holds them (no conversion) and the bytes, one
-// column of the product per (row, byte). A sum is at most 64 * 128 * 128 = 2^20, so
-// its FP32 value is exact, and the only roundings are x' to 2^(e - 23) and the
-// FP32 multiply-adds of the groups' sums by their scales. A row that holds an infinity or NaN is
-// computed by FP32 multiply-adds instead, column after column.
+// Mathematics. Each block of 128 W columns of a row of x (W steps of a wave, 1 to 4)
+// is written as integers, x = i 2^(e - 22), |i| <= 2^22, 2^e above its largest
+// magnitude, and i as three signed bytes, i = d0 + 256 d1 + 65536 d2. The INT8
+// matrix instruction then forms the exact sums of 16 channels' codes times the
+// bytes of up to five rows (eight in two instructions) over 64 columns: operands are
+// the codes as the tile holds them (no conversion) and the bytes, one column of
+// the product per (row, byte). A sum is at most 64 * 128 * 128 = 2^20, so its FP32
+// value is exact, and the only roundings are x to 2^(e - 23) and the FP32
+// multiply-adds of the groups' sums by their scales. The factor of a row (its scale,
+// or its RMS norm's, whose sum of squares is taken as the row goes by) multiplies
+// the finished sums. A row that holds an infinity or NaN is computed by FP32
+// multiply-adds instead, column after column.
 #include <type_traits>
 
 #include "linear4.hpp"
@@ -28,6 +30,7 @@ using namespace linear4;
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v4f_apart __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kWaves = 8;
 constexpr size_t kLdsBytes = 160 * 1024;
@@ -41,12 +44,17 @@ struct Args {
   const float *x, *row_scale;
   float *out;
   int m, n, k, group, steps, tiles_total, rms, epilogue;
-  // The rows as bytes, written by rows4_kernel (PRE): blocks and their weights as
-  // they stand in the GEMV's LDS, row factors, non-finite marks of `parts` parts.
+  // The rows as they are staged: x, but for rows of fewer than four columns, which are
+  // computed like those with an infinity (plain).
+  const float *staged;
+  int staged_k;
+  uint32_t plain;
+  // What rows4_kernel writes (PRE): the blocks and their weights as they stand in the
+  // GEMV's LDS, sums of squares [8][blocks] and non-finite marks [8][blocks].
   char *digits;
-  float *weights, *row_factors;
+  float *weights, *squares;
   uint32_t *marks;
-  int parts;
+  int blocks;
 };
 
 // The largest of the 16 lanes of a DPP row, in every one of them.
@@ -92,26 +100,34 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Four columns of a row, zeros past its end.
-__device__ __forceinline__ float4 load_x(const Args &a, bool vec, int r, int col) {
-  const float *row = a.x + static_cast<size_t>(r) * a.k;
-  if (vec) return col < a.k ? *reinterpret_cast<const float4 *>(row + col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  return make_float4(col < a.k ? row[col] : 0.0f, col + 1 < a.k ? row[col + 1] : 0.0f,
-                     col + 2 < a.k ? row[col + 2] : 0.0f, col + 3 < a.k ? row[col + 3] : 0.0f);
+// A load at a uniform address and a lane's offset: one register of it, not two.
+template <typename T>
+__device__ __forceinline__ T load_at(const void *base, uint32_t offset) {
+  return *reinterpret_cast<const T *>(static_cast<const char *>(base) + offset);
 }
-__device__ __forceinline__ bool rows_vec(const Args &a) {
-  return a.k % 4 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+
+// Four columns of row r (the same for the wave) in one load, which needs no more than
+// FP32's alignment: the row's last four past its end, `trim`med when they are used.
+__device__ __forceinline__ v4f load_x(const Args &a, int r, int col) {
+  return load_at<v4f_apart>(a.staged + static_cast<size_t>(r) * a.staged_k, 4u * (col < a.staged_k - 4 ? col : a.staged_k - 4));
+}
+// Their values: zeros past the row's end.
+__device__ __forceinline__ v4f trim(const Args &a, v4f v, int col) {
+  const int k = a.staged_k, over = col - (k - 4);  // positions that the load went back
+  if (k % 4 != 0) {
+    v = over == 1 ? v4f{v[1], v[2], v[3], 0.0f} : over == 2 ? v4f{v[2], v[3], 0.0f, 0.0f} : over == 3 ? v4f{v[3], 0.0f, 0.0f, 0.0f} : v;
+  }
+  return over < 4 ? v : v4f{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
 // 1 / sqrt(mean of squares + eps) from the sum of squares.
 __device__ __forceinline__ float rms_factor(float sum, int k) {
   return __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(sum, static_cast<float>(k)) + 1.1920929e-7f));
 }
-__device__ __forceinline__ float square_sum(float4 v, float sum) {
-  sum = fmaf_(v.x, v.x, sum);
-  sum = fmaf_(v.y, v.y, sum);
-  sum = fmaf_(v.z, v.z, sum);
-  return fmaf_(v.w, v.w, sum);
+__device__ __forceinline__ float square_sum(v4f v, float sum) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) sum = fmaf_(v[i], v[i], sum);
+  return sum;
 }
 
 // The product's columns: with one 16-column block column 5 d + r holds byte d of
@@ -128,32 +144,36 @@ struct Columns {
 template <int W>
 struct Block {
   static constexpr int kParts = (W + 1) / 2;
-  float4 v[kParts];
+  v4f v[kParts];
   __device__ static __forceinline__ bool holds(int p) { return 2 * p + (threadIdx.x & 63) / 32 < W; }
-  __device__ __forceinline__ void load(const Args &a, bool vec, int r, int col0) {
+  // Columns past the block's count as past the row.
+  __device__ static __forceinline__ int column(const Args &a, int col0, int p) {
+    return holds(p) ? col0 + 256 * p + 4 * (threadIdx.x & 63) : a.staged_k;
+  }
+  __device__ __forceinline__ void load(const Args &a, int r, int col0) {
 #pragma unroll
-    for (int p = 0; p < kParts; p++)
-      v[p] = holds(p) ? load_x(a, vec, r, col0 + 256 * p + 4 * (threadIdx.x & 63)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int p = 0; p < kParts; p++) v[p] = load_x(a, r, column(a, col0, p));
+  }
+  __device__ __forceinline__ void trim_to(const Args &a, int col0) {
+#pragma unroll
+    for (int p = 0; p < kParts; p++) v[p] = trim(a, v[p], column(a, col0, p));
   }
 };
 
-// A wave writes block v of row r, times `factor` if scaled: bytes to `digits`
-// [2 W groups], their weights to `weights` [columns]. True (in every lane) if a
-// value is not finite.
+// A wave writes block x of row r: bytes to `digits` [2 W groups], their weights to
+// `weights` [columns]. True (in every lane) if a value is not finite.
 template <int NB, int W>
-__device__ __forceinline__ bool stage_block(Block<W> x, int r, bool scaled, float factor, char *digits, float *weights) {
+__device__ __forceinline__ bool stage_block(const Block<W> &x, int r, char *digits, float *weights) {
   using C = Columns<NB>;
   constexpr int P = Block<W>::kParts;
   const int lane = threadIdx.x & 63, l16 = lane & 15;
-  float4(&v)[P] = x.v;
+  const v4f(&v)[P] = x.v;
   uint32_t big = 0;
 #pragma unroll
   for (int p = 0; p < P; p++) {
-    if (scaled) v[p] = make_float4(v[p].x * factor, v[p].y * factor, v[p].z * factor, v[p].w * factor);
-    const float u[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const uint32_t bits = __float_as_uint(u[i]) & 0x7fffffffu;
+      const uint32_t bits = __float_as_uint(v[p][i]) & 0x7fffffffu;
       big = bits > big ? bits : big;
     }
   }
@@ -169,7 +189,7 @@ __device__ __forceinline__ bool stage_block(Block<W> x, int r, bool scaled, floa
   };
 #pragma unroll
   for (int p = 0; p < P; p++) {
-    const uint32_t w0 = bytes(v[p].x), w1 = bytes(v[p].y), w2 = bytes(v[p].z), w3 = bytes(v[p].w);
+    const uint32_t w0 = bytes(v[p][0]), w1 = bytes(v[p][1]), w2 = bytes(v[p][2]), w3 = bytes(v[p][3]);
     const uint32_t a01 = __builtin_amdgcn_perm(w1, w0, 0x05010400u), a23 = __builtin_amdgcn_perm(w3, w2, 0x05010400u);
     const uint32_t b01 = __builtin_amdgcn_perm(w1, w0, 0x0c0c0602u), b23 = __builtin_amdgcn_perm(w3, w2, 0x0c0c0602u);
     const uint32_t d[3] = {__builtin_amdgcn_perm(a23, a01, 0x05040100u), __builtin_amdgcn_perm(a23, a01, 0x07060302u),
@@ -184,59 +204,45 @@ __device__ __forceinline__ bool stage_block(Block<W> x, int r, bool scaled, floa
   return bad;
 }
 
-// Steps of a wave's turn where the rows come as bytes.
-constexpr int kPreSteps = 4;
-
-// The rows as bytes in memory, for large calls: a wave for each block (blockIdx.x,
-// wave) of row blockIdx.y, after the sum of squares of the whole row if it is
-// normalized.
-template <int NB>
-__global__ __launch_bounds__(256) void rows4_kernel(Args a, int blocks) {
+// The rows as bytes in memory, for large calls: a wave for each block of a row.
+template <int NB, int W>
+__global__ __launch_bounds__(256) void rows4_kernel(Args a) {
   using C = Columns<NB>;
-  __shared__ float s_sum[4];
-  __shared__ uint32_t s_bad;
-  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const bool vec = rows_vec(a);
-  const int block = 4 * blockIdx.x + wave;
-  Block<kPreSteps> x;
-  x.load(a, vec, r, block * kPreSteps * kStep);
-  if (tid == 0) s_bad = 0;
-  float factor = a.row_scale ? a.row_scale[r] : 1.0f;
-  if (a.rms) {
-    float sum = 0.0f;
-    for (int col = 4 * tid; col < a.k; col += 8192) {
-      float4 v[8];  // in flight together
+  const int r = blockIdx.y, block = 4 * blockIdx.x + threadIdx.x / 64;
+  if (block >= a.blocks) return;
+  Block<W> x;
+  x.load(a, r, block * W * kStep);
+  x.trim_to(a, block * W * kStep);
+  const bool bad = stage_block<NB, W>(x, r, a.digits + static_cast<size_t>(block) * 2 * W * C::kGroup, a.weights + block * C::kWide);
+  float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] = load_x(a, vec, r, col + 1024 * i);
-#pragma unroll
-      for (int i = 0; i < 8; i++) sum = square_sum(v[i], sum);
-    }
-    sum = wave_sum(sum);
-    if (lane == 0) s_sum[wave] = sum;
-  }
-  __syncthreads();
-  if (a.rms) factor = rms_factor((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), a.k);
-  if (block < blocks &&
-      stage_block<NB, kPreSteps>(x, r, a.rms || a.row_scale, factor,
-                                 a.digits + static_cast<size_t>(block) * 2 * kPreSteps * C::kGroup,
-                                 a.weights + block * C::kWide))
-    s_bad = 1;
-  __syncthreads();
-  if (tid == 0) {
-    a.marks[blockIdx.x * 8 + r] = s_bad;
-    a.row_factors[r] = factor;
+  for (int p = 0; p < Block<W>::kParts; p++) sum = square_sum(x.v[p], sum);
+  sum = wave_sum(sum);
+  if (threadIdx.x % 64 == 0) {
+    a.marks[r * a.blocks + block] = bad;
+    a.squares[r * a.blocks + block] = sum;
   }
 }
 
 // The workgroup's LDS accesses so far, and no load from memory, are waited for.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// Waves of a SIMD that the registers leave room for: two workgroups of a compute
+// unit, or one where LDS holds no more (or the scales of 32 columns take the registers).
+template <int NB, int SK, int W, int G, bool PRE>
+constexpr int resident() {
+  return (G == 32 && W > 2) || (PRE ? 2 : 1) * SK * 2 * W * Columns<NB>::kGroup > 80 * 1024 ? 2 : 4;
+}
+
 // NB: 16-column blocks of the product (Columns). SK: waves that share a tile's
 // columns, each W steps of a turn. G: columns per scale. PRE: the rows come as bytes
 // from rows4_kernel and pass through LDS turn by turn; otherwise the workgroup
 // writes all of them to LDS itself.
+// Bound: the codes, read once. A wave's load is 1 KB, a tile's step, and W of them
+// with their scales are on their way while W others are used; a load under a branch,
+// or a spilled register, would make the wave wait for all of them.
 template <int NB, int SK, int W, int G, bool PRE>
-__global__ __launch_bounds__(64 * kWaves, G == 32 && W > 2 ? 2 : 4) void gemv4_kernel(Args a) {
+__global__ __launch_bounds__(64 * kWaves, (resident<NB, SK, W, G, PRE>())) void gemv4_kernel(Args a) {
   using C = Columns<NB>;
   constexpr int NS = kStep / G;             // scales of a channel per step
   constexpr int SLOTS = kWaves / SK;        // tiles a workgroup has at once
@@ -244,15 +250,14 @@ __global__ __launch_bounds__(64 * kWaves, G == 32 && W > 2 ? 2 : 4) void gemv4_k
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int steps = a.steps, M = a.m, k = a.k;
   const int turns = (steps + W * SK - 1) / (W * SK);
-  const int held = PRE ? 2 * SK : turns * SK;                    // blocks in LDS (PRE: two turns)
-  float *weights = reinterpret_cast<float *>(lds + held * BLOCK);  // [held][columns]
-  float *red = weights + held * C::kWide;                        // [kWaves][8][16]
-  float *row_factor = red + kWaves * 8 * 16;                     // [8]
-  uint32_t *bad = reinterpret_cast<uint32_t *>(row_factor + 8);  // [8]
+  const int held = PRE ? 2 * SK : turns * SK;                          // blocks in LDS
+  float *const weights = reinterpret_cast<float *>(lds + held * BLOCK);  // [held][columns]
+  float *const red = weights + held * C::kWide;                         // [kWaves][8][16]
+  float *const squares = red + kWaves * 8 * 16;                         // [8][SK]
+  uint32_t *const bad = reinterpret_cast<uint32_t *>(squares + 8 * SK);  // [8]
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int slot = wave / SK, part = wave % SK;
-  const bool scaled = a.rms || a.row_scale;
 
   // The wave's work: of tiles first, first + stride, ... block part of every
   // turn: W steps, whose bytes are zeros past the last one.
@@ -266,21 +271,25 @@ __global__ __launch_bounds__(64 * kWaves, G == 32 && W > 2 ? 2 : 4) void gemv4_k
     int step = (turn * SK + part) * W + i;
     step = step < steps ? step : steps - 1;
     const size_t at = static_cast<size_t>(tile) * steps + step;
-    codes[i] = reinterpret_cast<const v4u *>(a.tiles)[at * 64 + lane];
+    codes[i] = load_at<v4u>(a.tiles + at * 64, 16u * lane);
 #pragma unroll
-    for (int q = 0; q < NS; q++) scales[i][q] = *reinterpret_cast<const v4f *>(a.scales + (at * NS + q) * kTile + 4 * kg);
+    for (int q = 0; q < NS; q++) scales[i][q] = load_at<v4f>(a.scales + (at * NS + q) * kTile, 16u * kg);
   };
 
   // PRE: a turn's bytes from memory to registers and on to LDS, and its weights to
   // registers.
-  constexpr int PER = PRE ? SK * BLOCK / 16 / (64 * kWaves) : 1;  // 16-byte pieces of a thread
-  static_assert(!PRE || SK * BLOCK % (16 * 64 * kWaves) == 0, "whole pieces");
+  constexpr int PIECES = SK * BLOCK / 16;  // 16 bytes each
+  constexpr int PER = PRE ? (PIECES + 64 * kWaves - 1) / (64 * kWaves) : 1;
   v4u moved[PER];
   float weight[NB];
+  // A thread with no piece left moves its last one again: no branch, no wait in one.
+  auto piece_of = [&](int p) {
+    const int piece = tid + 64 * kWaves * p;
+    return piece < PIECES ? piece : piece - 64 * kWaves;
+  };
   auto fetch = [&](int turn) {
 #pragma unroll
-    for (int p = 0; p < PER; p++)
-      moved[p] = reinterpret_cast<const v4u *>(a.digits)[turn * (SK * BLOCK / 16) + tid + 64 * kWaves * p];
+    for (int p = 0; p < PER; p++) moved[p] = load_at<v4u>(a.digits + static_cast<size_t>(turn) * PIECES * 16, 16u * piece_of(p));
   };
   auto fetch_weight = [&](int turn) {
 #pragma unroll
@@ -288,83 +297,75 @@ __global__ __launch_bounds__(64 * kWaves, G == 32 && W > 2 ? 2 : 4) void gemv4_k
   };
   auto place = [&](int buffer) {
 #pragma unroll
-    for (int p = 0; p < PER; p++) reinterpret_cast<v4u *>(lds)[buffer * (SK * BLOCK / 16) + tid + 64 * kWaves * p] = moved[p];
+    for (int p = 0; p < PER; p++) reinterpret_cast<v4u *>(lds)[buffer * PIECES + piece_of(p)] = moved[p];
   };
   if constexpr (PRE) {
     fetch(0);
     fetch_weight(0);
 #pragma unroll
     for (int i = 0; i < W; i++) load(i, 0, 0);
-    if (tid < 8) {
+    // Wave r sums row r's squares and marks over its blocks.
+    if (wave < M) {
+      float sum = 0.0f;
       uint32_t any = 0;
-      for (int p = 0; p < a.parts; p++) any |= tid < M ? a.marks[p * 8 + tid] : 0;
-      bad[tid] = any;
-      row_factor[tid] = tid < M ? a.row_factors[tid] : 1.0f;
+      for (int block = lane; block < a.blocks; block += 64) {
+        sum = sum + a.squares[wave * a.blocks + block];
+        any |= a.marks[wave * a.blocks + block];
+      }
+      sum = wave_sum(sum);
+      const bool found = __any(any != 0);
+      if (lane < SK) squares[wave * SK + lane] = lane == 0 ? sum : 0.0f;
+      if (lane == 0) bad[wave] = found;
     }
     place(0);
+    lds_barrier();
   } else {
     // The rows' loads go before the codes': loads arrive in order, and so the rows
     // are written while the codes are on their way. This wave writes block
-    // turn * SK + part of rows slot, slot + SLOTS, ...: a turn's at a time, the
-    // first one's from registers.
+    // turn * SK + part of rows slot, slot + SLOTS, ...
     constexpr int ROWS = (C::kRows + SLOTS - 1) / SLOTS;
-    const bool vec = rows_vec(a);
-    float row_scale = 1.0f;
-    if (tid < 8 && a.row_scale) row_scale = a.row_scale[tid < M ? tid : 0];
     Block<W> x[ROWS];
-    auto load_rows = [&](int t) {
+    float sum[ROWS];
 #pragma unroll
-      for (int i = 0; i < ROWS; i++)
-        if (slot + SLOTS * i < M) x[i].load(a, vec, slot + SLOTS * i, (t * SK + part) * W * kStep);
+    for (int i = 0; i < ROWS; i++) sum[i] = 0.0f;
+    // Past the call's rows, the last one again (not written).
+    auto load_rows = [&](int turn) {
+#pragma unroll
+      for (int i = 0; i < ROWS; i++) {
+        const int r = slot + SLOTS * i;
+        x[i].load(a, r < M ? r : M - 1, (turn * SK + part) * W * kStep);
+      }
     };
     load_rows(0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < W; i++) load(i, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
-    if (tid < 8) {
-      bad[tid] = 0;
-      row_factor[tid] = row_scale;
-    }
-    if (a.rms) {
-      float sum[ROWS];
-#pragma unroll
-      for (int i = 0; i < ROWS; i++) sum[i] = 0.0f;
-      for (int t = 0; t < turns; t++) {
-        if (t > 0) load_rows(t);
-#pragma unroll
-        for (int i = 0; i < ROWS; i++)
-          if (slot + SLOTS * i < M)
-#pragma unroll
-            for (int p = 0; p < Block<W>::kParts; p++) sum[i] = square_sum(x[i].v[p], sum[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < ROWS; i++) {
-        const float total = wave_sum(sum[i]);
-        if (lane == 0 && slot + SLOTS * i < M) red[(slot + SLOTS * i) * SK + part] = total;
-      }
-      lds_barrier();
-      if (tid < M) {
-        float total = red[tid * SK];
-        for (int q = 1; q < SK; q++) total += red[tid * SK + q];
-        row_factor[tid] = rms_factor(total, k);
-      }
-      if (turns > 1) load_rows(0);
-    }
+    if (tid < 8) bad[tid] = a.plain;
     lds_barrier();
-    for (int t = 0; t < turns; t++) {
-      if (t > 0) load_rows(t);
-      const int block = t * SK + part;
+    for (int turn = 0; turn < turns; turn++) {
+      if (turn > 0) load_rows(turn);
+      const int block = turn * SK + part;
 #pragma unroll
       for (int i = 0; i < ROWS; i++) {
         const int r = slot + SLOTS * i;
-        if (r < M &&
-            stage_block<NB, W>(x[i], r, scaled, row_factor[r], lds + block * BLOCK, weights + block * C::kWide))
-          bad[r] = 1;
+        if (r >= M) continue;
+        x[i].trim_to(a, block * W * kStep);
+        if (a.rms)
+#pragma unroll
+          for (int p = 0; p < Block<W>::kParts; p++) sum[i] = square_sum(x[i].v[p], sum[i]);
+        if (stage_block<NB, W>(x[i], r, lds + block * BLOCK, weights + block * C::kWide)) bad[r] = 1;
       }
     }
+    // The rows' sums of squares by waves, for `finish`.
+    if (a.rms)
+#pragma unroll
+      for (int i = 0; i < ROWS; i++) {
+        const float total = wave_sum(sum[i]);
+        if (lane == 0 && slot + SLOTS * i < M) squares[(slot + SLOTS * i) * SK + part] = total;
+      }
+    lds_barrier();
   }
-  lds_barrier();
 
   float acc[NB][4];
 #pragma unroll
@@ -449,8 +450,24 @@ __global__ __launch_bounds__(64 * kWaves, G == 32 && W > 2 ? 2 : 4) void gemv4_k
     const int r = l16, ch = tile * kTile + 4 * kg;
     if (r >= M || tile >= a.tiles_total || ch >= a.n) return;
     const float *row = a.x + static_cast<size_t>(r) * k;
-    const float rf = row_factor[r];
-    auto x_at = [&](int col) { return scaled ? row[col] * rf : row[col]; };
+    const bool scaled = a.rms || a.row_scale;
+    float factor = 1.0f;
+    if (a.rms) {
+      float total_squares = squares[r * SK];
+#pragma unroll
+      for (int p = 1; p < SK; p++) total_squares += squares[r * SK + p];
+      if (a.plain) {
+        total_squares = 0.0f;
+        for (int col = 0; col < k; col++) total_squares = fmaf_(row[col], row[col], total_squares);
+      }
+      factor = rms_factor(total_squares, k);
+    } else if (a.row_scale) {
+      factor = a.row_scale[r];
+    }
+    if (scaled)
+#pragma unroll
+      for (int i = 0; i < 4; i++) total[i] = total[i] * factor;
+    auto x_at = [&](int col) { return scaled ? row[col] * factor : row[col]; };
     if (bad[r]) {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -499,23 +516,23 @@ __global__ __launch_bounds__(64 * kWaves, G == 32 && W > 2 ? 2 : 4) void gemv4_k
     if (ends && a.epilogue == FOCR_EPI_ADD) load_residual(round);
     if constexpr (PRE && kMore) fetch(next_turn);
     const int block = PRE ? buffer * SK + part : turn * SK + part;
-    float sum[NB][4], f[NB];
+    float block_sum[NB][4], f[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++) {
       f[b] = PRE ? weight[b] : weights[block * C::kWide + 16 * b + l16];
 #pragma unroll
-      for (int i = 0; i < 4; i++) sum[b][i] = 0.0f;
+      for (int i = 0; i < 4; i++) block_sum[b][i] = 0.0f;
     }
     if constexpr (PRE && kMore) fetch_weight(next_turn);
 #pragma unroll
     for (int i = 0; i < W; i++) {
-      consume(codes[i], scales[i], lds + block * BLOCK + 2 * i * C::kGroup, sum);
+      consume(codes[i], scales[i], lds + block * BLOCK + 2 * i * C::kGroup, block_sum);
       if constexpr (kMore) load(i, next_round, next_turn);
     }
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) acc[b][i] = fmaf_(sum[b][i], f[b], acc[b][i]);
+      for (int i = 0; i < 4; i++) acc[b][i] = fmaf_(block_sum[b][i], f[b], acc[b][i]);
     if constexpr (PRE && kMore) {
       buffer ^= 1;
       place(buffer);
@@ -529,75 +546,94 @@ __global__ __launch_bounds__(64 * kWaves, G == 32 && W > 2 ? 2 : 4) void gemv4_k
   take(std::false_type());
 }
 
+// Turns of a row, and the fewest steps of a turn that take all of it in them.
+constexpr int turns_of(int steps, int sk) { return (steps + 4 * sk - 1) / (4 * sk); }
+constexpr int width_of(int steps, int sk) {
+  const int turns = turns_of(steps, sk);
+  return (steps + sk * turns - 1) / (sk * turns);
+}
+// LDS of a workgroup.
+size_t lds_of(int nb, int sk, int w, size_t held) {
+  return held * (2 * w * 64 * 16 * nb + 16 * nb * 4) + kWaves * 8 * 16 * 4 + 8 * sk * 4 + 8 * 4;
+}
+
 template <int NB, int SK, int W, int G, bool PRE>
 int launch_one(Ctx *ctx, const Args &a) {
-  using C = Columns<NB>;
-  const size_t turns = (static_cast<size_t>(a.steps) + W * SK - 1) / (W * SK), held = PRE ? 2 * SK : turns * SK;
-  const size_t lds = held * (2 * W * C::kGroup + C::kWide * 4) + kWaves * 8 * 16 * 4 + 8 * 4 + 8 * 4;
-  FOCR_REQUIRE(lds <= kLdsBytes, FOCR_E_SHAPE, "GEMV: in_dim too large for the rows of x in LDS");
+  if constexpr (PRE) {
+    hipLaunchKernelGGL((rows4_kernel<NB, W>), dim3((a.blocks + 3) / 4, a.m), dim3(256), 0, ctx->stream, a);
+    FOCR_HIP_CHECK(hipGetLastError());
+  }
+  const size_t turns = (a.steps + W * SK - 1) / (W * SK), lds = lds_of(NB, SK, W, PRE ? 2 * SK : turns * SK);
+  FOCR_REQUIRE(lds <= kLdsBytes, FOCR_E_SHAPE, "GEMV: the rows of x exceed LDS");
   // Above 64 KB the kernel has to be allowed it, on each device.
   if (lds > 64 * 1024)
     FOCR_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(gemv4_kernel<NB, SK, W, G, PRE>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLdsBytes)));
   constexpr int slots = kWaves / SK;
   const int want = (a.tiles_total + slots - 1) / slots;
-  const int blocks = want < 512 ? want : 512;
+  const int most = lds > kLdsBytes / 2 ? 256 : 512;  // workgroups that 256 compute units hold at once
+  const int blocks = want < most ? want : most;
   hipLaunchKernelGGL((gemv4_kernel<NB, SK, W, G, PRE>), dim3(blocks), dim3(64 * kWaves), lds, ctx->stream, a);
   FOCR_HIP_CHECK(hipGetLastError());
   return FOCR_OK;
 }
 
-// The fewest steps of a turn that take all of a row, at most 4.
 template <int NB, int SK, int G>
 int launch_steps(Ctx *ctx, const Args &a) {
-  switch ((a.steps + SK - 1) / SK) {
+  switch (width_of(a.steps, SK)) {
     case 1: return launch_one<NB, SK, 1, G, false>(ctx, a);
     case 2: return launch_one<NB, SK, 2, G, false>(ctx, a);
     case 3: return launch_one<NB, SK, 3, G, false>(ctx, a);
     default: return launch_one<NB, SK, 4, G, false>(ctx, a);
   }
 }
+// Rows as bytes: more than one turn, so that W is 3 or 4.
+template <int NB, int SK, int G>
+int launch_pre(Ctx *ctx, Args a) {
+  using C = Columns<NB>;
+  const int turns = turns_of(a.steps, SK) < 2 ? 2 : turns_of(a.steps, SK), w = (a.steps + SK * turns - 1) / (SK * turns) <= 3 ? 3 : 4;
+  const size_t blocks = static_cast<size_t>((a.steps + w * SK - 1) / (w * SK)) * SK;
+  const size_t digits = blocks * 2 * w * C::kGroup;
+  const int rc = ensure_scratch(ctx, digits + blocks * (C::kWide * 4 + 8 * 4 + 8 * 4));
+  if (rc != FOCR_OK) return rc;
+  a.blocks = static_cast<int>(blocks);
+  a.digits = static_cast<char *>(ctx->scratch);
+  a.weights = reinterpret_cast<float *>(a.digits + digits);
+  a.squares = a.weights + blocks * C::kWide;
+  a.marks = reinterpret_cast<uint32_t *>(a.squares + 8 * blocks);
+  return w == 3 ? launch_one<NB, SK, 3, G, true>(ctx, a) : launch_one<NB, SK, 4, G, true>(ctx, a);
+}
+
+// Few tiles are shared by many waves, so that every SIMD has work: 4,096 x 8,192 for
+// one row takes 8.4 us with eight waves a tile and 14.4 with two, and 27,807 x 2,132
+// for two rows 12.8 with two and 15.5 with four. Bytes from memory reach LDS once for
+// a turn of all the workgroup's tiles, so that half as many waves a tile are right
+// there: 20,000 x 5,000 for four rows takes 15.5 us with one and 16.7 with two.
+constexpr int waves_of(int tiles) { return tiles >= 1024 ? 2 : tiles >= 512 ? 4 : 8; }
+
+// Above this many columns in all rows a kernel of its own writes their bytes once:
+// at 32,768 columns 11,008 channels take 11.9 us with it and 14.2 with the rows
+// written by every workgroup; a launch more costs what 16,384 columns gain (8,192
+// channels: 7.2 us without it, 4,096: 6.9 without it and 9.5 with it).
+constexpr long kPreColumns = 16384;
 
 template <int NB, int G>
-int launch_parts(Ctx *ctx, const Args &a, bool pre) {
-  // Waves per tile: enough to give each SIMD two.
-  if (pre) {
-    if (a.tiles_total >= 2048) return launch_one<NB, 1, kPreSteps, G, true>(ctx, a);
-    if (a.tiles_total >= 512) return launch_one<NB, 2, kPreSteps, G, true>(ctx, a);
-    return launch_one<NB, 4, kPreSteps, G, true>(ctx, a);
-  }
-  if (a.tiles_total >= 2048) return launch_steps<NB, 2, G>(ctx, a);
-  if (a.tiles_total >= 512) return launch_steps<NB, 4, G>(ctx, a);
-  return launch_steps<NB, 8, G>(ctx, a);
+int launch_parts(Ctx *ctx, const Args &a) {
+  const int sk = waves_of(a.tiles_total);
+  const size_t lds = lds_of(NB, sk, width_of(a.steps, sk), static_cast<size_t>(turns_of(a.steps, sk)) * sk);
+  const bool pre = static_cast<long>(a.m) * a.k > kPreColumns || lds > kLdsBytes;
+  if (sk == 2) return pre ? launch_pre<NB, 1, G>(ctx, a) : launch_steps<NB, 2, G>(ctx, a);
+  if (sk == 4) return pre ? launch_pre<NB, 2, G>(ctx, a) : launch_steps<NB, 4, G>(ctx, a);
+  return pre ? launch_pre<NB, 4, G>(ctx, a) : launch_steps<NB, 8, G>(ctx, a);
 }
-
-// Blocks of the rows' bytes: whole turns of up to four waves.
-size_t pre_blocks(size_t steps) { return (steps + 4 * kPreSteps - 1) / (4 * kPreSteps) * 4; }
 
 template <int NB>
-int launch_group(Ctx *ctx, Args a, bool pre) {
-  using C = Columns<NB>;
-  if (pre) {
-    const size_t blocks = pre_blocks(a.steps);
-    a.parts = static_cast<int>(blocks / 4);
-    a.digits = static_cast<char *>(ctx->scratch);
-    a.weights = reinterpret_cast<float *>(a.digits + blocks * 2 * kPreSteps * C::kGroup);
-    a.row_factors = a.weights + blocks * C::kWide;
-    a.marks = reinterpret_cast<uint32_t *>(a.row_factors + 8);
-    hipLaunchKernelGGL(rows4_kernel<NB>, dim3(a.parts, a.m), dim3(256), 0, ctx->stream, a, static_cast<int>(blocks));
-    FOCR_HIP_CHECK(hipGetLastError());
-  }
+int launch_group(Ctx *ctx, const Args &a) {
   switch (a.group) {
-    case 32: return launch_parts<NB, 32>(ctx, a, pre);
-    case 64: return launch_parts<NB, 64>(ctx, a, pre);
-    default: return launch_parts<NB, 128>(ctx, a, pre);
+    case 32: return launch_parts<NB, 32>(ctx, a);
+    case 64: return launch_parts<NB, 64>(ctx, a);
+    default: return launch_parts<NB, 128>(ctx, a);
   }
-}
-
-// Scratch of a call whose rows are written as bytes first.
-size_t rows_bytes(size_t m, size_t steps) {
-  const size_t blocks = pre_blocks(steps), wide = m <= 5 ? Columns<1>::kWide : Columns<2>::kWide;
-  return blocks * (2 * kPreSteps * 64 * wide + wide * 4) + 8 * 4 + blocks / 4 * 8 * 4;
 }
 
 // ---- storage -------------------------------------------------------------------
@@ -711,12 +747,23 @@ int launch_gemv4(Ctx *ctx, const Linear *lin, const float *x, size_t rows, const
   a.tiles_total = static_cast<int>(lin->gemv_tiles);
   a.rms = rms_norm ? 1 : 0;
   a.epilogue = epilogue;
-  const bool pre = rows * lin->k > 16384 || lin->k > 8192;
-  if (pre) {
-    const int rc = ensure_scratch(ctx, rows_bytes(rows, steps));
-    if (rc != FOCR_OK) return rc;
+  a.staged = lin->k < 4 ? lin->gemv_scales : x;  // 16 floats at least
+  a.staged_k = lin->k < 4 ? 4 : a.k;
+  a.plain = lin->k < 4;
+  if (a.plain && a.m > 1) {
+    // One row at a time: the scales of one tile are the rows.
+    for (size_t r = 0; r < rows; r++) {
+      Args one = a;
+      one.m = 1;
+      one.x = x + r * lin->k;
+      one.row_scale = row_scale ? row_scale + r : nullptr;
+      one.out = out + r * (epilogue == FOCR_EPI_GLU ? lin->n / 2 : lin->n);
+      const int rc = launch_group<1>(ctx, one);
+      if (rc != FOCR_OK) return rc;
+    }
+    return FOCR_OK;
   }
-  return rows <= 5 ? launch_group<1>(ctx, a, pre) : launch_group<2>(ctx, a, pre);
+  return rows <= 5 ? launch_group<1>(ctx, a) : launch_group<2>(ctx, a);
 }
 
 int pack_linear4(Ctx *ctx, Linear *lin, const int8_t *codes, size_t *total) {
