@@ -280,6 +280,7 @@ __global__ __launch_bounds__(64 * kWaves, (resident<NB, SK, W, G, PRE>())) void 
   // registers.
   constexpr int PIECES = SK * BLOCK / 16;  // 16 bytes each
   constexpr int PER = PRE ? (PIECES + 64 * kWaves - 1) / (64 * kWaves) : 1;
+  static_assert(!PRE || PIECES >= 64 * kWaves, "a piece for each thread");
   v4u moved[PER];
   float weight[NB];
   // A thread with no piece left moves its last one again: no branch, no wait in one.
@@ -587,11 +588,13 @@ int launch_steps(Ctx *ctx, const Args &a) {
     default: return launch_one<NB, SK, 4, G, false>(ctx, a);
   }
 }
-// Rows as bytes: more than one turn, so that W is 3 or 4.
+// Rows as bytes: more than one turn, so that W is 3 or 4 (one wave a tile: many
+// turns, and 4).
 template <int NB, int SK, int G>
 int launch_pre(Ctx *ctx, Args a) {
   using C = Columns<NB>;
-  const int turns = turns_of(a.steps, SK) < 2 ? 2 : turns_of(a.steps, SK), w = (a.steps + SK * turns - 1) / (SK * turns) <= 3 ? 3 : 4;
+  const int turns = turns_of(a.steps, SK) < 2 ? 2 : turns_of(a.steps, SK);
+  const int w = SK > 1 && (a.steps + SK * turns - 1) / (SK * turns) <= 3 ? 3 : 4;
   const size_t blocks = static_cast<size_t>((a.steps + w * SK - 1) / (w * SK)) * SK;
   const size_t digits = blocks * 2 * w * C::kGroup;
   const int rc = ensure_scratch(ctx, digits + blocks * (C::kWide * 4 + 8 * 4 + 8 * 4));
@@ -601,7 +604,9 @@ int launch_pre(Ctx *ctx, Args a) {
   a.weights = reinterpret_cast<float *>(a.digits + digits);
   a.squares = a.weights + blocks * C::kWide;
   a.marks = reinterpret_cast<uint32_t *>(a.squares + 8 * blocks);
-  return w == 3 ? launch_one<NB, SK, 3, G, true>(ctx, a) : launch_one<NB, SK, 4, G, true>(ctx, a);
+  if constexpr (SK > 1)
+    if (w == 3) return launch_one<NB, SK, 3, G, true>(ctx, a);
+  return launch_one<NB, SK, 4, G, true>(ctx, a);
 }
 
 // Few tiles are shared by many waves, so that every SIMD has work: 4,096 x 8,192 for
