@@ -297,6 +297,7 @@ int focr_linear_upload(focr_ctx *handle, int bits, size_t n, size_t k, size_t gr
   FOCR_REQUIRE(n > 0 && k > 0, FOCR_E_SHAPE, "focr_linear_upload: empty matrix");
   FOCR_REQUIRE(n <= (size_t(1) << 31) / 1 && k <= (size_t(1) << 24), FOCR_E_SHAPE,
                "focr_linear_upload: matrix too large");
+  FOCR_REQUIRE(bits != 4 || n <= INT32_MAX - 15, FOCR_E_SHAPE, "focr_linear_upload: matrix too large for 4-bit tiles");
   if (bits != 32) {
     FOCR_REQUIRE(group == 32 || group == 64 || group == 128, FOCR_E_SHAPE,
                  "focr_linear_upload: group must be 32, 64 or 128");

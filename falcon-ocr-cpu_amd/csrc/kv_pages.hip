@@ -427,7 +427,7 @@ struct AttendArgs {
   const float *q, *sinks;
   float *out;
   float *part_o, *part_md;  // [row][head][part][64], [..][2]
-  int max_len, chunk, parts, tiles, most;  // most: rows of a sequence at most
+  int max_len, chunk, parts, tiles;  // tiles: of 16 columns, for as many rows as a sequence can have
 };
 
 // A sequence's rows for attention; false where there is nothing to do (n = 0) or it
@@ -938,13 +938,12 @@ Cache cache_of(const Pages *kv, size_t rows, const int32_t *row_start, const int
 // What every call over a batch checks.
 int check_batch(const char *name, const Ctx *ctx, const Pages *kv, size_t rows, const int32_t *row_start,
                 const int32_t *lens, size_t n_seqs) {
-  const std::string at = std::string(name) + ": ";
-  FOCR_REQUIRE(ctx && kv, FOCR_E_ARG, at + "null argument");
-  FOCR_REQUIRE(kv->device == ctx->device, FOCR_E_ARG, at + "the cache is on another device than the context");
-  FOCR_REQUIRE(n_seqs <= kv->n_seqs, FOCR_E_SHAPE, at + "more sequences than the cache has");
-  FOCR_REQUIRE(rows < (size_t(1) << 24), FOCR_E_SHAPE, at + "too many rows");
-  FOCR_REQUIRE(row_start || rows == n_seqs, FOCR_E_SHAPE, at + "without row_start every sequence has one row");
-  FOCR_REQUIRE(rows == 0 || n_seqs == 0 || lens, FOCR_E_ARG, at + "null lengths");
+  FOCR_REQUIRE(ctx && kv, FOCR_E_ARG, std::string(name) + ": null argument");
+  FOCR_REQUIRE(kv->device == ctx->device, FOCR_E_ARG, std::string(name) + ": the cache is on another device than the context");
+  FOCR_REQUIRE(n_seqs <= kv->n_seqs, FOCR_E_SHAPE, std::string(name) + ": more sequences than the cache has");
+  FOCR_REQUIRE(rows < (size_t(1) << 24), FOCR_E_SHAPE, std::string(name) + ": too many rows");
+  FOCR_REQUIRE(row_start || rows == n_seqs, FOCR_E_SHAPE, std::string(name) + ": without row_start every sequence has one row");
+  FOCR_REQUIRE(rows == 0 || n_seqs == 0 || lens, FOCR_E_ARG, std::string(name) + ": null lengths");
   return FOCR_OK;
 }
 
@@ -1130,9 +1129,9 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
   a.sinks = sinks;
   a.out = out;
   a.max_len = static_cast<int>(max_len);
-  a.most = row_start ? static_cast<int>(rows < 8 ? rows : 8) : 1;
+  const size_t most = row_start ? std::min<size_t>(rows, 8) : 1;
   const size_t group = kv->n_heads / kv->key_heads;
-  a.tiles = static_cast<int>((group * a.most + 15) / 16);
+  a.tiles = static_cast<int>((group * most + 15) / 16);
   // Parts of whole 256 keys, at most 4,096 (the longest run) up to a million
   // positions. Few sequences need only fill the chip (us a call with 512 / 1,024 /
   // 2,048 workgroups: one of 131,072 positions 33.1 / 36.2 / 37.3, four of up to

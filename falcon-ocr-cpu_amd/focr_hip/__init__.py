@@ -171,11 +171,11 @@ class Context:
         self.handle = handle
         self.device = device
         with torch.cuda.device(device):
-            stream = torch.cuda.current_stream(device)
-        _check(lib().focr_ctx_set_stream(self.handle, ctypes.c_void_p(stream.cuda_stream)))
+            self.use_stream(torch.cuda.current_stream(device))
 
     def use_stream(self, stream) -> None:
         """Run on a torch stream (None: the context's own stream)."""
+        self.stream = None if stream is None else stream.cuda_stream
         if stream is None:
             _check(lib().focr_ctx_use_own_stream(self.handle))
         else:
@@ -658,15 +658,6 @@ class KvSplit:
             pass
 
 
-def _int32(t, count: int, what: str):
-    """Device pointer of an int32 CUDA tensor of `count` values."""
-    if t is None:
-        return None
-    if t.numel() != count or t.dtype != _torch().int32:
-        raise FocrError(-2, f"{what}: {count} int32 values")
-    return _dev(t)
-
-
 class KvPages:
     """An 8-bit cache of pages for a batch of sequences (no reference
     counterpart): blocks of 16 positions and one head share a scale.
@@ -684,6 +675,7 @@ class KvPages:
         self.n_pages, self.page_size, self.n_seqs, self.seq_pages = n_pages, page_size, n_seqs, seq_pages
         self.n_heads, self.n_kv_heads = n_heads, n_kv_heads
         self.key_heads = n_kv_heads if key_heads is None else key_heads
+        self._types = _torch().float32, _torch().int32
         handle = ctypes.c_void_p()
         _check(lib().focr_kv_pages_create(self.ctx.handle, n_pages, page_size, n_seqs, seq_pages, n_heads,
                                           self.key_heads, n_kv_heads, 64, ctypes.byref(handle)))
@@ -697,17 +689,31 @@ class KvPages:
         _check(lib().focr_kv_pages_map(self.ctx.handle, self.handle, seq, first, len(ids),
                                        ids.ctypes.data_as(ctypes.c_void_p)))
 
-    def _batch(self, rows: int, lens, row_start):
+    def _ptr(self, t, kind: int = 0):
+        """Device pointer of a contiguous tensor on the cache's device: float32, or (kind 1) int32."""
+        if t is None:
+            return None
+        if t.get_device() != self.ctx.device:
+            raise FocrError(-1, "expected a CUDA tensor on the cache's device")
+        if t.dtype != self._types[kind]:
+            raise FocrError(-2, f"expected {self._types[kind]}, not {t.dtype}")
+        if not t.is_contiguous():
+            raise FocrError(-2, "expected a contiguous tensor")
+        return t.data_ptr()
+
+    def _batch(self, lens, row_start):
         seqs = lens.numel()
-        return _int32(row_start, seqs + 1, "row_start"), _int32(lens, seqs, "lens"), seqs
+        if row_start is not None and row_start.numel() != seqs + 1:
+            raise FocrError(-2, "row_start has a value more than lens")
+        return self._ptr(row_start, 1), self._ptr(lens, 1), seqs
 
     def append(self, k, v, lens, row_start=None) -> None:
         """Keys [rows][key_heads][64] and values [rows][n_kv_heads][64] at the batch's positions."""
         rows = v.numel() // (self.n_kv_heads * 64)
         if k.numel() != rows * self.key_heads * 64 or v.numel() != rows * self.n_kv_heads * 64:
             raise FocrError(-2, "keys [rows][key_heads][64] and values [rows][n_kv_heads][64]")
-        _check(lib().focr_kv_pages_append(self.ctx.handle, self.handle, _dev(k), _dev(v), rows,
-                                          *self._batch(rows, lens, row_start)))
+        _check(lib().focr_kv_pages_append(self.ctx.handle, self.handle, self._ptr(k), self._ptr(v), rows,
+                                          *self._batch(lens, row_start)))
 
     def qkv_rows(self, qkv, rope, lens, row_start=None, q=None):
         """`qkv_rows` with its keys and values appended: queries [rows][n_heads][64]."""
@@ -719,8 +725,8 @@ class KvPages:
             q = qkv.new_empty((rows, self.n_heads, 64))
         elif q.numel() != rows * width:
             raise FocrError(-2, "queries [rows][n_heads][64]")
-        _check(lib().focr_kv_pages_qkv_rows(self.ctx.handle, self.handle, _dev(qkv), rows, _dev(rope),
-                                            *self._batch(rows, lens, row_start), _dev(q)))
+        _check(lib().focr_kv_pages_qkv_rows(self.ctx.handle, self.handle, self._ptr(qkv), rows, self._ptr(rope),
+                                            *self._batch(lens, row_start), self._ptr(q)))
         return q
 
     def attention(self, q, lens, max_len: int, row_start=None, sinks=None, out=None):
@@ -735,8 +741,8 @@ class KvPages:
             out = q.new_empty((rows, self.n_heads, 64))
         elif out.numel() != q.numel():
             raise FocrError(-2, "outputs [rows][n_heads][64]")
-        _check(lib().focr_kv_pages_attention(self.ctx.handle, self.handle, _dev(q), rows,
-                                             *self._batch(rows, lens, row_start), max_len, _dev(sinks), _dev(out)))
+        _check(lib().focr_kv_pages_attention(self.ctx.handle, self.handle, self._ptr(q), rows,
+                                             *self._batch(lens, row_start), max_len, self._ptr(sinks), self._ptr(out)))
         return out
 
     def dequantize(self, rows: int, lens, row_start=None):
@@ -744,8 +750,8 @@ class KvPages:
         torch = _torch()
         k = lens.new_empty((rows, self.key_heads, 64), dtype=torch.float32)
         v = lens.new_empty((rows, self.n_kv_heads, 64), dtype=torch.float32)
-        _check(lib().focr_kv_pages_dequantize(self.ctx.handle, self.handle, rows, *self._batch(rows, lens, row_start),
-                                              _dev(k), _dev(v)))
+        _check(lib().focr_kv_pages_dequantize(self.ctx.handle, self.handle, rows, *self._batch(lens, row_start),
+                                              self._ptr(k), self._ptr(v)))
         return k, v
 
     def refused(self):

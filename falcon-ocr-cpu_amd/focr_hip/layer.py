@@ -98,6 +98,7 @@ class DecoderLayer:
         self.prefix_len = 0
         self.image = (0, 0)
         self._work = {}
+        self._outgrown = []
 
     def _buf(self, name: str, shape):
         import torch
@@ -110,6 +111,20 @@ class DecoderLayer:
             t = torch.empty(n, dtype=torch.float32, device=f"cuda:{self.ctx.device}")
             self._work[name] = t
         return t[:n].view(*shape)
+
+    def _step_buf(self, name: str, shape):
+        """`_buf` for `decode_pages`: one that is outgrown is kept for steps that were
+        captured with it (its successor is at least twice as large)."""
+        import torch
+
+        t = self._work.get(name)
+        n = 1
+        for s in shape:
+            n *= s
+        if t is not None and t.numel() < n:
+            self._outgrown.append(t)
+            self._work[name] = torch.empty(max(n, 2 * t.numel()), dtype=t.dtype, device=t.device)
+        return self._buf(name, shape)
 
     def kv(self, total: int) -> CompactKv:
         """The cache's first `total` positions as a CompactKv."""
@@ -234,6 +249,8 @@ class DecoderLayer:
     def _pages(self, pages: KvPages) -> None:
         if (pages.n_heads, pages.n_kv_heads) != (self.n_heads, self.n_kv_heads):
             raise FocrError(-2, "the pages' heads are not the layer's")
+        if pages.ctx is not self.ctx:
+            raise FocrError(-1, "the pages belong to another context")
 
     def enter_pages(self, pages: KvPages, seq: int) -> None:
         """Appends this layer's prefilled prompt to `pages` as sequence `seq`
@@ -257,32 +274,35 @@ class DecoderLayer:
         batch[1, seq + 1] = n
         lens, row_start = batch[0, :seq + 1].to(self.v.device), batch[1].to(self.v.device)
         pages.append(self.prefix_k[:n], self.v[:n], lens, row_start=row_start)
+        if self.ctx.stream != torch.cuda.current_stream(self.ctx.device).cuda_stream:
+            self.ctx.sync()  # the batch's arrays are free for torch's stream from here on
 
     def decode_pages(self, h, rope, pages: KvPages, lens, max_len: int, row_start=None, clock=None):
         """One step of a batch of sequences: updates `h` [rows][dim] in place
         and appends to `pages` at the positions `lens` (see `KvPages`; no
-        sequence has more than `max_len`, these rows included)."""
+        sequence has more than `max_len`, these rows included). Rows that are
+        no sequence's, or a refused one's, come out without meaning."""
         self._pages(pages)
         rows = h.shape[0]
+        if h.shape[1:] != (self.dim,):
+            raise FocrError(-2, "h [rows][dim]")
         if rows == 0:
             return h
         ctx, panel = self.ctx, rows > 8
-        if pages.ctx is not ctx:
-            raise FocrError(-1, "the pages belong to another context")
         mark = clock or (lambda stage: None)
-        qkv = self._buf("pqkv", (rows, self.qkv.out_dim))
+        qkv = self._step_buf("pqkv", (rows, self.qkv.out_dim))
         if panel:
-            rs = row_scales(h, self.dim, out=self._buf("prs", (rows,)), ctx=ctx)
+            rs = row_scales(h, self.dim, out=self._step_buf("prs", (rows,)), ctx=ctx)
             self.qkv.prefill(h, rows, row_scale=rs, kernel=self.projection, out=qkv)
         else:
             self.qkv.linear_ex(h, rows, rms_norm=True, out=qkv)
         mark("qkv")
-        q = pages.qkv_rows(qkv, rope, lens, row_start=row_start, q=self._buf("pq", (rows, self.n_heads, 64)))
+        q = pages.qkv_rows(qkv, rope, lens, row_start=row_start, q=self._step_buf("pq", (rows, self.n_heads, 64)))
         mark("qkv_rows")
         attn = pages.attention(q, lens, max_len, row_start=row_start, sinks=self.sinks,
-                               out=self._buf("pattn", (rows, self.n_heads, 64)))
+                               out=self._step_buf("pattn", (rows, self.n_heads, 64)))
         mark("attention")
-        gated = self._buf("pgated", (rows, self.w13.out_dim // 2))
+        gated = self._step_buf("pgated", (rows, self.w13.out_dim // 2))
         if panel:
             self.wo.prefill(attn, rows, epilogue=Epilogue.ADD, out=h, kernel=self.projection)
             mark("wo")

@@ -195,3 +195,68 @@ def test_captured_batch_steps(fh):
         got = host(h)
         want = layer.decode_pages(to_dev(x), rope, caches[1], int32(start + step), 64)
         assert_bitwise(got, host(want), f"step {step}")
+
+
+def test_a_captured_step_keeps_its_buffers(fh):
+    # A larger batch in between must not leave the graph writing memory that others have.
+    import torch
+
+    m, _ = matrices(fh)
+    ctx = fh.default_context()
+    layer = layer_of(fh, m, to_dev(np.zeros(H, F32)), 8, fh.PrefillProjection.I16)
+    n = 7
+    caches = [fh.KvPages(n, 16, n, 1, H, G) for _ in range(2)]
+    for pages in caches:
+        for i in range(n):
+            pages.map(i, 0, [i])
+    rope = to_dev(rope_table(n, 3, alike=True))
+    x = gen.normal((n, DIM), 1.0, 11)
+    zeros = int32([0] * n)
+    layer.decode_pages(to_dev(x[:2]), rope[:2], caches[1], zeros[:2], 16)
+    h = torch.zeros(2, DIM, device="cuda:0")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ctx.use_stream(torch.cuda.current_stream())
+        layer.decode_pages(h, rope[:2], caches[0], zeros[:2], 16)
+    ctx.use_stream(torch.cuda.current_stream())
+    layer.decode_pages(to_dev(x), rope, caches[1], zeros, 16)
+    others = [torch.full((2, w), 7.0, device="cuda:0") for w in ((H + 2 * G) * 64, H * 64, H * 64, FFN) for _ in range(4)]
+    want = host(layer.decode_pages(to_dev(x[:2]), rope[:2], caches[1], zeros[:2], 16))
+    for step in range(3):
+        h.copy_(to_dev(x[:2]))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert_bitwise(host(h), want, f"replay {step}")
+    assert all((host(t) == 7.0).all() for t in others)
+
+
+def test_entering_on_another_stream(fh):
+    # The context runs on its own stream, the batch's arrays are made on torch's.
+    import torch
+
+    m, _ = matrices(fh)
+    got = []
+    for own in (False, True):
+        ctx = fh.Context(0)
+        layer = fh.DecoderLayer(m["qkv"], m["wo"], m["w13"], m["w2"], to_dev(np.zeros(H, F32)), 40, ctx=ctx)
+        pages = fh.KvPages(6, 16, 2, 3, H, G, key_heads=H, ctx=ctx)
+        pages.map(1, 0, [4, 2, 5])
+        layer.prefix_k[:40] = to_dev(gen.normal((40, H, 64), 1.0, 21))
+        layer.v[:40] = to_dev(gen.normal((40, G, 64), 1.0, 22))
+        layer.len = layer.prefix_len = 40
+        torch.cuda.synchronize()
+        if own:
+            ctx.use_stream(None)
+        layer.enter_pages(pages, 1)
+        junk = [torch.full((n,), 1 << 28, dtype=torch.int32, device="cuda:0") for n in (2, 3, 2, 3)]
+        ctx.sync()
+        assert len(junk) == 4 and pages.refused() == []
+        ctx.use_stream(torch.cuda.current_stream())
+        got.append([host(t) for t in pages.dequantize(40, int32([-1, 0]), row_start=int32([0, 0, 40]))])
+        with pytest.raises(fh.FocrError) as e:
+            layer.enter_pages(fh.KvPages(6, 16, 2, 3, H, G, key_heads=H), 1)  # of another context
+        assert e.value.code == -1
+    for a, b in zip(*got):
+        assert_bitwise(a, b)

@@ -347,3 +347,14 @@ def test_refusals(fh):
     with pytest.raises(fh.FocrError) as e:
         lin.linear(x, 9)
     assert e.value.code == -2
+
+
+def test_channels_past_31_bits_are_refused(fh):
+    # Refused by its sizes alone, before any code is read.
+    import ctypes
+
+    codes, scales, out = np.zeros(1, np.int8), np.zeros(1, np.float32), ctypes.c_void_p()
+    ptr = lambda a: a.ctypes.data_as(ctypes.c_void_p)  # noqa: E731
+    rc = fh.lib().focr_linear_upload(fh.default_context().handle, 4, 2 ** 31 - 15, 1, 64, ptr(codes), ptr(scales), None,
+                                     None, 0, ctypes.byref(out))
+    assert rc == -2 and out.value is None

@@ -597,3 +597,26 @@ def test_refusals(fh):
     refused(-2, lambda: kv.dequantize(3, lens))
 
 
+
+
+def test_refusals_of_types(fh):
+    # A tensor of fewer bytes than its elements would take would be read past its end.
+    import torch
+
+    kv = fh.KvPages(4, 16, 2, 4)
+    x = lambda *shape: torch.zeros(shape, device="cuda:0")  # noqa: E731
+    lens = int32([0, 0])
+    calls = [lambda: kv.attention(x(2, 16, 64).half(), lens, 16),
+             lambda: kv.attention(x(2, 16, 64), lens, 16, sinks=x(16).bfloat16()),
+             lambda: kv.attention(x(2, 16, 64), lens, 16, out=x(2, 16, 64).half()),
+             lambda: kv.append(x(2, 8, 64).half(), x(2, 8, 64), lens),
+             lambda: kv.append(x(2, 8, 64), x(2, 8, 64).half(), lens),
+             lambda: kv.append(x(2, 8, 64), x(2, 8, 64), lens, row_start=x(3)),
+             lambda: kv.qkv_rows(x(2, 32 * 64).half(), x(2, 16, 32, 2), lens),
+             lambda: kv.qkv_rows(x(2, 32 * 64), x(2, 16, 32, 2).half(), lens),
+             lambda: kv.dequantize(2, lens.float())]
+    for call in calls:
+        with pytest.raises(fh.FocrError) as e:
+            call()
+        assert e.value.code == -2, str(e.value)
+    assert kv.refused() == []
