@@ -236,6 +236,10 @@ __device__ __forceinline__ void turn_bytes(uint32_t (&w)[4]) {
 // a query head. Lane (r, c): elements 4 c .. + 3 of the block's positions 4 r + s, s =
 // 0 .. 3, so that a load or store of FP32 rows is 1 KB, key codes go to memory as
 // they stand (256 bytes for each s) and a dim's codes of four positions are one word.
+// Bound: the rows and factors read, the queries written. 15,243 rows of four prompts
+// (16 query and key heads, 8 value heads) take 70 us for 250 MB read and 87 written,
+// 4.8 TB/s where a copy reaches 5.1; a row of each of 64 sequences 5.9 us, which is
+// the launch and three dependent trips to memory (batch, table, rows).
 template <bool QKV>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const Cache &c = a.c;
@@ -384,7 +388,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 }
 
 // ---- reading back --------------------------------------------------------------
-// A wave takes one block of a sequence's rows and one stored head.
+// A wave takes one block of a sequence's rows and one stored head. Bound by the FP32
+// rows written: 15,243 rows of 24 heads take 27 us (118 MB moved, 4.4 TB/s).
 __global__ __launch_bounds__(256) void read_kernel(Cache c, float *__restrict__ k, float *__restrict__ v) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = blockIdx.y * 4 + wave, stored = c.key_heads + c.kv_heads;
@@ -488,13 +493,20 @@ __device__ __forceinline__ float row_max(float v) {
 // product holds byte d of query q, column j of key tile t is key 4 j + t as its codes
 // stand: lane (j, q) gets the three exact sums of its four keys with its query,
 // and nothing is computed twice. Weights. exp2(s - m) times the block's value scale,
-// over the power of two above the largest such scale so far, rounded to 2^-30, as four
-// signed bytes (half a step a key: of its run's largest value, and a run is 4,096
-// keys at most, so together at most 2^-18, usually some 2^-25, of that): byte d of query q is column 4 d + q of the second product, whose
-// operands are the value codes as they stand (lane group g: block g) and these
-// bytes, turned through 1 KB of LDS. Its sums are exact integers too, and stay in
-// the accumulators while m and the power of two do; when one of them changes
-// they are added to FP32 ones, which are scaled.
+// over the power of two above the largest such scale so far, rounded to 2^-30, as
+// four signed bytes (half a step a key: of its run's largest value, and a run is 4,096
+// keys at most, so together at most 2^-18, usually some 2^-25, of that): byte d of
+// query q is column 4 d + q of the second product, whose operands are the value codes
+// as they stand (lane group g: block g) and these bytes, turned through 1 KB of LDS.
+// Its sums are exact integers too, and stay in the accumulators while m and the power
+// of two do; when one of them changes they are added to FP32 ones, which are scaled.
+//
+// Bound: the codes, read once. 64 sequences of up to 8,192 positions (346,572 in all,
+// 16 key and 8 value heads) take 102 us, 618 MB from memory at 6.1 TB/s; 535 MB
+// are needed, as two key heads' workgroups do not read all of their values together
+// (both in one workgroup: 549 MB, but 110 us, as fewer bytes are on their way). One
+// sequence of 131,072 takes 22 us (137 MB, 6.1 TB/s) and its merge 5; 101
+// positions take 5.5 us, the launch and four dependent trips to memory.
 struct Stage {
   v4i k[4], v[4];
   float k_scale, v_scale;
@@ -815,7 +827,8 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
 }
 
 // The parts of a sequence's rows of one head: as many of the waves for each row as
-// there are, lane = element, eight parts of a wave in flight.
+// there are, lane = element, eight parts of a wave in flight. Bound by the launch and
+// the trips to memory: 4.7 us for 7 parts of 25 rows as for 57 parts of two.
 template <int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttendArgs a) {
   const Cache &c = a.c;
@@ -1162,7 +1175,10 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
   FOCR_HIP_CHECK(hipGetLastError());
   if (a.parts > 1) {
     const dim3 each(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(n_seqs));
-    if (a.parts <= 16)
+    // Parts of all a sequence's rows (us a call with 4 / 16 waves: 26 parts of one row
+    // 10.2 / 11.2, 3 of one in 64 sequences 109 / 117; 57 of two 34.9 / 33.7, 59 of
+    // eight 37.7 / 28.5).
+    if (a.parts * most <= 64)
       hipLaunchKernelGGL(merge_kernel<4>, each, dim3(256), 0, ctx->stream, a);
     else
       hipLaunchKernelGGL(merge_kernel<16>, each, dim3(1024), 0, ctx->stream, a);

@@ -151,13 +151,13 @@ int focr_linear_dequantize(focr_ctx *ctx, const focr_linear *lin, float *out_dev
  * (src/kernels/mod.rs:407-432). x_dev [rows][in], out_dev [rows][out].
  * Bitwise equal to the reference's AVX2/NEON/portable dot_q / dot order.
  * Bits 4: the inputs of each block of 128 to 512 columns are taken to 2^-22 of
- * their largest magnitude, the products with the codes of 64 columns (32 for
- * group 32) are summed exactly, and these sums times their scales are added in
- * FP32 (the same for the two calls below); a row scale or norm multiplies the
- * finished sums; rows that hold an infinity or NaN are computed by FP32
- * multiply-adds. A large call (rows * in above 16,384, or rows that do not fit a
- * workgroup) keeps its inputs as bytes, 16 a column (32 for more than five
- * rows), in the context scratch. */
+ * their largest magnitude (2^-118 at the least), the products with the codes of
+ * 64 columns (32 for group 32) are summed exactly, and these sums times their
+ * scales are added in FP32 (the same for the two calls below); a row scale or
+ * norm multiplies the finished sums; rows that hold an infinity or NaN are
+ * computed by FP32 multiply-adds. A large call (rows * in above 16,384, or rows
+ * that do not fit a workgroup) keeps its inputs as bytes, 16 a column (32 for
+ * more than five rows), in the context scratch. */
 int focr_linear_decode(focr_ctx *ctx, const focr_linear *lin, const float *x_dev, size_t rows,
                        float *out_dev);
 /* QuantLinear::linear_glu / kernels::linear_glu_with_simd for 1..=8 rows
