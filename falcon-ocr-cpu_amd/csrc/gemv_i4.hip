@@ -238,26 +238,26 @@ constexpr int resident() {
 // NB: 16-column blocks of the product (Columns). SK: waves that share a tile's
 // columns, each W steps of a turn. G: columns per scale. PRE: the rows come as bytes
 // from rows4_kernel and pass through LDS turn by turn; otherwise the workgroup
-// writes all of them to LDS itself.
+// writes all of them to LDS itself. NW: waves of a workgroup.
 // Bound: the codes, read once. A wave's load is 1 KB, a tile's step, and W of them
 // with their scales are on their way while W others are used; a load under a branch,
 // or a spilled register, would make the wave wait for all of them. 24,576 x 8,192 in
 // groups of 64 take 24.6 us for eight rows (114 MB, 4.6 TB/s), 65,536 x 768 in groups
 // of 128 7.9 us for one (27 MB, 3.4 TB/s: a third of it is the launch and the rows);
 // 2,048 x 768 take 4.4 us, all launch, rows and one trip to memory.
-template <int NB, int SK, int W, int G, bool PRE>
-__global__ __launch_bounds__(64 * kWaves, (resident<NB, SK, W, G, PRE>())) void gemv4_kernel(Args a) {
+template <int NB, int SK, int W, int G, bool PRE, int NW>
+__global__ __launch_bounds__(64 * NW, (resident<NB, SK, W, G, PRE>())) void gemv4_kernel(Args a) {
   using C = Columns<NB>;
   constexpr int NS = kStep / G;             // scales of a channel per step
-  constexpr int SLOTS = kWaves / SK;        // tiles a workgroup has at once
+  constexpr int SLOTS = NW / SK;        // tiles a workgroup has at once
   constexpr int BLOCK = 2 * W * C::kGroup;  // bytes of a block
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int steps = a.steps, M = a.m, k = a.k;
   const int turns = (steps + W * SK - 1) / (W * SK);
   const int held = PRE ? 2 * SK : turns * SK;                          // blocks in LDS
   float *const weights = reinterpret_cast<float *>(lds + held * BLOCK);  // [held][columns]
-  float *const red = weights + held * C::kWide;                         // [kWaves][8][16]
-  float *const squares = red + kWaves * 8 * 16;                         // [8][SK]
+  float *const red = weights + held * C::kWide;                         // [NW][8][16]
+  float *const squares = red + NW * 8 * 16;                         // [8][SK]
   uint32_t *const bad = reinterpret_cast<uint32_t *>(squares + 8 * SK);  // [8]
   const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, kg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -283,14 +283,14 @@ __global__ __launch_bounds__(64 * kWaves, (resident<NB, SK, W, G, PRE>())) void 
   // PRE: a turn's bytes from memory to registers and on to LDS, and its weights to
   // registers.
   constexpr int PIECES = SK * BLOCK / 16;  // 16 bytes each
-  constexpr int PER = PRE ? (PIECES + 64 * kWaves - 1) / (64 * kWaves) : 1;
-  static_assert(!PRE || PIECES >= 64 * kWaves, "a piece for each thread");
+  constexpr int PER = PRE ? (PIECES + 64 * NW - 1) / (64 * NW) : 1;
+  static_assert(!PRE || PIECES >= 64 * NW, "a piece for each thread");
   v4u moved[PER];
   float weight[NB];
   // A thread with no piece left moves its last one again: no branch, no wait in one.
   auto piece_of = [&](int p) {
-    const int piece = tid + 64 * kWaves * p;
-    return piece < PIECES ? piece : piece - 64 * kWaves;
+    const int piece = tid + 64 * NW * p;
+    return piece < PIECES ? piece : piece - 64 * NW;
   };
   auto fetch = [&](int turn) {
 #pragma unroll
@@ -309,18 +309,18 @@ __global__ __launch_bounds__(64 * kWaves, (resident<NB, SK, W, G, PRE>())) void 
     fetch_weight(0);
 #pragma unroll
     for (int i = 0; i < W; i++) load(i, 0, 0);
-    // Wave r sums row r's squares and marks over its blocks.
-    if (wave < M) {
+    // A wave sums a row's squares and marks over its blocks.
+    for (int r = wave; r < M; r += NW) {
       float sum = 0.0f;
       uint32_t any = 0;
       for (int block = lane; block < a.blocks; block += 64) {
-        sum = sum + a.squares[wave * a.blocks + block];
-        any |= a.marks[wave * a.blocks + block];
+        sum = sum + a.squares[r * a.blocks + block];
+        any |= a.marks[r * a.blocks + block];
       }
       sum = wave_sum(sum);
       const bool found = __any(any != 0);
-      if (lane < SK) squares[wave * SK + lane] = lane == 0 ? sum : 0.0f;
-      if (lane == 0) bad[wave] = found;
+      if (lane < SK) squares[r * SK + lane] = lane == 0 ? sum : 0.0f;
+      if (lane == 0) bad[r] = found;
     }
     place(0);
     lds_barrier();
@@ -562,7 +562,7 @@ size_t lds_of(int nb, int sk, int w, size_t held) {
   return held * (2 * w * 64 * 16 * nb + 16 * nb * 4) + kWaves * 8 * 16 * 4 + 8 * sk * 4 + 8 * 4;
 }
 
-template <int NB, int SK, int W, int G, bool PRE>
+template <int NB, int SK, int W, int G, bool PRE, int NW = kWaves>
 int launch_one(Ctx *ctx, const Args &a) {
   if constexpr (PRE) {
     hipLaunchKernelGGL((rows4_kernel<NB, W>), dim3((a.blocks + 3) / 4, a.m), dim3(256), 0, ctx->stream, a);
@@ -572,13 +572,13 @@ int launch_one(Ctx *ctx, const Args &a) {
   FOCR_REQUIRE(lds <= kLdsBytes, FOCR_E_SHAPE, "GEMV: the rows of x exceed LDS");
   // Above 64 KB the kernel has to be allowed it, on each device.
   if (lds > 64 * 1024)
-    FOCR_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(gemv4_kernel<NB, SK, W, G, PRE>),
+    FOCR_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(gemv4_kernel<NB, SK, W, G, PRE, NW>),
                                        hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kLdsBytes)));
-  constexpr int slots = kWaves / SK;
+  constexpr int slots = NW / SK;
   const int want = (a.tiles_total + slots - 1) / slots;
   const int most = lds > kLdsBytes / 2 ? 256 : 512;  // workgroups that 256 compute units hold at once
   const int blocks = want < most ? want : most;
-  hipLaunchKernelGGL((gemv4_kernel<NB, SK, W, G, PRE>), dim3(blocks), dim3(64 * kWaves), lds, ctx->stream, a);
+  hipLaunchKernelGGL((gemv4_kernel<NB, SK, W, G, PRE, NW>), dim3(blocks), dim3(64 * NW), lds, ctx->stream, a);
   FOCR_HIP_CHECK(hipGetLastError());
   return FOCR_OK;
 }
@@ -608,8 +608,19 @@ int launch_pre(Ctx *ctx, Args a) {
   a.weights = reinterpret_cast<float *>(a.digits + digits);
   a.squares = a.weights + blocks * C::kWide;
   a.marks = reinterpret_cast<uint32_t *>(a.squares + 8 * blocks);
-  if constexpr (SK > 1)
+  if constexpr (SK > 1) {
     if (w == 3) return launch_one<NB, SK, 3, G, true>(ctx, a);
+  } else if constexpr (NB == 1) {
+    // The tiles of the busiest compute unit, with workgroups of eight tiles or of six
+    // (us with eight / six: 24,576 x 8,192 for five rows 30.3 / 27.5, 40,000 x 5,000
+    // for four 32.9 / 29.9; for more than five rows the products leave no gain, 32.9
+    // / 33.5).
+    auto busiest = [&](int nw) {
+      const int groups = (a.tiles_total + nw - 1) / nw;
+      return groups > 512 ? a.tiles_total : (groups + 255) / 256 * nw;
+    };
+    if (busiest(6) < busiest(8)) return launch_one<NB, SK, 4, G, true, 6>(ctx, a);
+  }
   return launch_one<NB, SK, 4, G, true>(ctx, a);
 }
 
