@@ -90,7 +90,7 @@ def test_decode_against_64_bits(fh, n, k, group):
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("n,k", [(20, 20000), (300, 8200), (1000, 4100), (9000, 2304), (33000, 2200)])
+@pytest.mark.parametrize("n,k", [(20, 20000), (300, 8200), (1000, 4100), (9000, 2304), (9000, 4100), (33000, 2200)])
 def test_decode_of_large_calls(fh, n, k, group):
     # Rows written as bytes by a kernel of their own, and passed through LDS in turns.
     codes, scales, _ = matrix(n, k, group, n + k)
@@ -101,6 +101,21 @@ def test_decode_of_large_calls(fh, n, k, group):
         x[:, k // 3] *= 50.0
         got = host(lin.linear(to_dev(x), rows))
         check(got, *product(x.astype(np.float64), w), f"n {n} k {k} group {group} rows {rows}")
+
+
+@pytest.mark.parametrize("n,k,group", [(16400, 3300, 32), (16400, 3300, 64), (16400, 3300, 128), (32768, 3300, 64)])
+def test_decode_of_large_calls_with_many_channels(fh, n, k, group):
+    # One wave a tile, in workgroups of six tiles and of eight.
+    codes, scales, _ = matrix(n, k, group, n + k)
+    lin = fh.QuantLinear.from_parts(n, k, group, codes, scales, bits=4)
+    x = gen.normal((5, k), 2.0, 5)
+    x[3, k // 3] = 40.0
+    want, bound = product(x.astype(np.float64), weights64(codes, scales, group))
+    check(host(lin.linear(to_dev(x), 5)), want, bound, f"n {n} k {k} group {group}")
+    h = gen.normal((5, n), 1.0, 6)
+    out = to_dev(h)
+    lin.linear_ex(to_dev(x), 5, epilogue=fh.Epilogue.ADD, out=out)
+    check(host(out), h + want, bound + EPS * (np.abs(h + want) + bound), f"ADD n {n} k {k} group {group}")
 
 
 @pytest.mark.parametrize("n,k,group", [(64, 96, 32), (2048, 768, 64), (1030, 1300, 128), (4608, 768, 64), (70, 4500, 64)])
