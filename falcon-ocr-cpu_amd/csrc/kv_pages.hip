@@ -153,6 +153,10 @@ struct AppendArgs {
   const float *qkv, *rope;  // QKV rows and factors, or
   const float *k, *v;       // ready keys [rows][key heads][64] and values [rows][KV heads][64]
   float *q;
+  // Workgroups go to the 8 XCDs in turn. Near: those of one unit's heads, which take
+  // the same factors and some the same keys, follow one another on the same one;
+  // otherwise all units of four heads do.
+  int near;
 };
 
 // The largest magnitude's bits in a wave, in every lane.
@@ -237,22 +241,23 @@ __device__ __forceinline__ void turn_bytes(uint32_t (&w)[4]) {
 // 0 .. 3, so that a load or store of FP32 rows is 1 KB, key codes go to memory as
 // they stand (256 bytes for each s) and a dim's codes of four positions are one word.
 // Bound: the rows and factors read, the queries written. 15,243 rows of four prompts
-// (16 query and key heads, 8 value heads) take 70 us for 250 MB read and 87 written,
-// 4.8 TB/s where a copy reaches 5.1; a row of each of 64 sequences 5.9 us, which is
+// (16 query and key heads, 8 value heads) take 62 us for 188 MB read and 87 written,
+// 4.4 TB/s where a copy reaches 5.1; a row of each of 64 sequences 5.9 us, which is
 // the launch and three dependent trips to memory (batch, table, rows).
 template <bool QKV>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, r4 = lane / 16 * 4, e4 = lane % 16 * 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.y * 4 + wave, stored = c.key_heads + c.kv_heads;
+  const int at_unit = a.near ? (blockIdx.z * gridDim.y + blockIdx.y) * 8 + blockIdx.x % 8 : blockIdx.x;
+  const int head = (a.near ? blockIdx.x / 8 : blockIdx.y) * 4 + wave, stored = c.key_heads + c.kv_heads;
   const auto of = [](int len, int n) {
     const int blocks = touched(len, n);
     return blocks <= 3 ? 1 : blocks - 2;
   };
   Unit unit;
-  const bool found = find_unit(c, blockIdx.x, of, unit);
-  if (blockIdx.x == 0 && head == 0 && c.row_start) {
+  const bool found = find_unit(c, at_unit, of, unit);
+  if (at_unit == 0 && head == 0 && c.row_start) {
     // Marks every refused sequence.
     Unit none;
     find_unit(c, 0x7fffffff, of, none);
@@ -960,14 +965,23 @@ int check_batch(const char *name, const Ctx *ctx, const Pages *kv, size_t rows, 
   return FOCR_OK;
 }
 
-int launch_append(Ctx *ctx, const AppendArgs &a, bool qkv) {
+int launch_append(Ctx *ctx, AppendArgs a, bool qkv) {
   const Cache &c = a.c;
   // Units: n rows touch at most (n + 14) / 16 + 1 blocks, three of which are one
   // unit, so at most n / 16 units, or one.
   const int units = c.row_start ? c.rows / kBlock + (c.rows < c.n_seqs ? c.rows : c.n_seqs) : c.n_seqs;
   const int heads = c.key_heads + c.kv_heads + (qkv ? c.n_heads : 0);
   FOCR_HIP_CHECK(hipSetDevice(ctx->device));
-  const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>((heads + 3) / 4));
+  const unsigned groups = static_cast<unsigned>((heads + 3) / 4);
+  // Long prompts are near (us a call with its reading back, near / not: four of up to
+  // 6,544 rows 89 / 104, one of 1,500 17.5 / 18.7; sixteen of up to 300 23.7 / 22.8, 200
+  // of up to five 26.4 / 25.5: a sequence's first unit has three blocks' work).
+  a.near = c.rows / c.n_seqs >= 1024;
+  dim3 grid(static_cast<unsigned>(units), groups);
+  if (a.near) {
+    const unsigned eights = static_cast<unsigned>((units + 7) / 8), y = std::min(eights, 32768u);
+    grid = dim3(8 * groups, y, (eights + y - 1) / y);
+  }
   if (qkv)
     hipLaunchKernelGGL(append_kernel<true>, grid, dim3(256), 0, ctx->stream, a);
   else

@@ -184,6 +184,36 @@ def test_row_step_is_the_two_calls(fh, heads, kv_heads, key_heads):
         assert_bitwise(host(a), host(b))
 
 
+@pytest.mark.parametrize("heads,kv_heads,key_heads", HEADS)
+@pytest.mark.parametrize("counts,before", [([1500], [5]), ([1400, 0, 2, 3000], [0, 40, 33, 17])])
+def test_long_prompts_are_their_parts(fh, heads, kv_heads, key_heads, counts, before):
+    # A thousand rows a sequence and more in one call, or as many calls as it takes of up to 300.
+    totals = [a + b for a, b in zip(counts, before)]
+    rows, n = sum(counts), len(counts)
+    qkv = to_dev(gen.normal((rows, (heads + 2 * kv_heads) * 64), 1.0, 61))
+    angle = gen.uniform((rows, heads, 32), -9.0, 9.0, 62)
+    rope = to_dev(np.stack([np.cos(angle), np.sin(angle)], axis=-1).astype(F32))
+    one, two = (make(fh, totals, 64, heads, kv_heads, key_heads, seed=s) for s in (1, 2))
+    k0, v0 = cat(rows_of(before, key_heads, 63)), cat(rows_of(before, kv_heads, 64))
+    zero = int32([0] * n)
+    for kv in (one, two):
+        kv.append(k0, v0, zero, row_start=starts(before))
+    q = host(one.qkv_rows(qkv, rope, int32(before), row_start=starts(counts)))
+    first = np.cumsum([0] + counts)
+    for i in range(n):
+        for at in range(0, counts[i], 300):
+            size = min(300, counts[i] - at)
+            lens, row_start = [-1] * n, [0] * (i + 1) + [size] * (n - i)
+            lens[i] = before[i] + at
+            here = slice(first[i] + at, first[i] + at + size)
+            part = two.qkv_rows(qkv[here].contiguous(), rope[here].contiguous(), int32(lens), row_start=int32(row_start))
+            assert_bitwise(q[here], host(part), f"queries of sequence {i} from {at}")
+    for a, b in zip(one.dequantize(sum(totals), zero, row_start=starts(totals)),
+                    two.dequantize(sum(totals), zero, row_start=starts(totals))):
+        assert_bitwise(host(a), host(b))
+    assert one.refused() == [] and two.refused() == []
+
+
 def attention64(q, k, v, first, sinks):
     """64-bit attention of rows [n][H][64] at positions first.. over decoded keys and
     values, and how far FP32's may be from it.
