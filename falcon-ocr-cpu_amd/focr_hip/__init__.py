@@ -675,7 +675,7 @@ class KvPages:
         self.n_pages, self.page_size, self.n_seqs, self.seq_pages = n_pages, page_size, n_seqs, seq_pages
         self.n_heads, self.n_kv_heads = n_heads, n_kv_heads
         self.key_heads = n_kv_heads if key_heads is None else key_heads
-        self._types = _torch().float32, _torch().int32
+        self._float, self._int, self._device = _torch().float32, _torch().int32, self.ctx.device
         handle = ctypes.c_void_p()
         _check(lib().focr_kv_pages_create(self.ctx.handle, n_pages, page_size, n_seqs, seq_pages, n_heads,
                                           self.key_heads, n_kv_heads, 64, ctypes.byref(handle)))
@@ -689,31 +689,36 @@ class KvPages:
         _check(lib().focr_kv_pages_map(self.ctx.handle, self.handle, seq, first, len(ids),
                                        ids.ctypes.data_as(ctypes.c_void_p)))
 
-    def _ptr(self, t, kind: int = 0):
-        """Device pointer of a contiguous tensor on the cache's device: float32, or (kind 1) int32."""
-        if t is None:
-            return None
-        if t.get_device() != self.ctx.device:
-            raise FocrError(-1, "expected a CUDA tensor on the cache's device")
-        if t.dtype != self._types[kind]:
-            raise FocrError(-2, f"expected {self._types[kind]}, not {t.dtype}")
-        if not t.is_contiguous():
-            raise FocrError(-2, "expected a contiguous tensor")
-        return t.data_ptr()
+    def _ptr(self, t):
+        """Device pointer of a contiguous float32 tensor on the cache's device."""
+        if t is None or (t.dtype is self._float and t.get_device() == self._device and t.is_contiguous()):
+            return None if t is None else t.data_ptr()
+        raise self._misfit(t, self._float)
+
+    def _misfit(self, t, dtype) -> FocrError:
+        if t.get_device() != self._device:
+            return FocrError(-1, "expected a CUDA tensor on the cache's device")
+        return FocrError(-2, "expected a contiguous tensor" if t.dtype is dtype else f"expected {dtype}, not {t.dtype}")
 
     def _batch(self, lens, row_start):
         seqs = lens.numel()
-        if row_start is not None and row_start.numel() != seqs + 1:
+        if not (lens.dtype is self._int and lens.get_device() == self._device and lens.is_contiguous()):
+            raise self._misfit(lens, self._int)
+        if row_start is None:
+            return None, lens.data_ptr(), seqs
+        if row_start.numel() != seqs + 1:
             raise FocrError(-2, "row_start has a value more than lens")
-        return self._ptr(row_start, 1), self._ptr(lens, 1), seqs
+        if not (row_start.dtype is self._int and row_start.get_device() == self._device and row_start.is_contiguous()):
+            raise self._misfit(row_start, self._int)
+        return row_start.data_ptr(), lens.data_ptr(), seqs
 
     def append(self, k, v, lens, row_start=None) -> None:
         """Keys [rows][key_heads][64] and values [rows][n_kv_heads][64] at the batch's positions."""
         rows = v.numel() // (self.n_kv_heads * 64)
         if k.numel() != rows * self.key_heads * 64 or v.numel() != rows * self.n_kv_heads * 64:
             raise FocrError(-2, "keys [rows][key_heads][64] and values [rows][n_kv_heads][64]")
-        _check(lib().focr_kv_pages_append(self.ctx.handle, self.handle, self._ptr(k), self._ptr(v), rows,
-                                          *self._batch(lens, row_start)))
+        start, lens, seqs = self._batch(lens, row_start)
+        _check(lib().focr_kv_pages_append(self.ctx.handle, self.handle, self._ptr(k), self._ptr(v), rows, start, lens, seqs))
 
     def qkv_rows(self, qkv, rope, lens, row_start=None, q=None):
         """`qkv_rows` with its keys and values appended: queries [rows][n_heads][64]."""
@@ -723,10 +728,14 @@ class KvPages:
             raise FocrError(-2, "QKV rows [rows][qdim + 2 kdim] and factors [rows][n_heads][32][2]")
         if q is None:
             q = qkv.new_empty((rows, self.n_heads, 64))
+            to = q.data_ptr()
         elif q.numel() != rows * width:
             raise FocrError(-2, "queries [rows][n_heads][64]")
+        else:
+            to = self._ptr(q)
+        start, lens, seqs = self._batch(lens, row_start)
         _check(lib().focr_kv_pages_qkv_rows(self.ctx.handle, self.handle, self._ptr(qkv), rows, self._ptr(rope),
-                                            *self._batch(lens, row_start), self._ptr(q)))
+                                            start, lens, seqs, to))
         return q
 
     def attention(self, q, lens, max_len: int, row_start=None, sinks=None, out=None):
@@ -739,19 +748,23 @@ class KvPages:
             raise FocrError(-2, "max_len is positive")
         if out is None:
             out = q.new_empty((rows, self.n_heads, 64))
+            to = out.data_ptr()
         elif out.numel() != q.numel():
             raise FocrError(-2, "outputs [rows][n_heads][64]")
-        _check(lib().focr_kv_pages_attention(self.ctx.handle, self.handle, self._ptr(q), rows,
-                                             *self._batch(lens, row_start), max_len, self._ptr(sinks), self._ptr(out)))
+        else:
+            to = self._ptr(out)
+        start, lens, seqs = self._batch(lens, row_start)
+        _check(lib().focr_kv_pages_attention(self.ctx.handle, self.handle, self._ptr(q), rows, start, lens, seqs, max_len,
+                                             self._ptr(sinks), to))
         return out
 
     def dequantize(self, rows: int, lens, row_start=None):
         """What the cache holds at the batch's positions: keys [rows][key_heads][64], values [rows][n_kv_heads][64]."""
-        torch = _torch()
-        k = lens.new_empty((rows, self.key_heads, 64), dtype=torch.float32)
-        v = lens.new_empty((rows, self.n_kv_heads, 64), dtype=torch.float32)
-        _check(lib().focr_kv_pages_dequantize(self.ctx.handle, self.handle, rows, *self._batch(lens, row_start),
-                                              self._ptr(k), self._ptr(v)))
+        k = lens.new_empty((rows, self.key_heads, 64), dtype=self._float)
+        v = lens.new_empty((rows, self.n_kv_heads, 64), dtype=self._float)
+        start, lens, seqs = self._batch(lens, row_start)
+        _check(lib().focr_kv_pages_dequantize(self.ctx.handle, self.handle, rows, start, lens, seqs, k.data_ptr(),
+                                              v.data_ptr()))
         return k, v
 
     def refused(self):
