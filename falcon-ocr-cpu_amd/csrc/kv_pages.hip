@@ -55,7 +55,7 @@ struct Cache {
   const int32_t *table;
   float *open;
   int32_t *tags, *refused;
-  int shift, seq_pages, n_pages, n_heads, key_heads, kv_heads;
+  int shift, seq_pages, n_heads, key_heads, kv_heads;
   const int32_t *row_start, *lens;  // row_start null: row r is sequence r's
   int rows, n_seqs;
 
@@ -942,7 +942,6 @@ Cache cache_of(const Pages *kv, size_t rows, const int32_t *row_start, const int
   c.refused = kv->refused;
   c.shift = kv->shift;
   c.seq_pages = static_cast<int>(kv->seq_pages);
-  c.n_pages = static_cast<int>(kv->n_pages);
   c.n_heads = static_cast<int>(kv->n_heads);
   c.key_heads = static_cast<int>(kv->key_heads);
   c.kv_heads = static_cast<int>(kv->kv_heads);
