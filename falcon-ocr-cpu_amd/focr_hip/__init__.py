@@ -683,9 +683,12 @@ class KvPages:
 
     def map(self, seq: int, first: int, pages) -> None:
         """Pages (numbers, -1: none) of the sequence from its page `first` on."""
-        ids = np.ascontiguousarray(pages, dtype=np.int32)
+        ids = np.asarray(pages)
         if ids.ndim != 1 or seq < 0 or first < 0:
             raise FocrError(-2, "pages of a sequence: a list from page `first` on")
+        if ids.size and (ids.dtype.kind not in "iu" or ids.min() < -1 or ids.max() >= self.n_pages):
+            raise FocrError(-5, "no such page")
+        ids = np.ascontiguousarray(ids, dtype=np.int32)
         _check(lib().focr_kv_pages_map(self.ctx.handle, self.handle, seq, first, len(ids),
                                        ids.ctypes.data_as(ctypes.c_void_p)))
 

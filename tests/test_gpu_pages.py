@@ -650,3 +650,13 @@ def test_refusals_of_types(fh):
             call()
         assert e.value.code == -2, str(e.value)
     assert kv.refused() == []
+
+
+def test_page_numbers_are_not_cut_to_32_bits(fh):
+    kv = fh.KvPages(4, 16, 2, 4)
+    for bad in (np.array([2 ** 32 + 1]), np.array([1.5]), [2 ** 40]):
+        with pytest.raises(fh.FocrError) as e:
+            kv.map(0, 0, bad)
+        assert e.value.code == -5
+    kv.map(0, 0, [])
+    kv.map(0, 1, np.array([3, -1, 0], dtype=np.int64))
