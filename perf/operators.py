@@ -13,7 +13,6 @@ a KV head rotate differently, for each query head (``keys`` 16).
 
 With ``own`` false ``run`` is made of elementary torch operations; with it true it makes the framework's calls.
 """
-import functools
 import math
 import random
 import sys
@@ -27,7 +26,6 @@ own = False
 HEAD, BLOCK = 64, 16
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
     path = str(Path(__file__).resolve().parents[1] / "falcon-ocr-cpu_amd")
     if path not in sys.path:
