@@ -238,18 +238,29 @@ class Linear:
     4-bit codes come as int8 in -8..7, one an element; the device holds two a byte."""
 
     def __init__(self, bits, codes, scales, group, exc_cols=None, exc_vals=None, ctx: Optional[Context] = None):
-        self.ctx = ctx or default_context()
         codes = np.ascontiguousarray(codes)
+        if bits not in (4, 8, 16, 32) or codes.ndim != 2:
+            raise FocrError(-1, "a matrix [out][in] of 4, 8, 16 or 32 bits")
         n, k = codes.shape
         dtype = {4: np.int8, 8: np.int8, 16: np.int16, 32: np.float32}[bits]
-        codes = codes.astype(dtype, copy=False)
+        given, codes = codes, codes.astype(dtype, copy=False)
+        if bits != 32 and given.dtype != dtype and not np.array_equal(codes, given):
+            raise FocrError(-5, f"codes outside {np.dtype(dtype).name}")
         sc = None if scales is None else np.ascontiguousarray(scales, dtype=np.float32)
+        # The upload reads a scale for each group of the rows; it refuses other groups.
+        if sc is not None and group in (32, 64, 128) and bits != 32:
+            groups = -(-k // group)
+            if sc.shape not in ((n, groups), (n * groups,)):
+                raise FocrError(-2, "scales [out][ceil(in / group)]")
         cols = vals = None
         n_exc = 0
         if exc_cols is not None and len(exc_cols):
             cols = np.ascontiguousarray(exc_cols, dtype=np.int32)
             vals = np.ascontiguousarray(exc_vals, dtype=np.float32)
             n_exc = len(cols)
+            if cols.ndim != 1 or vals.shape not in ((n, n_exc), (n * n_exc,)):
+                raise FocrError(-2, "exception columns [n_exc] and their weights [out][n_exc]")
+        self.ctx = ctx or default_context()
         handle = ctypes.c_void_p()
         ptr = lambda a: None if a is None else a.ctypes.data_as(ctypes.c_void_p)
         _check(lib().focr_linear_upload(self.ctx.handle, bits, n, k, group if bits != 32 else 0, ptr(codes), ptr(sc),
