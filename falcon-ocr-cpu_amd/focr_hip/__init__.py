@@ -150,12 +150,14 @@ def _torch():
     return torch
 
 
-def _dev(t) -> Optional[int]:
-    """Device pointer of a CUDA tensor (None passes NULL)."""
+def _dev(t, device: Optional[int] = None) -> Optional[int]:
+    """Device pointer of a contiguous float32 CUDA tensor, on `device` if that is given (None passes NULL)."""
     if t is None:
         return None
-    if not t.is_cuda:
-        raise FocrError(-1, "expected a CUDA tensor")
+    if not t.is_cuda or (device is not None and t.get_device() != device):
+        raise FocrError(-1, "expected a CUDA tensor" if device is None else f"expected a CUDA tensor on device {device}")
+    if t.dtype is not _torch().float32:
+        raise FocrError(-2, f"expected float32, not {t.dtype}")
     if not t.is_contiguous():
         raise FocrError(-2, "expected a contiguous tensor")
     return t.data_ptr()
@@ -295,10 +297,16 @@ class Linear:
             pass
 
     # -- operators ---------------------------------------------------------
+    def _dev(self, t, count: Optional[int] = None) -> Optional[int]:
+        """`_dev` on the matrix's device, for a tensor of `count` elements."""
+        if t is not None and count is not None and t.numel() != count:
+            raise FocrError(-2, f"expected {count} elements, not {t.numel()}")
+        return _dev(t, self.ctx.device)
+
     def dequantize(self):
         torch = _torch()
         out = torch.empty((self.out_dim, self.in_dim), dtype=torch.float32, device=f"cuda:{self.ctx.device}")
-        _check(lib().focr_linear_dequantize(self.ctx.handle, self.handle, _dev(out)))
+        _check(lib().focr_linear_dequantize(self.ctx.handle, self.handle, self._dev(out)))
         return out
 
     def linear(self, input, rows: int, output=None):
@@ -310,7 +318,7 @@ class Linear:
             output = torch.empty((rows, self.out_dim), dtype=torch.float32, device=input.device)
         elif output.numel() != rows * self.out_dim:
             raise FocrError(-2, "W8 output shape")
-        _check(lib().focr_linear_decode(self.ctx.handle, self.handle, _dev(input), rows, _dev(output)))
+        _check(lib().focr_linear_decode(self.ctx.handle, self.handle, self._dev(input), rows, self._dev(output)))
         return output
 
     def linear_glu(self, input, rows: int, gated=None):
@@ -320,7 +328,8 @@ class Linear:
             raise FocrError(-2, "W8 input shape")
         if gated is None:
             gated = torch.empty((rows, self.out_dim // 2), dtype=torch.float32, device=input.device)
-        _check(lib().focr_linear_decode_glu(self.ctx.handle, self.handle, _dev(input), rows, _dev(gated)))
+        _check(lib().focr_linear_decode_glu(self.ctx.handle, self.handle, self._dev(input), rows,
+                                            self._dev(gated, rows * (self.out_dim // 2))))
         return gated
 
     def linear_ex(self, input, rows: int, row_scale=None, epilogue: Epilogue = Epilogue.STORE, out=None,
@@ -340,8 +349,9 @@ class Linear:
             out = torch.empty((rows, width), dtype=torch.float32, device=input.device)
         elif out.numel() != rows * width:
             raise FocrError(-2, "W8 output shape")
-        _check(lib().focr_linear_decode_ex(self.ctx.handle, self.handle, _dev(input), rows, _dev(row_scale),
-                                           int(bool(rms_norm)), int(epilogue), _dev(out)))
+        _check(lib().focr_linear_decode_ex(self.ctx.handle, self.handle, self._dev(input), rows,
+                                           self._dev(row_scale, rows), int(bool(rms_norm)), int(epilogue),
+                                           self._dev(out)))
         return out
 
     def prefill(self, input, rows: int, row_scale=None, epilogue: Epilogue = Epilogue.STORE, out=None,
@@ -357,8 +367,8 @@ class Linear:
             if epilogue == Epilogue.ADD:
                 raise FocrError(-1, "Epilogue.ADD needs the residual `out`")
             out = torch.empty((rows, width), dtype=torch.float32, device=input.device)
-        _check(lib().focr_linear_prefill(self.ctx.handle, self.handle, _dev(input), rows, _dev(row_scale),
-                                         int(epilogue), int(kernel), _dev(out)))
+        _check(lib().focr_linear_prefill(self.ctx.handle, self.handle, self._dev(input), rows, self._dev(row_scale, rows),
+                                         int(epilogue), int(kernel), self._dev(out, rows * width)))
         return out
 
 

@@ -286,6 +286,7 @@ class DecoderLayer:
         rows = h.shape[0]
         if h.shape[1:] != (self.dim,):
             raise FocrError(-2, "h [rows][dim]")
+        pages._ptr(h)  # a contiguous float32 tensor on the layer's device
         if rows == 0:
             return h
         ctx, panel = self.ctx, rows > 8

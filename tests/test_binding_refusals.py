@@ -1,7 +1,10 @@
-"""What the binding refuses before the library sees it, without a GPU: arrays
-of fewer bytes than the call would read."""
+"""What the binding refuses before the library sees it, without a GPU: arrays and
+tensors of fewer bytes than the call would read or write."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
+import torch
 
 import focr_hip
 
@@ -49,3 +52,56 @@ def test_codes_are_not_cut(bits, bad):
 def test_other_matrices():
     refused(-1, lambda: focr_hip.Linear(5, codes(), np.ones((32, 3), F32), 64))
     refused(-1, lambda: focr_hip.Linear(8, codes()[0], np.ones((32, 3), F32), 64))
+
+
+def cuda(*shape, dtype=torch.float32, device=0, contiguous=True):
+    """Stands in for a CUDA tensor."""
+    return SimpleNamespace(is_cuda=True, dtype=dtype, get_device=lambda: device, is_contiguous=lambda: contiguous,
+                           data_ptr=lambda: 4096, numel=lambda: int(np.prod(shape)), shape=torch.Size(shape), device="meta")
+
+
+def test_tensors_of_other_types_and_devices():
+    dev = focr_hip._dev
+    assert dev(cuda(4)) == 4096 and dev(cuda(4), 0) == 4096 and dev(None) is None
+    for dtype in (torch.float16, torch.bfloat16, torch.float64, torch.int32):
+        refused(-2, lambda: dev(cuda(4, dtype=dtype)))
+    refused(-2, lambda: dev(cuda(4, contiguous=False)))
+    refused(-1, lambda: dev(cuda(4, device=1), 0))
+    refused(-1, lambda: dev(torch.zeros(4)))
+
+
+def test_projections_refuse_what_they_would_read_or_write_past():
+    lin = object.__new__(focr_hip.Linear)
+    lin.ctx, lin.handle = SimpleNamespace(handle=None, device=0), None
+    lin.out_dim, lin.in_dim = 32, 64
+    x = cuda(2, 64)
+    add = focr_hip.Epilogue.ADD
+    for bad in (dict(dtype=torch.float16), dict(dtype=torch.bfloat16)):
+        half = cuda(2, 64, **bad)
+        for call in (lambda: lin.linear(half, 2, output=cuda(2, 32)), lambda: lin.linear(x, 2, output=cuda(2, 32, **bad)),
+                     lambda: lin.linear_glu(half, 2, gated=cuda(2, 16)), lambda: lin.linear_glu(x, 2, gated=cuda(2, 16, **bad)),
+                     lambda: lin.linear_ex(half, 2, out=cuda(2, 32)),
+                     lambda: lin.linear_ex(x, 2, epilogue=add, out=cuda(2, 32, **bad)),
+                     lambda: lin.linear_ex(x, 2, row_scale=cuda(2, **bad), out=cuda(2, 32)),
+                     lambda: lin.prefill(half, 2, out=cuda(2, 32)),
+                     lambda: lin.prefill(x, 2, epilogue=add, out=cuda(2, 32, **bad)),
+                     lambda: focr_hip.row_scales(half, 64, out=cuda(2), ctx=lin.ctx)):
+            refused(-2, call)
+    for call in (lambda: lin.linear_glu(x, 2, gated=cuda(2, 15)), lambda: lin.linear_ex(x, 2, row_scale=cuda(1), out=cuda(2, 32)),
+                 lambda: lin.prefill(x, 2, row_scale=cuda(1), out=cuda(2, 32)), lambda: lin.prefill(x, 2, out=cuda(1, 32))):
+        refused(-2, call)
+    for call in (lambda: lin.linear_ex(cuda(2, 64, device=1), 2, out=cuda(2, 32)),
+                 lambda: lin.prefill(x, 2, epilogue=add, out=cuda(2, 32, device=1))):
+        refused(-1, call)
+
+
+def test_steps_refuse_other_hidden_states():
+    layer, pages, ctx = object.__new__(focr_hip.DecoderLayer), object.__new__(focr_hip.KvPages), SimpleNamespace(handle=None, device=0)
+    layer.ctx = pages.ctx = ctx
+    layer.n_heads = pages.n_heads = 16
+    layer.n_kv_heads = pages.n_kv_heads = 8
+    layer.dim, pages.handle = 64, None
+    pages._float, pages._int, pages._device = torch.float32, torch.int32, 0
+    for code, h in ((-2, cuda(2, 64, dtype=torch.float16)), (-2, cuda(2, 64, dtype=torch.bfloat16)),
+                    (-2, cuda(2, 64, contiguous=False)), (-1, cuda(2, 64, device=1)), (-2, cuda(2, 63))):
+        refused(code, lambda: layer.decode_pages(h, None, pages, None, 16))
