@@ -150,14 +150,20 @@ def _torch():
     return torch
 
 
+_float32 = None  # torch's, which is not imported with the package
+
+
 def _dev(t, device: Optional[int] = None) -> Optional[int]:
     """Device pointer of a contiguous float32 CUDA tensor, on `device` if that is given (None passes NULL)."""
+    global _float32
     if t is None:
         return None
-    if not t.is_cuda or (device is not None and t.get_device() != device):
+    if not (t.is_cuda if device is None else t.get_device() == device):
         raise FocrError(-1, "expected a CUDA tensor" if device is None else f"expected a CUDA tensor on device {device}")
-    if t.dtype is not _torch().float32:
-        raise FocrError(-2, f"expected float32, not {t.dtype}")
+    if t.dtype is not _float32:
+        _float32 = _torch().float32
+        if t.dtype is not _float32:
+            raise FocrError(-2, f"expected float32, not {t.dtype}")
     if not t.is_contiguous():
         raise FocrError(-2, "expected a contiguous tensor")
     return t.data_ptr()
@@ -299,7 +305,9 @@ class Linear:
     # -- operators ---------------------------------------------------------
     def _dev(self, t, count: Optional[int] = None) -> Optional[int]:
         """`_dev` on the matrix's device, for a tensor of `count` elements."""
-        if t is not None and count is not None and t.numel() != count:
+        if t is None:
+            return None
+        if count is not None and t.numel() != count:
             raise FocrError(-2, f"expected {count} elements, not {t.numel()}")
         return _dev(t, self.ctx.device)
 
