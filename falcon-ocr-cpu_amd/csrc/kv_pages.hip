@@ -34,6 +34,7 @@ constexpr int kBlock = 16, kBlockBytes = kBlock * 64;
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 struct Pages {
   int device = 0, shift = 0;  // log2 of the blocks of a page
@@ -497,14 +498,16 @@ __device__ __forceinline__ float row_max(float v) {
 // its largest element, so to 2^-22 of it). Row 4 q + d of the INT8 matrix
 // product holds byte d of query q, column j of key tile t is key 4 j + t as its codes
 // stand: lane (j, q) gets the three exact sums of its four keys with its query,
-// and nothing is computed twice. Weights. exp2(s - m) times the block's value scale,
-// over the power of two above the largest such scale so far, rounded to 2^-30, as
-// four signed bytes (half a step a key: of its run's largest value, and a run is 4,096
-// keys at most, so together at most 2^-18, usually some 2^-25, of that): byte d of
-// query q is column 4 d + q of the second product, whose operands are the value codes
-// as they stand (lane group g: block g) and these bytes, turned through 1 KB of LDS.
-// Its sums are exact integers too, and stay in the accumulators while m and the power
-// of two do; when one of them changes they are added to FP32 ones, which are scaled.
+// and nothing is computed twice. Weights. w = exp2(s - m) times the block's value
+// scale in FP32, over the power of two above the largest such scale so far and times
+// 2^64 (so that weights 2^-174 below that keep all their bits), is the sum of three
+// BF16 numbers, its own bits eight at a time: part d of query q is column 4 d + q of
+// the second product, whose operands are the value codes as BF16 numbers (exact) and
+// these parts, turned through LDS. So every product is exact, whatever the
+// magnitudes of the other keys' weights and values, and sums round as FP32's do; a
+// weight on one scale for a run's keys (integers) would lose those far below the
+// largest. The sums stay in the accumulators, which are scaled when m or the power of
+// two changes.
 //
 // Bound: the codes, read once. 64 sequences of up to 8,192 positions (346,572 in all,
 // 16 key and 8 value heads) take 102 us, 618 MB from memory at 6.1 TB/s; 535 MB
@@ -665,21 +668,19 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   const float ninf = -__builtin_inff();
   float m = ninf, den = 0.0f;
   int power = -300;  // 2^power above every block scale of the values so far
-  v4i sums[4];
   v4f acc[4];
 #pragma unroll
-  for (int d = 0; d < 4; d++) {
-    sums[d] = v4i{0, 0, 0, 0};
-    acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  // The bytes of the weights: [column 4 d + q][64 keys], a wave's own.
-  __shared__ __attribute__((aligned(16))) char turned[4][16 * 64];
-  char *const turn_to = turned[wave] + g * 64 + 4 * l16;
-  const char *const turn_from = turned[wave] + l16 * 64 + 16 * g;
+  for (int d = 0; d < 4; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  // The parts of the weights: [column 4 d + q][64 keys], a wave's own. Rows of 72, so
+  // that 16 columns' 16 bytes lie in different banks; there is no fourth part.
+  constexpr int kTurned = 72;
+  __shared__ __attribute__((aligned(16))) uint16_t turned[4][16 * kTurned];
+  uint16_t *const turn_to = turned[wave] + g * kTurned + 4 * l16;
+  const uint16_t *const turn_from = turned[wave] + l16 * kTurned + 16 * g;
+  *reinterpret_cast<uint2 *>(turn_to + 12 * kTurned) = make_uint2(0, 0);
 
-  // The integer sums to the FP32 ones, times `scaled` of query g: column 4 d + q's
-  // lanes take that of query q.
-  auto flush = [&](float scaled) {
+  // The sums times `scaled` of query g: column 4 d + q's lanes take that of query q.
+  auto rescale = [&](float scaled) {
     const float s0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 0));
     const float s1 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 16));
     const float s2 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 32));
@@ -688,17 +689,34 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
 #pragma unroll
     for (int d = 0; d < 4; d++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        acc[d][i] = (acc[d][i] + static_cast<float>(sums[d][i])) * f;
-        sums[d][i] = 0;
-      }
+      for (int i = 0; i < 4; i++) acc[d][i] = acc[d][i] * f;
   };
 
-  auto consume = [&](const Stage &s, int key0, bool overflow) {
+  // Two FP32 numbers' upper halves, the first one's low.
+  auto upper = [](uint32_t second, uint32_t first) { return __builtin_amdgcn_perm(second, first, 0x07060302u); };
+  auto as_bf = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const v4i words = {static_cast<int>(a), static_cast<int>(b), static_cast<int>(c), static_cast<int>(d)};
+    return __builtin_bit_cast(v8bf, words);
+  };
+  // Eight codes as BF16 numbers.
+  auto codes_of = [&](int first, int second) {
+    const uint32_t w[2] = {static_cast<uint32_t>(first), static_cast<uint32_t>(second)};
+    uint32_t to[4];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      to[2 * i] = upper(__float_as_uint(sdwa_cvt<1>(w[i])), __float_as_uint(sdwa_cvt<0>(w[i])));
+      to[2 * i + 1] = upper(__float_as_uint(sdwa_cvt<3>(w[i])), __float_as_uint(sdwa_cvt<2>(w[i])));
+    }
+    return as_bf(to[0], to[1], to[2], to[3]);
+  };
+
+  auto consume = [&](const Stage &s, int key0) {
     // Blocks that hold none of the sequence's positions do not count; NaN reaches a
-    // row by its scores, as integers have none for the weights.
-    const float v_scale = key0 / kBlock + l16 / 4 <= last_block ? s.v_scale : 0.0f;
-    const float k_scale = s.none || v_scale != v_scale ? __builtin_nanf("") : s.k_scale;
+    // row by its scores, which are those of the keys it sees.
+    float v_scale = key0 / kBlock + l16 / 4 <= last_block ? s.v_scale : 0.0f;
+    const bool bad = v_scale != v_scale;
+    const float k_scale = s.none || bad ? __builtin_nanf("") : s.k_scale;
+    v_scale = bad ? 0.0f : v_scale;
     // The largest value scale of the four blocks (lanes 4 b .. + 3 of a row).
     float widest = __builtin_fmaxf(v_scale, row_ror<4>(v_scale));
     widest = __builtin_fmaxf(widest, row_ror<8>(widest));
@@ -706,7 +724,7 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
     const int lower = power - above;
     power = above;
-    const float weight = __builtin_ldexpf(v_scale, 30 - power);
+    const float weight = __builtin_ldexpf(v_scale, 64 - power);
     float p[4];
     const float factor = q_factor * k_scale;
 #pragma unroll
@@ -720,44 +738,47 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     float top = __builtin_fmaxf(__builtin_fmaxf(p[0], p[1]), __builtin_fmaxf(p[2], p[3]));
     top = __builtin_fmaxf(m, row_max(top));
     const float from = top == ninf ? 0.0f : top;
-    if (__any(top > m) || lower < 0 || overflow) {
+    if (__any(top > m) || lower < 0) {
       const float keep = __builtin_amdgcn_exp2f(m - from);
       den = den * keep;
-      flush(__builtin_ldexpf(keep, lower));
+      rescale(__builtin_ldexpf(keep, lower));
       m = top;
     }
-    uint32_t w[4];
+    uint32_t part[3][4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       const float e = __builtin_amdgcn_exp2f(p[t] - from);
       den = den + e;
-      w[t] = (static_cast<uint32_t>(static_cast<int>(fmaf_(e, weight, 0.5f))) + 0x80808080u) ^ 0x80808080u;
+      float left = e * weight;
+#pragma unroll
+      for (int d = 0; d < 3; d++) {
+        part[d][t] = __float_as_uint(left);
+        left = left - __uint_as_float(part[d][t] & 0xffff0000u);
+      }
     }
-    // Bytes of four values to values of four bytes.
-    const uint32_t a01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), a23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
-    const uint32_t b01 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), b23 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
-    asm volatile("" ::: "memory");
-    *reinterpret_cast<uint32_t *>(turn_to) = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
-    *reinterpret_cast<uint32_t *>(turn_to + 4 * 64) = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
-    *reinterpret_cast<uint32_t *>(turn_to + 8 * 64) = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
-    *reinterpret_cast<uint32_t *>(turn_to + 12 * 64) = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    const v4i weights = *reinterpret_cast<const v4i *>(turn_from);
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int d = 0; d < 4; d++) sums[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(s.v[d], weights, sums[d], 0, 0, 0);
+    for (int d = 0; d < 3; d++)
+      *reinterpret_cast<uint2 *>(turn_to + 4 * d * kTurned) = make_uint2(upper(part[d][1], part[d][0]), upper(part[d][3], part[d][2]));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const v8bf low = *reinterpret_cast<const v8bf *>(turn_from), high = *reinterpret_cast<const v8bf *>(turn_from + 8);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_of(s.v[d][0], s.v[d][1]), low, acc[d], 0, 0, 0);
+      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_of(s.v[d][2], s.v[d][3]), high, acc[d], 0, 0, 0);
+    }
   };
   // While one 64 keys are worked on, the next are on their way, and before them the
   // pages of those after: no load is under a branch, so the waits count what is
-  // still out. A sum grows by at most 2^20 with 64 keys: it is flushed every 1,024
-  // times.
+  // still out.
   auto turn = [&](const Stage &now, Stage &then, int key0, auto more) {
     if constexpr (decltype(more)::value) {
       const Found after = find(key0 + 128);
       load(next, key0 + 64, then);
       next = after;
     }
-    consume(now, key0, ((key0 - begin) & 0xffff) == 0xffc0);
+    consume(now, key0);
   };
   if (works) {
     const std::true_type more;
@@ -779,8 +800,6 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   // The waves' states meet in LDS: [run][column], 16 in all.
   __shared__ float s_m[16], s_den[16];
   __shared__ __attribute__((aligned(16))) float s_o[16][68];
-  const float back = __builtin_ldexpf(1.0f, power - 30);
-  flush(1.0f);
   den = den + row_ror<8>(den);
   den = den + row_ror<4>(den);
   den = den + row_ror<2>(den);
@@ -794,10 +813,9 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     v4f o;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      // Lane l16 < 4: byte sums of lanes l16, + 4, + 8, + 12.
+      // Lane l16 < 4: the sums of lanes l16, + 4, + 8, the upper part's first.
       const float x = acc[d][i];
-      const float sum = fmaf_(row_ror<4>(x), 16777216.0f, fmaf_(row_ror<8>(x), 65536.0f, fmaf_(row_ror<12>(x), 256.0f, x)));
-      o[i] = sum * back;
+      o[i] = __builtin_ldexpf((row_ror<8>(x) + row_ror<12>(x)) + x, power - 64);
     }
     if (l16 < 4) *reinterpret_cast<v4f *>(&s_o[4 * wave + l16][16 * d + 4 * g]) = o;
   }
