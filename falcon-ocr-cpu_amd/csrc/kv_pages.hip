@@ -494,11 +494,11 @@ __device__ __forceinline__ float row_max(float v) {
 // four columns and one run of the part's keys, 64 (four blocks) at a time: up to four
 // columns leave each wave a run of its own, up to eight two waves, more all four.
 //
-// Scores. A query row is integers i 2^(e - 22) of three signed bytes (2^e above
-// its largest element, so to 2^-22 of it). Row 4 q + d of the INT8 matrix
-// product holds byte d of query q, column j of key tile t is key 4 j + t as its codes
-// stand: lane (j, q) gets the three exact sums of its four keys with its query,
-// and nothing is computed twice. Weights. w = exp2(s - m) times the block's value
+// Scores. A query row is integers i 2^(e - 30) of four signed bytes (2^e above its
+// largest element, so to 2^-30 of it: elements down to 2^-6 of it keep all their
+// bits). Row 4 q + d of the INT8 matrix product holds byte d of query q, column j of
+// key tile t is key 4 j + t as its codes stand: lane (j, q) gets the four exact sums of
+// its four keys with its query, and nothing is computed twice. Weights. w = exp2(s - m) times the block's value
 // scale in FP32, over the power of two above the largest such scale so far and times
 // 2^64 (so that weights 2^-174 below that keep all their bits), is the sum of three
 // BF16 numbers, its own bits eight at a time: part d of query q is column 4 d + q of
@@ -643,18 +643,18 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     big = p[0] > p[1] ? p[0] : p[1];
     const bool finite = big < 0x7f800000u;
     int e = !finite || big == 0 ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(big));
-    e = e < -96 ? -96 : e;
+    e = e < -90 ? -90 : e;
     // log2(e) / 8: scores in powers of two. From query l16 / 4 to query g.
-    const float factor = finite ? __builtin_ldexpf(0.180336880111120426f, e - 22) : __builtin_nanf("");
+    const float factor = finite ? __builtin_ldexpf(0.180336880111120426f, e - 30) : __builtin_nanf("");
     q_factor = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (4 * g), __float_as_int(factor)));
-    // 1.5 2^23 + i holds the integer i in its low bits; adding 128 to each byte of
-    // i and inverting their top bits leaves signed bytes whose weighted sum is i.
+    // Adding 128 to each lower byte of i and inverting their top bits leaves signed
+    // bytes whose weighted sum is i.
     auto bytes = [&](float f) {
-      const float t = __builtin_ldexpf(f, 22 - e) + 12582912.0f;
-      return (__float_as_uint(t) + (0x00808080u - 0x4b400000u)) ^ 0x00808080u;
+      const int i = finite ? static_cast<int>(__builtin_rintf(__builtin_ldexpf(f, 30 - e))) : 0;
+      return (static_cast<uint32_t>(i) + 0x00808080u) ^ 0x00808080u;
     };
-    // Byte l16 % 4 of four values; the fourth is none.
-    const uint32_t pick = l16 % 4 == 3 ? 0x0c0c0c0cu : 0x0c0c0400u + 0x0101u * (l16 % 4);
+    // Byte l16 % 4 of four values.
+    const uint32_t pick = 0x0c0c0400u + 0x0101u * (l16 % 4);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const uint32_t lo = __builtin_amdgcn_perm(bytes(x[i].y), bytes(x[i].x), pick);
@@ -731,7 +731,8 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     for (int t = 0; t < 4; t++) {
       const v4i zero = {0, 0, 0, 0};
       const v4i dots = __builtin_amdgcn_mfma_i32_16x16x64_i8(digit, s.k[t], zero, 0, 0, 0);
-      const float sum = fmaf_(static_cast<float>(dots[2]), 65536.0f, static_cast<float>((dots[1] << 8) + dots[0]));
+      // A sum is below 2^20, so two of them fit 32 bits.
+      const float sum = fmaf_(static_cast<float>((dots[3] << 8) + dots[2]), 65536.0f, static_cast<float>((dots[1] << 8) + dots[0]));
       p[t] = sum * factor;
       if (key0 + 4 * l16 + t >= visible) p[t] = ninf;
     }

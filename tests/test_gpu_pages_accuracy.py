@@ -26,7 +26,7 @@ def attention64(q, k, v, first):
     """64-bit attention of rows [n][heads][64] at positions first.., and how far FP32's may
     be from it.
 
-    A score is off by the query's step (2^-22 of its largest element) times the key, and by
+    A score is off by the query's step (2^-22 of its largest element at most) times the key, and by
     a few roundings of itself and of its exponent; a weight by the exponential of twice that
     (its own and the maximum's). A weighted value passes a rounding, of up to a whole step
     where a matrix instruction cuts, for each of the terms that are added to it, of which a
@@ -110,3 +110,28 @@ def test_large_values_behind_a_row(fh, ratio, page):
 def test_values_of_one_small_or_large_magnitude(fh, scale):
     k, v, q = inputs(300, 53)
     attend(fh, k, v * F32(scale), q, 299)
+
+
+@pytest.mark.parametrize("total", [40, 1100])
+@pytest.mark.parametrize("large", [1e4, 3e5])
+def test_a_large_query_element_that_meets_no_key(fh, total, large):
+    # Scores come from elements far below the largest one. They are off by 2^-30 of that (half a
+    # step of an integer that twice the largest bounds by 2^30) times the key, and by the roundings
+    # of their own terms' sum and of the exponent.
+    k, v, q = inputs(total, 59)
+    k[:, :, 5] = 0
+    q[:, :, 5] = large
+    kv = fh.KvPages(-(-total // 64), 64, 1, -(-total // 64), HEADS, HEADS)
+    kv.map(0, 0, list(range(-(-total // 64))))
+    kv.append(to_dev(k), to_dev(v), int32([0]), row_start=int32([0, total]))
+    gk, gv = (host(x).astype(np.float64) for x in kv.dequantize(total, int32([0]), row_start=int32([0, total])))
+    got = host(kv.attention(to_dev(q), int32([total - 1]), total)).astype(np.float64)
+    for h in range(HEADS):
+        s = gk[:, h] @ q[0, h].astype(np.float64) / 8.0
+        w = np.exp(s - s.max())
+        w /= w.sum()
+        step = 2.0 ** -30 * large * np.abs(gk[:, h]).sum(axis=1).max() / 8
+        off = step + EPS * (6 * (np.abs(gk[:, h]) @ np.abs(q[0, h])).max() / 8 + 8 * np.abs(s).max() + 16)
+        bound = w @ np.abs(gv[:, h]) * (2.2 * off + EPS * (2 * min(total, 1024) + 112))
+        over = np.abs(got[0, h] - w @ gv[:, h]) / bound
+        assert (over <= 1).all(), f"head {h}: {over.max()} times what is allowed"
