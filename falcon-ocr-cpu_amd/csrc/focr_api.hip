@@ -377,7 +377,7 @@ int focr_linear_upload(focr_ctx *handle, int bits, size_t n, size_t k, size_t gr
   if (n_exc) {
     std::vector<int32_t> cols(exc_cols, exc_cols + n_exc);
     std::vector<float> vals(exc_vals, exc_vals + n * n_exc);
-    std::vector<int16_t> index(k, -1);
+    std::vector<int16_t> index((k + 3) / 4 * 4, -1);  // whole fours, as the 4-bit GEMV loads them
     for (size_t e = 0; e < n_exc; e++) index[size_t(exc_cols[e])] = int16_t(e);
     if ((rc = upload_vector(cols, &lin->exc_cols, &total)) != FOCR_OK) return fail(rc);
     if ((rc = upload_vector(vals, &lin->exc_vals, &total)) != FOCR_OK) return fail(rc);

@@ -81,7 +81,7 @@ struct Linear {
   float *scales = nullptr; // [n][groups] (bits 4/8/16)
   int32_t *exc_cols = nullptr;  // [n_exc]
   float *exc_vals = nullptr;    // [n][n_exc]
-  int16_t *exc_index = nullptr; // [k]: exception number of a column, or -1
+  int16_t *exc_index = nullptr; // [k, up to whole fours]: exception number of a column, or -1
   // GEMV tiles (bits 4: tiles of 16 channels x 128 columns, linear4.hpp).
   void *gemv_codes = nullptr;    // [tiles][steps][64 lanes][16 B]
   float *gemv_scales = nullptr;  // [tiles][steps][2 halves][2 ch][sps]

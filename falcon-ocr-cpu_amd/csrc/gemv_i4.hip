@@ -8,7 +8,9 @@
 //
 // Mathematics. Each block of 128 W columns of a row of x (W steps of a wave, 1 to 4)
 // is written as integers, x = i 2^(e - 22), |i| <= 2^22, 2^e above its largest
-// magnitude, and i as three signed bytes, i = d0 + 256 d1 + 65536 d2. The INT8
+// magnitude, and i as three signed bytes, i = d0 + 256 d1 + 65536 d2. Exception columns
+// count as zeros in this: their codes are, and their inputs, which may be far larger
+// than the others', are added by themselves in FP32. The INT8
 // matrix instruction then forms the exact sums of 16 channels' codes times the
 // bytes of up to five rows (eight in two instructions) over 64 columns: operands are
 // the codes as the tile holds them (no conversion) and the bytes, one column of
@@ -40,6 +42,7 @@ struct Args {
   const float *scales;
   const int32_t *exc_cols;
   const float *exc_vals;
+  const int16_t *exc_index;  // [k up to whole fours]: below 0 where a column is no exception; null: none
   int n_exc;
   const float *x, *row_scale;
   float *out;
@@ -154,6 +157,20 @@ struct Block {
 #pragma unroll
     for (int p = 0; p < kParts; p++) v[p] = load_x(a, r, column(a, col0, p));
   }
+  // Which of the lane's columns are exceptions: bit 4 p + i, the same for all rows.
+  __device__ static __forceinline__ uint32_t exceptions(const Args &a, int col0) {
+    uint32_t marks = 0;
+    if (a.exc_index) {
+      const int last = (a.staged_k - 1) / 4 * 4;
+#pragma unroll
+      for (int p = 0; p < kParts; p++) {
+        const int col = column(a, col0, p);
+        const uint2 index = load_at<uint2>(a.exc_index, 2u * (col < last ? col : last));
+        marks |= ((~index.x >> 15 & 1) | (~index.x >> 30 & 2) | (~index.y >> 13 & 4) | (~index.y >> 28 & 8)) << (4 * p);
+      }
+    }
+    return marks;
+  }
   __device__ __forceinline__ void trim_to(const Args &a, int col0) {
 #pragma unroll
     for (int p = 0; p < kParts; p++) v[p] = trim(a, v[p], column(a, col0, p));
@@ -161,13 +178,27 @@ struct Block {
 };
 
 // A wave writes block x of row r: bytes to `digits` [2 W groups], their weights to
-// `weights` [columns]. True (in every lane) if a value is not finite.
+// `weights` [columns]; exceptions become zeros. True (in every lane) if a value is not
+// finite.
 template <int NB, int W>
-__device__ __forceinline__ bool stage_block(const Block<W> &x, int r, char *digits, float *weights) {
+__device__ __forceinline__ bool stage_block(Block<W> &x, uint32_t exceptions, int r, char *digits, float *weights) {
   using C = Columns<NB>;
   constexpr int P = Block<W>::kParts;
   const int lane = threadIdx.x & 63, l16 = lane & 15;
-  const v4f(&v)[P] = x.v;
+  v4f(&v)[P] = x.v;
+  bool outlier = false;  // an exception that is not finite
+  if (__any(exceptions != 0)) {
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const bool taken = exceptions >> (4 * p + i) & 1;
+        outlier |= taken && (__float_as_uint(v[p][i]) & 0x7fffffffu) >= 0x7f800000u;
+        v[p][i] = taken ? 0.0f : v[p][i];
+      }
+    }
+    outlier = __any(outlier);
+  }
   uint32_t big = 0;
 #pragma unroll
   for (int p = 0; p < P; p++) {
@@ -201,7 +232,7 @@ __device__ __forceinline__ bool stage_block(const Block<W> &x, int r, char *digi
     }
   }
   if (lane < 3) weights[lane * C::kRows + r] = __builtin_ldexpf(1.0f, e - 26 + 8 * lane);
-  return bad;
+  return bad || outlier;
 }
 
 // The rows as bytes in memory, for large calls: a wave for each block of a row.
@@ -213,12 +244,14 @@ __global__ __launch_bounds__(256) void rows4_kernel(Args a) {
   if (block >= a.blocks) return;
   Block<W> x;
   x.load(a, r, block * W * kStep);
+  const uint32_t exceptions = Block<W>::exceptions(a, block * W * kStep);
   x.trim_to(a, block * W * kStep);
-  const bool bad = stage_block<NB, W>(x, r, a.digits + static_cast<size_t>(block) * 2 * W * C::kGroup, a.weights + block * C::kWide);
   float sum = 0.0f;
 #pragma unroll
   for (int p = 0; p < Block<W>::kParts; p++) sum = square_sum(x.v[p], sum);
   sum = wave_sum(sum);
+  const bool bad = stage_block<NB, W>(x, exceptions, r, a.digits + static_cast<size_t>(block) * 2 * W * C::kGroup,
+                                      a.weights + block * C::kWide);
   if (threadIdx.x % 64 == 0) {
     a.marks[r * a.blocks + block] = bad;
     a.squares[r * a.blocks + block] = sum;
@@ -333,6 +366,7 @@ __global__ __launch_bounds__(64 * NW, (resident<NB, SK, W, G, PRE>())) void gemv
     float sum[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) sum[i] = 0.0f;
+    uint32_t exceptions = 0;
     // Past the call's rows, the last one again (not written).
     auto load_rows = [&](int turn) {
 #pragma unroll
@@ -340,6 +374,7 @@ __global__ __launch_bounds__(64 * NW, (resident<NB, SK, W, G, PRE>())) void gemv
         const int r = slot + SLOTS * i;
         x[i].load(a, r < M ? r : M - 1, (turn * SK + part) * W * kStep);
       }
+      exceptions = Block<W>::exceptions(a, (turn * SK + part) * W * kStep);
     };
     load_rows(0);
     __builtin_amdgcn_sched_barrier(0);
@@ -359,7 +394,7 @@ __global__ __launch_bounds__(64 * NW, (resident<NB, SK, W, G, PRE>())) void gemv
         if (a.rms)
 #pragma unroll
           for (int p = 0; p < Block<W>::kParts; p++) sum[i] = square_sum(x[i].v[p], sum[i]);
-        if (stage_block<NB, W>(x[i], r, lds + block * BLOCK, weights + block * C::kWide)) bad[r] = 1;
+        if (stage_block<NB, W>(x[i], exceptions, r, lds + block * BLOCK, weights + block * C::kWide)) bad[r] = 1;
       }
     }
     // The rows' sums of squares by waves, for `finish`.
@@ -755,6 +790,7 @@ int launch_gemv4(Ctx *ctx, const Linear *lin, const float *x, size_t rows, const
   a.scales = lin->gemv_scales;
   a.exc_cols = lin->exc_cols;
   a.exc_vals = lin->exc_vals;
+  a.exc_index = lin->n_exc ? lin->exc_index : nullptr;
   a.n_exc = static_cast<int>(lin->n_exc);
   a.x = x;
   a.row_scale = row_scale;

@@ -152,7 +152,8 @@ int focr_linear_dequantize(focr_ctx *ctx, const focr_linear *lin, float *out_dev
  * (src/kernels/mod.rs:407-432). x_dev [rows][in], out_dev [rows][out].
  * Bitwise equal to the reference's AVX2/NEON/portable dot_q / dot order.
  * Bits 4: the inputs of each block of 128 to 512 columns are taken to 2^-22 of
- * their largest magnitude (2^-118 at the least), the products with the codes of
+ * their largest magnitude (2^-118 at the least; exception columns, whose products
+ * are added in FP32, do not count in it), the products with the codes of
  * 64 columns (32 for group 32) are summed exactly, and these sums times their
  * scales are added in FP32 (the same for the two calls below); a row scale or
  * norm multiplies the finished sums; rows that hold an infinity or NaN are
