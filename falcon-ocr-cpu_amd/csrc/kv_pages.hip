@@ -442,11 +442,40 @@ struct AttendArgs {
 };
 
 // A sequence's rows for attention; false where there is nothing to do (n = 0) or it
-// is refused (bad).
+// is refused (bad), but for what `overlaps` says.
 __device__ __forceinline__ bool attend_span(const AttendArgs &a, int seq, int &len, int &first, int &n, bool &bad) {
   bad = !a.c.span(seq, len, first, n);
   if (n > 8 || (n > 0 && len + n > a.max_len)) bad = true;
   return n > 0 && !bad;
+}
+
+// Whether a sequence's rows, from `first` on, begin before those of a sequence before it
+// end, as find_unit refuses them. A wave's question. Starts that do not decrease never
+// do, so mostly these are all that is looked at: each lane's of the first 64 (`start_of`,
+// loaded ahead of the question), and of 256 at a time.
+__device__ __forceinline__ int start_of(const Cache &c, int seq) {
+  const int at = 1 + static_cast<int>(threadIdx.x & 63);
+  return c.row_start ? c.row_start[at < seq ? at : seq] : 0;
+}
+__device__ __forceinline__ bool overlaps(const Cache &c, int seq, int first, int start) {
+  if (!c.row_start) return false;
+  const int lane = threadIdx.x & 63;
+  int top = start;
+  for (int base = 65; base < seq; base += 256) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int at = base + 64 * i + lane, other = c.row_start[at < seq ? at : seq];
+      top = other > top ? other : top;
+    }
+  }
+  if (!__any(top > first)) return false;
+  bool found = false;
+  for (int base = 0; base < seq; base += 64) {
+    int len, other, n;
+    const int at = base + lane;
+    if (at < seq && c.span(at, len, other, n) && n > 0 && other + n > first) found = true;
+  }
+  return __any(found);
 }
 
 // out = o / den / (1 + exp(sink - lse)), lse = (m + log2(den)) ln 2.
@@ -465,14 +494,30 @@ __device__ __forceinline__ float state_weight(float m, float den, float top) {
   return __builtin_amdgcn_exp2f(m - top);
 }
 
-// The rows of a refused sequence, where they are rows of the call: NaN.
+// The rows of a refused sequence, where they are rows of the call: NaN. Only those that
+// can be no other sequence's: behind all starts before its own and before all later ones.
 __device__ __forceinline__ void refuse_rows(const AttendArgs &a, int seq, int head0, int heads) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63;
   const int begin = c.row_start ? c.row_start[seq] : seq, end = c.row_start ? c.row_start[seq + 1] : seq + 1;
   if (lane == 0) c.refused[seq] = 1;
   if (begin < 0 || end > c.rows) return;
-  for (int row = begin; row < end; row++)
+  int from = begin, to = end;
+  if (c.row_start) {
+    for (int at = lane; at <= c.n_seqs; at += 64) {
+      const int start = c.row_start[at];
+      if (at <= seq)
+        from = start > from ? start : from;
+      else
+        to = start < to ? start : to;
+    }
+    for (int d = 1; d < 64; d *= 2) {
+      const int f = __shfl_xor(from, d), t = __shfl_xor(to, d);
+      from = f > from ? f : from;
+      to = t < to ? t : to;
+    }
+  }
+  for (int row = from; row < to; row++)
     for (int h = head0; h < head0 + heads; h++)
       a.out[(static_cast<size_t>(row) * c.n_heads + h) * 64 + lane] = __builtin_nanf("");
 }
@@ -538,6 +583,7 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   const int group = c.n_heads / c.key_heads, value_head = key_head * c.kv_heads / c.key_heads;
   int len, first, n;
   bool bad;
+  const int start = start_of(c, seq);
   if (!attend_span(a, seq, len, first, n, bad)) {
     if (bad && a.parts == 1 && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
     return;
@@ -664,7 +710,6 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     const int mine = column0 + g;
     visible = len + (mine < columns ? mine : columns - 1) % n + 1;
   }
-
   const float ninf = -__builtin_inff();
   float m = ninf, den = 0.0f;
   int power = -300;  // 2^power above every block scale of the values so far
@@ -797,6 +842,11 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     }
   }
   if (__any(missing) && lane == 0) c.refused[seq] = 1;
+  // Asked here, where no load is waited for.
+  if (overlaps(c, seq, first, start)) {
+    if (a.parts == 1 && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
+    return;
+  }
 
   // The waves' states meet in LDS: [run][column], 16 in all.
   __shared__ float s_m[16], s_den[16];
@@ -862,6 +912,7 @@ __global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttendArgs a) {
   __shared__ float s_m[WAVES], s_den[WAVES], s_o[WAVES][64];
   int len, first, n;
   bool bad;
+  const int start = start_of(c, seq);
   const bool live = attend_span(a, seq, len, first, n, bad);
   if (bad && wave == 0) refuse_rows(a, seq, head, 1);
   if (!live) return;
@@ -905,7 +956,7 @@ __global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttendArgs a) {
     }
     s_o[wave][lane] = o;
     __syncthreads();
-    if (own == 0 && r < n) {
+    if (own == 0 && r < n && !overlaps(c, seq, first, start)) {
       float top = m;
       for (int w = 1; w < waves; w++) top = __builtin_fmaxf(top, s_m[wave + w]);
       float total = 0.0f;
@@ -919,6 +970,7 @@ __global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttendArgs a) {
     }
     __syncthreads();
   }
+  if (wave == 0 && overlaps(c, seq, first, start)) refuse_rows(a, seq, head, 1);
 }
 
 // ---- pages of a sequence ---------------------------------------------------------

@@ -456,8 +456,9 @@ int focr_kv_free(focr_kv_split *kv);
  * kernels read and the caller advances, so a captured step replays with new
  * lengths. Rows of sequences that take no part, and rows before the first or
  * behind the last sequence, are neither read nor written. A sequence whose
- * entries do not fit (rows out of range, positions past seq_pages pages or
- * without a page) is refused alone: focr_kv_pages_refused names it. */
+ * entries do not fit (rows out of range or of a sequence before it, positions
+ * past seq_pages pages or without a page) is refused alone:
+ * focr_kv_pages_refused names it. */
 int focr_kv_pages_create(focr_ctx *ctx, size_t n_pages, size_t page_size, size_t n_seqs, size_t seq_pages,
                          size_t n_heads, size_t n_key_heads, size_t n_kv_heads, size_t head_dim,
                          focr_kv_pages **out);
@@ -493,8 +494,8 @@ int focr_kv_pages_qkv_rows(focr_ctx *ctx, focr_kv_pages *kv, const float *qkv_de
  * the per-head sink (sinks_dev [n_heads], NULL: none), scale 1/8. q_dev, out_dev
  * [rows][n_heads][64]. max_len: no sequence has more positions, the call's rows
  * included; the call's work is dealt out by it. A refused sequence (also one
- * with more than 8 rows or max_len positions) gets NaN rows, as does a
- * non-finite query. Within FP32 rounding of the decoded values' attention;
+ * with more than 8 rows or max_len positions) gets NaN rows, but for those that
+ * another sequence's entries reach; so does a non-finite query. Within FP32 rounding of the decoded values' attention;
  * queries are taken to 2^-30 of their largest element (2^-120 at the least).
  * Uses the context scratch. */
 int focr_kv_pages_attention(focr_ctx *ctx, const focr_kv_pages *kv, const float *q_dev, size_t rows,
