@@ -156,8 +156,8 @@ int focr_linear_dequantize(focr_ctx *ctx, const focr_linear *lin, float *out_dev
  * are added in FP32, do not count in it), the products with the codes of
  * 64 columns (32 for group 32) are summed exactly, and these sums times their
  * scales are added in FP32 (the same for the two calls below); a row scale or
- * norm multiplies the finished sums; rows that hold an infinity or NaN are
- * computed by FP32 multiply-adds. A large call (rows * in above 16,384, or rows
+ * norm multiplies the finished sums; rows that hold an infinity or NaN have the
+ * infinities and NaNs of their products' sums. A large call (rows * in above 16,384, or rows
  * that do not fit a workgroup) keeps its inputs as bytes, 16 a column (32 for
  * more than five rows), in the context scratch. */
 int focr_linear_decode(focr_ctx *ctx, const focr_linear *lin, const float *x_dev, size_t rows,
