@@ -46,7 +46,8 @@ Sessions that are decoded together keep their positions in a `KvPages` cache
 (one for each layer): `enter_pages` appends a prefilled prompt as one of its
 sequences, and `decode_pages` runs one step of the whole batch::
 
-    rms_norm(h) . qkv -> qkv                 the decode GEMV up to 8 rows in all, else the panels
+    rms_norm(h) . qkv -> qkv                 the decode GEMV up to 8 rows in all (or 32, eight at a
+                                             time, where the prompts' kernel is INT16's), else panels
     KvPages.qkv_rows -> q, codes             split, norm, rotation, append
     KvPages.attention                        each sequence's rows over its pages
     wo, w13, w2                              as in `decode` or `prefill`
@@ -277,11 +278,27 @@ class DecoderLayer:
         if self.ctx.stream != torch.cuda.current_stream(self.ctx.device).cuda_stream:
             self.ctx.sync()  # the batch's arrays are free for torch's stream from here on
 
-    def decode_pages(self, h, rope, pages: KvPages, lens, max_len: int, row_start=None, clock=None):
+    @staticmethod
+    def _eights(matrix, x, out, **kw) -> None:
+        """`linear_ex` of any number of rows, eight at a time."""
+        rows = x.shape[0]
+        if rows <= 8:
+            matrix.linear_ex(x, rows, out=out, **kw)
+            return
+        for at in range(0, rows, 8):
+            matrix.linear_ex(x[at:at + 8], min(8, rows - at), out=out[at:at + 8], **kw)
+
+    def decode_pages(self, h, rope, pages: KvPages, lens, max_len: int, row_start=None, clock=None,
+                     projection: Optional[PrefillProjection] = None):
         """One step of a batch of sequences: updates `h` [rows][dim] in place
         and appends to `pages` at the positions `lens` (see `KvPages`; no
         sequence has more than `max_len`, these rows included). Rows that are
-        no sequence's, or a refused one's, come out without meaning."""
+        no sequence's, or a refused one's, come out without meaning.
+
+        More than 8 rows in all take the kernel `projection`: by default the
+        layer's, but where that is INT16's FP32 products, as `decode` has
+        them, so that a session's step does not lose accuracy by the number
+        of others'."""
         self._pages(pages)
         rows = h.shape[0]
         if h.shape[1:] != (self.dim,):
@@ -289,14 +306,20 @@ class DecoderLayer:
         pages._ptr(h)  # a contiguous float32 tensor on the layer's device
         if rows == 0:
             return h
-        ctx, panel = self.ctx, rows > 8
+        if projection is None and self.projection != PrefillProjection.I16:
+            projection = self.projection
+        if projection is None and rows > 32:
+            # Up to 32 rows the GEMV takes eight at a time (us for a layer's four 4-bit matrices of
+            # 768 .. 4,608, calls of eight / FP32 panels: 16 rows 63 / 141, 64 rows 252 / 141).
+            projection = PrefillProjection.F32_MFMA
+        ctx, panel = self.ctx, rows > 8 and projection is not None
         mark = clock or (lambda stage: None)
         qkv = self._step_buf("pqkv", (rows, self.qkv.out_dim))
         if panel:
             rs = row_scales(h, self.dim, out=self._step_buf("prs", (rows,)), ctx=ctx)
-            self.qkv.prefill(h, rows, row_scale=rs, kernel=self.projection, out=qkv)
+            self.qkv.prefill(h, rows, row_scale=rs, kernel=projection, out=qkv)
         else:
-            self.qkv.linear_ex(h, rows, rms_norm=True, out=qkv)
+            self._eights(self.qkv, h, qkv, rms_norm=True)
         mark("qkv")
         q = pages.qkv_rows(qkv, rope, lens, row_start=row_start, q=self._step_buf("pq", (rows, self.n_heads, 64)))
         mark("qkv_rows")
@@ -305,18 +328,18 @@ class DecoderLayer:
         mark("attention")
         gated = self._step_buf("pgated", (rows, self.w13.out_dim // 2))
         if panel:
-            self.wo.prefill(attn, rows, epilogue=Epilogue.ADD, out=h, kernel=self.projection)
+            self.wo.prefill(attn, rows, epilogue=Epilogue.ADD, out=h, kernel=projection)
             mark("wo")
             rs = row_scales(h, self.dim, out=rs, ctx=ctx)
-            self.w13.prefill(h, rows, row_scale=rs, epilogue=Epilogue.GLU, kernel=self.projection, out=gated)
+            self.w13.prefill(h, rows, row_scale=rs, epilogue=Epilogue.GLU, kernel=projection, out=gated)
             mark("w13")
-            self.w2.prefill(gated, rows, epilogue=Epilogue.ADD, out=h, kernel=self.projection)
+            self.w2.prefill(gated, rows, epilogue=Epilogue.ADD, out=h, kernel=projection)
         else:
-            self.wo.linear_ex(attn, rows, epilogue=Epilogue.ADD, out=h)
+            self._eights(self.wo, attn, h, epilogue=Epilogue.ADD)
             mark("wo")
-            self.w13.linear_ex(h, rows, rms_norm=True, epilogue=Epilogue.GLU, out=gated)
+            self._eights(self.w13, h, gated, rms_norm=True, epilogue=Epilogue.GLU)
             mark("w13")
-            self.w2.linear_ex(gated, rows, epilogue=Epilogue.ADD, out=h)
+            self._eights(self.w2, gated, h, epilogue=Epilogue.ADD)
         mark("w2")
         return h
 
