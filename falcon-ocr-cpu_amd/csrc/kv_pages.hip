@@ -18,8 +18,9 @@
 // blocks of a sequence are also kept in FP32 beside the pages (two, so that a step
 // that takes back up to 16 positions finds them too): what the cache holds depends
 // on the rows appended, and not on how many at a time. Where a block is not
-// there (a sequence that goes on from pages it was given, or goes back further),
-// its earlier positions are taken from its codes.
+// there (a sequence that goes on from pages it was given, or goes back further), or
+// another sequence wrote the page's block since, its earlier positions are taken from
+// its codes.
 #include <algorithm>
 #include <new>
 #include <type_traits>
@@ -42,6 +43,7 @@ struct Pages {
   int8_t *k_codes = nullptr;   // [page][key head][block][1 KB]
   int8_t *v_codes = nullptr;   // [page][KV head][block][1 KB]
   float *k_scales = nullptr, *v_scales = nullptr;  // [page][head][block]
+  int32_t *k_writers = nullptr, *v_writers = nullptr;  // [page][head][block]: the sequence that wrote it, or -1
   int32_t *table = nullptr;    // [sequence][seq_pages], -1: no page
   float *open = nullptr;       // [sequence][key heads, then KV heads][block % 2][16][64]
   int32_t *tags = nullptr;     // [sequence][heads][2]: the block that `open` holds, or -1
@@ -53,6 +55,7 @@ struct Pages {
 struct Cache {
   int8_t *k_codes, *v_codes;
   float *k_scales, *v_scales;
+  int32_t *k_writers, *v_writers;
   const int32_t *table;
   float *open;
   int32_t *tags, *refused;
@@ -327,7 +330,8 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     }
     int8_t *const codes = (is_key ? c.k_codes : c.v_codes) + number * kBlockBytes;
     float *const scale_at = (is_key ? c.k_scales : c.v_scales) + number;
-    const bool kept = earlier && c.tags[slot + block % 2] == block;
+    int32_t *const writer_at = (is_key ? c.k_writers : c.v_writers) + number;
+    const bool kept = earlier && c.tags[slot + block % 2] == block && *writer_at == unit.seq;
     if (earlier && !kept) {
       // From the codes.
       const float scale = *scale_at;
@@ -373,7 +377,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 #pragma unroll
     for (int s = 0; s < 4; s++)
       *reinterpret_cast<uint32_t *>(is_key ? codes + s * 256 + lane * 4 : codes + (e4 + s) * kBlock + r4) = w[s];
-    if (lane == 0) *scale_at = scale;
+    if (lane == 0) {
+      *scale_at = scale;
+      *writer_at = unit.seq;
+    }
     if (block >= last_block - 1) {
 #pragma unroll
       for (int s = 0; s < 4; s++) {
@@ -981,13 +988,14 @@ struct MapArgs {
   int32_t pages[kMapped];
 };
 
-// Writes table entries, and forgets the FP32 blocks that stood in those pages.
+// Writes table entries, and forgets the FP32 blocks that stood where other pages come.
 __global__ __launch_bounds__(256) void map_kernel(MapArgs a) {
-  for (int i = threadIdx.x; i < a.count; i += 256) a.table[a.first + i] = a.pages[i];
   for (int i = threadIdx.x; i < 2 * a.heads; i += 256) {
     const int block = a.tags[i], at = block >> a.shift;
-    if (block >= 0 && at >= a.first && at < a.first + a.count) a.tags[i] = -1;
+    if (block >= 0 && at >= a.first && at < a.first + a.count && a.table[at] != a.pages[at - a.first]) a.tags[i] = -1;
   }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.count; i += 256) a.table[a.first + i] = a.pages[i];
 }
 
 __global__ __launch_bounds__(256) void fill_kernel(int32_t *to, size_t count, int32_t value) {
@@ -996,7 +1004,8 @@ __global__ __launch_bounds__(256) void fill_kernel(int32_t *to, size_t count, in
 }
 
 void free_pages(Pages *kv) {
-  void *buffers[] = {kv->k_codes, kv->v_codes, kv->k_scales, kv->v_scales, kv->table, kv->open, kv->tags, kv->refused};
+  void *buffers[] = {kv->k_codes,   kv->v_codes, kv->k_scales, kv->v_scales, kv->k_writers,
+                     kv->v_writers, kv->table,   kv->open,     kv->tags,     kv->refused};
   for (void *p : buffers)
     if (p) (void)hipFree(p);
 }
@@ -1007,6 +1016,8 @@ Cache cache_of(const Pages *kv, size_t rows, const int32_t *row_start, const int
   c.v_codes = kv->v_codes;
   c.k_scales = kv->k_scales;
   c.v_scales = kv->v_scales;
+  c.k_writers = kv->k_writers;
+  c.v_writers = kv->v_writers;
   c.table = kv->table;
   c.open = kv->open;
   c.tags = kv->tags;
@@ -1102,6 +1113,8 @@ int focr_kv_pages_create(focr_ctx *handle, size_t n_pages, size_t page_size, siz
                  {reinterpret_cast<void **>(&kv->v_codes), blocks * n_kv_heads * kBlockBytes, 0},
                  {reinterpret_cast<void **>(&kv->k_scales), blocks * n_key_heads * sizeof(float), 0},
                  {reinterpret_cast<void **>(&kv->v_scales), blocks * n_kv_heads * sizeof(float), 0},
+                 {reinterpret_cast<void **>(&kv->k_writers), blocks * n_key_heads * sizeof(int32_t), -1},
+                 {reinterpret_cast<void **>(&kv->v_writers), blocks * n_kv_heads * sizeof(int32_t), -1},
                  {reinterpret_cast<void **>(&kv->table), n_seqs * seq_pages * sizeof(int32_t), -1},
                  {reinterpret_cast<void **>(&kv->open), n_seqs * heads * 2 * kBlock * 64 * sizeof(float), 0},
                  {reinterpret_cast<void **>(&kv->tags), n_seqs * heads * 2 * sizeof(int32_t), -1},

@@ -477,8 +477,9 @@ int focr_kv_pages_map(focr_ctx *ctx, focr_kv_pages *kv, size_t seq, size_t first
  * values that a block held before are coded again from FP32 (the last two
  * blocks of a sequence are kept in it), so the cache depends on the rows and
  * not on the calls they came in, also after up to 16 positions were taken back
- * (lens_dev lowered); further back, or in pages that the sequence was mapped
- * and did not write, the block's codes are coded again. Positions without a
+ * (lens_dev lowered) and when pages are mapped again where they stand; further
+ * back, or in pages that the sequence was mapped and did not write last, the
+ * block's codes are coded again. Positions without a
  * page are left out. */
 int focr_kv_pages_append(focr_ctx *ctx, focr_kv_pages *kv, const float *k_dev, const float *v_dev, size_t rows,
                          const int32_t *row_start_dev, const int32_t *lens_dev, size_t n_seqs);
