@@ -237,7 +237,7 @@ __device__ __forceinline__ bool stage_block(Block<W> &x, uint32_t exceptions, in
 }
 
 // The rows as bytes in memory, for large calls: a wave for each block of a row.
-// Bound by its launch: eight rows of 8,192 take 4.9 us and move 0.7 MB.
+// Bound by its launch: eight rows of 8,192 take 3.2 us and move 0.7 MB.
 template <int NB, int W>
 __global__ __launch_bounds__(256) void rows4_kernel(Args a) {
   using C = Columns<NB>;
@@ -276,9 +276,9 @@ constexpr int resident() {
 // Bound: the codes, read once. A wave's load is 1 KB, a tile's step, and W of them
 // with their scales are on their way while W others are used; a load under a branch,
 // or a spilled register, would make the wave wait for all of them. 24,576 x 8,192 in
-// groups of 64 take 24.6 us for eight rows (114 MB, 4.6 TB/s), 65,536 x 768 in groups
-// of 128 7.9 us for one (27 MB, 3.4 TB/s: a third of it is the launch and the rows);
-// 2,048 x 768 take 4.4 us, all launch, rows and one trip to memory.
+// groups of 64 take 26.1 us for eight rows (114 MB, 4.4 TB/s), 65,536 x 768 in groups
+// of 128 7.7 us for one (27 MB, 3.5 TB/s: a third of it is the launch and the rows);
+// 2,048 x 768 take 4.7 us, all launch, rows and one trip to memory.
 template <int NB, int SK, int W, int G, bool PRE, int NW>
 __global__ __launch_bounds__(64 * NW, (resident<NB, SK, W, G, PRE>())) void gemv4_kernel(Args a) {
   using C = Columns<NB>;

@@ -246,7 +246,7 @@ __device__ __forceinline__ void turn_bytes(uint32_t (&w)[4]) {
 // they stand (256 bytes for each s) and a dim's codes of four positions are one word.
 // Bound: the rows and factors read, the queries written. 15,243 rows of four prompts
 // (16 query and key heads, 8 value heads) take 62 us for 188 MB read and 87 written,
-// 4.4 TB/s where a copy reaches 5.1; a row of each of 64 sequences 5.9 us, which is
+// 4.4 TB/s where a copy reaches 5.1; a row of each of 64 sequences 6.4 us, which is
 // the launch and three dependent trips to memory (batch, table, rows).
 template <bool QKV>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 
 // ---- reading back --------------------------------------------------------------
 // A wave takes one block of a sequence's rows and one stored head. Bound by the FP32
-// rows written: 15,243 rows of 24 heads take 27 us (118 MB moved, 4.4 TB/s).
+// rows written: 15,243 rows of 24 heads take 25 us (118 MB moved, 4.7 TB/s).
 __global__ __launch_bounds__(256) void read_kernel(Cache c, float *__restrict__ k, float *__restrict__ v) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int head = blockIdx.y * 4 + wave, stored = c.key_heads + c.kv_heads;
@@ -562,11 +562,11 @@ __device__ __forceinline__ float row_max(float v) {
 // two changes.
 //
 // Bound: the codes, read once. 64 sequences of up to 8,192 positions (346,572 in all,
-// 16 key and 8 value heads) take 102 us, 618 MB from memory at 6.1 TB/s; 535 MB
+// 16 key and 8 value heads) take 107 us, 623 MB from memory at 5.8 TB/s; 535 MB
 // are needed, as two key heads' workgroups do not read all of their values together
-// (both in one workgroup: 549 MB, but 110 us, as fewer bytes are on their way). One
-// sequence of 131,072 takes 22 us (137 MB, 6.1 TB/s) and its merge 5; 101
-// positions take 5.5 us, the launch and four dependent trips to memory.
+// (both in one workgroup: 549 MB, but 8 % longer, as fewer bytes are on their way). One
+// sequence of 131,072 takes 25 us (137 MB, 5.6 TB/s) and its merge 5; 101
+// positions take 5.7 us, the launch and four dependent trips to memory.
 struct Stage {
   v4i k[4], v[4];
   float k_scale, v_scale;
@@ -909,7 +909,7 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
 
 // The parts of a sequence's rows of one head: as many of the waves for each row as
 // there are, lane = element, eight parts of a wave in flight. Bound by the launch and
-// the trips to memory: 4.7 us for 7 parts of 25 rows as for 57 parts of two.
+// the trips to memory: 4.4 us for 7 parts of 25 rows, 5.3 for 57 parts of two.
 template <int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttendArgs a) {
   const Cache &c = a.c;
@@ -1056,7 +1056,8 @@ int launch_append(Ctx *ctx, AppendArgs a, bool qkv) {
   const unsigned groups = static_cast<unsigned>((heads + 3) / 4);
   // Long prompts are near (us a call with its reading back, near / not: four of up to
   // 6,544 rows 89 / 104, one of 1,500 17.5 / 18.7; sixteen of up to 300 23.7 / 22.8, 200
-  // of up to five 26.4 / 25.5: a sequence's first unit has three blocks' work).
+  // of up to five 26.4 / 25.5: a sequence's first unit has three blocks' work), by the
+  // mean over all the call's sequences: one prompt among many idle ones is not.
   a.near = c.rows / c.n_seqs >= 1024;
   dim3 grid(static_cast<unsigned>(units), groups);
   if (a.near) {
@@ -1242,12 +1243,12 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
   const size_t most = row_start ? std::min<size_t>(rows, 8) : 1;
   const size_t group = kv->n_heads / kv->key_heads;
   a.tiles = static_cast<int>((group * most + 15) / 16);
-  // Parts of whole 256 keys, at most 4,096 (the longest run) up to a million
-  // positions. Few sequences need only fill the chip (us a call with 512 / 1,024 /
-  // 2,048 workgroups: one of 131,072 positions 33.1 / 36.2 / 37.3, four of up to
-  // 16,000 16.8 / 16.7 / 19.2); more, of different lengths, want parts to spare
-  // (20 of up to 9,000 49.4 / 44.9 / 45.0, 40 of up to 5,000 with up to 8 rows 88.9 /
-  // 59.7 / 54.0).
+  // Parts of whole 256 keys, at most 4,096 up to a million positions. Few sequences
+  // need only fill the chip (us a call with 512 / 1,024 / 2,048 workgroups: one of
+  // 131,072 positions 32.9 / 36.8 / 37.7, four of up to 16,000 16.3 / 17.8 / 18.8; six of
+  // up to 3,000 with up to 8 rows 17.6 / 15.4 / 15.9); more, of different lengths, want
+  // parts to spare (20 of up to 9,000 49.0 / 47.1 / 44.7, 40 of up to 5,000 with up to 8
+  // rows 84.7 / 84.8 / 63.7).
   const size_t heads = n_seqs * kv->key_heads * a.tiles;
   const size_t enough = n_seqs <= 2 ? 512 : n_seqs <= 8 ? 1024 : 2048;
   const size_t want = heads >= enough ? 1 : enough / heads;
@@ -1273,8 +1274,8 @@ int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const 
   if (a.parts > 1) {
     const dim3 each(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(n_seqs));
     // Parts of all a sequence's rows (us a call with 4 / 16 waves: 26 parts of one row
-    // 10.2 / 11.2, 3 of one in 64 sequences 109 / 117; 57 of two 34.9 / 33.7, 59 of
-    // eight 37.7 / 28.5).
+    // 9.8 / 10.4, 3 of one in 64 sequences 112 / 120; 57 of two 34.8 / 32.8, 59 of
+    // eight 33.3 / 20.3).
     if (a.parts * most <= 64)
       hipLaunchKernelGGL(merge_kernel<4>, each, dim3(256), 0, ctx->stream, a);
     else

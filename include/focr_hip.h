@@ -496,9 +496,10 @@ int focr_kv_pages_qkv_rows(focr_ctx *ctx, focr_kv_pages *kv, const float *qkv_de
  * [rows][n_heads][64]. max_len: no sequence has more positions, the call's rows
  * included; the call's work is dealt out by it. A refused sequence (also one
  * with more than 8 rows or max_len positions) gets NaN rows, but for those that
- * another sequence's entries reach; so does a non-finite query. Within FP32 rounding of the decoded values' attention;
- * queries are taken to 2^-30 of their largest element (2^-120 at the least).
- * Uses the context scratch. */
+ * another sequence's entries reach; so does a non-finite query. Within FP32
+ * rounding of the decoded values' attention: queries are taken to 2^-30 of their
+ * largest element (2^-120 at the least), and value blocks whose scales are up to
+ * 2^140 apart keep all their bits. Uses the context scratch. */
 int focr_kv_pages_attention(focr_ctx *ctx, const focr_kv_pages *kv, const float *q_dev, size_t rows,
                             const int32_t *row_start_dev, const int32_t *lens_dev, size_t n_seqs, size_t max_len,
                             const float *sinks_dev, float *out_dev);

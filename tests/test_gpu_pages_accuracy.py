@@ -135,3 +135,15 @@ def test_a_large_query_element_that_meets_no_key(fh, total, large):
         bound = w @ np.abs(gv[:, h]) * (2.2 * off + EPS * (2 * min(total, 1024) + 112))
         over = np.abs(got[0, h] - w @ gv[:, h]) / bound
         assert (over <= 1).all(), f"head {h}: {over.max()} times what is allowed"
+
+
+@pytest.mark.parametrize("total", [130, 1100])
+def test_value_blocks_far_apart_in_scale(fh, total):
+    # Scales 2^133 apart: the smaller ones' products stay whole, before the large block and behind it.
+    for at in (0, total // 2 // 16 * 16):
+        k, v, q = inputs(total, 61 + at)
+        k[at:at + 16] = key_for(q, -100.0)
+        large = v[at:at + 16] * F32(1e20)
+        v *= F32(1e-20)
+        v[at:at + 16] = large
+        attend(fh, k, v, q, total - 1)
