@@ -550,14 +550,14 @@ __device__ __forceinline__ float row_max(float v) {
 // largest element, so to 2^-30 of it: elements down to 2^-6 of it keep all their
 // bits). Row 4 q + d of the INT8 matrix product holds byte d of query q, column j of
 // key tile t is key 4 j + t as its codes stand: lane (j, q) gets the four exact sums of
-// its four keys with its query, and nothing is computed twice. Weights. w = exp2(s - m) times the block's value
-// scale in FP32, over the power of two above the largest such scale so far and times
-// 2^64 (so that weights 2^-174 below that keep all their bits), is the sum of three
-// BF16 numbers, its own bits eight at a time: part d of query q is column 4 d + q of
-// the second product, whose operands are the value codes as BF16 numbers (exact) and
-// these parts, turned through LDS. So every product is exact, whatever the
-// magnitudes of the other keys' weights and values, and sums round as FP32's do; a
-// weight on one scale for a run's keys (integers) would lose those far below the
+// its four keys with its query, and nothing is computed twice. Weights. w = exp2(s - m)
+// times the block's value scale in FP32, over the power of two above the largest such
+// scale so far and times 2^64 (so that weights 2^-174 below that keep all their bits),
+// is the sum of three BF16 numbers, its own bits eight at a time: part d of query q is
+// column 4 d + q of the second product, whose operands are the value codes as BF16
+// numbers (exact) and these parts, turned through LDS. So every product is exact,
+// whatever the magnitudes of the other keys' weights and values, and sums round as
+// FP32's do; integers of one step for a run's weights would lose those far below the
 // largest. The sums stay in the accumulators, which are scaled when m or the power of
 // two changes.
 //
