@@ -53,6 +53,9 @@ struct Ctx {
   size_t argmax_parts = 0;
   float *rms_dev = nullptr;  // [8] row scales of a decode GEMV whose width has no in-kernel rms_norm
   uint32_t *flags = nullptr;  // [16] words of pinned host memory that kernels write and a synchronous call reads
+  // focr_logits_select: how many of a row's workgroups have arrived (device; 0 between calls).
+  static constexpr int kSplitRows = 512, kSegments = 64;
+  uint32_t *arrived = nullptr;  // [kSplitRows]
   hipEvent_t order = nullptr;  // orders a new stream after the old one (focr_ctx_set_stream)
 };
 

@@ -27,6 +27,7 @@
 
 #include "decode_common.hpp"
 #include "rms_tree.hpp"
+#include "rotary.hpp"
 
 namespace focr {
 namespace {
@@ -156,6 +157,8 @@ struct AppendArgs {
   Cache c;
   const float *qkv, *rope;  // QKV rows and factors, or
   const float *k, *v;       // ready keys [rows][key heads][64] and values [rows][KV heads][64]
+  const float *positions, *frequencies;  // in the factors' place: [rows][axes], [axes][n_heads][32]
+  int axes;
   float *q;
   // Workgroups go to the 8 XCDs in turn. Near: those of one unit's heads, which take
   // the same factors and some the same keys, follow one another on the same one;
@@ -248,7 +251,10 @@ __device__ __forceinline__ void turn_bytes(uint32_t (&w)[4]) {
 // (16 query and key heads, 8 value heads) take 62 us for 188 MB read and 87 written,
 // 4.4 TB/s where a copy reaches 5.1; a row of each of 64 sequences 6.4 us, which is
 // the launch and three dependent trips to memory (batch, table, rows).
-template <bool QKV>
+//
+// With ANGLES the factors are formed from positions (rotary.hpp), bitwise those of
+// focr_rotary_factors.
+template <bool QKV, bool ANGLES>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, r4 = lane / 16 * 4, e4 = lane % 16 * 4;
@@ -289,6 +295,14 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     source = (is_key ? a.k : a.v) + (is_key ? head : head - c.key_heads) * 64;
   }
   const bool turned = QKV && (is_key || is_query);
+  float2 speed[kMaxAxes];
+  if constexpr (ANGLES)
+    if (turned) {
+#pragma unroll
+      for (int x = 0; x < kMaxAxes; x++)
+        if (x < a.axes)
+          speed[x] = *reinterpret_cast<const float2 *>(a.frequencies + (static_cast<size_t>(x) * c.n_heads + pair) * 32 + e4 / 2);
+    }
   const int first_block = unit.len / kBlock, blocks = touched(unit.len, unit.n), last_block = first_block + blocks - 1;
   const int held = is_key ? c.key_heads : c.kv_heads, at_head = is_key ? head : head - c.key_heads;
   const size_t slot = (static_cast<size_t>(unit.seq) * stored + head) * 2;
@@ -305,9 +319,33 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       const size_t at = unit.first + (row < 0 ? 0 : row < unit.n ? row : unit.n - 1);
       const float *from = earlier && row < 0 ? open + (r4 + s) * 64 : source + at * width;
       x[s] = *reinterpret_cast<const v4f *>(from + e4);
-      if (turned) f[s] = *reinterpret_cast<const v4f *>(a.rope + (at * c.n_heads + pair) * 64 + e4);
+      if constexpr (!ANGLES)
+        if (turned) f[s] = *reinterpret_cast<const v4f *>(a.rope + (at * c.n_heads + pair) * 64 + e4);
     }
     if (turned) {
+      if constexpr (ANGLES) {
+        float place[4][kMaxAxes];
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+          const int row = row0 + r4 + s;
+          const size_t at = unit.first + (row < 0 ? 0 : row < unit.n ? row : unit.n - 1);
+#pragma unroll
+          for (int x = 0; x < kMaxAxes; x++)
+            if (x < a.axes) place[s][x] = a.positions[at * a.axes + x];
+        }
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+          double angle[2] = {static_cast<double>(place[s][0]) * speed[0].x, static_cast<double>(place[s][0]) * speed[0].y};
+#pragma unroll
+          for (int x = 1; x < kMaxAxes; x++)
+            if (x < a.axes) {
+              angle[0] = __builtin_fma(static_cast<double>(place[s][x]), static_cast<double>(speed[x].x), angle[0]);
+              angle[1] = __builtin_fma(static_cast<double>(place[s][x]), static_cast<double>(speed[x].y), angle[1]);
+            }
+          const float2 u = cos_sin(angle[0]), v = cos_sin(angle[1]);
+          f[s] = v4f{u.x, u.y, v.x, v.y};
+        }
+      }
       v4f y[4] = {x[0], x[1], x[2], x[3]};
       norm_rotate(y, f);
       if (is_query) {
@@ -446,13 +484,16 @@ struct AttendArgs {
   float *out;
   float *part_o, *part_md;  // [row][head][part][64], [..][2]
   int max_len, chunk, parts, tiles;  // tiles: of 16 columns, for as many rows as a sequence can have
+  // Positions below base are those of sequence `prefix`, in the first first_part of the
+  // parts; own_parts hold a sequence's own.
+  int own_parts, first_part, base, prefix, prefix_chunk, beside;
 };
 
 // A sequence's rows for attention; false where there is nothing to do (n = 0) or it
 // is refused (bad), but for what `overlaps` says.
 __device__ __forceinline__ bool attend_span(const AttendArgs &a, int seq, int &len, int &first, int &n, bool &bad) {
   bad = !a.c.span(seq, len, first, n);
-  if (n > 8 || (n > 0 && len + n > a.max_len)) bad = true;
+  if (n > 8 || (n > 0 && (len + n > a.max_len || len < a.base))) bad = true;
   return n > 0 && !bad;
 }
 
@@ -541,6 +582,28 @@ __device__ __forceinline__ float row_max(float v) {
   return __builtin_fmaxf(v, row_ror<1>(v));
 }
 
+// A column's state from those of its runs, [run][column] in LDS: four dims of it.
+__device__ __forceinline__ v4f join_runs(const float *s_m, const float *s_den, const float (*s_o)[68], int col, int wide,
+                                         int runs, int dim, float &top, float &total) {
+  top = s_m[col];
+  total = 0.0f;
+  for (int w = 1; w < runs; w++) top = __builtin_fmaxf(top, s_m[w * wide + col]);
+  v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int w = 0; w < runs; w++) {
+    const int at = w * wide + col;
+    const float f = state_weight(s_m[at], s_den[at], top);
+    total = fmaf_(s_den[at], f, total);
+    const v4f x = *reinterpret_cast<const v4f *>(&s_o[at][dim]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = fmaf_(x[i], f, o[i]);
+  }
+  return o;
+}
+__device__ __forceinline__ void store_part(const AttendArgs &a, size_t at, int dim, const v4f &o, float top, float total) {
+  *reinterpret_cast<v4f *>(a.part_o + at * 64 + dim) = o;
+  if (dim == 0) *reinterpret_cast<float2 *>(a.part_md + at * 2) = make_float2(top, total);
+}
+
 // A workgroup takes one sequence, one key head's queries (its query heads times the
 // sequence's rows: columns, up to 16 of them) and one part of the keys. A wave takes
 // four columns and one run of the part's keys, 64 (four blocks) at a time: up to four
@@ -572,51 +635,28 @@ struct Stage {
   float k_scale, v_scale;
   bool none;
 };
-template <bool WIDE>
-__global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
-  const Cache &c = a.c;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // Workgroups go to the 8 XCDs in turn: those of the key heads of one value head
-  // follow one another on the same one, whose L2 then holds the values for all.
-  const int share = c.key_heads / c.kv_heads, turn_of = blockIdx.x / 8;
-  int task = (turn_of / share * 8 + blockIdx.x % 8) * share + turn_of % share;
-  const int key_head = task % c.key_heads;
-  task /= c.key_heads;
-  const int tile = task % a.tiles;
-  task /= a.tiles;
-  const int part = task % a.parts, seq = task / a.parts;
-  if (seq >= c.n_seqs) return;
-  const int group = c.n_heads / c.key_heads, value_head = key_head * c.kv_heads / c.key_heads;
-  int len, first, n;
-  bool bad;
-  const int start = start_of(c, seq);
-  if (!attend_span(a, seq, len, first, n, bad)) {
-    if (bad && a.parts == 1 && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
-    return;
-  }
-  const int limit = len + n, from_key = part * a.chunk;
-  if (16 * tile >= group * n || from_key >= limit) return;
-  // Waves: runs of the part's keys, in whole 64s, times quads of columns.
-  const int columns = group * n, left = columns - 16 * tile;
-  const int quads = left <= 4 ? 1 : left <= 8 ? 2 : 4, runs = 4 / quads, run = wave / quads, quad = wave % quads;
-  const int to_key = from_key + a.chunk < limit ? from_key + a.chunk : limit;
-  const int each = (to_key - from_key + 64 * runs - 1) / (64 * runs) * 64;
-  const int begin = from_key + run * each, end = begin + each < to_key ? begin + each : to_key;
-  const int column0 = 16 * tile + 4 * quad;
+struct Found {
+  int k_page, v_page;
+};
 
-  // 64 keys: lane's key block is l16 / 4 of four, its value block g. In a page of 64
-  // positions or more (WIDE) they follow one another, and their addresses are scalar
-  // but for the lane's share; otherwise each lane looks its blocks' pages up (past the
-  // last block, that one again). A block without a page is NaN.
-  const int last_block = (limit - 1) / kBlock, blocks_mask = (1 << c.shift) - 1;
-  const int32_t *table = c.table + static_cast<size_t>(seq) * c.seq_pages;
+// 64 keys: lane's key block is l16 / 4 of four, its value block g. In a page of 64
+// positions or more (WIDE) they follow one another, and their addresses are scalar
+// but for the lane's share; otherwise each lane looks its blocks' pages up (past the
+// last block, that one again). A block without a page is NaN.
+template <bool WIDE>
+struct Reader {
   typedef __attribute__((address_space(4))) const int32_t scalar_table;  // read by scalar loads
+  const Cache &c;
+  const int32_t *table;
+  int key_head, value_head, last_block;
   bool missing = false;
-  struct Found {
-    int k_page, v_page;
-  };
-  auto find = [&](int key0) {
+
+  __device__ __forceinline__ Reader(const Cache &cache, int seq, int head, int limit)
+      : c(cache), table(cache.table + static_cast<size_t>(seq) * cache.seq_pages), key_head(head),
+        value_head(head * cache.kv_heads / cache.key_heads), last_block((limit - 1) / kBlock) {}
+
+  __device__ __forceinline__ Found find(int key0) const {
+    const int l16 = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
     Found f;
     const int b = key0 / kBlock;
     if constexpr (WIDE) {
@@ -627,9 +667,10 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
       f.v_page = table[(b + g < last_block ? b + g : last_block) >> c.shift];
     }
     return f;
-  };
-  const int k_lane = l16 % 4 * 64 + g * 16, v_lane = l16 * 16;
-  auto load = [&](const Found &f, int key0, Stage &s) {
+  }
+  __device__ __forceinline__ void load(const Found &f, int key0, Stage &s) {
+    const int l16 = threadIdx.x & 15, g = threadIdx.x >> 4 & 3, blocks_mask = (1 << c.shift) - 1;
+    const int k_lane = l16 % 4 * 64 + g * 16, v_lane = l16 * 16;
     const int b = key0 / kBlock;
     const bool none = f.k_page < 0;
     missing |= none;
@@ -660,26 +701,20 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
 #pragma unroll
       for (int d = 0; d < 4; d++) s.v[d] = *reinterpret_cast<const v4i *>(v + d * 256);
     }
-  };
-  Found next;
-  Stage stage[2];
-  const bool works = begin < end && column0 < columns;
-  if (works) next = find(begin);
+  }
+};
 
-  // Column column0 + q: query row first + column % n, head key_head * group +
-  // column / n. Lane l16 brings row l16 of the first product (query l16 / 4, byte
-  // l16 % 4), lane (l16, g) works on query g.
+// Four columns of a wave. Lane l16 holds row l16 of the first product (query l16 / 4,
+// byte l16 % 4), lane (l16, g) works on query g.
+struct Quad {
   v4i digit;
-  float q_factor;
-  int visible;
-  if (works) {
-    float4 x[4];
-    const int wanted = column0 + l16 / 4, column = wanted < columns ? wanted : columns - 1;
-    const float *q = a.q + (static_cast<size_t>(first + column % n) * c.n_heads + key_head * group + column / n) * 64 + 16 * g;
-#pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = reinterpret_cast<const float4 *>(q)[i];
-    load(next, begin, stage[0]);
-    next = find(begin + 64);
+  float factor, m, den;
+  int visible;  // keys that query g sees
+  v4f acc[4];
+
+  // From 16 elements of query l16 / 4 (lane (l16, g): 16 g .. + 15).
+  __device__ __forceinline__ void begin(const float4 (&x)[4]) {
+    const int l16 = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
     uint32_t big = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -698,8 +733,8 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     int e = !finite || big == 0 ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(big));
     e = e < -90 ? -90 : e;
     // log2(e) / 8: scores in powers of two. From query l16 / 4 to query g.
-    const float factor = finite ? __builtin_ldexpf(0.180336880111120426f, e - 30) : __builtin_nanf("");
-    q_factor = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (4 * g), __float_as_int(factor)));
+    const float scale = finite ? __builtin_ldexpf(0.180336880111120426f, e - 30) : __builtin_nanf("");
+    factor = __int_as_float(__builtin_amdgcn_ds_bpermute(4 * (4 * g), __float_as_int(scale)));
     // Adding 128 to each lower byte of i and inverting their top bits leaves signed
     // bytes whose weighted sum is i.
     auto bytes = [&](float f) {
@@ -714,25 +749,15 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
       const uint32_t hi = __builtin_amdgcn_perm(bytes(x[i].w), bytes(x[i].z), pick);
       digit[i] = static_cast<int>(lo | hi << 16);
     }
-    const int mine = column0 + g;
-    visible = len + (mine < columns ? mine : columns - 1) % n + 1;
-  }
-  const float ninf = -__builtin_inff();
-  float m = ninf, den = 0.0f;
-  int power = -300;  // 2^power above every block scale of the values so far
-  v4f acc[4];
+    m = -__builtin_inff();
+    den = 0.0f;
 #pragma unroll
-  for (int d = 0; d < 4; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  // The parts of the weights: [column 4 d + q][64 keys], a wave's own. Rows of 72, so
-  // that 16 columns' 16 bytes lie in different banks; there is no fourth part.
-  constexpr int kTurned = 72;
-  __shared__ __attribute__((aligned(16))) uint16_t turned[4][16 * kTurned];
-  uint16_t *const turn_to = turned[wave] + g * kTurned + 4 * l16;
-  const uint16_t *const turn_from = turned[wave] + l16 * kTurned + 16 * g;
-  *reinterpret_cast<uint2 *>(turn_to + 12 * kTurned) = make_uint2(0, 0);
+    for (int d = 0; d < 4; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
 
   // The sums times `scaled` of query g: column 4 d + q's lanes take that of query q.
-  auto rescale = [&](float scaled) {
+  __device__ __forceinline__ void rescale(float scaled) {
+    const int l16 = threadIdx.x & 15;
     const float s0 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 0));
     const float s1 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 16));
     const float s2 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(scaled), 32));
@@ -742,66 +767,105 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     for (int d = 0; d < 4; d++)
 #pragma unroll
       for (int i = 0; i < 4; i++) acc[d][i] = acc[d][i] * f;
-  };
+  }
 
-  // Two FP32 numbers' upper halves, the first one's low.
-  auto upper = [](uint32_t second, uint32_t first) { return __builtin_amdgcn_perm(second, first, 0x07060302u); };
-  auto as_bf = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    const v4i words = {static_cast<int>(a), static_cast<int>(b), static_cast<int>(c), static_cast<int>(d)};
-    return __builtin_bit_cast(v8bf, words);
-  };
-  // Eight codes as BF16 numbers.
-  auto codes_of = [&](int first, int second) {
-    const uint32_t w[2] = {static_cast<uint32_t>(first), static_cast<uint32_t>(second)};
-    uint32_t to[4];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      to[2 * i] = upper(__float_as_uint(sdwa_cvt<1>(w[i])), __float_as_uint(sdwa_cvt<0>(w[i])));
-      to[2 * i + 1] = upper(__float_as_uint(sdwa_cvt<3>(w[i])), __float_as_uint(sdwa_cvt<2>(w[i])));
+  // The run's state to LDS: the four columns' m and den, and their sums [column][68].
+  __device__ __forceinline__ void end(int power, float *to_m, float *to_den, float (*to_o)[68]) {
+    const int l16 = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+    den = den + row_ror<8>(den);
+    den = den + row_ror<4>(den);
+    den = den + row_ror<2>(den);
+    den = den + row_ror<1>(den);
+    if (l16 == 0) {
+      to_m[g] = m;
+      to_den[g] = den;
     }
-    return as_bf(to[0], to[1], to[2], to[3]);
-  };
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+      v4f o;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        // Lane l16 < 4: the sums of lanes l16, + 4, + 8, the upper part's first.
+        const float x = acc[d][i];
+        o[i] = __builtin_ldexpf((row_ror<8>(x) + row_ror<12>(x)) + x, power - 64);
+      }
+      if (l16 < 4) *reinterpret_cast<v4f *>(&to_o[l16][16 * d + 4 * g]) = o;
+    }
+  }
+};
 
-  auto consume = [&](const Stage &s, int key0) {
-    // Blocks that hold none of the sequence's positions do not count; NaN reaches a
-    // row by its scores, which are those of the keys it sees.
-    float v_scale = key0 / kBlock + l16 / 4 <= last_block ? s.v_scale : 0.0f;
-    const bool bad = v_scale != v_scale;
-    const float k_scale = s.none || bad ? __builtin_nanf("") : s.k_scale;
-    v_scale = bad ? 0.0f : v_scale;
-    // The largest value scale of the four blocks (lanes 4 b .. + 3 of a row).
-    float widest = __builtin_fmaxf(v_scale, row_ror<4>(v_scale));
-    widest = __builtin_fmaxf(widest, row_ror<8>(widest));
-    int above = widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -300;
-    above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
-    const int lower = power - above;
-    power = above;
-    const float weight = __builtin_ldexpf(v_scale, 64 - power);
+// Two FP32 numbers' upper halves, the first one's low.
+__device__ __forceinline__ uint32_t upper(uint32_t second, uint32_t first) {
+  return __builtin_amdgcn_perm(second, first, 0x07060302u);
+}
+// Eight codes as BF16 numbers.
+__device__ __forceinline__ v8bf codes_of(int first, int second) {
+  const uint32_t w[2] = {static_cast<uint32_t>(first), static_cast<uint32_t>(second)};
+  v4i to;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    to[2 * i] = static_cast<int>(upper(__float_as_uint(sdwa_cvt<1>(w[i])), __float_as_uint(sdwa_cvt<0>(w[i]))));
+    to[2 * i + 1] = static_cast<int>(upper(__float_as_uint(sdwa_cvt<3>(w[i])), __float_as_uint(sdwa_cvt<2>(w[i]))));
+  }
+  return __builtin_bit_cast(v8bf, to);
+}
+
+// The parts of the weights: [column 4 d + q][64 keys], a wave's own for four columns.
+// Rows of 72, so that 16 columns' 16 bytes lie in different banks; there is no fourth part.
+constexpr int kTurned = 72;
+
+// 64 keys from key0 on for all of a wave's columns. `turned` is the wave's own. 2^power
+// is above every block scale of the values so far.
+template <int QUADS>
+__device__ __forceinline__ void consume(Quad (&quad)[QUADS], int &power, const Stage &s, int key0, int last_block,
+                                        uint16_t *turned) {
+  const int l16 = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
+  const float ninf = -__builtin_inff();
+  // Blocks that hold none of the sequence's positions do not count; NaN reaches a
+  // row by its scores, which are those of the keys it sees.
+  float v_scale = key0 / kBlock + l16 / 4 <= last_block ? s.v_scale : 0.0f;
+  const bool bad = v_scale != v_scale;
+  const float k_scale = s.none || bad ? __builtin_nanf("") : s.k_scale;
+  v_scale = bad ? 0.0f : v_scale;
+  // The largest value scale of the four blocks (lanes 4 b .. + 3 of a row).
+  float widest = __builtin_fmaxf(v_scale, row_ror<4>(v_scale));
+  widest = __builtin_fmaxf(widest, row_ror<8>(widest));
+  int above = widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -300;
+  above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
+  const int lower = power - above;
+  power = above;
+  const float weight = __builtin_ldexpf(v_scale, 64 - power);
+  uint16_t *const turn_to = turned + g * kTurned + 4 * l16;
+  const uint16_t *const turn_from = turned + l16 * kTurned + 16 * g;
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < QUADS; i++) {
+    Quad &u = quad[i];
     float p[4];
-    const float factor = q_factor * k_scale;
+    const float factor = u.factor * k_scale;
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       const v4i zero = {0, 0, 0, 0};
-      const v4i dots = __builtin_amdgcn_mfma_i32_16x16x64_i8(digit, s.k[t], zero, 0, 0, 0);
+      const v4i dots = __builtin_amdgcn_mfma_i32_16x16x64_i8(u.digit, s.k[t], zero, 0, 0, 0);
       // A sum is below 2^20, so two of them fit 32 bits.
       const float sum = fmaf_(static_cast<float>((dots[3] << 8) + dots[2]), 65536.0f, static_cast<float>((dots[1] << 8) + dots[0]));
       p[t] = sum * factor;
-      if (key0 + 4 * l16 + t >= visible) p[t] = ninf;
+      if (key0 + 4 * l16 + t >= u.visible) p[t] = ninf;
     }
     float top = __builtin_fmaxf(__builtin_fmaxf(p[0], p[1]), __builtin_fmaxf(p[2], p[3]));
-    top = __builtin_fmaxf(m, row_max(top));
+    top = __builtin_fmaxf(u.m, row_max(top));
     const float from = top == ninf ? 0.0f : top;
-    if (__any(top > m) || lower < 0) {
-      const float keep = __builtin_amdgcn_exp2f(m - from);
-      den = den * keep;
-      rescale(__builtin_ldexpf(keep, lower));
-      m = top;
+    if (__any(top > u.m) || lower < 0) {
+      const float keep = __builtin_amdgcn_exp2f(u.m - from);
+      u.den = u.den * keep;
+      u.rescale(__builtin_ldexpf(keep, lower));
+      u.m = top;
     }
     uint32_t part[3][4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
       const float e = __builtin_amdgcn_exp2f(p[t] - from);
-      den = den + e;
+      u.den = u.den + e;
       float left = e * weight;
 #pragma unroll
       for (int d = 0; d < 3; d++) {
@@ -809,46 +873,120 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
         left = left - __uint_as_float(part[d][t] & 0xffff0000u);
       }
     }
-    asm volatile("" ::: "memory");
 #pragma unroll
     for (int d = 0; d < 3; d++)
-      *reinterpret_cast<uint2 *>(turn_to + 4 * d * kTurned) = make_uint2(upper(part[d][1], part[d][0]), upper(part[d][3], part[d][2]));
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    const v8bf low = *reinterpret_cast<const v8bf *>(turn_from), high = *reinterpret_cast<const v8bf *>(turn_from + 8);
-    asm volatile("" ::: "memory");
+      *reinterpret_cast<uint2 *>(turn_to + (16 * i + 4 * d) * kTurned) =
+          make_uint2(upper(part[d][1], part[d][0]), upper(part[d][3], part[d][2]));
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  v8bf low[QUADS], high[QUADS];
 #pragma unroll
-    for (int d = 0; d < 4; d++) {
-      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_of(s.v[d][0], s.v[d][1]), low, acc[d], 0, 0, 0);
-      acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_of(s.v[d][2], s.v[d][3]), high, acc[d], 0, 0, 0);
-    }
-  };
-  // While one 64 keys are worked on, the next are on their way, and before them the
-  // pages of those after: no load is under a branch, so the waits count what is
-  // still out.
-  auto turn = [&](const Stage &now, Stage &then, int key0, auto more) {
-    if constexpr (decltype(more)::value) {
-      const Found after = find(key0 + 128);
-      load(next, key0 + 64, then);
-      next = after;
-    }
-    consume(now, key0);
-  };
-  if (works) {
-    const std::true_type more;
-    const std::false_type no_more;
-    int key0 = begin;
-    for (; key0 + 128 < end; key0 += 128) {
-      turn(stage[0], stage[1], key0, more);
-      turn(stage[1], stage[0], key0 + 64, more);
-    }
-    if (key0 + 64 < end) {
-      turn(stage[0], stage[1], key0, more);
-      turn(stage[1], stage[0], key0 + 64, no_more);
-    } else {
-      turn(stage[0], stage[1], key0, no_more);
+  for (int i = 0; i < QUADS; i++) {
+    low[i] = *reinterpret_cast<const v8bf *>(turn_from + 16 * i * kTurned);
+    high[i] = *reinterpret_cast<const v8bf *>(turn_from + 16 * i * kTurned + 8);
+  }
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int d = 0; d < 4; d++) {
+    const v8bf first = codes_of(s.v[d][0], s.v[d][1]), second = codes_of(s.v[d][2], s.v[d][3]);
+#pragma unroll
+    for (int i = 0; i < QUADS; i++) {
+      quad[i].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(first, low[i], quad[i].acc[d], 0, 0, 0);
+      quad[i].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(second, high[i], quad[i].acc[d], 0, 0, 0);
     }
   }
-  if (__any(missing) && lane == 0) c.refused[seq] = 1;
+}
+
+// A wave's run of keys. While one 64 keys are worked on, the next are on their way,
+// and before them the pages of those after: no load is under a branch, so the waits
+// count what is still out. stage[0] holds the first 64, `next` the pages of the second.
+template <int QUADS, bool WIDE>
+__device__ __forceinline__ void walk(Quad (&quad)[QUADS], int &power, Reader<WIDE> &reader, Stage (&stage)[2], Found next,
+                                     int begin, int end, uint16_t *turned) {
+  auto turn = [&](const Stage &now, Stage &then, int key0, auto more) {
+    if constexpr (decltype(more)::value) {
+      const Found after = reader.find(key0 + 128);
+      reader.load(next, key0 + 64, then);
+      next = after;
+    }
+    consume<QUADS>(quad, power, now, key0, reader.last_block, turned);
+  };
+  const std::true_type more;
+  const std::false_type no_more;
+  int key0 = begin;
+  for (; key0 + 128 < end; key0 += 128) {
+    turn(stage[0], stage[1], key0, more);
+    turn(stage[1], stage[0], key0 + 64, more);
+  }
+  if (key0 + 64 < end) {
+    turn(stage[0], stage[1], key0, more);
+    turn(stage[1], stage[0], key0 + 64, no_more);
+  } else {
+    turn(stage[0], stage[1], key0, no_more);
+  }
+}
+
+template <bool WIDE>
+__global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Workgroups go to the 8 XCDs in turn: those of the key heads of one value head
+  // follow one another on the same one, whose L2 then holds the values for all.
+  const int share = c.key_heads / c.kv_heads, turn_of = blockIdx.x / 8;
+  int task = (turn_of / share * 8 + blockIdx.x % 8) * share + turn_of % share;
+  const int key_head = task % c.key_heads;
+  task /= c.key_heads;
+  const int tile = task % a.tiles;
+  task /= a.tiles;
+  const int part = task % a.own_parts, seq = task / a.own_parts;
+  if (seq >= c.n_seqs) return;
+  const int group = c.n_heads / c.key_heads;
+  int len, first, n;
+  bool bad;
+  const int start = start_of(c, seq);
+  if (!attend_span(a, seq, len, first, n, bad)) {
+    if (bad && a.parts == 1 && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
+    return;
+  }
+  const int limit = len + n, from_key = a.base + part * a.chunk;
+  if (16 * tile >= group * n || from_key >= limit) return;
+  // Waves: runs of the part's keys, in whole 64s, times quads of columns.
+  const int columns = group * n, left = columns - 16 * tile;
+  const int quads = left <= 4 ? 1 : left <= 8 ? 2 : 4, runs = 4 / quads, run = wave / quads, at_quad = wave % quads;
+  const int to_key = from_key + a.chunk < limit ? from_key + a.chunk : limit;
+  const int each = (to_key - from_key + 64 * runs - 1) / (64 * runs) * 64;
+  const int begin = from_key + run * each, end = begin + each < to_key ? begin + each : to_key;
+  const int column0 = 16 * tile + 4 * at_quad;
+
+  Reader<WIDE> reader(c, seq, key_head, limit);
+  Found next;
+  Stage stage[2];
+  Quad quad[1];
+  quad[0].m = -__builtin_inff();
+  quad[0].den = 0.0f;
+#pragma unroll
+  for (int d = 0; d < 4; d++) quad[0].acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  int power = -300;
+  __shared__ __attribute__((aligned(16))) uint16_t turned[4][16 * kTurned];
+  *reinterpret_cast<uint2 *>(turned[wave] + (12 + g) * kTurned + 4 * l16) = make_uint2(0, 0);
+  const bool works = begin < end && column0 < columns;
+  if (works) {
+    next = reader.find(begin);
+    // Column column0 + q: query row first + column % n, head key_head * group + column / n.
+    float4 x[4];
+    const int wanted = column0 + l16 / 4, column = wanted < columns ? wanted : columns - 1;
+    const float *q = a.q + (static_cast<size_t>(first + column % n) * c.n_heads + key_head * group + column / n) * 64 + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = reinterpret_cast<const float4 *>(q)[i];
+    reader.load(next, begin, stage[0]);
+    next = reader.find(begin + 64);
+    quad[0].begin(x);
+    const int mine = column0 + g;
+    quad[0].visible = len + (mine < columns ? mine : columns - 1) % n + 1;
+    walk<1, WIDE>(quad, power, reader, stage, next, begin, end, turned[wave]);
+  }
+  if (__any(reader.missing) && lane == 0) c.refused[seq] = 1;
   // Asked here, where no load is waited for.
   if (overlaps(c, seq, first, start)) {
     if (a.parts == 1 && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
@@ -858,53 +996,135 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   // The waves' states meet in LDS: [run][column], 16 in all.
   __shared__ float s_m[16], s_den[16];
   __shared__ __attribute__((aligned(16))) float s_o[16][68];
-  den = den + row_ror<8>(den);
-  den = den + row_ror<4>(den);
-  den = den + row_ror<2>(den);
-  den = den + row_ror<1>(den);
-  if (l16 == 0) {
-    s_m[4 * wave + g] = m;
-    s_den[4 * wave + g] = den;
-  }
-#pragma unroll
-  for (int d = 0; d < 4; d++) {
-    v4f o;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      // Lane l16 < 4: the sums of lanes l16, + 4, + 8, the upper part's first.
-      const float x = acc[d][i];
-      o[i] = __builtin_ldexpf((row_ror<8>(x) + row_ror<12>(x)) + x, power - 64);
-    }
-    if (l16 < 4) *reinterpret_cast<v4f *>(&s_o[4 * wave + l16][16 * d + 4 * g]) = o;
-  }
+  quad[0].end(power, s_m + 4 * wave, s_den + 4 * wave, s_o + 4 * wave);
   __syncthreads();
   // Thread: a column and four dims.
   const int col = threadIdx.x / 16, dim = threadIdx.x % 16 * 4, wide = 4 * quads;
   const int out_column = 16 * tile + col;
   if (col >= wide || out_column >= columns) return;
-  float top = s_m[col], total = 0.0f;
-  for (int w = 1; w < runs; w++) top = __builtin_fmaxf(top, s_m[w * wide + col]);
-  v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int w = 0; w < runs; w++) {
-    const int at = w * wide + col;
-    const float f = state_weight(s_m[at], s_den[at], top);
-    total = fmaf_(s_den[at], f, total);
-    const v4f x = *reinterpret_cast<const v4f *>(&s_o[at][dim]);
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = fmaf_(x[i], f, o[i]);
-  }
+  float top, total;
+  const v4f o = join_runs(s_m, s_den, s_o, col, wide, runs, dim, top, total);
   const int out_head = key_head * group + out_column / n;
   const size_t out_row = static_cast<size_t>(first + out_column % n) * c.n_heads + out_head;
   if (a.parts == 1) {
     const float factor = sink_factor(a.sinks, out_head, top, total);
+    v4f y;
 #pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = __fdiv_rn(o[i], total) * factor;
-    *reinterpret_cast<v4f *>(a.out + out_row * 64 + dim) = o;
+    for (int i = 0; i < 4; i++) y[i] = __fdiv_rn(o[i], total) * factor;
+    *reinterpret_cast<v4f *>(a.out + out_row * 64 + dim) = y;
     return;
   }
-  const size_t at = out_row * a.parts + part;
-  *reinterpret_cast<v4f *>(a.part_o + at * 64 + dim) = o;
-  if (dim == 0) *reinterpret_cast<float2 *>(a.part_md + at * 2) = make_float2(top, total);
+  store_part(a, out_row * a.parts + a.first_part + part, dim, o, top, total);
+}
+
+// ---- attention over a prefix that the batch shares ----------------------------------
+// The rows of a call see positions below `base` in the pages of one sequence, the
+// prefix, each row all of them, so all rows' queries of a key head are columns of the same
+// products, and the keys are read once for 64 columns at a time. What a row sees behind
+// `base` are its own sequence's positions (attend_kernel), and merge_kernel joins both:
+// with states (m_i, d_i, o_i) of disjoint keys, m = max m_i, o = sum 2^(m_i - m) o_i /
+// sum 2^(m_i - m) d_i.
+//
+// A wave takes 4 QUADS columns, so that a key's codes are loaded, and its values' turned
+// to BF16, once for all of them; a workgroup's four waves stand side by side over
+// up to 16 QUADS columns (`beside` of them), or over one run of the keys each.
+template <bool WIDE, int QUADS>
+__global__ __launch_bounds__(256, QUADS == 4 ? 2 : 3) void prefix_kernel(AttendArgs a) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // The key heads of one value head, and all tiles of their columns, follow one
+  // another on one XCD.
+  const int share = c.key_heads / c.kv_heads;
+  int task = blockIdx.x / 8;
+  const int sharer = task % share;
+  task /= share;
+  const int tile = task % a.tiles;
+  task = task / a.tiles * 8 + blockIdx.x % 8;
+  const int value_head = task % c.kv_heads, part = task / c.kv_heads;
+  if (part >= a.first_part) return;
+  const int key_head = value_head * share + sharer, group = c.n_heads / c.key_heads, columns = group * c.rows;
+  const int beside = a.beside, across = 4 * QUADS * beside, runs = 4 / beside, run = wave / beside;
+  const int tile0 = tile * across, column0 = tile0 + wave % beside * 4 * QUADS;
+  // The tile's rows, and which sequence each is of (-1: none that takes part).
+  const int row0 = tile0 / group, row_end = (tile0 + across - 1) / group + 1;
+  const int rows = (row_end < c.rows ? row_end : c.rows) - row0;
+  __shared__ int owner[16 * QUADS];
+  if (threadIdx.x < 16 * QUADS) owner[threadIdx.x] = -1;
+  __syncthreads();
+  const int seq0 = c.row_start ? 0 : row0, seq_end = c.row_start ? c.n_seqs : row0 + rows;
+  for (int seq = seq0 + threadIdx.x; seq < seq_end; seq += 256) {
+    int len, first, n;
+    bool bad;
+    if (!attend_span(a, seq, len, first, n, bad)) continue;
+    for (int r = first > row0 ? first : row0; r < first + n && r < row0 + rows; r++) atomicMax(owner + (r - row0), seq);
+  }
+  __syncthreads();
+  const unsigned long long live = __ballot(lane < rows && owner[lane < rows ? lane : 0] >= 0);
+  if (live == 0) return;
+  const int some = __ffsll(live) - 1;
+
+  const int from_key = part * a.prefix_chunk, to_key = from_key + a.prefix_chunk < a.base ? from_key + a.prefix_chunk : a.base;
+  const int each = (to_key - from_key + 64 * runs - 1) / (64 * runs) * 64;
+  const int begin = from_key + run * each, end = begin + each < to_key ? begin + each : to_key;
+  Reader<WIDE> reader(c, a.prefix, key_head, a.base);
+  Stage stage[2];
+  Quad quad[QUADS];
+#pragma unroll
+  for (int i = 0; i < QUADS; i++) {
+    quad[i].m = -__builtin_inff();
+    quad[i].den = 0.0f;
+#pragma unroll
+    for (int d = 0; d < 4; d++) quad[i].acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  int power = -300;
+  __shared__ __attribute__((aligned(16))) uint16_t turned[4][QUADS * 16 * kTurned];
+#pragma unroll
+  for (int i = 0; i < QUADS; i++)
+    *reinterpret_cast<uint2 *>(turned[wave] + (16 * i + 12 + g) * kTurned + 4 * l16) = make_uint2(0, 0);
+  if (begin < end && column0 < columns) {
+    Found next = reader.find(begin);
+    // Column column0 + q: row column / group, head key_head * group + column % group. A
+    // column that is no row's takes another's query, and is left out in the end.
+    float4 x[QUADS][4];
+#pragma unroll
+    for (int i = 0; i < QUADS; i++) {
+      const int wanted = column0 + 4 * i + l16 / 4, column = wanted < columns ? wanted : columns - 1;
+      int row = column / group - row0;
+      row = live >> row & 1 ? row : some;
+      const float *q = a.q + (static_cast<size_t>(row0 + row) * c.n_heads + key_head * group + column % group) * 64 + 16 * g;
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[i][j] = reinterpret_cast<const float4 *>(q)[j];
+    }
+    reader.load(next, begin, stage[0]);
+    next = reader.find(begin + 64);
+#pragma unroll
+    for (int i = 0; i < QUADS; i++) {
+      quad[i].begin(x[i]);
+      quad[i].visible = a.base;
+    }
+    walk<QUADS, WIDE>(quad, power, reader, stage, next, begin, end, turned[wave]);
+  }
+  if (__any(reader.missing) && lane < rows && owner[lane] >= 0) c.refused[owner[lane]] = 1;
+
+  // The waves' states meet in LDS: [run][column].
+  __shared__ float s_m[16 * QUADS], s_den[16 * QUADS];
+  __shared__ __attribute__((aligned(16))) float s_o[16 * QUADS][68];
+#pragma unroll
+  for (int i = 0; i < QUADS; i++) {
+    const int at = 4 * QUADS * wave + 4 * i;
+    quad[i].end(power, s_m + at, s_den + at, s_o + at);
+  }
+  __syncthreads();
+  const int dim = threadIdx.x % 16 * 4;
+  for (int col = threadIdx.x / 16; col < across; col += 16) {
+    const int column = tile0 + col;
+    if (column >= columns || owner[column / group - row0] < 0) continue;
+    float top, total;
+    const v4f o = join_runs(s_m, s_den, s_o, col, across, runs, dim, top, total);
+    const size_t out_row = static_cast<size_t>(column / group) * c.n_heads + key_head * group + column % group;
+    store_part(a, out_row * a.parts + part, dim, o, top, total);
+  }
 }
 
 // The parts of a sequence's rows of one head: as many of the waves for each row as
@@ -925,7 +1145,7 @@ __global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttendArgs a) {
   if (!live) return;
   const int spread = n == 1 ? 1 : n == 2 ? 2 : n <= 4 ? 4 : 8;
   const int waves = spread < WAVES ? WAVES / spread : 1, own = wave % waves;
-  const int parts = (len + n - 1) / a.chunk + 1;
+  const int parts = a.first_part + (len + n - a.base - 1) / a.chunk + 1;
   for (int r0 = 0; r0 < n; r0 += WAVES / waves) {
     const int r = r0 + wave / waves;
     const size_t row = static_cast<size_t>(first + (r < n ? r : 0)) * c.n_heads + head, at = row * a.parts;
@@ -1064,11 +1284,107 @@ int launch_append(Ctx *ctx, AppendArgs a, bool qkv) {
     const unsigned eights = static_cast<unsigned>((units + 7) / 8), y = std::min(eights, 32768u);
     grid = dim3(8 * groups, y, (eights + y - 1) / y);
   }
-  if (qkv)
-    hipLaunchKernelGGL(append_kernel<true>, grid, dim3(256), 0, ctx->stream, a);
+  if (a.positions)
+    hipLaunchKernelGGL((append_kernel<true, true>), grid, dim3(256), 0, ctx->stream, a);
+  else if (qkv)
+    hipLaunchKernelGGL((append_kernel<true, false>), grid, dim3(256), 0, ctx->stream, a);
   else
-    hipLaunchKernelGGL(append_kernel<false>, grid, dim3(256), 0, ctx->stream, a);
+    hipLaunchKernelGGL((append_kernel<false, false>), grid, dim3(256), 0, ctx->stream, a);
   FOCR_HIP_CHECK(hipGetLastError());
+  return FOCR_OK;
+}
+
+// Attention, where shared > 0 over that many positions of sequence `prefix` first.
+int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, size_t rows, const int32_t *row_start,
+                  const int32_t *lens, size_t n_seqs, size_t max_len, size_t prefix, size_t shared, const float *sinks,
+                  float *out) {
+  int rc = check_batch(name, ctx, kv, rows, row_start, lens, n_seqs);
+  if (rc != FOCR_OK) return rc;
+  FOCR_REQUIRE(prefix < kv->n_seqs, FOCR_E_SHAPE, std::string(name) + ": the cache has no such sequence");
+  FOCR_REQUIRE(shared % kv->page == 0 && shared <= kv->seq_pages * kv->page, FOCR_E_SHAPE,
+               std::string(name) + ": the shared positions are whole pages of a sequence");
+  if (rows == 0 || n_seqs == 0) return FOCR_OK;
+  FOCR_REQUIRE(q && out, FOCR_E_ARG, std::string(name) + ": null buffer");
+  FOCR_REQUIRE(max_len > shared && max_len <= kv->seq_pages * kv->page, FOCR_E_SHAPE,
+               std::string(name) + ": max_len is more than the shared positions, up to what a sequence's pages hold");
+  AttendArgs a = {};
+  a.c = cache_of(kv, rows, row_start, lens, n_seqs);
+  a.q = q;
+  a.sinks = sinks;
+  a.out = out;
+  a.max_len = static_cast<int>(max_len);
+  a.base = static_cast<int>(shared);
+  a.prefix = static_cast<int>(prefix);
+  const size_t most = row_start ? std::min<size_t>(rows, 8) : 1;
+  const size_t group = kv->n_heads / kv->key_heads, own = max_len - shared;
+  a.tiles = static_cast<int>((group * most + 15) / 16);
+  // Parts of whole 256 keys, at most 4,096 up to a million positions. Few sequences
+  // need only fill the chip (us a call with 512 / 1,024 / 2,048 workgroups: one of
+  // 131,072 positions 32.9 / 36.8 / 37.7, four of up to 16,000 16.3 / 17.8 / 18.8; six of
+  // up to 3,000 with up to 8 rows 17.6 / 15.4 / 15.9); more, of different lengths, want
+  // parts to spare (20 of up to 9,000 49.0 / 47.1 / 44.7, 40 of up to 5,000 with up to 8
+  // rows 84.7 / 84.8 / 63.7).
+  const size_t heads = n_seqs * kv->key_heads * a.tiles;
+  const size_t enough = n_seqs <= 2 ? 512 : n_seqs <= 8 ? 1024 : 2048;
+  const size_t want = heads >= enough ? 1 : enough / heads;
+  const size_t chunk = std::max(std::min<size_t>((own + want - 1) / want, 4096), (own + kMaxParts - 1) / kMaxParts);
+  a.chunk = static_cast<int>((chunk + 255) / 256 * 256);
+  a.own_parts = static_cast<int>((own + a.chunk - 1) / a.chunk);
+  const size_t share = kv->key_heads / kv->kv_heads;
+  const size_t grid = (heads * a.own_parts + 8 * share - 1) / (8 * share) * (8 * share);
+  FOCR_REQUIRE(grid < (size_t(1) << 31), FOCR_E_SHAPE, std::string(name) + ": too many sequences and heads");
+  AttendArgs before = a;  // the prefix's kernel: other tiles
+  size_t before_grid = 0;
+  int quads = 0;
+  if (shared > 0) {
+    const size_t columns = group * rows;
+    quads = columns <= 4 ? 1 : columns <= 8 ? 2 : 4;
+    a.beside = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
+    const size_t across = 4 * quads * a.beside, tiles = (columns + across - 1) / across;
+    const size_t each = kv->key_heads * tiles, parts = each >= 512 ? 1 : 512 / each;
+    const size_t prefix_chunk = std::max((shared + parts - 1) / parts, (shared + kMaxParts - 1) / kMaxParts);
+    a.prefix_chunk = static_cast<int>((prefix_chunk + 63) / 64 * 64);
+    a.first_part = static_cast<int>((shared + a.prefix_chunk - 1) / a.prefix_chunk);
+    before_grid = (kv->kv_heads * a.first_part + 7) / 8 * 8 * share * tiles;
+    FOCR_REQUIRE(before_grid < (size_t(1) << 31), FOCR_E_SHAPE, std::string(name) + ": too many rows and heads");
+    before = a;
+    before.tiles = static_cast<int>(tiles);
+  }
+  a.parts = before.parts = a.first_part + a.own_parts;
+  const size_t slots = rows * kv->n_heads * a.parts;
+  FOCR_HIP_CHECK(hipSetDevice(ctx->device));
+  if (a.parts > 1) {
+    rc = ensure_scratch(ctx, slots * 66 * sizeof(float));
+    if (rc != FOCR_OK) return rc;
+    a.part_o = before.part_o = static_cast<float *>(ctx->scratch);
+    a.part_md = before.part_md = a.part_o + slots * 64;
+  }
+  const bool wide = kv->page >= 64;
+  if (before_grid > 0) {
+    const dim3 all(static_cast<unsigned>(before_grid));
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, all, dim3(256), 0, ctx->stream, before); };
+    if (wide)
+      launch(quads == 1 ? prefix_kernel<true, 1> : quads == 2 ? prefix_kernel<true, 2> : prefix_kernel<true, 4>);
+    else
+      launch(quads == 1 ? prefix_kernel<false, 1> : quads == 2 ? prefix_kernel<false, 2> : prefix_kernel<false, 4>);
+    FOCR_HIP_CHECK(hipGetLastError());
+  }
+  if (wide)
+    hipLaunchKernelGGL(attend_kernel<true>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
+  else
+    hipLaunchKernelGGL(attend_kernel<false>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
+  FOCR_HIP_CHECK(hipGetLastError());
+  if (a.parts > 1) {
+    const dim3 each(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(n_seqs));
+    // Parts of all a sequence's rows (us a call with 4 / 16 waves: 26 parts of one row
+    // 9.8 / 10.4, 3 of one in 64 sequences 112 / 120; 57 of two 34.8 / 32.8, 59 of
+    // eight 33.3 / 20.3).
+    if (a.parts * most <= 64)
+      hipLaunchKernelGGL(merge_kernel<4>, each, dim3(256), 0, ctx->stream, a);
+    else
+      hipLaunchKernelGGL(merge_kernel<16>, each, dim3(1024), 0, ctx->stream, a);
+    FOCR_HIP_CHECK(hipGetLastError());
+  }
   return FOCR_OK;
 }
 
@@ -1224,65 +1540,41 @@ int focr_kv_pages_qkv_rows(focr_ctx *handle, focr_kv_pages *pages, const float *
   return launch_append(ctx, a, true);
 }
 
+int focr_kv_pages_qkv_rows_at(focr_ctx *handle, focr_kv_pages *pages, const float *qkv, size_t rows,
+                              const float *positions, size_t axes, const float *frequencies, const int32_t *row_start,
+                              const int32_t *lens, size_t n_seqs, float *q) {
+  Ctx *ctx = reinterpret_cast<Ctx *>(handle);
+  Pages *kv = reinterpret_cast<Pages *>(pages);
+  const int rc = check_batch("focr_kv_pages_qkv_rows_at", ctx, kv, rows, row_start, lens, n_seqs);
+  if (rc != FOCR_OK) return rc;
+  FOCR_REQUIRE(axes >= 1 && axes <= kMaxAxes, FOCR_E_SHAPE, "focr_kv_pages_qkv_rows_at: 1 to 4 axes");
+  if (rows == 0 || n_seqs == 0) return FOCR_OK;
+  FOCR_REQUIRE(qkv && positions && frequencies && q, FOCR_E_ARG, "focr_kv_pages_qkv_rows_at: null buffer");
+  FOCR_REQUIRE(reinterpret_cast<uintptr_t>(frequencies) % 8 == 0, FOCR_E_ARG,
+               "focr_kv_pages_qkv_rows_at: frequencies stand on 8 bytes");
+  AppendArgs a = {};
+  a.c = cache_of(kv, rows, row_start, lens, n_seqs);
+  a.qkv = qkv;
+  a.positions = positions;
+  a.frequencies = frequencies;
+  a.axes = static_cast<int>(axes);
+  a.q = q;
+  return launch_append(ctx, a, true);
+}
+
 int focr_kv_pages_attention(focr_ctx *handle, const focr_kv_pages *pages, const float *q, size_t rows,
                             const int32_t *row_start, const int32_t *lens, size_t n_seqs, size_t max_len,
                             const float *sinks, float *out) {
-  Ctx *ctx = reinterpret_cast<Ctx *>(handle);
-  const Pages *kv = reinterpret_cast<const Pages *>(pages);
-  int rc = check_batch("focr_kv_pages_attention", ctx, kv, rows, row_start, lens, n_seqs);
-  if (rc != FOCR_OK || rows == 0 || n_seqs == 0) return rc;
-  FOCR_REQUIRE(q && out, FOCR_E_ARG, "focr_kv_pages_attention: null buffer");
-  FOCR_REQUIRE(max_len > 0 && max_len <= kv->seq_pages * kv->page, FOCR_E_SHAPE,
-               "focr_kv_pages_attention: max_len is 1 .. what a sequence's pages hold");
-  AttendArgs a = {};
-  a.c = cache_of(kv, rows, row_start, lens, n_seqs);
-  a.q = q;
-  a.sinks = sinks;
-  a.out = out;
-  a.max_len = static_cast<int>(max_len);
-  const size_t most = row_start ? std::min<size_t>(rows, 8) : 1;
-  const size_t group = kv->n_heads / kv->key_heads;
-  a.tiles = static_cast<int>((group * most + 15) / 16);
-  // Parts of whole 256 keys, at most 4,096 up to a million positions. Few sequences
-  // need only fill the chip (us a call with 512 / 1,024 / 2,048 workgroups: one of
-  // 131,072 positions 32.9 / 36.8 / 37.7, four of up to 16,000 16.3 / 17.8 / 18.8; six of
-  // up to 3,000 with up to 8 rows 17.6 / 15.4 / 15.9); more, of different lengths, want
-  // parts to spare (20 of up to 9,000 49.0 / 47.1 / 44.7, 40 of up to 5,000 with up to 8
-  // rows 84.7 / 84.8 / 63.7).
-  const size_t heads = n_seqs * kv->key_heads * a.tiles;
-  const size_t enough = n_seqs <= 2 ? 512 : n_seqs <= 8 ? 1024 : 2048;
-  const size_t want = heads >= enough ? 1 : enough / heads;
-  const size_t chunk = std::max(std::min<size_t>((max_len + want - 1) / want, 4096), (max_len + kMaxParts - 1) / kMaxParts);
-  a.chunk = static_cast<int>((chunk + 255) / 256 * 256);
-  a.parts = static_cast<int>((max_len + a.chunk - 1) / a.chunk);
-  const size_t share = kv->key_heads / kv->kv_heads;
-  const size_t grid = (heads * a.parts + 8 * share - 1) / (8 * share) * (8 * share);
-  FOCR_REQUIRE(grid < (size_t(1) << 31), FOCR_E_SHAPE, "focr_kv_pages_attention: too many sequences and heads");
-  const size_t slots = rows * kv->n_heads * a.parts;
-  FOCR_HIP_CHECK(hipSetDevice(ctx->device));
-  if (a.parts > 1) {
-    rc = ensure_scratch(ctx, slots * 66 * sizeof(float));
-    if (rc != FOCR_OK) return rc;
-    a.part_o = static_cast<float *>(ctx->scratch);
-    a.part_md = a.part_o + slots * 64;
-  }
-  if (kv->page >= 64)
-    hipLaunchKernelGGL(attend_kernel<true>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
-  else
-    hipLaunchKernelGGL(attend_kernel<false>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
-  FOCR_HIP_CHECK(hipGetLastError());
-  if (a.parts > 1) {
-    const dim3 each(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(n_seqs));
-    // Parts of all a sequence's rows (us a call with 4 / 16 waves: 26 parts of one row
-    // 9.8 / 10.4, 3 of one in 64 sequences 112 / 120; 57 of two 34.8 / 32.8, 59 of
-    // eight 33.3 / 20.3).
-    if (a.parts * most <= 64)
-      hipLaunchKernelGGL(merge_kernel<4>, each, dim3(256), 0, ctx->stream, a);
-    else
-      hipLaunchKernelGGL(merge_kernel<16>, each, dim3(1024), 0, ctx->stream, a);
-    FOCR_HIP_CHECK(hipGetLastError());
-  }
-  return FOCR_OK;
+  return launch_attend("focr_kv_pages_attention", reinterpret_cast<Ctx *>(handle), reinterpret_cast<const Pages *>(pages), q,
+                       rows, row_start, lens, n_seqs, max_len, 0, 0, sinks, out);
+}
+
+int focr_kv_pages_attention_shared(focr_ctx *handle, const focr_kv_pages *pages, const float *q, size_t rows,
+                                   const int32_t *row_start, const int32_t *lens, size_t n_seqs, size_t max_len,
+                                   size_t prefix_seq, size_t shared_len, const float *sinks, float *out) {
+  return launch_attend("focr_kv_pages_attention_shared", reinterpret_cast<Ctx *>(handle),
+                       reinterpret_cast<const Pages *>(pages), q, rows, row_start, lens, n_seqs, max_len, prefix_seq,
+                       shared_len, sinks, out);
 }
 
 int focr_kv_pages_dequantize(focr_ctx *handle, const focr_kv_pages *pages, size_t rows, const int32_t *row_start,

@@ -264,6 +264,37 @@ extern "C" {
     ) -> c_int;
 
     // ---- A9: greedy selection
+    pub fn focr_rotary_factors(
+        ctx: *mut focr_ctx,
+        positions_dev: *const f32,
+        rows: usize,
+        axes: usize,
+        frequencies_dev: *const f32,
+        n_heads: usize,
+        head_dim: usize,
+        out_dev: *mut f32,
+    ) -> c_int;
+    pub fn focr_logits_select(
+        ctx: *mut focr_ctx,
+        logits_dev: *const f32,
+        rows: usize,
+        vocab: usize,
+        history_dev: *mut i32,
+        history_len_dev: *mut i32,
+        history_cap: usize,
+        recent: usize,
+        penalties_dev: *const f32,
+        penalty_rows: usize,
+        bias_tokens_dev: *const i32,
+        bias_dev: *const f32,
+        n_bias: usize,
+        bias_rows: usize,
+        allowed_dev: *const u32,
+        allowed_rows: usize,
+        append: c_int,
+        adjusted_dev: *mut f32,
+        tokens_dev: *mut i32,
+    ) -> c_int;
     pub fn focr_argmax(
         ctx: *mut focr_ctx,
         logits_dev: *const f32,
@@ -403,6 +434,33 @@ extern "C" {
         lens_dev: *const i32,
         n_seqs: usize,
         q_dev: *mut f32,
+    ) -> c_int;
+    pub fn focr_kv_pages_qkv_rows_at(
+        ctx: *mut focr_ctx,
+        kv: *mut focr_kv_pages,
+        qkv_dev: *const f32,
+        rows: usize,
+        positions_dev: *const f32,
+        axes: usize,
+        frequencies_dev: *const f32,
+        row_start_dev: *const i32,
+        lens_dev: *const i32,
+        n_seqs: usize,
+        q_dev: *mut f32,
+    ) -> c_int;
+    pub fn focr_kv_pages_attention_shared(
+        ctx: *mut focr_ctx,
+        kv: *const focr_kv_pages,
+        q_dev: *const f32,
+        rows: usize,
+        row_start_dev: *const i32,
+        lens_dev: *const i32,
+        n_seqs: usize,
+        max_len: usize,
+        prefix_seq: usize,
+        shared_len: usize,
+        sinks_dev: *const f32,
+        out_dev: *mut f32,
     ) -> c_int;
     pub fn focr_kv_pages_attention(
         ctx: *mut focr_ctx,

@@ -20,6 +20,9 @@ Names and argument meanings follow the reference (amazingvince/falcon-ocr-cpu):
   argmax                 (runner/mod.rs:916-930)
   qkv_rows               fused_prefix_rows / split_norm_rope + LayerCache::append
                          (model/fused.rs:17-123, model/rope.rs:14-86, model/cache.rs:117-216)
+  Rotary                 rotary_factors on the device (model/rope.rs:103-142), several axes
+  LogitRules, select_tokens, adjust_logits
+                         penalties, biases and masks on logits, a batch's greedy tokens (no counterpart)
   DecoderLayer           one layer of Model::forward_layers (model/mod.rs:513-691):
                          prefill and decode steps over a device-resident compact cache
 
@@ -77,6 +80,8 @@ SIGNATURES = {
     "focr_attention_prefill_split": (_I, [_P, _P, _P, _P, _P, _Z, _Z, _Z, _Z, _Z, _Z, _Z, _Z, _Z, _P, _I, _I, _P]),
     "focr_attention_prefill_bf16": (_I, [_P, _P, _P, _P, _Z, _Z, _Z, _Z, _Z, _Z, _P, _I, _I, _P]),
     "focr_argmax": (_I, [_P, _P, _Z, _Z, _P]),
+    "focr_rotary_factors": (_I, [_P, _P, _Z, _Z, _P, _Z, _Z, _P]),
+    "focr_logits_select": (_I, [_P, _P, _Z, _Z, _P, _P, _Z, _Z, _P, _Z, _P, _P, _Z, _Z, _P, _Z, _I, _P, _P]),
     "focr_kv_seal": (_I, [_P, _I, _P, _P, _Z, _Z, _Z, _Z, _Z, ctypes.POINTER(_P)]),
     "focr_kv_reseal": (_I, [_P, _P, _P, _P, _Z, _Z]),
     "focr_kv_append": (_I, [_P, _P, _P, _P, _Z]),
@@ -96,6 +101,8 @@ SIGNATURES = {
     "focr_kv_pages_map": (_I, [_P, _P, _Z, _Z, _Z, _P]),
     "focr_kv_pages_append": (_I, [_P, _P, _P, _P, _Z, _P, _P, _Z]),
     "focr_kv_pages_qkv_rows": (_I, [_P, _P, _P, _Z, _P, _P, _P, _Z, _P]),
+    "focr_kv_pages_qkv_rows_at": (_I, [_P, _P, _P, _Z, _P, _Z, _P, _P, _P, _Z, _P]),
+    "focr_kv_pages_attention_shared": (_I, [_P, _P, _P, _Z, _P, _P, _Z, _Z, _Z, _Z, _P, _P]),
     "focr_kv_pages_attention": (_I, [_P, _P, _P, _Z, _P, _P, _Z, _Z, _P, _P]),
     "focr_kv_pages_dequantize": (_I, [_P, _P, _Z, _P, _P, _Z, _P, _P]),
     "focr_kv_pages_refused": (_I, [_P, _P, _P]),
@@ -150,7 +157,26 @@ def _torch():
     return torch
 
 
-_float32 = None  # torch's, which is not imported with the package
+_float32 = _int32 = None  # torch's, which is not imported with the package
+
+
+def _misfit(t, dtype, device: int) -> FocrError:
+    """Why a tensor does not pass."""
+    if t.get_device() != device:
+        return FocrError(-1, f"expected a CUDA tensor on device {device}")
+    return FocrError(-2, "expected a contiguous tensor" if t.dtype is dtype else f"expected {dtype}, not {t.dtype}")
+
+
+def _dev_int(t, device: int) -> Optional[int]:
+    """Device pointer of a contiguous int32 CUDA tensor on `device` (None passes NULL)."""
+    global _int32
+    if t is None:
+        return None
+    if _int32 is None:
+        _int32 = _torch().int32
+    if t.dtype is not _int32 or t.get_device() != device or not t.is_contiguous():
+        raise _misfit(t, _int32, device)
+    return t.data_ptr()
 
 
 def _dev(t, device: Optional[int] = None) -> Optional[int]:
@@ -564,6 +590,140 @@ def argmax(logits, rows: int, vocab: int, ctx: Optional[Context] = None):
     return list(tokens)
 
 
+class Rotary:
+    """Rotary positions with 1 to 4 axes (time, height, width, ..): the pair of elements
+    2 p, 2 p + 1 of head h is turned by the sum over the axes of position times
+    `frequencies` [axes][n_heads][32] (radians; 0 where an axis does not turn a pair).
+    Angles are formed in FP64, and cos and sin rounded to FP32 once."""
+
+    def __init__(self, frequencies, ctx: Optional[Context] = None):
+        torch = _torch()
+        self.ctx = ctx or default_context()
+        table = torch.as_tensor(frequencies)
+        if table.ndim != 3 or not 1 <= table.shape[0] <= 4 or table.shape[2] != 32:
+            raise FocrError(-2, "frequencies [axes][n_heads][32] of 1 to 4 axes")
+        # A copy of its own: what the caller does with theirs later does not reach it.
+        self.frequencies = table.to(device=f"cuda:{self.ctx.device}", dtype=torch.float32, copy=True).contiguous()
+        self.axes, self.n_heads = int(table.shape[0]), int(table.shape[1])
+        self._table = self.frequencies.data_ptr()
+        if self.ctx.stream != torch.cuda.current_stream(self.ctx.device).cuda_stream:
+            torch.cuda.current_stream(self.ctx.device).synchronize()  # the table is there for the context's stream
+
+    def factors(self, positions, out=None):
+        """cos and sin [rows][n_heads][32][2] of positions [rows][axes], as every row step takes them (`rope`)."""
+        rows = self._rows(positions)
+        if out is None:
+            out = positions.new_empty((rows, self.n_heads, 32, 2))
+        elif out.numel() != rows * self.n_heads * 64:
+            raise FocrError(-2, "factors [rows][n_heads][32][2]")
+        device = self.ctx.device
+        _check(lib().focr_rotary_factors(self.ctx.handle, _dev(positions, device), rows, self.axes, self._table,
+                                         self.n_heads, 64, _dev(out, device)))
+        return out
+
+    def at(self, positions) -> "RotaryRows":
+        """Positions [rows][axes] in the place of factors (`KvPages.qkv_rows`, `DecoderLayer.decode_pages`)."""
+        self._rows(positions)
+        return RotaryRows(self, positions)
+
+    def _rows(self, positions) -> int:
+        rows, rest = divmod(positions.numel(), self.axes)
+        if rest or positions.shape[-1] != self.axes:
+            raise FocrError(-2, "positions [rows][axes]")
+        return rows
+
+
+class RotaryRows:
+    """`Rotary.at`: the rows' positions, which the row step reads when it runs."""
+
+    __slots__ = ("rotary", "positions")
+
+    def __init__(self, rotary: Rotary, positions):
+        self.rotary, self.positions = rotary, positions
+
+
+@dataclass
+class LogitRules:
+    """Rules on the logits [rows][vocab] of a batch; tensors on the GPU, each may be None.
+
+    history     int32 [rows][room]: each row's tokens so far, the first lengths[r] of them
+    lengths     int32 [rows]
+    recent      penalties look at the last `recent` of these (0: at all)
+    penalties   float32 [rows or 1][3]: repetition (a counted token's logit is divided by it
+                above 0 and multiplied by it below), presence, frequency (times the count;
+                both taken from the logit)
+    bias_tokens int32 [rows or 1][n], bias float32 of that shape: added to these tokens'
+                logits (the last one where a token comes twice; below 0: none)
+    allowed     int32 [rows or 1][ceil(vocab / 32)]: bit t % 32 of word t / 32 allows token t
+    """
+
+    history: object = None
+    lengths: object = None
+    recent: int = 0
+    penalties: object = None
+    bias_tokens: object = None
+    bias: object = None
+    allowed: object = None
+
+
+def _logits(name, logits, rows, vocab, rules, adjusted, tokens, append, ctx) -> None:
+    device = ctx.device
+    if logits.numel() != rows * vocab or (adjusted is not None and adjusted.numel() != rows * vocab):
+        raise FocrError(-2, f"{name}: logits [rows][vocab]")
+    if tokens is not None and tokens.numel() != rows:
+        raise FocrError(-2, f"{name}: tokens [rows]")
+    if rules.recent < 0:
+        raise FocrError(-2, f"{name}: recent is not negative")
+
+    def shaped(t, width, what):
+        """How many rows a rule has: 1 or `rows`."""
+        if t is None:
+            return 0
+        if width == 0 or t.numel() not in (width, rows * width):
+            raise FocrError(-2, f"{name}: {what}")
+        return 1 if t.numel() == width else rows
+
+    room = n_bias = 0
+    if rules.history is not None and rows:
+        room = rules.history.shape[-1]
+        if rules.history.numel() != rows * room or rules.lengths is None or rules.lengths.numel() != rows:
+            raise FocrError(-2, f"{name}: history [rows][room] and lengths [rows]")
+    if (rules.bias_tokens is None) != (rules.bias is None):
+        raise FocrError(-1, f"{name}: biases and their tokens")
+    if rules.bias is not None:
+        n_bias = rules.bias.shape[-1]
+        if rules.bias_tokens.shape != rules.bias.shape:
+            raise FocrError(-2, f"{name}: a bias for each of its tokens")
+    bias_rows = shaped(rules.bias, n_bias, "biases [rows or 1][n]") if n_bias else 0
+    _check(lib().focr_logits_select(
+        ctx.handle, _dev(logits, device), rows, vocab, _dev_int(rules.history, device), _dev_int(rules.lengths, device),
+        room, rules.recent, _dev(rules.penalties, device), shaped(rules.penalties, 3, "penalties [rows or 1][3]"),
+        _dev_int(rules.bias_tokens, device), _dev(rules.bias, device), n_bias, bias_rows,
+        _dev_int(rules.allowed, device), shaped(rules.allowed, (vocab + 31) // 32, "allowed [rows or 1][ceil(vocab / 32)]"),
+        int(append), _dev(adjusted, device), _dev_int(tokens, device)))
+
+
+def select_tokens(logits, rows: int, vocab: int, rules: LogitRules = LogitRules(), adjusted=None, tokens=None,
+                  append: bool = False, ctx: Optional[Context] = None):
+    """Greedy tokens int32 [rows] of `rows` rows under `rules`, on the device and without waiting: the lowest index of
+    the largest logit, -1 where the rules leave none, -2 where one is NaN or +infinity. `adjusted` [rows][vocab] (may
+    be `logits` itself) receives the logits under the rules; `append` adds the tokens to the history."""
+    ctx = ctx or default_context()
+    if tokens is None:
+        tokens = logits.new_empty(rows, dtype=_torch().int32)
+    _logits("select_tokens", logits, rows, vocab, rules, adjusted, tokens, append, ctx)
+    return tokens
+
+
+def adjust_logits(logits, rows: int, vocab: int, rules: LogitRules, out=None, ctx: Optional[Context] = None):
+    """The logits [rows][vocab] under `rules`, for a sampler (`out` may be `logits` itself)."""
+    ctx = ctx or default_context()
+    if out is None:
+        out = logits.new_empty((rows, vocab))
+    _logits("adjust_logits", logits, rows, vocab, rules, out, None, False, ctx)
+    return out
+
+
 def default_fast_exp(kv_bits: int, fast_exps: bool, requested: Optional[bool] = None) -> bool:
     """`default_fast_exp` (src/quant/kv.rs:176-184): the fast decode exp for
     8-bit records when the run allows fast exps (ExpMode::FAST), the exact one
@@ -753,10 +913,18 @@ class KvPages:
         _check(lib().focr_kv_pages_append(self.ctx.handle, self.handle, self._ptr(k), self._ptr(v), rows, start, lens, seqs))
 
     def qkv_rows(self, qkv, rope, lens, row_start=None, q=None):
-        """`qkv_rows` with its keys and values appended: queries [rows][n_heads][64]."""
+        """`qkv_rows` with its keys and values appended: queries [rows][n_heads][64].
+        `rope`: factors, or positions (`Rotary.at`), bitwise those of `Rotary.factors`."""
         width = self.n_heads * 64
         rows, rest = divmod(qkv.numel(), width + 2 * self.n_kv_heads * 64)
-        if rest or rope.numel() != rows * width:
+        angles = type(rope) is RotaryRows
+        if angles:
+            rotary, positions = rope.rotary, rope.positions
+            if rest or positions.numel() != rows * rotary.axes or rotary.n_heads != self.n_heads:
+                raise FocrError(-2, "QKV rows [rows][qdim + 2 kdim] and positions [rows][axes] of as many heads")
+            if rotary.ctx.device != self._device:
+                raise FocrError(-1, "the frequencies are on another device than the cache")
+        elif rest or rope.numel() != rows * width:
             raise FocrError(-2, "QKV rows [rows][qdim + 2 kdim] and factors [rows][n_heads][32][2]")
         if q is None:
             q = qkv.new_empty((rows, self.n_heads, 64))
@@ -766,6 +934,10 @@ class KvPages:
         else:
             to = self._ptr(q)
         start, lens, seqs = self._batch(lens, row_start)
+        if angles:
+            _check(lib().focr_kv_pages_qkv_rows_at(self.ctx.handle, self.handle, self._ptr(qkv), rows, self._ptr(positions),
+                                                   rotary.axes, rotary._table, start, lens, seqs, to))
+            return q
         _check(lib().focr_kv_pages_qkv_rows(self.ctx.handle, self.handle, self._ptr(qkv), rows, self._ptr(rope),
                                             start, lens, seqs, to))
         return q
@@ -773,6 +945,17 @@ class KvPages:
     def attention(self, q, lens, max_len: int, row_start=None, sinks=None, out=None):
         """Attention of the batch's rows (1..8 of a sequence), appended before:
         [rows][n_heads][64]. No sequence has more than `max_len` positions, these included."""
+        return self._attention(q, lens, max_len, row_start, sinks, out, 0, 0)
+
+    def attention_shared(self, q, lens, max_len: int, shared: int, prefix: int = 0, row_start=None, sinks=None, out=None):
+        """`attention` of a batch that begins alike: the positions below `shared` (whole pages) are those of the
+        cache's sequence `prefix`, read once for all rows; from there on each sequence has its own. A sequence
+        that stands before `shared` is refused."""
+        if not 0 <= prefix < self.n_seqs or shared < 0:
+            raise FocrError(-2, "the shared positions are of a sequence of the cache")
+        return self._attention(q, lens, max_len, row_start, sinks, out, prefix, shared)
+
+    def _attention(self, q, lens, max_len, row_start, sinks, out, prefix, shared):
         rows, rest = divmod(q.numel(), self.n_heads * 64)
         if rest or (sinks is not None and sinks.numel() != self.n_heads):
             raise FocrError(-2, "queries [rows][n_heads][64] and sinks [n_heads]")
@@ -786,6 +969,10 @@ class KvPages:
         else:
             to = self._ptr(out)
         start, lens, seqs = self._batch(lens, row_start)
+        if shared:
+            _check(lib().focr_kv_pages_attention_shared(self.ctx.handle, self.handle, self._ptr(q), rows, start, lens, seqs,
+                                                        max_len, prefix, shared, self._ptr(sinks), to))
+            return out
         _check(lib().focr_kv_pages_attention(self.ctx.handle, self.handle, self._ptr(q), rows, start, lens, seqs, max_len,
                                              self._ptr(sinks), to))
         return out

@@ -289,11 +289,13 @@ class DecoderLayer:
             matrix.linear_ex(x[at:at + 8], min(8, rows - at), out=out[at:at + 8], **kw)
 
     def decode_pages(self, h, rope, pages: KvPages, lens, max_len: int, row_start=None, clock=None,
-                     projection: Optional[PrefillProjection] = None):
+                     projection: Optional[PrefillProjection] = None, shared: int = 0, prefix: int = 0):
         """One step of a batch of sequences: updates `h` [rows][dim] in place
         and appends to `pages` at the positions `lens` (see `KvPages`; no
         sequence has more than `max_len`, these rows included). Rows that are
-        no sequence's, or a refused one's, come out without meaning.
+        no sequence's, or a refused one's, come out without meaning. `rope`:
+        factors, or the rows' positions (`Rotary.at`). `shared`, `prefix`: the
+        positions that all have from sequence `prefix` (`KvPages.attention_shared`).
 
         More than 8 rows in all take the kernel `projection`: by default the
         layer's, but where that is INT16's FP32 products, as `decode` has
@@ -323,8 +325,11 @@ class DecoderLayer:
         mark("qkv")
         q = pages.qkv_rows(qkv, rope, lens, row_start=row_start, q=self._step_buf("pq", (rows, self.n_heads, 64)))
         mark("qkv_rows")
-        attn = pages.attention(q, lens, max_len, row_start=row_start, sinks=self.sinks,
-                               out=self._step_buf("pattn", (rows, self.n_heads, 64)))
+        attn = self._step_buf("pattn", (rows, self.n_heads, 64))
+        if shared:
+            pages.attention_shared(q, lens, max_len, shared, prefix, row_start=row_start, sinks=self.sinks, out=attn)
+        else:
+            pages.attention(q, lens, max_len, row_start=row_start, sinks=self.sinks, out=attn)
         mark("attention")
         gated = self._step_buf("pgated", (rows, self.w13.out_dim // 2))
         if panel:

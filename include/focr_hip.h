@@ -103,9 +103,10 @@ int focr_ctx_sync(focr_ctx *ctx);
  * use). Graphs captured on one context hold the same scratch: replay them one
  * after another; those that run side by side come from contexts of their own.
  * Device buffers a context owns, and so the only addresses of its own that a
- * captured graph can hold: the scratch (above) and an 8-float row-scale
- * array allocated at creation (focr_argmax's result words are read back to
- * the host within the call, which therefore cannot be captured). No
+ * captured graph can hold: the scratch (above), an 8-float row-scale array and
+ * focr_logits_select's 512 counters, both allocated at creation (focr_argmax's
+ * result words are read back to the host within the call, which therefore cannot
+ * be captured). No
  * context buffer holds weights past the call that unpacked them (4-bit codes):
  * prefill on INT8/INT16 codes reads the codes and forms fl(code * scale) in
  * registers. */
@@ -288,6 +289,18 @@ int focr_qkv_rows(focr_ctx *ctx, const float *qkv_dev, size_t rows, const float 
                   size_t n_heads, size_t n_kv_heads, size_t head_dim, size_t prefix_rows,
                   float *q_dev, float *prefix_k_dev, float *generated_k_dev, float *v_dev);
 
+/* The factors that the row steps take as rope_dev, of rotary positions with
+ * several axes (time, height, width, ..), on the device: no reference counterpart
+ * (its rotary_factors, src/model/rope.rs:103-142, is host code).
+ *   positions_dev [rows][axes], frequencies_dev [axes][n_heads][32] (radians for a
+ *   step of the axis; 0 where it does not turn the pair; 8-byte aligned), axes 1..4,
+ *   out_dev [rows][n_heads][32][2] (16-byte aligned), head_dim 64:
+ *   out = (cos, sin) of the sum over the axes, in order, of position * frequency.
+ * Products are exact and sums round in FP64; cos and sin are those of the FP64 sum to
+ * about 2^-52, rounded to FP32 once. A sum of 2^50 or more, and what is not finite, gives NaN. */
+int focr_rotary_factors(focr_ctx *ctx, const float *positions_dev, size_t rows, size_t axes,
+                        const float *frequencies_dev, size_t n_heads, size_t head_dim, float *out_dev);
+
 /* ---- decode / draft-verify attention -------------------------------------- */
 /* kernels::attention_with for 1..=8 query rows over a compact cache with
  * generated keys (src/kernels/attention/mod.rs:256-311 -> online::head,
@@ -329,6 +342,34 @@ int focr_attention_decode_row(focr_ctx *ctx, const float *qkv_dev, const float *
  * logits_dev [rows][vocab]; tokens (host) [rows]. Synchronous. */
 int focr_argmax(focr_ctx *ctx, const float *logits_dev, size_t rows, size_t vocab,
                 uint32_t *tokens);
+
+/* Rules on the logits of a batch, and its greedy tokens, on the device: no
+ * reference counterpart (its greedy step has no rules). For token t of row r, whose
+ * logit is z, every step rounded to FP32:
+ *   penalties_dev [penalty_rows][3]: repetition, presence, frequency (NULL: none).
+ *     c is how often t stands among the last `recent` (0: all) of the row's
+ *     history, the first history_len_dev[r] (held to 0 .. history_cap) entries of
+ *     history_dev [rows][history_cap]; entries that are no token do not count.
+ *     c > 0: z = z > 0 ? z / repetition : z * repetition, then
+ *            z = z - (c * frequency + presence)
+ *   bias_tokens_dev, bias_dev [bias_rows][n_bias]: z = z + the bias of t, the last
+ *     one where the list names t more than once; entries that are no token are none.
+ *   allowed_dev [allowed_rows][ceil(vocab / 32)]: -infinity unless bit t % 32 of
+ *     word t / 32 is 1 (NULL: all are allowed).
+ * penalty_rows, bias_rows, allowed_rows: rows, or 1 (the same for every row).
+ * adjusted_dev [rows][vocab] (NULL: not kept; logits_dev itself: in place, no other
+ * overlap) receives z. tokens_dev [rows] (NULL: none) receives the lowest
+ * index of the largest z, -1 where all are -infinity, -2 where a z is NaN or
+ * +infinity (what is not allowed is -infinity, whatever stood there).
+ * append 1: a token that is not negative is written behind the row's history and
+ * its length advanced, where there is room.
+ * Asynchronous; 2^18 - 1 counted tokens and 2^14 - 1 biases at most. Uses the
+ * context scratch. */
+int focr_logits_select(focr_ctx *ctx, const float *logits_dev, size_t rows, size_t vocab, int32_t *history_dev,
+                       int32_t *history_len_dev, size_t history_cap, size_t recent, const float *penalties_dev,
+                       size_t penalty_rows, const int32_t *bias_tokens_dev, const float *bias_dev, size_t n_bias,
+                       size_t bias_rows, const uint32_t *allowed_dev, size_t allowed_rows, int append,
+                       float *adjusted_dev, int32_t *tokens_dev);
 
 /* ---- Sealed split KV cache, Kv::Q8 / Kv::Q16 (src/quant/kv.rs) ---------- */
 /* SplitPrefix::from_compact / seal (src/quant/kv.rs:225-421): seals the
@@ -490,6 +531,12 @@ int focr_kv_pages_append(focr_ctx *ctx, focr_kv_pages *kv, const float *k_dev, c
 int focr_kv_pages_qkv_rows(focr_ctx *ctx, focr_kv_pages *kv, const float *qkv_dev, size_t rows,
                            const float *rope_dev, const int32_t *row_start_dev, const int32_t *lens_dev,
                            size_t n_seqs, float *q_dev);
+/* The same, rotated by positions_dev [rows][axes] and frequencies_dev
+ * [axes][n_heads][32] in the factors' place: bitwise focr_rotary_factors, then
+ * focr_kv_pages_qkv_rows. */
+int focr_kv_pages_qkv_rows_at(focr_ctx *ctx, focr_kv_pages *kv, const float *qkv_dev, size_t rows,
+                              const float *positions_dev, size_t axes, const float *frequencies_dev,
+                              const int32_t *row_start_dev, const int32_t *lens_dev, size_t n_seqs, float *q_dev);
 /* Attention of 1..8 rows of each sequence, appended before: row r of a sequence
  * (at position lens_dev[i] + r) attends to the positions up to its own, with
  * the per-head sink (sinks_dev [n_heads], NULL: none), scale 1/8. q_dev, out_dev
@@ -503,6 +550,18 @@ int focr_kv_pages_qkv_rows(focr_ctx *ctx, focr_kv_pages *kv, const float *qkv_de
 int focr_kv_pages_attention(focr_ctx *ctx, const focr_kv_pages *kv, const float *q_dev, size_t rows,
                             const int32_t *row_start_dev, const int32_t *lens_dev, size_t n_seqs, size_t max_len,
                             const float *sinks_dev, float *out_dev);
+/* The same for a batch whose sequences begin alike: positions below shared_len are
+ * those of sequence prefix_seq (of the cache; it may be of the batch or not), read
+ * once for all rows, and what each sequence has mapped there is not looked at; from
+ * shared_len on each has its own. shared_len: whole pages (0: focr_kv_pages_attention). A
+ * sequence that stands before shared_len (lens_dev[i] below it) is refused; where the
+ * prefix has no page, all are. Other sequences than the prefix's, or none, go in calls of
+ * their own, whose lens_dev say -1 for the rest. Within FP32 rounding of
+ * focr_kv_pages_attention on the same positions. */
+int focr_kv_pages_attention_shared(focr_ctx *ctx, const focr_kv_pages *kv, const float *q_dev, size_t rows,
+                                   const int32_t *row_start_dev, const int32_t *lens_dev, size_t n_seqs,
+                                   size_t max_len, size_t prefix_seq, size_t shared_len, const float *sinks_dev,
+                                   float *out_dev);
 /* What the cache holds of the batch's rows: k_dev [rows][n_key_heads][64],
  * v_dev [rows][n_kv_heads][64] (NaN without a page). */
 int focr_kv_pages_dequantize(focr_ctx *ctx, const focr_kv_pages *kv, size_t rows, const int32_t *row_start_dev,
