@@ -814,11 +814,9 @@ __device__ __forceinline__ v8bf codes_of(int first, int second) {
 // Rows of 72, so that 16 columns' 16 bytes lie in different banks; there is no fourth part.
 constexpr int kTurned = 72;
 
-// 64 keys from key0 on for all of a wave's columns. `turned` is the wave's own. 2^power
+// 64 keys from key0 on for a wave's four columns. `turned` is the wave's own. 2^power
 // is above every block scale of the values so far.
-template <int QUADS>
-__device__ __forceinline__ void consume(Quad (&quad)[QUADS], int &power, const Stage &s, int key0, int last_block,
-                                        uint16_t *turned) {
+__device__ __forceinline__ void consume(Quad &u, int &power, const Stage &s, int key0, int last_block, uint16_t *turned) {
   const int l16 = threadIdx.x & 15, g = threadIdx.x >> 4 & 3;
   const float ninf = -__builtin_inff();
   // Blocks that hold none of the sequence's positions do not count; NaN reaches a
@@ -837,79 +835,65 @@ __device__ __forceinline__ void consume(Quad (&quad)[QUADS], int &power, const S
   const float weight = __builtin_ldexpf(v_scale, 64 - power);
   uint16_t *const turn_to = turned + g * kTurned + 4 * l16;
   const uint16_t *const turn_from = turned + l16 * kTurned + 16 * g;
+  float p[4];
+  const float factor = u.factor * k_scale;
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    const v4i zero = {0, 0, 0, 0};
+    const v4i dots = __builtin_amdgcn_mfma_i32_16x16x64_i8(u.digit, s.k[t], zero, 0, 0, 0);
+    // A sum is below 2^20, so two of them fit 32 bits.
+    const float sum = fmaf_(static_cast<float>((dots[3] << 8) + dots[2]), 65536.0f, static_cast<float>((dots[1] << 8) + dots[0]));
+    p[t] = sum * factor;
+    if (key0 + 4 * l16 + t >= u.visible) p[t] = ninf;
+  }
+  float top = __builtin_fmaxf(__builtin_fmaxf(p[0], p[1]), __builtin_fmaxf(p[2], p[3]));
+  top = __builtin_fmaxf(u.m, row_max(top));
+  const float from = top == ninf ? 0.0f : top;
+  if (__any(top > u.m) || lower < 0) {
+    const float keep = __builtin_amdgcn_exp2f(u.m - from);
+    u.den = u.den * keep;
+    u.rescale(__builtin_ldexpf(keep, lower));
+    u.m = top;
+  }
+  uint32_t part[3][4];
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    const float e = __builtin_amdgcn_exp2f(p[t] - from);
+    u.den = u.den + e;
+    float left = e * weight;
+#pragma unroll
+    for (int d = 0; d < 3; d++) {
+      part[d][t] = __float_as_uint(left);
+      left = left - __uint_as_float(part[d][t] & 0xffff0000u);
+    }
+  }
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < QUADS; i++) {
-    Quad &u = quad[i];
-    float p[4];
-    const float factor = u.factor * k_scale;
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-      const v4i zero = {0, 0, 0, 0};
-      const v4i dots = __builtin_amdgcn_mfma_i32_16x16x64_i8(u.digit, s.k[t], zero, 0, 0, 0);
-      // A sum is below 2^20, so two of them fit 32 bits.
-      const float sum = fmaf_(static_cast<float>((dots[3] << 8) + dots[2]), 65536.0f, static_cast<float>((dots[1] << 8) + dots[0]));
-      p[t] = sum * factor;
-      if (key0 + 4 * l16 + t >= u.visible) p[t] = ninf;
-    }
-    float top = __builtin_fmaxf(__builtin_fmaxf(p[0], p[1]), __builtin_fmaxf(p[2], p[3]));
-    top = __builtin_fmaxf(u.m, row_max(top));
-    const float from = top == ninf ? 0.0f : top;
-    if (__any(top > u.m) || lower < 0) {
-      const float keep = __builtin_amdgcn_exp2f(u.m - from);
-      u.den = u.den * keep;
-      u.rescale(__builtin_ldexpf(keep, lower));
-      u.m = top;
-    }
-    uint32_t part[3][4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-      const float e = __builtin_amdgcn_exp2f(p[t] - from);
-      u.den = u.den + e;
-      float left = e * weight;
-#pragma unroll
-      for (int d = 0; d < 3; d++) {
-        part[d][t] = __float_as_uint(left);
-        left = left - __uint_as_float(part[d][t] & 0xffff0000u);
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < 3; d++)
-      *reinterpret_cast<uint2 *>(turn_to + (16 * i + 4 * d) * kTurned) =
-          make_uint2(upper(part[d][1], part[d][0]), upper(part[d][3], part[d][2]));
-  }
+  for (int d = 0; d < 3; d++)
+    *reinterpret_cast<uint2 *>(turn_to + 4 * d * kTurned) = make_uint2(upper(part[d][1], part[d][0]), upper(part[d][3], part[d][2]));
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  v8bf low[QUADS], high[QUADS];
-#pragma unroll
-  for (int i = 0; i < QUADS; i++) {
-    low[i] = *reinterpret_cast<const v8bf *>(turn_from + 16 * i * kTurned);
-    high[i] = *reinterpret_cast<const v8bf *>(turn_from + 16 * i * kTurned + 8);
-  }
+  const v8bf low = *reinterpret_cast<const v8bf *>(turn_from), high = *reinterpret_cast<const v8bf *>(turn_from + 8);
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int d = 0; d < 4; d++) {
-    const v8bf first = codes_of(s.v[d][0], s.v[d][1]), second = codes_of(s.v[d][2], s.v[d][3]);
-#pragma unroll
-    for (int i = 0; i < QUADS; i++) {
-      quad[i].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(first, low[i], quad[i].acc[d], 0, 0, 0);
-      quad[i].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(second, high[i], quad[i].acc[d], 0, 0, 0);
-    }
+    u.acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_of(s.v[d][0], s.v[d][1]), low, u.acc[d], 0, 0, 0);
+    u.acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes_of(s.v[d][2], s.v[d][3]), high, u.acc[d], 0, 0, 0);
   }
 }
 
-// A wave's run of keys. While one 64 keys are worked on, the next are on their way,
-// and before them the pages of those after: no load is under a branch, so the waits
-// count what is still out. stage[0] holds the first 64, `next` the pages of the second.
-template <int QUADS, bool WIDE>
-__device__ __forceinline__ void walk(Quad (&quad)[QUADS], int &power, Reader<WIDE> &reader, Stage (&stage)[2], Found next,
-                                     int begin, int end, uint16_t *turned) {
-  auto turn = [&](const Stage &now, Stage &then, int key0, auto more) {
+// A wave's run of keys, 64 at a time. While one 64 keys are worked on, the next are on
+// their way, and before them the pages of those after: no load is under a branch, so
+// the waits count what is still out. stage[0] holds the first 64, `next` the pages of
+// the second.
+template <typename R, typename S, typename Step>
+__device__ __forceinline__ void walk(R &reader, S (&stage)[2], Found next, int begin, int end, const Step &step) {
+  auto turn = [&](const S &now, S &then, int key0, auto more) {
     if constexpr (decltype(more)::value) {
       const Found after = reader.find(key0 + 128);
       reader.load(next, key0 + 64, then);
       next = after;
     }
-    consume<QUADS>(quad, power, now, key0, reader.last_block, turned);
+    step(now, key0);
   };
   const std::true_type more;
   const std::false_type no_more;
@@ -962,11 +946,11 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   Reader<WIDE> reader(c, seq, key_head, limit);
   Found next;
   Stage stage[2];
-  Quad quad[1];
-  quad[0].m = -__builtin_inff();
-  quad[0].den = 0.0f;
+  Quad quad;
+  quad.m = -__builtin_inff();
+  quad.den = 0.0f;
 #pragma unroll
-  for (int d = 0; d < 4; d++) quad[0].acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int d = 0; d < 4; d++) quad.acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   int power = -300;
   __shared__ __attribute__((aligned(16))) uint16_t turned[4][16 * kTurned];
   *reinterpret_cast<uint2 *>(turned[wave] + (12 + g) * kTurned + 4 * l16) = make_uint2(0, 0);
@@ -981,10 +965,11 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     for (int i = 0; i < 4; i++) x[i] = reinterpret_cast<const float4 *>(q)[i];
     reader.load(next, begin, stage[0]);
     next = reader.find(begin + 64);
-    quad[0].begin(x);
+    quad.begin(x);
     const int mine = column0 + g;
-    quad[0].visible = len + (mine < columns ? mine : columns - 1) % n + 1;
-    walk<1, WIDE>(quad, power, reader, stage, next, begin, end, turned[wave]);
+    quad.visible = len + (mine < columns ? mine : columns - 1) % n + 1;
+    walk(reader, stage, next, begin, end,
+         [&](const Stage &now, int key0) { consume(quad, power, now, key0, reader.last_block, turned[wave]); });
   }
   if (__any(reader.missing) && lane == 0) c.refused[seq] = 1;
   // Asked here, where no load is waited for.
@@ -996,7 +981,7 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   // The waves' states meet in LDS: [run][column], 16 in all.
   __shared__ float s_m[16], s_den[16];
   __shared__ __attribute__((aligned(16))) float s_o[16][68];
-  quad[0].end(power, s_m + 4 * wave, s_den + 4 * wave, s_o + 4 * wave);
+  quad.end(power, s_m + 4 * wave, s_den + 4 * wave, s_o + 4 * wave);
   __syncthreads();
   // Thread: a column and four dims.
   const int col = threadIdx.x / 16, dim = threadIdx.x % 16 * 4, wide = 4 * quads;
@@ -1025,105 +1010,361 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
 // with states (m_i, d_i, o_i) of disjoint keys, m = max m_i, o = sum 2^(m_i - m) o_i /
 // sum 2^(m_i - m) d_i.
 //
-// A wave takes 4 QUADS columns, so that a key's codes are loaded, and its values' turned
-// to BF16, once for all of them; a workgroup's four waves stand side by side over
-// up to 16 QUADS columns (`beside` of them), or over one run of the keys each.
-template <bool WIDE, int QUADS>
-__global__ __launch_bounds__(256, QUADS == 4 ? 2 : 3) void prefix_kernel(AttendArgs a) {
+// A wave takes 16 GROUPS columns and holds all that is theirs in its lanes. Scores. Lane
+// (l16, g) has column l16's query as two FP16 numbers an element, of 2^14 times the
+// power of two above the largest (so 24 bits of each element down to 2^-14 of the largest, and 2^-39 of that one for all); a key's
+// codes are FP16 numbers, so products are exact, and their sums round as FP32's do. Row m
+// of key tile t is key 4 m + t, as the codes stand, so that lane (l16, g) gets the scores
+// of column l16 with the 16 keys of block g, one scale for all of them. Weights. exp2(s - m)
+// times the block's value scale is three BF16 numbers, as in attend_kernel, which
+// stand where the second product takes them: its operand is lane (l16, g)'s eight keys of block g
+// by column l16, the other the value codes of dim l16 and these keys, as they stand.
+struct WideStage {
+  v4i k[4], v[4];
+  float k_scale, v_scale;  // of block g
+};
+template <bool WIDE>
+struct WideReader {
+  Reader<WIDE> reader;
+  __device__ __forceinline__ Found find(int key0) const { return reader.find(key0); }
+  __device__ __forceinline__ void load(const Found &f, int key0, WideStage &s) {
+    const Cache &c = reader.c;
+    const int g = threadIdx.x >> 4 & 3, at = key0 / kBlock + g;
+    Stage plain;
+    reader.load(f, key0, plain);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      s.k[i] = plain.k[i];
+      s.v[i] = plain.v[i];
+    }
+    // The scales of block g, whose page the lane has for its values.
+    const int in = (at < reader.last_block ? at : reader.last_block) & ((1 << c.shift) - 1);
+    const long page = f.v_page < 0 ? 0 : f.v_page;
+    const float k_scale = c.k_scales[((page * c.key_heads + reader.key_head) << c.shift) + in];
+    const float v_scale = c.v_scales[((page * c.kv_heads + reader.value_head) << c.shift) + in];
+    s.k_scale = f.v_page < 0 ? __builtin_nanf("") : k_scale;
+    s.v_scale = v_scale;
+  }
+};
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
+// Eight codes as FP16 numbers: 1024 + 128 + code has the code, its top bit turned, in its
+// low byte.
+__device__ __forceinline__ v8h halves_of(int first, int second) {
+  const uint32_t w[2] = {static_cast<uint32_t>(first) ^ 0x80808080u, static_cast<uint32_t>(second) ^ 0x80808080u};
+  v4i to;
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const uint32_t bits = __builtin_amdgcn_perm(0x64646464u, w[i], j == 0 ? 0x04010400u : 0x04030402u);
+      to[2 * i + j] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, bits) - v2h{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)});
+    }
+  return __builtin_bit_cast(v8h, to);
+}
+
+// Largest over the four lanes (l16, 0 .. 3).
+__device__ __forceinline__ float across_max(float v) {
+  auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __builtin_fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __builtin_fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+__device__ __forceinline__ float across_sum(float v) {
+  auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+}
+
+// 16 columns of a wave: lane (l16, g) has column l16.
+struct Column {
+  v8h q[2][2];  // the two parts of dims 16 g + 8 h .. + 7
+  float factor, m, den;
+  v4f acc[4];   // dims 16 d + 4 g + i
+
+  __device__ __forceinline__ void clear() {
+    m = -__builtin_inff();
+    den = 0.0f;
+#pragma unroll
+    for (int d = 0; d < 4; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  // From dims 16 g .. + 15.
+  __device__ __forceinline__ void begin(const float4 (&x)[4]) {
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint32_t bits = __float_as_uint(y[j]) & 0x7fffffffu;
+        big = bits > big ? bits : big;
+      }
+    }
+    auto p = __builtin_amdgcn_permlane16_swap(big, big, false, false);
+    big = p[0] > p[1] ? p[0] : p[1];
+    p = __builtin_amdgcn_permlane32_swap(big, big, false, false);
+    big = p[0] > p[1] ? p[0] : p[1];
+    const bool finite = big < 0x7f800000u;
+    int e = !finite || big == 0 ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(big));
+    e = e < -90 ? -90 : e;
+    // log2(e) / 8: scores in powers of two.
+    factor = finite ? __builtin_ldexpf(0.180336880111120426f, e - 14) : __builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float scaled = finite ? __builtin_ldexpf(y[j], 14 - e) : 0.0f;
+        const _Float16 high = static_cast<_Float16>(scaled);
+        q[0][i / 2][i % 2 * 4 + j] = high;
+        q[1][i / 2][i % 2 * 4 + j] = static_cast<_Float16>(scaled - static_cast<float>(high));
+      }
+    }
+  }
+};
+
+template <int GROUPS>
+__device__ __forceinline__ void consume_wide(Column (&column)[GROUPS], int &power, const WideStage &s, int key0, int last_block) {
+  const int g = threadIdx.x >> 4 & 3;
+  const float ninf = -__builtin_inff();
+  const bool none = key0 / kBlock + g > last_block;  // a block behind the last
+  float v_scale = none ? 0.0f : s.v_scale;
+  const bool bad = v_scale != v_scale;
+  const float k_scale = bad ? __builtin_nanf("") : s.k_scale;
+  v_scale = bad ? 0.0f : v_scale;
+  const float widest = across_max(v_scale);
+  int above = widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -300;
+  above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
+  const int lower = power - above;
+  power = above;
+  const float weight = __builtin_ldexpf(v_scale, 64 - power);
+  v4f sums[GROUPS][4];
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    const v8h first = halves_of(s.k[t][0], s.k[t][1]), second = halves_of(s.k[t][2], s.k[t][3]);
+#pragma unroll
+    for (int c = 0; c < GROUPS; c++) {
+      v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int part = 1; part >= 0; part--) {
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(first, column[c].q[part][0], sum, 0, 0, 0);
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(second, column[c].q[part][1], sum, 0, 0, 0);
+      }
+      sums[c][t] = sum;
+    }
+  }
+  v8bf weights[GROUPS][3][2];
+#pragma unroll
+  for (int c = 0; c < GROUPS; c++) {
+    Column &u = column[c];
+    const float factor = none ? 0.0f : u.factor * k_scale;
+    float top = sums[c][0][0];
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) top = __builtin_fmaxf(top, sums[c][t][i]);
+    top = none ? ninf : top * factor;
+    top = __builtin_fmaxf(u.m, across_max(top));
+    const float from = top == ninf ? 0.0f : top;
+    if (__any(top > u.m) || lower < 0) {
+      const float keep = __builtin_amdgcn_exp2f(u.m - from), scaled = __builtin_ldexpf(keep, lower);
+      u.den = u.den * keep;
+#pragma unroll
+      for (int d = 0; d < 4; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) u.acc[d][i] = u.acc[d][i] * scaled;
+      u.m = top;
+    }
+    const float minus = none ? ninf : -from;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      v4i words[3];
+#pragma unroll
+      for (int pair = 0; pair < 4; pair++) {
+        uint32_t bits[3][2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          // Position 8 half + 2 pair + j of the block: row i, tile t.
+          const int i = 2 * half + pair / 2, t = pair % 2 * 2 + j;
+          const float e = __builtin_amdgcn_exp2f(fmaf_(sums[c][t][i], factor, minus));
+          u.den = u.den + e;
+          float left = e * weight;
+#pragma unroll
+          for (int d = 0; d < 3; d++) {
+            bits[d][j] = __float_as_uint(left);
+            left = left - __uint_as_float(bits[d][j] & 0xffff0000u);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < 3; d++) words[d][pair] = static_cast<int>(upper(bits[d][1], bits[d][0]));
+      }
+#pragma unroll
+      for (int d = 0; d < 3; d++) weights[c][d][half] = __builtin_bit_cast(v8bf, words[d]);
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < 4; d++) {
+    const v8bf first = codes_of(s.v[d][0], s.v[d][1]), second = codes_of(s.v[d][2], s.v[d][3]);
+#pragma unroll
+    for (int c = 0; c < GROUPS; c++)
+#pragma unroll
+      for (int part = 2; part >= 0; part--) {
+        column[c].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(first, weights[c][part][0], column[c].acc[d], 0, 0, 0);
+        column[c].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(second, weights[c][part][1], column[c].acc[d], 0, 0, 0);
+      }
+  }
+}
+
+// The sequence of each of a tile's rows row0 .. row0 + rows - 1 that one which takes part
+// has, by the threads of a workgroup or wave; `owner` begins at -1. False if none was found.
+__device__ __forceinline__ bool find_owners(const AttendArgs &a, int row0, int rows, int *owner, int thread, int threads) {
   const Cache &c = a.c;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // The key heads of one value head, and all tiles of their columns, follow one
-  // another on one XCD.
-  const int share = c.key_heads / c.kv_heads;
-  int task = blockIdx.x / 8;
-  const int sharer = task % share;
-  task /= share;
-  const int tile = task % a.tiles;
-  task = task / a.tiles * 8 + blockIdx.x % 8;
-  const int value_head = task % c.kv_heads, part = task / c.kv_heads;
-  if (part >= a.first_part) return;
-  const int key_head = value_head * share + sharer, group = c.n_heads / c.key_heads, columns = group * c.rows;
-  const int beside = a.beside, across = 4 * QUADS * beside, runs = 4 / beside, run = wave / beside;
-  const int tile0 = tile * across, column0 = tile0 + wave % beside * 4 * QUADS;
-  // The tile's rows, and which sequence each is of (-1: none that takes part).
-  const int row0 = tile0 / group, row_end = (tile0 + across - 1) / group + 1;
-  const int rows = (row_end < c.rows ? row_end : c.rows) - row0;
-  __shared__ int owner[16 * QUADS];
-  if (threadIdx.x < 16 * QUADS) owner[threadIdx.x] = -1;
-  __syncthreads();
   const int seq0 = c.row_start ? 0 : row0, seq_end = c.row_start ? c.n_seqs : row0 + rows;
-  for (int seq = seq0 + threadIdx.x; seq < seq_end; seq += 256) {
+  bool any = false;
+  for (int seq = seq0 + thread; seq < seq_end; seq += threads) {
     int len, first, n;
     bool bad;
     if (!attend_span(a, seq, len, first, n, bad)) continue;
-    for (int r = first > row0 ? first : row0; r < first + n && r < row0 + rows; r++) atomicMax(owner + (r - row0), seq);
+    for (int r = first > row0 ? first : row0; r < first + n && r < row0 + rows; r++) {
+      atomicMax(owner + (r - row0), seq);
+      any = true;
+    }
   }
-  __syncthreads();
-  const unsigned long long live = __ballot(lane < rows && owner[lane < rows ? lane : 0] >= 0);
-  if (live == 0) return;
-  const int some = __ffsll(live) - 1;
+  return any;
+}
 
+// A wave's keys begin .. end - 1 for its columns from column0 on, whose rows from row0 on
+// have these owners. Leaves the sums of `den` in every lane.
+template <bool WIDE, int GROUPS>
+__device__ __forceinline__ void walk_prefix(const AttendArgs &a, Column (&column)[GROUPS], int &power, int key_head, int column0,
+                                            int row0, int rows, const int *owner, int begin, int end) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int group = c.n_heads / c.key_heads, columns = group * c.rows;
+#pragma unroll
+  for (int i = 0; i < GROUPS; i++) column[i].clear();
+  power = -300;
+  if (begin >= end || column0 >= columns) return;
+  WideReader<WIDE> reader{Reader<WIDE>(c, a.prefix, key_head, a.base)};
+  WideStage stage[2];
+  Found next = reader.find(begin);
+  // Column column0 + l16: row column / group, head key_head * group + column % group.
+  // One that is no row's has a query of zeros, and is left out in the end.
+  float4 x[GROUPS][4];
+#pragma unroll
+  for (int i = 0; i < GROUPS; i++) {
+    const int at = column0 + 16 * i + l16;
+    const bool live = at < columns && owner[at / group - row0] >= 0;
+    const float *q = a.q + (static_cast<size_t>(at / group) * c.n_heads + key_head * group + at % group) * 64 + 16 * g;
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[i][j] = live ? reinterpret_cast<const float4 *>(q)[j] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  reader.load(next, begin, stage[0]);
+  next = reader.find(begin + 64);
+#pragma unroll
+  for (int i = 0; i < GROUPS; i++) column[i].begin(x[i]);
+  walk(reader, stage, next, begin, end,
+       [&](const WideStage &now, int key0) { consume_wide<GROUPS>(column, power, now, key0, reader.reader.last_block); });
+  if (__any(reader.reader.missing))
+    for (int r = lane; r < rows; r += 64)
+      if (owner[r] >= 0) c.refused[owner[r]] = 1;
+#pragma unroll
+  for (int i = 0; i < GROUPS; i++) column[i].den = across_sum(column[i].den);
+}
+
+// Up to 64 columns: a workgroup for a part of the keys, its four waves side by side over
+// the columns (`beside` of them) and the part's runs.
+template <bool WIDE>
+__global__ __launch_bounds__(256, 3) void prefix_few_kernel(AttendArgs a) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // The key heads of one value head follow one another on one XCD.
+  const int share = c.key_heads / c.kv_heads, turn_of = blockIdx.x / 8;
+  const int task = turn_of / share * 8 + blockIdx.x % 8;
+  const int key_head = task % c.kv_heads * share + turn_of % share, part = task / c.kv_heads;
+  if (part >= a.first_part) return;
+  const int group = c.n_heads / c.key_heads, columns = group * c.rows;
+  const int beside = a.beside, across = 16 * beside, runs = 4 / beside, run = wave / beside, column0 = wave % beside * 16;
+  __shared__ int owner[64];
+  if (threadIdx.x < 64) owner[threadIdx.x] = -1;
+  __syncthreads();
+  if (!__syncthreads_or(find_owners(a, 0, c.rows, owner, threadIdx.x, 256))) return;
   const int from_key = part * a.prefix_chunk, to_key = from_key + a.prefix_chunk < a.base ? from_key + a.prefix_chunk : a.base;
   const int each = (to_key - from_key + 64 * runs - 1) / (64 * runs) * 64;
   const int begin = from_key + run * each, end = begin + each < to_key ? begin + each : to_key;
-  Reader<WIDE> reader(c, a.prefix, key_head, a.base);
-  Stage stage[2];
-  Quad quad[QUADS];
-#pragma unroll
-  for (int i = 0; i < QUADS; i++) {
-    quad[i].m = -__builtin_inff();
-    quad[i].den = 0.0f;
-#pragma unroll
-    for (int d = 0; d < 4; d++) quad[i].acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  int power = -300;
-  __shared__ __attribute__((aligned(16))) uint16_t turned[4][QUADS * 16 * kTurned];
-#pragma unroll
-  for (int i = 0; i < QUADS; i++)
-    *reinterpret_cast<uint2 *>(turned[wave] + (16 * i + 12 + g) * kTurned + 4 * l16) = make_uint2(0, 0);
-  if (begin < end && column0 < columns) {
-    Found next = reader.find(begin);
-    // Column column0 + q: row column / group, head key_head * group + column % group. A
-    // column that is no row's takes another's query, and is left out in the end.
-    float4 x[QUADS][4];
-#pragma unroll
-    for (int i = 0; i < QUADS; i++) {
-      const int wanted = column0 + 4 * i + l16 / 4, column = wanted < columns ? wanted : columns - 1;
-      int row = column / group - row0;
-      row = live >> row & 1 ? row : some;
-      const float *q = a.q + (static_cast<size_t>(row0 + row) * c.n_heads + key_head * group + column % group) * 64 + 16 * g;
-#pragma unroll
-      for (int j = 0; j < 4; j++) x[i][j] = reinterpret_cast<const float4 *>(q)[j];
-    }
-    reader.load(next, begin, stage[0]);
-    next = reader.find(begin + 64);
-#pragma unroll
-    for (int i = 0; i < QUADS; i++) {
-      quad[i].begin(x[i]);
-      quad[i].visible = a.base;
-    }
-    walk<QUADS, WIDE>(quad, power, reader, stage, next, begin, end, turned[wave]);
-  }
-  if (__any(reader.missing) && lane < rows && owner[lane] >= 0) c.refused[owner[lane]] = 1;
-
+  Column column[1];
+  int power;
+  walk_prefix<WIDE, 1>(a, column, power, key_head, column0, 0, c.rows, owner, begin, end);
   // The waves' states meet in LDS: [run][column].
-  __shared__ float s_m[16 * QUADS], s_den[16 * QUADS];
-  __shared__ __attribute__((aligned(16))) float s_o[16 * QUADS][68];
+  __shared__ float s_m[64], s_den[64];
+  __shared__ __attribute__((aligned(16))) float s_o[64][68];
+  const int to = 16 * wave + l16;
+  if (g == 0) {
+    s_m[to] = column[0].m;
+    s_den[to] = column[0].den;
+  }
 #pragma unroll
-  for (int i = 0; i < QUADS; i++) {
-    const int at = 4 * QUADS * wave + 4 * i;
-    quad[i].end(power, s_m + at, s_den + at, s_o + at);
+  for (int d = 0; d < 4; d++) {
+    v4f o;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] = __builtin_ldexpf(column[0].acc[d][j], power - 64);
+    *reinterpret_cast<v4f *>(&s_o[to][16 * d + 4 * g]) = o;
   }
   __syncthreads();
   const int dim = threadIdx.x % 16 * 4;
-  for (int col = threadIdx.x / 16; col < across; col += 16) {
-    const int column = tile0 + col;
-    if (column >= columns || owner[column / group - row0] < 0) continue;
+  for (int at = threadIdx.x / 16; at < across; at += 16) {
+    if (at >= columns || owner[at / group] < 0) continue;
     float top, total;
-    const v4f o = join_runs(s_m, s_den, s_o, col, across, runs, dim, top, total);
-    const size_t out_row = static_cast<size_t>(column / group) * c.n_heads + key_head * group + column % group;
-    store_part(a, out_row * a.parts + part, dim, o, top, total);
+    const v4f o = join_runs(s_m, s_den, s_o, at, across, runs, dim, top, total);
+    const size_t slot = (static_cast<size_t>(at / group) * c.n_heads + key_head * group + at % group) * a.parts + part;
+    store_part(a, slot, dim, o, top, total);
+  }
+}
+
+// More columns: every wave has 32 of them and a part of the keys to itself, so that any number of
+// columns leaves no wave idle. Waves follow one another by column, key head of one value
+// head, then part and value head, and each XCD has a stretch of them.
+template <bool WIDE>
+__global__ __launch_bounds__(256, 2) void prefix_kernel(AttendArgs a) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int share = c.key_heads / c.kv_heads, group = c.n_heads / c.key_heads, columns = group * c.rows;
+  int task = (blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8) * 4 + wave;
+  const int tile = task % a.tiles;
+  task /= a.tiles;
+  const int sharer = task % share;
+  task /= share;
+  const int key_head = task % c.kv_heads * share + sharer, part = task / c.kv_heads;
+  if (part >= a.first_part) return;
+  const int column0 = 32 * tile, row0 = column0 / group, row_end = (column0 + 31) / group + 1;
+  const int rows = (row_end < c.rows ? row_end : c.rows) - row0;
+  __shared__ int all_owners[4][32];
+  int *const owner = all_owners[wave];
+  if (lane < 32) owner[lane] = -1;
+  asm volatile("" ::: "memory");
+  if (!__any(find_owners(a, row0, rows, owner, lane, 64))) return;
+  asm volatile("" ::: "memory");
+  const int begin = part * a.prefix_chunk, end = begin + a.prefix_chunk < a.base ? begin + a.prefix_chunk : a.base;
+  Column column[2];
+  int power;
+  walk_prefix<WIDE, 2>(a, column, power, key_head, column0, row0, rows, owner, begin, end);
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int at = column0 + 16 * i + l16;
+    if (at >= columns || owner[at / group - row0] < 0) continue;
+    const size_t slot = (static_cast<size_t>(at / group) * c.n_heads + key_head * group + at % group) * a.parts + part;
+#pragma unroll
+    for (int d = 0; d < 4; d++) {
+      v4f o;
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = __builtin_ldexpf(column[i].acc[d][j], power - 64);
+      store_part(a, slot, 16 * d + 4 * g, o, column[i].m, column[i].den);
+    }
   }
 }
 
@@ -1325,7 +1566,7 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
   // parts to spare (20 of up to 9,000 49.0 / 47.1 / 44.7, 40 of up to 5,000 with up to 8
   // rows 84.7 / 84.8 / 63.7).
   const size_t heads = n_seqs * kv->key_heads * a.tiles;
-  const size_t enough = n_seqs <= 2 ? 512 : n_seqs <= 8 ? 1024 : 2048;
+  const size_t enough = n_seqs <= 2 ? 512 : n_seqs <= 8 || shared > 0 ? 1024 : 2048;
   const size_t want = heads >= enough ? 1 : enough / heads;
   const size_t chunk = std::max(std::min<size_t>((own + want - 1) / want, 4096), (own + kMaxParts - 1) / kMaxParts);
   a.chunk = static_cast<int>((chunk + 255) / 256 * 256);
@@ -1335,18 +1576,19 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
   FOCR_REQUIRE(grid < (size_t(1) << 31), FOCR_E_SHAPE, std::string(name) + ": too many sequences and heads");
   AttendArgs before = a;  // the prefix's kernel: other tiles
   size_t before_grid = 0;
-  int quads = 0;
+  bool few = false;
   if (shared > 0) {
     const size_t columns = group * rows;
-    quads = columns <= 4 ? 1 : columns <= 8 ? 2 : 4;
+    few = columns <= 64;
+    // Few columns: 512 workgroups, more: 2,048 waves, which all run at once.
     a.beside = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
-    const size_t across = 4 * quads * a.beside, tiles = (columns + across - 1) / across;
-    const size_t each = kv->key_heads * tiles, parts = each >= 512 ? 1 : 512 / each;
+    const size_t tiles = few ? 1 : (columns + 31) / 32, all = few ? 512 : 2048;
+    const size_t each = kv->key_heads * tiles, parts = each >= all ? 1 : all / each;
     const size_t prefix_chunk = std::max((shared + parts - 1) / parts, (shared + kMaxParts - 1) / kMaxParts);
     a.prefix_chunk = static_cast<int>((prefix_chunk + 63) / 64 * 64);
     a.first_part = static_cast<int>((shared + a.prefix_chunk - 1) / a.prefix_chunk);
-    before_grid = (kv->kv_heads * a.first_part + 7) / 8 * 8 * share * tiles;
-    FOCR_REQUIRE(before_grid < (size_t(1) << 31), FOCR_E_SHAPE, std::string(name) + ": too many rows and heads");
+    before_grid = few ? (kv->kv_heads * a.first_part + 7) / 8 * 8 * share : (each * a.first_part + 31) / 32 * 8;
+    FOCR_REQUIRE(before_grid < (size_t(1) << 29), FOCR_E_SHAPE, std::string(name) + ": too many rows and heads");
     before = a;
     before.tiles = static_cast<int>(tiles);
   }
@@ -1364,9 +1606,9 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
     const dim3 all(static_cast<unsigned>(before_grid));
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, all, dim3(256), 0, ctx->stream, before); };
     if (wide)
-      launch(quads == 1 ? prefix_kernel<true, 1> : quads == 2 ? prefix_kernel<true, 2> : prefix_kernel<true, 4>);
+      launch(few ? prefix_few_kernel<true> : prefix_kernel<true>);
     else
-      launch(quads == 1 ? prefix_kernel<false, 1> : quads == 2 ? prefix_kernel<false, 2> : prefix_kernel<false, 4>);
+      launch(few ? prefix_few_kernel<false> : prefix_kernel<false>);
     FOCR_HIP_CHECK(hipGetLastError());
   }
   if (wide)
@@ -1379,7 +1621,7 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
     // Parts of all a sequence's rows (us a call with 4 / 16 waves: 26 parts of one row
     // 9.8 / 10.4, 3 of one in 64 sequences 112 / 120; 57 of two 34.8 / 32.8, 59 of
     // eight 33.3 / 20.3).
-    if (a.parts * most <= 64)
+    if (a.parts * (shared > 0 ? (rows + n_seqs - 1) / n_seqs : most) <= 64)
       hipLaunchKernelGGL(merge_kernel<4>, each, dim3(256), 0, ctx->stream, a);
     else
       hipLaunchKernelGGL(merge_kernel<16>, each, dim3(1024), 0, ctx->stream, a);
