@@ -885,11 +885,11 @@ __device__ __forceinline__ void consume(Quad &u, int &power, const Stage &s, int
 // their way, and before them the pages of those after: no load is under a branch, so
 // the waits count what is still out. stage[0] holds the first 64, `next` the pages of
 // the second.
-template <typename R, typename S, typename Step>
-__device__ __forceinline__ void walk(R &reader, S (&stage)[2], Found next, int begin, int end, const Step &step) {
+template <typename R, typename S, typename F, typename Step>
+__device__ __forceinline__ void walk(R &reader, S (&stage)[2], F next, int begin, int end, const Step &step) {
   auto turn = [&](const S &now, S &then, int key0, auto more) {
     if constexpr (decltype(more)::value) {
-      const Found after = reader.find(key0 + 128);
+      const F after = reader.find(key0 + 128);
       reader.load(next, key0 + 64, then);
       next = after;
     }
@@ -1325,13 +1325,233 @@ __global__ __launch_bounds__(256, 3) void prefix_few_kernel(AttendArgs a) {
   }
 }
 
-// More columns: every wave has 32 of them and a part of the keys to itself, so that any number of
+// More columns: 32 of a wave, on the matrix instructions of 32 by 32, which leave the
+// vector instructions more of the registers' ports (2 waves' 128 fused multiply-adds with
+// as many products: 542 cycles, with those of 16 by 16 658; byte permutations 600 and 690).
+// As above with lane (l32, h): row m of key tile t is position m % 4 + 4 (m / 8) of block
+// 2 t + m / 4 % 2, so that lane (l32, h) gets column l32's scores with the 16 keys of
+// blocks h and 2 + h, and its weights stand where the second product takes them.
+struct Stage32 {
+  v4i k[2][2], v[2][2];  // [key tile][16 dims 2 j + h], [key tile][32 dims]
+  float k_scale[2], v_scale[2];  // of block 2 t + h
+};
+template <bool WIDE>
+struct Reader32 {
+  struct Pages {
+    int k[2], v[2];
+  };
+  const Cache &c;
+  const int32_t *table;
+  int key_head, value_head, last_block;
+  bool missing = false;
+
+  __device__ __forceinline__ Reader32(const Cache &cache, int seq, int head, int limit)
+      : c(cache), table(cache.table + static_cast<size_t>(seq) * cache.seq_pages), key_head(head),
+        value_head(head * cache.kv_heads / cache.key_heads), last_block((limit - 1) / kBlock) {}
+
+  __device__ __forceinline__ int held(int block) const { return block < last_block ? block : last_block; }
+  __device__ __forceinline__ Pages find(int key0) const {
+    typedef __attribute__((address_space(4))) const int32_t scalar_table;  // read by scalar loads
+    const int b = key0 / kBlock;
+    Pages f;
+    if constexpr (WIDE) {
+      f.k[0] = f.k[1] = f.v[0] = f.v[1] = reinterpret_cast<scalar_table *>(reinterpret_cast<uintptr_t>(table))[held(b) >> c.shift];
+    } else {
+      const int of_k = threadIdx.x >> 2 & 1, of_v = threadIdx.x >> 5 & 1;
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        f.k[t] = table[held(b + 2 * t + of_k) >> c.shift];
+        f.v[t] = table[held(b + 2 * t + of_v) >> c.shift];
+      }
+    }
+    return f;
+  }
+  __device__ __forceinline__ void load(const Pages &f, int key0, Stage32 &s) {
+    const int l32 = threadIdx.x & 31, h = threadIdx.x >> 5 & 1, of_k = l32 >> 2 & 1, mask = (1 << c.shift) - 1;
+    const int b = key0 / kBlock;
+    const int k_lane = (l32 & 3) * 256 + (l32 >> 3) * 64 + 16 * h, v_lane = l32 * 16;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      missing |= f.k[t] < 0;
+      const long kp = f.k[t] < 0 ? 0 : f.k[t], vp = f.v[t] < 0 ? 0 : f.v[t];
+      const int8_t *k, *v;
+      if constexpr (WIDE) {
+        const long kn = ((kp * c.key_heads + key_head) << c.shift) + (b & mask) + 2 * t;
+        const long vn = ((vp * c.kv_heads + value_head) << c.shift) + (b & mask) + 2 * t;
+        k = c.k_codes + kn * kBlockBytes + (of_k * kBlockBytes + k_lane);
+        v = c.v_codes + vn * kBlockBytes + (h * kBlockBytes + v_lane);
+        s.k_scale[t] = (c.k_scales + kn)[h];
+        s.v_scale[t] = (c.v_scales + vn)[h];
+      } else {
+        const int v_in = held(b + 2 * t + h) & mask;
+        const long vn = ((vp * c.kv_heads + value_head) << c.shift) + v_in;
+        k = c.k_codes + (((kp * c.key_heads + key_head) << c.shift) + (held(b + 2 * t + of_k) & mask)) * kBlockBytes + k_lane;
+        v = c.v_codes + vn * kBlockBytes + v_lane;
+        s.k_scale[t] = c.k_scales[((vp * c.key_heads + key_head) << c.shift) + v_in];
+        s.v_scale[t] = c.v_scales[vn];
+      }
+      s.k_scale[t] = f.v[t] < 0 ? __builtin_nanf("") : s.k_scale[t];
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        s.k[t][j] = *reinterpret_cast<const v4i *>(k + 32 * j);
+        s.v[t][j] = *reinterpret_cast<const v4i *>(v + 512 * j);
+      }
+    }
+  }
+};
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ float halves_max(float v) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __builtin_fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+
+struct Columns32 {
+  v8h q[2][4];  // the two parts of dims 16 (2 j + h) + 8 i .. + 7, at 2 j + i
+  float factor, m, den;
+  v16f acc[2];  // dims 32 d + 8 (i / 4) + 4 h + i % 4
+  int power;
+
+  __device__ __forceinline__ void clear() {
+    m = -__builtin_inff();
+    den = 0.0f;
+    power = -300;
+#pragma unroll
+    for (int d = 0; d < 2; d++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
+  }
+  // From dims 16 (2 j + h) .. + 15 of the lane's column.
+  __device__ __forceinline__ void begin(const float4 (&x)[2][4]) {
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float y[4] = {x[i / 4][i % 4].x, x[i / 4][i % 4].y, x[i / 4][i % 4].z, x[i / 4][i % 4].w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint32_t bits = __float_as_uint(y[j]) & 0x7fffffffu;
+        big = bits > big ? bits : big;
+      }
+    }
+    const auto p = __builtin_amdgcn_permlane32_swap(big, big, false, false);
+    big = p[0] > p[1] ? p[0] : p[1];
+    const bool finite = big < 0x7f800000u;
+    int e = !finite || big == 0 ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(big));
+    e = e < -90 ? -90 : e;
+    // log2(e) / 8: scores in powers of two.
+    factor = finite ? __builtin_ldexpf(0.180336880111120426f, e - 14) : __builtin_nanf("");
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float y[4] = {x[i / 4][i % 4].x, x[i / 4][i % 4].y, x[i / 4][i % 4].z, x[i / 4][i % 4].w};
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float scaled = finite ? __builtin_ldexpf(y[j], 14 - e) : 0.0f;
+        const _Float16 high = static_cast<_Float16>(scaled);
+        q[0][i / 2][i % 2 * 4 + j] = high;
+        q[1][i / 2][i % 2 * 4 + j] = static_cast<_Float16>(scaled - static_cast<float>(high));
+      }
+    }
+  }
+
+  __device__ __forceinline__ void consume(const Stage32 &s, int key0, int last_block) {
+    const int h = threadIdx.x >> 5 & 1;
+    const float ninf = -__builtin_inff();
+    bool none[2];
+    float k_scale[2], v_scale[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      none[t] = key0 / kBlock + 2 * t + h > last_block;  // a block behind the last
+      const float v = none[t] ? 0.0f : s.v_scale[t];
+      k_scale[t] = v != v ? __builtin_nanf("") : s.k_scale[t];
+      v_scale[t] = v != v ? 0.0f : v;
+    }
+    const float widest = halves_max(__builtin_fmaxf(v_scale[0], v_scale[1]));
+    int above = widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -300;
+    above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
+    const int lower = power - above;
+    power = above;
+    v16f sums[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      v16f sum;
+#pragma unroll
+      for (int i = 0; i < 16; i++) sum[i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const v8h first = halves_of(s.k[t][j][0], s.k[t][j][1]), second = halves_of(s.k[t][j][2], s.k[t][j][3]);
+#pragma unroll
+        for (int part = 1; part >= 0; part--) {
+          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(first, q[part][2 * j], sum, 0, 0, 0);
+          sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(second, q[part][2 * j + 1], sum, 0, 0, 0);
+        }
+      }
+      sums[t] = sum;
+    }
+    float scale[2], top = ninf;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      scale[t] = none[t] ? 0.0f : factor * k_scale[t];
+      float most = sums[t][0];
+#pragma unroll
+      for (int i = 1; i < 16; i++) most = __builtin_fmaxf(most, sums[t][i]);
+      top = __builtin_fmaxf(top, none[t] ? ninf : most * scale[t]);
+    }
+    top = __builtin_fmaxf(m, halves_max(top));
+    const float from = top == ninf ? 0.0f : top;
+    if (__any(top > m) || lower < 0) {
+      const float keep = __builtin_amdgcn_exp2f(m - from), scaled = __builtin_ldexpf(keep, lower);
+      den = den * keep;
+#pragma unroll
+      for (int d = 0; d < 2; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[d][i] = acc[d][i] * scaled;
+      m = top;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      const float minus = none[t] ? ninf : -from, weight = __builtin_ldexpf(v_scale[t], 64 - power);
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        // Positions 8 half .. + 7 of block 2 t + h.
+        v4i words[3];
+#pragma unroll
+        for (int pair = 0; pair < 4; pair++) {
+          uint32_t bits[3][2];
+#pragma unroll
+          for (int j = 0; j < 2; j++) {
+            const float e = __builtin_amdgcn_exp2f(fmaf_(sums[t][8 * half + 2 * pair + j], scale[t], minus));
+            den = den + e;
+            float left = e * weight;
+#pragma unroll
+            for (int d = 0; d < 3; d++) {
+              bits[d][j] = __float_as_uint(left);
+              left = left - __uint_as_float(bits[d][j] & 0xffff0000u);
+            }
+          }
+#pragma unroll
+          for (int d = 0; d < 3; d++) words[d][pair] = static_cast<int>(upper(bits[d][1], bits[d][0]));
+        }
+        v8bf codes[2];
+#pragma unroll
+        for (int d = 0; d < 2; d++) codes[d] = codes_of(s.v[t][d][2 * half], s.v[t][d][2 * half + 1]);
+#pragma unroll
+        for (int part = 2; part >= 0; part--)
+#pragma unroll
+          for (int d = 0; d < 2; d++)
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(codes[d], __builtin_bit_cast(v8bf, words[part]), acc[d], 0, 0, 0);
+      }
+    }
+  }
+};
+
+// Every wave has 32 columns and a part of the keys to itself, so that any number of
 // columns leaves no wave idle. Waves follow one another by column, key head of one value
 // head, then part and value head, and each XCD has a stretch of them.
 template <bool WIDE>
 __global__ __launch_bounds__(256, 2) void prefix_kernel(AttendArgs a) {
   const Cache &c = a.c;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int share = c.key_heads / c.kv_heads, group = c.n_heads / c.key_heads, columns = group * c.rows;
   int task = (blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8) * 4 + wave;
@@ -1350,22 +1570,40 @@ __global__ __launch_bounds__(256, 2) void prefix_kernel(AttendArgs a) {
   if (!__any(find_owners(a, row0, rows, owner, lane, 64))) return;
   asm volatile("" ::: "memory");
   const int begin = part * a.prefix_chunk, end = begin + a.prefix_chunk < a.base ? begin + a.prefix_chunk : a.base;
-  Column column[2];
-  int power;
-  walk_prefix<WIDE, 2>(a, column, power, key_head, column0, row0, rows, owner, begin, end);
+  // The lane's column: row column / group, head key_head * group + column % group. One that
+  // is no row's has a query of zeros, and is left out in the end.
+  const int column = column0 + l32, row = column / group;
+  const bool live = column < columns && owner[row - row0] >= 0;
+  const size_t at = static_cast<size_t>(row) * c.n_heads + key_head * group + column % group;
+  Reader32<WIDE> reader(c, a.prefix, key_head, a.base);
+  Stage32 stage[2];
+  auto next = reader.find(begin);
+  float4 x[2][4];
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int at = column0 + 16 * i + l16;
-    if (at >= columns || owner[at / group - row0] < 0) continue;
-    const size_t slot = (static_cast<size_t>(at / group) * c.n_heads + key_head * group + at % group) * a.parts + part;
+  for (int j = 0; j < 2; j++)
 #pragma unroll
-    for (int d = 0; d < 4; d++) {
+    for (int i = 0; i < 4; i++)
+      x[j][i] = live ? reinterpret_cast<const float4 *>(a.q + at * 64 + 16 * (2 * j + h))[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  reader.load(next, begin, stage[0]);
+  next = reader.find(begin + 64);
+  Columns32 state;
+  state.clear();
+  state.begin(x);
+  walk(reader, stage, next, begin, end, [&](const Stage32 &now, int key0) { state.consume(now, key0, reader.last_block); });
+  if (__any(reader.missing) && lane < rows && owner[lane] >= 0) c.refused[owner[lane]] = 1;
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(state.den), __float_as_uint(state.den), false, false);
+  state.den = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+  if (!live) return;
+  const size_t slot = at * a.parts + part;
+#pragma unroll
+  for (int d = 0; d < 2; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
       v4f o;
 #pragma unroll
-      for (int j = 0; j < 4; j++) o[j] = __builtin_ldexpf(column[i].acc[d][j], power - 64);
-      store_part(a, slot, 16 * d + 4 * g, o, column[i].m, column[i].den);
+      for (int j = 0; j < 4; j++) o[j] = __builtin_ldexpf(state.acc[d][4 * i + j], state.power - 64);
+      store_part(a, slot, 32 * d + 8 * i + 4 * h, o, state.m, state.den);
     }
-  }
 }
 
 // The parts of a sequence's rows of one head: as many of the waves for each row as
