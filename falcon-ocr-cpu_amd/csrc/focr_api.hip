@@ -185,11 +185,11 @@ int focr_ctx_create(int device, focr_ctx **out) {
   err = hipMalloc(&ctx->rms_dev, 8 * sizeof(float));
   if (err == hipSuccess)
     err = hipHostMalloc(reinterpret_cast<void **>(&ctx->flags), 16 * sizeof(uint32_t), hipHostMallocDefault);
-  if (err == hipSuccess) err = hipMalloc(reinterpret_cast<void **>(&ctx->arrived), Ctx::kSplitRows * sizeof(uint32_t));
-  if (err == hipSuccess) err = hipMemsetAsync(ctx->arrived, 0, Ctx::kSplitRows * sizeof(uint32_t), ctx->own);
+  if (err == hipSuccess) err = hipMalloc(reinterpret_cast<void **>(&ctx->joins), kJoinRows * sizeof(RowJoin));
+  if (err == hipSuccess) err = hipMemsetAsync(ctx->joins, 0, kJoinRows * sizeof(RowJoin), ctx->own);
   if (err == hipSuccess) err = hipStreamSynchronize(ctx->own);
   if (err != hipSuccess) {
-    if (ctx->arrived) (void)hipFree(ctx->arrived);
+    if (ctx->joins) (void)hipFree(ctx->joins);
     if (ctx->flags) (void)hipHostFree(ctx->flags);
     if (ctx->rms_dev) (void)hipFree(ctx->rms_dev);
     (void)hipEventDestroy(ctx->order);
@@ -211,7 +211,7 @@ int focr_ctx_destroy(focr_ctx *handle) {
   if (ctx->argmax) FOCR_HIP_CHECK(hipHostFree(ctx->argmax));
   if (ctx->rms_dev) FOCR_HIP_CHECK(hipFree(ctx->rms_dev));
   if (ctx->flags) FOCR_HIP_CHECK(hipHostFree(ctx->flags));
-  if (ctx->arrived) FOCR_HIP_CHECK(hipFree(ctx->arrived));
+  if (ctx->joins) FOCR_HIP_CHECK(hipFree(ctx->joins));
   FOCR_HIP_CHECK(hipEventDestroy(ctx->order));
   FOCR_HIP_CHECK(hipStreamDestroy(ctx->own));
   delete ctx;

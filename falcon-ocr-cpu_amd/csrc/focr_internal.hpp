@@ -38,6 +38,15 @@ struct alignas(16) ArgmaxPart {
   uint32_t nonfinite, pad;
 };
 
+// Where the workgroups of a row of focr_logits_select join what they have found: the
+// largest key, and how many have arrived. A cache line each, as atomics on one line wait
+// for one another.
+struct alignas(128) RowJoin {
+  unsigned long long key;
+  uint32_t arrived;
+};
+constexpr int kJoinRows = 1024;
+
 // ---- context ---------------------------------------------------------------
 struct Ctx {
   int device = 0;
@@ -53,9 +62,7 @@ struct Ctx {
   size_t argmax_parts = 0;
   float *rms_dev = nullptr;  // [8] row scales of a decode GEMV whose width has no in-kernel rms_norm
   uint32_t *flags = nullptr;  // [16] words of pinned host memory that kernels write and a synchronous call reads
-  // focr_logits_select: how many of a row's workgroups have arrived (device; 0 between calls).
-  static constexpr int kSplitRows = 512, kSegments = 64;
-  uint32_t *arrived = nullptr;  // [kSplitRows]
+  RowJoin *joins = nullptr;  // [kJoinRows] (device; 0 between calls)
   hipEvent_t order = nullptr;  // orders a new stream after the old one (focr_ctx_set_stream)
 };
 

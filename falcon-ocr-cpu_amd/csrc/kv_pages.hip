@@ -1010,43 +1010,6 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
 // with states (m_i, d_i, o_i) of disjoint keys, m = max m_i, o = sum 2^(m_i - m) o_i /
 // sum 2^(m_i - m) d_i.
 //
-// A wave takes 16 GROUPS columns and holds all that is theirs in its lanes. Scores. Lane
-// (l16, g) has column l16's query as two FP16 numbers an element, of 2^14 times the
-// power of two above the largest (so 24 bits of each element down to 2^-14 of the largest, and 2^-39 of that one for all); a key's
-// codes are FP16 numbers, so products are exact, and their sums round as FP32's do. Row m
-// of key tile t is key 4 m + t, as the codes stand, so that lane (l16, g) gets the scores
-// of column l16 with the 16 keys of block g, one scale for all of them. Weights. exp2(s - m)
-// times the block's value scale is three BF16 numbers, as in attend_kernel, which
-// stand where the second product takes them: its operand is lane (l16, g)'s eight keys of block g
-// by column l16, the other the value codes of dim l16 and these keys, as they stand.
-struct WideStage {
-  v4i k[4], v[4];
-  float k_scale, v_scale;  // of block g
-};
-template <bool WIDE>
-struct WideReader {
-  Reader<WIDE> reader;
-  __device__ __forceinline__ Found find(int key0) const { return reader.find(key0); }
-  __device__ __forceinline__ void load(const Found &f, int key0, WideStage &s) {
-    const Cache &c = reader.c;
-    const int g = threadIdx.x >> 4 & 3, at = key0 / kBlock + g;
-    Stage plain;
-    reader.load(f, key0, plain);
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      s.k[i] = plain.k[i];
-      s.v[i] = plain.v[i];
-    }
-    // The scales of block g, whose page the lane has for its values.
-    const int in = (at < reader.last_block ? at : reader.last_block) & ((1 << c.shift) - 1);
-    const long page = f.v_page < 0 ? 0 : f.v_page;
-    const float k_scale = c.k_scales[((page * c.key_heads + reader.key_head) << c.shift) + in];
-    const float v_scale = c.v_scales[((page * c.kv_heads + reader.value_head) << c.shift) + in];
-    s.k_scale = f.v_page < 0 ? __builtin_nanf("") : k_scale;
-    s.v_scale = v_scale;
-  }
-};
-
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
@@ -1063,159 +1026,6 @@ __device__ __forceinline__ v8h halves_of(int first, int second) {
       to[2 * i + j] = __builtin_bit_cast(int, __builtin_bit_cast(v2h, bits) - v2h{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)});
     }
   return __builtin_bit_cast(v8h, to);
-}
-
-// Largest over the four lanes (l16, 0 .. 3).
-__device__ __forceinline__ float across_max(float v) {
-  auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __builtin_fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __builtin_fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
-}
-__device__ __forceinline__ float across_sum(float v) {
-  auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
-  p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(p[0]) + __uint_as_float(p[1]);
-}
-
-// 16 columns of a wave: lane (l16, g) has column l16.
-struct Column {
-  v8h q[2][2];  // the two parts of dims 16 g + 8 h .. + 7
-  float factor, m, den;
-  v4f acc[4];   // dims 16 d + 4 g + i
-
-  __device__ __forceinline__ void clear() {
-    m = -__builtin_inff();
-    den = 0.0f;
-#pragma unroll
-    for (int d = 0; d < 4; d++) acc[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  // From dims 16 g .. + 15.
-  __device__ __forceinline__ void begin(const float4 (&x)[4]) {
-    uint32_t big = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const uint32_t bits = __float_as_uint(y[j]) & 0x7fffffffu;
-        big = bits > big ? bits : big;
-      }
-    }
-    auto p = __builtin_amdgcn_permlane16_swap(big, big, false, false);
-    big = p[0] > p[1] ? p[0] : p[1];
-    p = __builtin_amdgcn_permlane32_swap(big, big, false, false);
-    big = p[0] > p[1] ? p[0] : p[1];
-    const bool finite = big < 0x7f800000u;
-    int e = !finite || big == 0 ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(big));
-    e = e < -90 ? -90 : e;
-    // log2(e) / 8: scores in powers of two.
-    factor = finite ? __builtin_ldexpf(0.180336880111120426f, e - 14) : __builtin_nanf("");
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const float scaled = finite ? __builtin_ldexpf(y[j], 14 - e) : 0.0f;
-        const _Float16 high = static_cast<_Float16>(scaled);
-        q[0][i / 2][i % 2 * 4 + j] = high;
-        q[1][i / 2][i % 2 * 4 + j] = static_cast<_Float16>(scaled - static_cast<float>(high));
-      }
-    }
-  }
-};
-
-template <int GROUPS>
-__device__ __forceinline__ void consume_wide(Column (&column)[GROUPS], int &power, const WideStage &s, int key0, int last_block) {
-  const int g = threadIdx.x >> 4 & 3;
-  const float ninf = -__builtin_inff();
-  const bool none = key0 / kBlock + g > last_block;  // a block behind the last
-  float v_scale = none ? 0.0f : s.v_scale;
-  const bool bad = v_scale != v_scale;
-  const float k_scale = bad ? __builtin_nanf("") : s.k_scale;
-  v_scale = bad ? 0.0f : v_scale;
-  const float widest = across_max(v_scale);
-  int above = widest > 0.0f ? __builtin_amdgcn_frexp_expf(widest) : -300;
-  above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
-  const int lower = power - above;
-  power = above;
-  const float weight = __builtin_ldexpf(v_scale, 64 - power);
-  v4f sums[GROUPS][4];
-#pragma unroll
-  for (int t = 0; t < 4; t++) {
-    const v8h first = halves_of(s.k[t][0], s.k[t][1]), second = halves_of(s.k[t][2], s.k[t][3]);
-#pragma unroll
-    for (int c = 0; c < GROUPS; c++) {
-      v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int part = 1; part >= 0; part--) {
-        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(first, column[c].q[part][0], sum, 0, 0, 0);
-        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(second, column[c].q[part][1], sum, 0, 0, 0);
-      }
-      sums[c][t] = sum;
-    }
-  }
-  v8bf weights[GROUPS][3][2];
-#pragma unroll
-  for (int c = 0; c < GROUPS; c++) {
-    Column &u = column[c];
-    const float factor = none ? 0.0f : u.factor * k_scale;
-    float top = sums[c][0][0];
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) top = __builtin_fmaxf(top, sums[c][t][i]);
-    top = none ? ninf : top * factor;
-    top = __builtin_fmaxf(u.m, across_max(top));
-    const float from = top == ninf ? 0.0f : top;
-    if (__any(top > u.m) || lower < 0) {
-      const float keep = __builtin_amdgcn_exp2f(u.m - from), scaled = __builtin_ldexpf(keep, lower);
-      u.den = u.den * keep;
-#pragma unroll
-      for (int d = 0; d < 4; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) u.acc[d][i] = u.acc[d][i] * scaled;
-      u.m = top;
-    }
-    const float minus = none ? ninf : -from;
-#pragma unroll
-    for (int half = 0; half < 2; half++) {
-      v4i words[3];
-#pragma unroll
-      for (int pair = 0; pair < 4; pair++) {
-        uint32_t bits[3][2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-          // Position 8 half + 2 pair + j of the block: row i, tile t.
-          const int i = 2 * half + pair / 2, t = pair % 2 * 2 + j;
-          const float e = __builtin_amdgcn_exp2f(fmaf_(sums[c][t][i], factor, minus));
-          u.den = u.den + e;
-          float left = e * weight;
-#pragma unroll
-          for (int d = 0; d < 3; d++) {
-            bits[d][j] = __float_as_uint(left);
-            left = left - __uint_as_float(bits[d][j] & 0xffff0000u);
-          }
-        }
-#pragma unroll
-        for (int d = 0; d < 3; d++) words[d][pair] = static_cast<int>(upper(bits[d][1], bits[d][0]));
-      }
-#pragma unroll
-      for (int d = 0; d < 3; d++) weights[c][d][half] = __builtin_bit_cast(v8bf, words[d]);
-    }
-  }
-#pragma unroll
-  for (int d = 0; d < 4; d++) {
-    const v8bf first = codes_of(s.v[d][0], s.v[d][1]), second = codes_of(s.v[d][2], s.v[d][3]);
-#pragma unroll
-    for (int c = 0; c < GROUPS; c++)
-#pragma unroll
-      for (int part = 2; part >= 0; part--) {
-        column[c].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(first, weights[c][part][0], column[c].acc[d], 0, 0, 0);
-        column[c].acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(second, weights[c][part][1], column[c].acc[d], 0, 0, 0);
-      }
-  }
 }
 
 // The sequence of each of a tile's rows row0 .. row0 + rows - 1 that one which takes part
@@ -1236,101 +1046,6 @@ __device__ __forceinline__ bool find_owners(const AttendArgs &a, int row0, int r
   return any;
 }
 
-// A wave's keys begin .. end - 1 for its columns from column0 on, whose rows from row0 on
-// have these owners. Leaves the sums of `den` in every lane.
-template <bool WIDE, int GROUPS>
-__device__ __forceinline__ void walk_prefix(const AttendArgs &a, Column (&column)[GROUPS], int &power, int key_head, int column0,
-                                            int row0, int rows, const int *owner, int begin, int end) {
-  const Cache &c = a.c;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int group = c.n_heads / c.key_heads, columns = group * c.rows;
-#pragma unroll
-  for (int i = 0; i < GROUPS; i++) column[i].clear();
-  power = -300;
-  if (begin >= end || column0 >= columns) return;
-  WideReader<WIDE> reader{Reader<WIDE>(c, a.prefix, key_head, a.base)};
-  WideStage stage[2];
-  Found next = reader.find(begin);
-  // Column column0 + l16: row column / group, head key_head * group + column % group.
-  // One that is no row's has a query of zeros, and is left out in the end.
-  float4 x[GROUPS][4];
-#pragma unroll
-  for (int i = 0; i < GROUPS; i++) {
-    const int at = column0 + 16 * i + l16;
-    const bool live = at < columns && owner[at / group - row0] >= 0;
-    const float *q = a.q + (static_cast<size_t>(at / group) * c.n_heads + key_head * group + at % group) * 64 + 16 * g;
-#pragma unroll
-    for (int j = 0; j < 4; j++) x[i][j] = live ? reinterpret_cast<const float4 *>(q)[j] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  }
-  reader.load(next, begin, stage[0]);
-  next = reader.find(begin + 64);
-#pragma unroll
-  for (int i = 0; i < GROUPS; i++) column[i].begin(x[i]);
-  walk(reader, stage, next, begin, end,
-       [&](const WideStage &now, int key0) { consume_wide<GROUPS>(column, power, now, key0, reader.reader.last_block); });
-  if (__any(reader.reader.missing))
-    for (int r = lane; r < rows; r += 64)
-      if (owner[r] >= 0) c.refused[owner[r]] = 1;
-#pragma unroll
-  for (int i = 0; i < GROUPS; i++) column[i].den = across_sum(column[i].den);
-}
-
-// Up to 64 columns: a workgroup for a part of the keys, its four waves side by side over
-// the columns (`beside` of them) and the part's runs.
-template <bool WIDE>
-__global__ __launch_bounds__(256, 3) void prefix_few_kernel(AttendArgs a) {
-  const Cache &c = a.c;
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // The key heads of one value head follow one another on one XCD.
-  const int share = c.key_heads / c.kv_heads, turn_of = blockIdx.x / 8;
-  const int task = turn_of / share * 8 + blockIdx.x % 8;
-  const int key_head = task % c.kv_heads * share + turn_of % share, part = task / c.kv_heads;
-  if (part >= a.first_part) return;
-  const int group = c.n_heads / c.key_heads, columns = group * c.rows;
-  const int beside = a.beside, across = 16 * beside, runs = 4 / beside, run = wave / beside, column0 = wave % beside * 16;
-  __shared__ int owner[64];
-  if (threadIdx.x < 64) owner[threadIdx.x] = -1;
-  __syncthreads();
-  if (!__syncthreads_or(find_owners(a, 0, c.rows, owner, threadIdx.x, 256))) return;
-  const int from_key = part * a.prefix_chunk, to_key = from_key + a.prefix_chunk < a.base ? from_key + a.prefix_chunk : a.base;
-  const int each = (to_key - from_key + 64 * runs - 1) / (64 * runs) * 64;
-  const int begin = from_key + run * each, end = begin + each < to_key ? begin + each : to_key;
-  Column column[1];
-  int power;
-  walk_prefix<WIDE, 1>(a, column, power, key_head, column0, 0, c.rows, owner, begin, end);
-  // The waves' states meet in LDS: [run][column].
-  __shared__ float s_m[64], s_den[64];
-  __shared__ __attribute__((aligned(16))) float s_o[64][68];
-  const int to = 16 * wave + l16;
-  if (g == 0) {
-    s_m[to] = column[0].m;
-    s_den[to] = column[0].den;
-  }
-#pragma unroll
-  for (int d = 0; d < 4; d++) {
-    v4f o;
-#pragma unroll
-    for (int j = 0; j < 4; j++) o[j] = __builtin_ldexpf(column[0].acc[d][j], power - 64);
-    *reinterpret_cast<v4f *>(&s_o[to][16 * d + 4 * g]) = o;
-  }
-  __syncthreads();
-  const int dim = threadIdx.x % 16 * 4;
-  for (int at = threadIdx.x / 16; at < across; at += 16) {
-    if (at >= columns || owner[at / group] < 0) continue;
-    float top, total;
-    const v4f o = join_runs(s_m, s_den, s_o, at, across, runs, dim, top, total);
-    const size_t slot = (static_cast<size_t>(at / group) * c.n_heads + key_head * group + at % group) * a.parts + part;
-    store_part(a, slot, dim, o, top, total);
-  }
-}
-
-// More columns: 32 of a wave, on the matrix instructions of 32 by 32, which leave the
-// vector instructions more of the registers' ports (2 waves' 128 fused multiply-adds with
-// as many products: 542 cycles, with those of 16 by 16 658; byte permutations 600 and 690).
-// As above with lane (l32, h): row m of key tile t is position m % 4 + 4 (m / 8) of block
-// 2 t + m / 4 % 2, so that lane (l32, h) gets column l32's scores with the 16 keys of
-// blocks h and 2 + h, and its weights stand where the second product takes them.
 struct Stage32 {
   v4i k[2][2], v[2][2];  // [key tile][16 dims 2 j + h], [key tile][32 dims]
   float k_scale[2], v_scale[2];  // of block 2 t + h
@@ -1545,9 +1260,93 @@ struct Columns32 {
   }
 };
 
-// Every wave has 32 columns and a part of the keys to itself, so that any number of
-// columns leaves no wave idle. Waves follow one another by column, key head of one value
-// head, then part and value head, and each XCD has a stretch of them.
+// What a wave of the prefix's kernels has: its columns from column0 on, of rows from row0 on
+// with these owners, and keys begin .. end - 1. `at`: the lane's column's number among
+// all rows and heads.
+template <bool WIDE>
+__device__ __forceinline__ void walk_prefix(const AttendArgs &a, Columns32 &state, int key_head, bool live, size_t at, int rows,
+                                            const int *owner, int begin, int end) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, h = lane >> 5;
+  Reader32<WIDE> reader(c, a.prefix, key_head, a.base);
+  Stage32 stage[2];
+  auto next = reader.find(begin);
+  float4 x[2][4];
+#pragma unroll
+  for (int j = 0; j < 2; j++)
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      x[j][i] = live ? reinterpret_cast<const float4 *>(a.q + at * 64 + 16 * (2 * j + h))[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  reader.load(next, begin, stage[0]);
+  next = reader.find(begin + 64);
+  state.begin(x);
+  walk(reader, stage, next, begin, end, [&](const Stage32 &now, int key0) { state.consume(now, key0, reader.last_block); });
+  if (__any(reader.missing))
+    for (int r = lane; r < rows; r += 64)
+      if (owner[r] >= 0) c.refused[owner[r]] = 1;
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(state.den), __float_as_uint(state.den), false, false);
+  state.den = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
+
+// Up to 64 columns: a workgroup for a part of the keys, its four waves side by side over
+// the columns (`beside` of them) and the part's runs.
+template <bool WIDE>
+__global__ __launch_bounds__(256, 2) void prefix_few_kernel(AttendArgs a) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // The key heads of one value head follow one another on one XCD.
+  const int share = c.key_heads / c.kv_heads, turn_of = blockIdx.x / 8;
+  const int task = turn_of / share * 8 + blockIdx.x % 8;
+  const int key_head = task % c.kv_heads * share + turn_of % share, part = task / c.kv_heads;
+  if (part >= a.first_part) return;
+  const int group = c.n_heads / c.key_heads, columns = group * c.rows;
+  const int beside = a.beside, across = 32 * beside, runs = 4 / beside, run = wave / beside;
+  __shared__ int owner[64];
+  if (threadIdx.x < 64) owner[threadIdx.x] = -1;
+  __syncthreads();
+  if (!__syncthreads_or(find_owners(a, 0, c.rows, owner, threadIdx.x, 256))) return;
+  const int from_key = part * a.prefix_chunk, to_key = from_key + a.prefix_chunk < a.base ? from_key + a.prefix_chunk : a.base;
+  const int each = (to_key - from_key + 64 * runs - 1) / (64 * runs) * 64;
+  const int begin = from_key + run * each, end = begin + each < to_key ? begin + each : to_key;
+  const int column = wave % beside * 32 + l32, row = column / group;
+  const bool live = column < columns && owner[row] >= 0;
+  Columns32 state;
+  state.clear();
+  if (begin < end && __any(live))
+    walk_prefix<WIDE>(a, state, key_head, live, static_cast<size_t>(row) * c.n_heads + key_head * group + column % group, c.rows,
+                      owner, begin, end);
+  // The waves' states meet in LDS: [run][column].
+  __shared__ float s_m[128], s_den[128];
+  __shared__ __attribute__((aligned(16))) float s_o[128][68];
+  const int to = 32 * wave + l32;
+  if (h == 0) {
+    s_m[to] = state.m;
+    s_den[to] = state.den;
+  }
+#pragma unroll
+  for (int d = 0; d < 2; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v4f o;
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = __builtin_ldexpf(state.acc[d][4 * i + j], state.power - 64);
+      *reinterpret_cast<v4f *>(&s_o[to][32 * d + 8 * i + 4 * h]) = o;
+    }
+  __syncthreads();
+  const int dim = threadIdx.x % 16 * 4;
+  for (int at = threadIdx.x / 16; at < columns; at += 16) {
+    if (owner[at / group] < 0) continue;
+    float top, total;
+    const v4f o = join_runs(s_m, s_den, s_o, at, across, runs, dim, top, total);
+    const size_t slot = (static_cast<size_t>(at / group) * c.n_heads + key_head * group + at % group) * a.parts + part;
+    store_part(a, slot, dim, o, top, total);
+  }
+}
+
+// More columns: every wave has 32 of them and a part of the keys to itself, so that any
+// number of columns leaves no wave idle. Waves follow one another by column, key head of
+// one value head, then part and value head, and each XCD has a stretch of them.
 template <bool WIDE>
 __global__ __launch_bounds__(256, 2) void prefix_kernel(AttendArgs a) {
   const Cache &c = a.c;
@@ -1575,24 +1374,9 @@ __global__ __launch_bounds__(256, 2) void prefix_kernel(AttendArgs a) {
   const int column = column0 + l32, row = column / group;
   const bool live = column < columns && owner[row - row0] >= 0;
   const size_t at = static_cast<size_t>(row) * c.n_heads + key_head * group + column % group;
-  Reader32<WIDE> reader(c, a.prefix, key_head, a.base);
-  Stage32 stage[2];
-  auto next = reader.find(begin);
-  float4 x[2][4];
-#pragma unroll
-  for (int j = 0; j < 2; j++)
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      x[j][i] = live ? reinterpret_cast<const float4 *>(a.q + at * 64 + 16 * (2 * j + h))[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  reader.load(next, begin, stage[0]);
-  next = reader.find(begin + 64);
   Columns32 state;
   state.clear();
-  state.begin(x);
-  walk(reader, stage, next, begin, end, [&](const Stage32 &now, int key0) { state.consume(now, key0, reader.last_block); });
-  if (__any(reader.missing) && lane < rows && owner[lane] >= 0) c.refused[owner[lane]] = 1;
-  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(state.den), __float_as_uint(state.den), false, false);
-  state.den = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+  walk_prefix<WIDE>(a, state, key_head, live, at, rows, owner, begin, end);
   if (!live) return;
   const size_t slot = at * a.parts + part;
 #pragma unroll
@@ -1819,7 +1603,7 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
     const size_t columns = group * rows;
     few = columns <= 64;
     // Few columns: 512 workgroups, more: 2,048 waves, which all run at once.
-    a.beside = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
+    a.beside = columns <= 32 ? 1 : 2;
     const size_t tiles = few ? 1 : (columns + 31) / 32, all = few ? 512 : 2048;
     const size_t each = kv->key_heads * tiles, parts = each >= all ? 1 : all / each;
     const size_t prefix_chunk = std::max((shared + parts - 1) / parts, (shared + kMaxParts - 1) / kMaxParts);

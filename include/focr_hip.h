@@ -104,7 +104,7 @@ int focr_ctx_sync(focr_ctx *ctx);
  * after another; those that run side by side come from contexts of their own.
  * Device buffers a context owns, and so the only addresses of its own that a
  * captured graph can hold: the scratch (above), an 8-float row-scale array and
- * focr_logits_select's 512 counters, both allocated at creation (focr_argmax's
+ * focr_logits_select's words for 1024 rows, both allocated at creation (focr_argmax's
  * result words are read back to the host within the call, which therefore cannot
  * be captured). No
  * context buffer holds weights past the call that unpacked them (4-bit codes):
@@ -363,8 +363,8 @@ int focr_argmax(focr_ctx *ctx, const float *logits_dev, size_t rows, size_t voca
  * +infinity (what is not allowed is -infinity, whatever stood there).
  * append 1: a token that is not negative is written behind the row's history and
  * its length advanced, where there is room.
- * Asynchronous; 2^18 - 1 counted tokens and 2^14 - 1 biases at most. Uses the
- * context scratch. */
+ * Asynchronous; 2^18 - 1 counted tokens and 2^14 - 1 biases at most. Uses words
+ * of the context's own, no scratch. */
 int focr_logits_select(focr_ctx *ctx, const float *logits_dev, size_t rows, size_t vocab, int32_t *history_dev,
                        int32_t *history_len_dev, size_t history_cap, size_t recent, const float *penalties_dev,
                        size_t penalty_rows, const int32_t *bias_tokens_dev, const float *bias_dev, size_t n_bias,
