@@ -243,6 +243,82 @@ __device__ __forceinline__ void turn_bytes(uint32_t (&w)[4]) {
   w[3] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
 }
 
+// Writes a block of a stored head: `x` holds its positions, those before the unit's rows
+// from the FP32 block `open` (row0 < 0) if that is still the block's.
+__device__ __forceinline__ void put_block(const Cache &c, const Unit &unit, bool is_key, int held, int at_head, size_t slot, int block,
+                                          int last_block, v4f (&x)[4]) {
+  const int lane = threadIdx.x & 63, r4 = lane / 16 * 4, e4 = lane % 16 * 4;
+  const int row0 = block * kBlock - unit.len;
+  float *const open = c.open + (slot + block % 2) * kBlock * 64;
+  const bool earlier = row0 < 0;
+  const long number = c.block_at(unit.seq, block, held, at_head);
+  if (number < 0) {
+    c.refused[unit.seq] = 1;
+    return;
+  }
+  int8_t *const codes = (is_key ? c.k_codes : c.v_codes) + number * kBlockBytes;
+  float *const scale_at = (is_key ? c.k_scales : c.v_scales) + number;
+  int32_t *const writer_at = (is_key ? c.k_writers : c.v_writers) + number;
+  const bool kept = earlier && c.tags[slot + block % 2] == block && *writer_at == unit.seq;
+  if (earlier && !kept) {
+    // From the codes.
+    const float scale = *scale_at;
+    uint32_t w[4];
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+      w[s] = *reinterpret_cast<const uint32_t *>(is_key ? codes + s * 256 + lane * 4 : codes + (e4 + s) * kBlock + r4);
+    if (!is_key) turn_bytes(w);
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+      if (row0 + r4 + s < 0)
+        x[s] = v4f{sdwa_cvt<0>(w[s]) * scale, sdwa_cvt<1>(w[s]) * scale, sdwa_cvt<2>(w[s]) * scale, sdwa_cvt<3>(w[s]) * scale};
+  }
+  uint32_t big = 0;
+#pragma unroll
+  for (int s = 0; s < 4; s++) {
+    if (row0 + r4 + s >= unit.n) x[s] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t bits = __float_as_uint(x[s][i]) & 0x7fffffffu;
+      big = bits > big ? bits : big;
+    }
+  }
+  big = wave_max_bits(big);
+  float scale = __fdiv_rn(__uint_as_float(big), 127.0f);
+  if (scale < 1.17549435e-38f) scale = 0.0f;
+  float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+  if (big >= 0x7f800000u) {
+    scale = __builtin_nanf("");
+    inverse = 0.0f;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int s = 0; s < 4; s++) {
+    // 1.5 2^23 + code, rounded to nearest even, holds the code in its low byte.
+    uint32_t bits[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) bits[i] = __float_as_uint(x[s][i] * inverse + 12582912.0f);
+    const uint32_t lo = __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400u);
+    w[s] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[3], bits[2], 0x0c0c0400u), lo, 0x05040100u);
+  }
+  if (!is_key) turn_bytes(w);
+#pragma unroll
+  for (int s = 0; s < 4; s++)
+    *reinterpret_cast<uint32_t *>(is_key ? codes + s * 256 + lane * 4 : codes + (e4 + s) * kBlock + r4) = w[s];
+  if (lane == 0) {
+    *scale_at = scale;
+    *writer_at = unit.seq;
+  }
+  if (block >= last_block - 1) {
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      const int row = row0 + r4 + s;
+      if (row < unit.n && (row >= 0 || !kept)) *reinterpret_cast<v4f *>(open + (r4 + s) * 64 + e4) = x[s];
+    }
+    if (lane == 0) c.tags[slot + block % 2] = block;
+  }
+}
+
 // A wave takes one unit and one head: a stored head (keys, then values), or with QKV
 // a query head. Lane (r, c): elements 4 c .. + 3 of the block's positions 4 r + s, s =
 // 0 .. 3, so that a load or store of FP32 rows is 1 KB, key codes go to memory as
@@ -251,10 +327,7 @@ __device__ __forceinline__ void turn_bytes(uint32_t (&w)[4]) {
 // (16 query and key heads, 8 value heads) take 62 us for 188 MB read and 87 written,
 // 4.4 TB/s where a copy reaches 5.1; a row of each of 64 sequences 6.4 us, which is
 // the launch and three dependent trips to memory (batch, table, rows).
-//
-// With ANGLES the factors are formed from positions (rotary.hpp), bitwise those of
-// focr_rotary_factors.
-template <bool QKV, bool ANGLES>
+template <bool QKV>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, r4 = lane / 16 * 4, e4 = lane % 16 * 4;
@@ -295,14 +368,6 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     source = (is_key ? a.k : a.v) + (is_key ? head : head - c.key_heads) * 64;
   }
   const bool turned = QKV && (is_key || is_query);
-  float2 speed[kMaxAxes];
-  if constexpr (ANGLES)
-    if (turned) {
-#pragma unroll
-      for (int x = 0; x < kMaxAxes; x++)
-        if (x < a.axes)
-          speed[x] = *reinterpret_cast<const float2 *>(a.frequencies + (static_cast<size_t>(x) * c.n_heads + pair) * 32 + e4 / 2);
-    }
   const int first_block = unit.len / kBlock, blocks = touched(unit.len, unit.n), last_block = first_block + blocks - 1;
   const int held = is_key ? c.key_heads : c.kv_heads, at_head = is_key ? head : head - c.key_heads;
   const size_t slot = (static_cast<size_t>(unit.seq) * stored + head) * 2;
@@ -319,33 +384,9 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       const size_t at = unit.first + (row < 0 ? 0 : row < unit.n ? row : unit.n - 1);
       const float *from = earlier && row < 0 ? open + (r4 + s) * 64 : source + at * width;
       x[s] = *reinterpret_cast<const v4f *>(from + e4);
-      if constexpr (!ANGLES)
-        if (turned) f[s] = *reinterpret_cast<const v4f *>(a.rope + (at * c.n_heads + pair) * 64 + e4);
+      if (turned) f[s] = *reinterpret_cast<const v4f *>(a.rope + (at * c.n_heads + pair) * 64 + e4);
     }
     if (turned) {
-      if constexpr (ANGLES) {
-        float place[4][kMaxAxes];
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-          const int row = row0 + r4 + s;
-          const size_t at = unit.first + (row < 0 ? 0 : row < unit.n ? row : unit.n - 1);
-#pragma unroll
-          for (int x = 0; x < kMaxAxes; x++)
-            if (x < a.axes) place[s][x] = a.positions[at * a.axes + x];
-        }
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-          double angle[2] = {static_cast<double>(place[s][0]) * speed[0].x, static_cast<double>(place[s][0]) * speed[0].y};
-#pragma unroll
-          for (int x = 1; x < kMaxAxes; x++)
-            if (x < a.axes) {
-              angle[0] = __builtin_fma(static_cast<double>(place[s][x]), static_cast<double>(speed[x].x), angle[0]);
-              angle[1] = __builtin_fma(static_cast<double>(place[s][x]), static_cast<double>(speed[x].y), angle[1]);
-            }
-          const float2 u = cos_sin(angle[0]), v = cos_sin(angle[1]);
-          f[s] = v4f{u.x, u.y, v.x, v.y};
-        }
-      }
       v4f y[4] = {x[0], x[1], x[2], x[3]};
       norm_rotate(y, f);
       if (is_query) {
@@ -361,72 +402,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       for (int s = 0; s < 4; s++)
         if (row0 + r4 + s >= 0) x[s] = y[s];
     }
-    const long number = c.block_at(unit.seq, block, held, at_head);
-    if (number < 0) {
-      c.refused[unit.seq] = 1;
-      return;
-    }
-    int8_t *const codes = (is_key ? c.k_codes : c.v_codes) + number * kBlockBytes;
-    float *const scale_at = (is_key ? c.k_scales : c.v_scales) + number;
-    int32_t *const writer_at = (is_key ? c.k_writers : c.v_writers) + number;
-    const bool kept = earlier && c.tags[slot + block % 2] == block && *writer_at == unit.seq;
-    if (earlier && !kept) {
-      // From the codes.
-      const float scale = *scale_at;
-      uint32_t w[4];
-#pragma unroll
-      for (int s = 0; s < 4; s++)
-        w[s] = *reinterpret_cast<const uint32_t *>(is_key ? codes + s * 256 + lane * 4 : codes + (e4 + s) * kBlock + r4);
-      if (!is_key) turn_bytes(w);
-#pragma unroll
-      for (int s = 0; s < 4; s++)
-        if (row0 + r4 + s < 0)
-          x[s] = v4f{sdwa_cvt<0>(w[s]) * scale, sdwa_cvt<1>(w[s]) * scale, sdwa_cvt<2>(w[s]) * scale, sdwa_cvt<3>(w[s]) * scale};
-    }
-    uint32_t big = 0;
-#pragma unroll
-    for (int s = 0; s < 4; s++) {
-      if (row0 + r4 + s >= unit.n) x[s] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint32_t bits = __float_as_uint(x[s][i]) & 0x7fffffffu;
-        big = bits > big ? bits : big;
-      }
-    }
-    big = wave_max_bits(big);
-    float scale = __fdiv_rn(__uint_as_float(big), 127.0f);
-    if (scale < 1.17549435e-38f) scale = 0.0f;
-    float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
-    if (big >= 0x7f800000u) {
-      scale = __builtin_nanf("");
-      inverse = 0.0f;
-    }
-    uint32_t w[4];
-#pragma unroll
-    for (int s = 0; s < 4; s++) {
-      // 1.5 2^23 + code, rounded to nearest even, holds the code in its low byte.
-      uint32_t bits[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) bits[i] = __float_as_uint(x[s][i] * inverse + 12582912.0f);
-      const uint32_t lo = __builtin_amdgcn_perm(bits[1], bits[0], 0x0c0c0400u);
-      w[s] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(bits[3], bits[2], 0x0c0c0400u), lo, 0x05040100u);
-    }
-    if (!is_key) turn_bytes(w);
-#pragma unroll
-    for (int s = 0; s < 4; s++)
-      *reinterpret_cast<uint32_t *>(is_key ? codes + s * 256 + lane * 4 : codes + (e4 + s) * kBlock + r4) = w[s];
-    if (lane == 0) {
-      *scale_at = scale;
-      *writer_at = unit.seq;
-    }
-    if (block >= last_block - 1) {
-#pragma unroll
-      for (int s = 0; s < 4; s++) {
-        const int row = row0 + r4 + s;
-        if (row < unit.n && (row >= 0 || !kept)) *reinterpret_cast<v4f *>(open + (r4 + s) * 64 + e4) = x[s];
-      }
-      if (lane == 0) c.tags[slot + block % 2] = block;
-    }
+    put_block(c, unit, is_key, held, at_head, slot, block, last_block, x);
   };
   if (unit.index > 0) {
     process(first_block + unit.index);
@@ -436,6 +412,106 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
   // The last two, which may be written where the first was read.
   for (int block = last_block - 1 > first_block ? last_block - 1 : first_block + 1; block <= last_block; block++)
     process(block);
+}
+
+// The row step from positions (rotary.hpp): a wave takes one unit and one query head, and with
+// it the key head that is turned by the same factors, or one value head. Lanes are as
+// in append_kernel; a lane forms the factors of its two pairs in its four rows, bitwise
+// those of focr_rotary_factors, while the rows are on their way.
+template <int AXES>
+__global__ __launch_bounds__(256) void turn_kernel(AppendArgs a) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, r4 = lane / 16 * 4, e4 = lane % 16 * 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int at_unit = a.near ? (blockIdx.z * gridDim.y + blockIdx.y) * 8 + blockIdx.x % 8 : blockIdx.x;
+  const int task = (a.near ? blockIdx.x / 8 : blockIdx.y) * 4 + wave;
+  const auto of = [](int len, int n) {
+    const int blocks = touched(len, n);
+    return blocks <= 3 ? 1 : blocks - 2;
+  };
+  Unit unit;
+  const bool found = find_unit(c, at_unit, of, unit);
+  if (at_unit == 0 && task == 0 && c.row_start) {
+    // Marks every refused sequence.
+    Unit none;
+    find_unit(c, 0x7fffffff, of, none);
+  }
+  if (!found || task >= c.n_heads + c.kv_heads) return;
+  const bool is_value = task >= c.n_heads;
+  const int query = task, repeat = c.n_heads / c.key_heads, value_head = task - c.n_heads;
+  const bool has_key = !is_value && query % repeat == 0;
+  const int key_head = query / repeat;
+  const size_t width = static_cast<size_t>(c.n_heads + 2 * c.kv_heads) * 64;
+  const int stored = c.key_heads + c.kv_heads, at_stored = is_value ? c.key_heads + value_head : key_head;
+  const size_t slot = (static_cast<size_t>(unit.seq) * stored + at_stored) * 2;
+  const float *const key_source = a.qkv + (is_value ? c.n_heads + c.kv_heads + value_head : c.n_heads + key_head * c.kv_heads / c.key_heads) * 64;
+  const int first_block = unit.len / kBlock, blocks = touched(unit.len, unit.n), last_block = first_block + blocks - 1;
+  float2 speed[AXES];
+#pragma unroll
+  for (int x = 0; x < AXES; x++)
+    speed[x] = is_value ? make_float2(0.0f, 0.0f)
+                        : *reinterpret_cast<const float2 *>(a.frequencies + (static_cast<size_t>(x) * c.n_heads + query) * 32 + e4 / 2);
+
+  auto process = [&](int block) {
+    const int row0 = block * kBlock - unit.len;  // the row of its first position
+    const float *const open = c.open + (slot + block % 2) * kBlock * 64;
+    v4f x[4], y[4];
+    float place[4][AXES];
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      const int row = row0 + r4 + s;
+      const size_t at = unit.first + (row < 0 ? 0 : row < unit.n ? row : unit.n - 1);
+      // Earlier positions from the FP32 block, new ones from the rows.
+      if (is_value || has_key) x[s] = *reinterpret_cast<const v4f *>((row < 0 ? open + (r4 + s) * 64 : key_source + at * width) + e4);
+      if (!is_value) {
+        y[s] = *reinterpret_cast<const v4f *>(a.qkv + query * 64 + at * width + e4);
+#pragma unroll
+        for (int i = 0; i < AXES; i++) place[s][i] = a.positions[at * AXES + i];
+      }
+    }
+    if (!is_value) {
+      v4f f[4];
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        // A step of few rows leaves most places of a block without one.
+        const int row = row0 + r4 + s;
+        f[s] = v4f{1.0f, 0.0f, 1.0f, 0.0f};
+        if (unit.n < kBlock && !__any(row >= 0 && row < unit.n)) continue;
+        double angle[2];
+#pragma unroll
+        for (int i = 0; i < AXES; i++) {
+          const double p = place[s][i];
+          angle[0] = i == 0 ? p * speed[i].x : __builtin_fma(p, static_cast<double>(speed[i].x), angle[0]);
+          angle[1] = i == 0 ? p * speed[i].y : __builtin_fma(p, static_cast<double>(speed[i].y), angle[1]);
+        }
+        const float2 u = cos_sin(angle[0]), v = cos_sin(angle[1]);
+        f[s] = v4f{u.x, u.y, v.x, v.y};
+      }
+      norm_rotate(y, f);
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        const int row = row0 + r4 + s;
+        if (row >= 0 && row < unit.n)
+          *reinterpret_cast<v4f *>(a.q + (static_cast<size_t>(unit.first + row) * c.n_heads + query) * 64 + e4) = y[s];
+      }
+      if (!has_key) return;
+      v4f turned[4] = {x[0], x[1], x[2], x[3]};
+      norm_rotate(turned, f);
+#pragma unroll
+      for (int s = 0; s < 4; s++)
+        if (row0 + r4 + s >= 0) x[s] = turned[s];
+    }
+    put_block(c, unit, !is_value, is_value ? c.kv_heads : c.key_heads, is_value ? value_head : key_head, slot, block, last_block, x);
+  };
+  // The first, or one of a long unit's, and with the first the last two, which may be
+  // written where the first was read.
+  int block = first_block + unit.index;
+  const int end = unit.index > 0 ? block : last_block;
+  while (true) {
+    process(block);
+    if (block >= end) break;
+    block = block + 1 > last_block - 1 ? block + 1 : last_block - 1;
+  }
 }
 
 // ---- reading back --------------------------------------------------------------
@@ -486,7 +562,7 @@ struct AttendArgs {
   int max_len, chunk, parts, tiles;  // tiles: of 16 columns, for as many rows as a sequence can have
   // Positions below base are those of sequence `prefix`, in the first first_part of the
   // parts; own_parts hold a sequence's own.
-  int own_parts, first_part, base, prefix, prefix_chunk, beside;
+  int own_parts, first_part, base, prefix, prefix_chunk, prefix_tiles, prefix_blocks, beside;
 };
 
 // A sequence's rows for attention; false where there is nothing to do (n = 0) or it
@@ -911,14 +987,14 @@ __device__ __forceinline__ void walk(R &reader, S (&stage)[2], F next, int begin
 }
 
 template <bool WIDE>
-__global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
+__device__ __forceinline__ void attend(const AttendArgs &a, int block) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go to the 8 XCDs in turn: those of the key heads of one value head
   // follow one another on the same one, whose L2 then holds the values for all.
-  const int share = c.key_heads / c.kv_heads, turn_of = blockIdx.x / 8;
-  int task = (turn_of / share * 8 + blockIdx.x % 8) * share + turn_of % share;
+  const int share = c.key_heads / c.kv_heads, turn_of = block / 8;
+  int task = (turn_of / share * 8 + block % 8) * share + turn_of % share;
   const int key_head = task % c.key_heads;
   task /= c.key_heads;
   const int tile = task % a.tiles;
@@ -1000,6 +1076,11 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
     return;
   }
   store_part(a, out_row * a.parts + a.first_part + part, dim, o, top, total);
+}
+
+template <bool WIDE>
+__global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
+  attend<WIDE>(a, blockIdx.x);
 }
 
 // ---- attention over a prefix that the batch shares ----------------------------------
@@ -1291,7 +1372,7 @@ __device__ __forceinline__ void walk_prefix(const AttendArgs &a, Columns32 &stat
 // Up to 64 columns: a workgroup for a part of the keys, its four waves side by side over
 // the columns (`beside` of them) and the part's runs.
 template <bool WIDE>
-__global__ __launch_bounds__(256, 2) void prefix_few_kernel(AttendArgs a) {
+__device__ __forceinline__ void attend_prefix_few(const AttendArgs &a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1348,14 +1429,14 @@ __global__ __launch_bounds__(256, 2) void prefix_few_kernel(AttendArgs a) {
 // number of columns leaves no wave idle. Waves follow one another by column, key head of
 // one value head, then part and value head, and each XCD has a stretch of them.
 template <bool WIDE>
-__global__ __launch_bounds__(256, 2) void prefix_kernel(AttendArgs a) {
+__device__ __forceinline__ void attend_prefix(const AttendArgs &a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int share = c.key_heads / c.kv_heads, group = c.n_heads / c.key_heads, columns = group * c.rows;
-  int task = (blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8) * 4 + wave;
-  const int tile = task % a.tiles;
-  task /= a.tiles;
+  int task = (blockIdx.x % 8 * (a.prefix_blocks / 8) + blockIdx.x / 8) * 4 + wave;
+  const int tile = task % a.prefix_tiles;
+  task /= a.prefix_tiles;
   const int sharer = task % share;
   task /= share;
   const int key_head = task % c.kv_heads * share + sharer, part = task / c.kv_heads;
@@ -1388,6 +1469,18 @@ __global__ __launch_bounds__(256, 2) void prefix_kernel(AttendArgs a) {
       for (int j = 0; j < 4; j++) o[j] = __builtin_ldexpf(state.acc[d][4 * i + j], state.power - 64);
       store_part(a, slot, 32 * d + 8 * i + 4 * h, o, state.m, state.den);
     }
+}
+
+// Both in one launch, the prefix's workgroups first: they take longer, and where their
+// vector instructions are the bound, the sequences' own keys come from memory meanwhile.
+template <bool WIDE, bool FEW>
+__global__ __launch_bounds__(256, 2) void shared_kernel(AttendArgs a) {
+  if (static_cast<int>(blockIdx.x) >= a.prefix_blocks)
+    attend<WIDE>(a, blockIdx.x - a.prefix_blocks);
+  else if constexpr (FEW)
+    attend_prefix_few<WIDE>(a);
+  else
+    attend_prefix<WIDE>(a);
 }
 
 // The parts of a sequence's rows of one head: as many of the waves for each row as
@@ -1534,7 +1627,7 @@ int launch_append(Ctx *ctx, AppendArgs a, bool qkv) {
   // Units: n rows touch at most (n + 14) / 16 + 1 blocks, three of which are one
   // unit, so at most n / 16 units, or one.
   const int units = c.row_start ? c.rows / kBlock + (c.rows < c.n_seqs ? c.rows : c.n_seqs) : c.n_seqs;
-  const int heads = c.key_heads + c.kv_heads + (qkv ? c.n_heads : 0);
+  const int heads = a.positions ? c.n_heads + c.kv_heads : c.key_heads + c.kv_heads + (qkv ? c.n_heads : 0);
   FOCR_HIP_CHECK(hipSetDevice(ctx->device));
   const unsigned groups = static_cast<unsigned>((heads + 3) / 4);
   // Long prompts are near (us a call with its reading back, near / not: four of up to
@@ -1547,12 +1640,11 @@ int launch_append(Ctx *ctx, AppendArgs a, bool qkv) {
     const unsigned eights = static_cast<unsigned>((units + 7) / 8), y = std::min(eights, 32768u);
     grid = dim3(8 * groups, y, (eights + y - 1) / y);
   }
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, ctx->stream, a); };
   if (a.positions)
-    hipLaunchKernelGGL((append_kernel<true, true>), grid, dim3(256), 0, ctx->stream, a);
-  else if (qkv)
-    hipLaunchKernelGGL((append_kernel<true, false>), grid, dim3(256), 0, ctx->stream, a);
+    launch(a.axes == 1 ? turn_kernel<1> : a.axes == 2 ? turn_kernel<2> : a.axes == 3 ? turn_kernel<3> : turn_kernel<4>);
   else
-    hipLaunchKernelGGL((append_kernel<false, false>), grid, dim3(256), 0, ctx->stream, a);
+    launch(qkv ? append_kernel<true> : append_kernel<false>);
   FOCR_HIP_CHECK(hipGetLastError());
   return FOCR_OK;
 }
@@ -1596,8 +1688,6 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
   const size_t share = kv->key_heads / kv->kv_heads;
   const size_t grid = (heads * a.own_parts + 8 * share - 1) / (8 * share) * (8 * share);
   FOCR_REQUIRE(grid < (size_t(1) << 31), FOCR_E_SHAPE, std::string(name) + ": too many sequences and heads");
-  AttendArgs before = a;  // the prefix's kernel: other tiles
-  size_t before_grid = 0;
   bool few = false;
   if (shared > 0) {
     const size_t columns = group * rows;
@@ -1609,34 +1699,30 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
     const size_t prefix_chunk = std::max((shared + parts - 1) / parts, (shared + kMaxParts - 1) / kMaxParts);
     a.prefix_chunk = static_cast<int>((prefix_chunk + 63) / 64 * 64);
     a.first_part = static_cast<int>((shared + a.prefix_chunk - 1) / a.prefix_chunk);
-    before_grid = few ? (kv->kv_heads * a.first_part + 7) / 8 * 8 * share : (each * a.first_part + 31) / 32 * 8;
-    FOCR_REQUIRE(before_grid < (size_t(1) << 29), FOCR_E_SHAPE, std::string(name) + ": too many rows and heads");
-    before = a;
-    before.tiles = static_cast<int>(tiles);
+    a.prefix_tiles = static_cast<int>(tiles);
+    const size_t blocks = few ? (kv->kv_heads * a.first_part + 7) / 8 * 8 * share : (each * a.first_part + 31) / 32 * 8;
+    FOCR_REQUIRE(blocks + grid < (size_t(1) << 31), FOCR_E_SHAPE, std::string(name) + ": too many rows and heads");
+    a.prefix_blocks = static_cast<int>(blocks);
   }
-  a.parts = before.parts = a.first_part + a.own_parts;
+  a.parts = a.first_part + a.own_parts;
   const size_t slots = rows * kv->n_heads * a.parts;
   FOCR_HIP_CHECK(hipSetDevice(ctx->device));
   if (a.parts > 1) {
     rc = ensure_scratch(ctx, slots * 66 * sizeof(float));
     if (rc != FOCR_OK) return rc;
-    a.part_o = before.part_o = static_cast<float *>(ctx->scratch);
-    a.part_md = before.part_md = a.part_o + slots * 64;
+    a.part_o = static_cast<float *>(ctx->scratch);
+    a.part_md = a.part_o + slots * 64;
   }
   const bool wide = kv->page >= 64;
-  if (before_grid > 0) {
-    const dim3 all(static_cast<unsigned>(before_grid));
-    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, all, dim3(256), 0, ctx->stream, before); };
-    if (wide)
-      launch(few ? prefix_few_kernel<true> : prefix_kernel<true>);
-    else
-      launch(few ? prefix_few_kernel<false> : prefix_kernel<false>);
-    FOCR_HIP_CHECK(hipGetLastError());
-  }
-  if (wide)
-    hipLaunchKernelGGL(attend_kernel<true>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.prefix_blocks + grid)), dim3(256), 0, ctx->stream, a);
+  };
+  if (shared == 0)
+    launch(wide ? attend_kernel<true> : attend_kernel<false>);
+  else if (few)
+    launch(wide ? shared_kernel<true, true> : shared_kernel<false, true>);
   else
-    hipLaunchKernelGGL(attend_kernel<false>, dim3(static_cast<unsigned>(grid)), dim3(256), 0, ctx->stream, a);
+    launch(wide ? shared_kernel<true, false> : shared_kernel<false, false>);
   FOCR_HIP_CHECK(hipGetLastError());
   if (a.parts > 1) {
     const dim3 each(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(n_seqs));

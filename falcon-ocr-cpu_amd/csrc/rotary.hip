@@ -27,17 +27,26 @@ __global__ __launch_bounds__(256) void factors_kernel(FactorArgs a) {
     f[x][1] = v.y;
   }
   const int row0 = blockIdx.x * a.rows_each, rest = a.rows - row0, rows = rest < a.rows_each ? rest : a.rows_each;
-  for (int i = 0; i < rows; i++) {
-    const float *at = a.positions + static_cast<size_t>(row0 + i) * AXES;
-    double angle[2];
+  // Four rows' positions at a time, so that only the first are waited for.
+  for (int base = 0; base < rows; base += 4) {
+    float p[4][AXES];
 #pragma unroll
-    for (int x = 0; x < AXES; x++) {
-      const double p = at[x];
+    for (int i = 0; i < 4; i++) {
+      const float *at = a.positions + static_cast<size_t>(row0 + (base + i < rows ? base + i : base)) * AXES;
 #pragma unroll
-      for (int j = 0; j < 2; j++) angle[j] = x == 0 ? p * f[x][j] : __builtin_fma(p, f[x][j], angle[j]);
+      for (int x = 0; x < AXES; x++) p[i][x] = at[x];
     }
-    const float2 u = cos_sin(angle[0]), v = cos_sin(angle[1]);
-    a.out[static_cast<size_t>(row0 + i) * a.slots + slot] = make_float4(u.x, u.y, v.x, v.y);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (base + i >= rows) break;
+      double angle[2];
+#pragma unroll
+      for (int x = 0; x < AXES; x++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) angle[j] = x == 0 ? p[i][x] * f[x][j] : __builtin_fma(static_cast<double>(p[i][x]), f[x][j], angle[j]);
+      const float2 u = cos_sin(angle[0]), v = cos_sin(angle[1]);
+      a.out[static_cast<size_t>(row0 + base + i) * a.slots + slot] = make_float4(u.x, u.y, v.x, v.y);
+    }
   }
 }
 
