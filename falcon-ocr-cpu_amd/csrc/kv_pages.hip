@@ -36,6 +36,7 @@ constexpr int kBlock = 16, kBlockBytes = kBlock * 64;
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 struct Pages {
@@ -1267,6 +1268,9 @@ struct Columns32 {
     above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
     const int lower = power - above;
     power = above;
+    // {-1, 0} and {0, -1} in BF16, in registers: as constants of the instruction both become the latter.
+    uint32_t less[2] = {0x0000bf80u, 0xbf800000u};
+    asm("" : "+v"(less[0]), "+v"(less[1]));
     v16f sums[2];
 #pragma unroll
     for (int t = 0; t < 2; t++) {
@@ -1309,24 +1313,27 @@ struct Columns32 {
       const float minus = none[t] ? ninf : -from, weight = __builtin_ldexpf(v_scale[t], 64 - power);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
-        // Positions 8 half .. + 7 of block 2 t + h.
+        // Positions 8 half .. + 7 of block 2 t + h. What a BF16 part leaves of a weight is one
+        // instruction: the sum of two products, with -1 and 0, and the weight, exact.
         v4i words[3];
 #pragma unroll
         for (int pair = 0; pair < 4; pair++) {
-          uint32_t bits[3][2];
+          float left[2];
 #pragma unroll
           for (int j = 0; j < 2; j++) {
             const float e = __builtin_amdgcn_exp2f(fmaf_(sums[t][8 * half + 2 * pair + j], scale[t], minus));
             den = den + e;
-            float left = e * weight;
-#pragma unroll
-            for (int d = 0; d < 3; d++) {
-              bits[d][j] = __float_as_uint(left);
-              left = left - __uint_as_float(bits[d][j] & 0xffff0000u);
-            }
+            left[j] = e * weight;
           }
 #pragma unroll
-          for (int d = 0; d < 3; d++) words[d][pair] = static_cast<int>(upper(bits[d][1], bits[d][0]));
+          for (int d = 0; d < 3; d++) {
+            const uint32_t word = upper(__float_as_uint(left[1]), __float_as_uint(left[0]));
+            words[d][pair] = static_cast<int>(word);
+            if (d < 2)
+#pragma unroll
+              for (int j = 0; j < 2; j++)
+                left[j] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, word), __builtin_bit_cast(v2bf, less[j]), left[j], false);
+          }
         }
         v8bf codes[2];
 #pragma unroll
@@ -1692,9 +1699,13 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
   if (shared > 0) {
     const size_t columns = group * rows;
     few = columns <= 64;
-    // Few columns: 512 workgroups, more: 2,048 waves, which all run at once.
+    // A workgroup, or a wave, for each compute unit or SIMD: the vector instructions are the
+    // bound, and one wave has them busy (us a call with 128 / 256 / 512 workgroups: 8
+    // sequences with up to 5 rows over 6,528 17.0 / 14.8 / 18.0, 64 with one 23.7 / 24.7 / 26.6, 4
+    // over 30,016 32.0 / 22.4 / 23.7; with 1,024 / 2,048 / 4,096 waves: 200 over 32,768
+    // 105 / 110 / 118, 100 with two rows over 8,192 41.8 / 44.8 / 52.2).
     a.beside = columns <= 32 ? 1 : 2;
-    const size_t tiles = few ? 1 : (columns + 31) / 32, all = few ? 512 : 2048;
+    const size_t tiles = few ? 1 : (columns + 31) / 32, all = few ? 256 : 1024;
     const size_t each = kv->key_heads * tiles, parts = each >= all ? 1 : all / each;
     const size_t prefix_chunk = std::max((shared + parts - 1) / parts, (shared + kMaxParts - 1) / kMaxParts);
     a.prefix_chunk = static_cast<int>((prefix_chunk + 63) / 64 * 64);
@@ -1729,7 +1740,8 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
     // Parts of all a sequence's rows (us a call with 4 / 16 waves: 26 parts of one row
     // 9.8 / 10.4, 3 of one in 64 sequences 112 / 120; 57 of two 34.8 / 32.8, 59 of
     // eight 33.3 / 20.3).
-    if (a.parts * (shared > 0 ? (rows + n_seqs - 1) / n_seqs : most) <= 64)
+    const bool four = shared > 0 ? n_seqs * kv->n_heads > 256 || a.parts * ((rows + n_seqs - 1) / n_seqs) <= 32 : a.parts * most <= 64;
+    if (four)
       hipLaunchKernelGGL(merge_kernel<4>, each, dim3(256), 0, ctx->stream, a);
     else
       hipLaunchKernelGGL(merge_kernel<16>, each, dim3(1024), 0, ctx->stream, a);
