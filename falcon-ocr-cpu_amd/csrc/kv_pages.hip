@@ -36,7 +36,6 @@ constexpr int kBlock = 16, kBlockBytes = kBlock * 64;
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 struct Pages {
@@ -1268,9 +1267,6 @@ struct Columns32 {
     above = __builtin_amdgcn_readfirstlane(above > power ? above : power);
     const int lower = power - above;
     power = above;
-    // {-1, 0} and {0, -1} in BF16, in registers: as constants of the instruction both become the latter.
-    uint32_t less[2] = {0x0000bf80u, 0xbf800000u};
-    asm("" : "+v"(less[0]), "+v"(less[1]));
     v16f sums[2];
 #pragma unroll
     for (int t = 0; t < 2; t++) {
@@ -1313,27 +1309,24 @@ struct Columns32 {
       const float minus = none[t] ? ninf : -from, weight = __builtin_ldexpf(v_scale[t], 64 - power);
 #pragma unroll
       for (int half = 0; half < 2; half++) {
-        // Positions 8 half .. + 7 of block 2 t + h. What a BF16 part leaves of a weight is one
-        // instruction: the sum of two products, with -1 and 0, and the weight, exact.
+        // Positions 8 half .. + 7 of block 2 t + h.
         v4i words[3];
 #pragma unroll
         for (int pair = 0; pair < 4; pair++) {
-          float left[2];
+          uint32_t bits[3][2];
 #pragma unroll
           for (int j = 0; j < 2; j++) {
             const float e = __builtin_amdgcn_exp2f(fmaf_(sums[t][8 * half + 2 * pair + j], scale[t], minus));
             den = den + e;
-            left[j] = e * weight;
+            float left = e * weight;
+#pragma unroll
+            for (int d = 0; d < 3; d++) {
+              bits[d][j] = __float_as_uint(left);
+              left = left - __uint_as_float(bits[d][j] & 0xffff0000u);
+            }
           }
 #pragma unroll
-          for (int d = 0; d < 3; d++) {
-            const uint32_t word = upper(__float_as_uint(left[1]), __float_as_uint(left[0]));
-            words[d][pair] = static_cast<int>(word);
-            if (d < 2)
-#pragma unroll
-              for (int j = 0; j < 2; j++)
-                left[j] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, word), __builtin_bit_cast(v2bf, less[j]), left[j], false);
-          }
+          for (int d = 0; d < 3; d++) words[d][pair] = static_cast<int>(upper(bits[d][1], bits[d][0]));
         }
         v8bf codes[2];
 #pragma unroll
