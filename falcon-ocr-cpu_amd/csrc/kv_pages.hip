@@ -560,16 +560,23 @@ struct AttendArgs {
   float *out;
   float *part_o, *part_md;  // [row][head][part][64], [..][2]
   int max_len, chunk, parts, tiles;  // tiles: of 16 columns, for as many rows as a sequence can have
-  // Positions below base are those of sequence `prefix`, in the first first_part of the
-  // parts; own_parts hold a sequence's own.
+};
+// Over a shared prefix: positions below base are those of sequence `prefix`, in the first
+// first_part of the parts; own_parts hold a sequence's own.
+struct SharedArgs : AttendArgs {
   int own_parts, first_part, base, prefix, prefix_chunk, prefix_tiles, prefix_blocks, beside;
 };
+template <typename Args>
+constexpr bool kShared = std::is_same<Args, SharedArgs>::value;
 
 // A sequence's rows for attention; false where there is nothing to do (n = 0) or it
 // is refused (bad), but for what `overlaps` says.
-__device__ __forceinline__ bool attend_span(const AttendArgs &a, int seq, int &len, int &first, int &n, bool &bad) {
+template <typename Args>
+__device__ __forceinline__ bool attend_span(const Args &a, int seq, int &len, int &first, int &n, bool &bad) {
   bad = !a.c.span(seq, len, first, n);
-  if (n > 8 || (n > 0 && (len + n > a.max_len || len < a.base))) bad = true;
+  if (n > 8 || (n > 0 && len + n > a.max_len)) bad = true;
+  if constexpr (kShared<Args>)
+    if (n > 0 && len < a.base) bad = true;
   return n > 0 && !bad;
 }
 
@@ -986,9 +993,18 @@ __device__ __forceinline__ void walk(R &reader, S (&stage)[2], F next, int begin
   }
 }
 
-template <bool WIDE>
-__device__ __forceinline__ void attend(const AttendArgs &a, int block) {
+//
+// Over a shared prefix it is the keys from `base` on, in the parts behind the prefix's.
+template <bool WIDE, typename Args>
+__device__ __forceinline__ void attend(const Args &a, int block) {
   const Cache &c = a.c;
+  int base = 0, own_parts = a.parts, first_part = 0;
+  if constexpr (kShared<Args>) {
+    base = a.base;
+    own_parts = a.own_parts;
+    first_part = a.first_part;
+  }
+  const bool whole = !kShared<Args> && own_parts == 1;  // no other part of a row: it is finished here
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Workgroups go to the 8 XCDs in turn: those of the key heads of one value head
@@ -999,17 +1015,17 @@ __device__ __forceinline__ void attend(const AttendArgs &a, int block) {
   task /= c.key_heads;
   const int tile = task % a.tiles;
   task /= a.tiles;
-  const int part = task % a.own_parts, seq = task / a.own_parts;
+  const int part = task % own_parts, seq = task / own_parts;
   if (seq >= c.n_seqs) return;
   const int group = c.n_heads / c.key_heads;
   int len, first, n;
   bool bad;
   const int start = start_of(c, seq);
   if (!attend_span(a, seq, len, first, n, bad)) {
-    if (bad && a.parts == 1 && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
+    if (bad && whole && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
     return;
   }
-  const int limit = len + n, from_key = a.base + part * a.chunk;
+  const int limit = len + n, from_key = base + part * a.chunk;
   if (16 * tile >= group * n || from_key >= limit) return;
   // Waves: runs of the part's keys, in whole 64s, times quads of columns.
   const int columns = group * n, left = columns - 16 * tile;
@@ -1050,7 +1066,7 @@ __device__ __forceinline__ void attend(const AttendArgs &a, int block) {
   if (__any(reader.missing) && lane == 0) c.refused[seq] = 1;
   // Asked here, where no load is waited for.
   if (overlaps(c, seq, first, start)) {
-    if (a.parts == 1 && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
+    if (whole && tile == 0 && wave == 0) refuse_rows(a, seq, key_head * group, group);
     return;
   }
 
@@ -1067,7 +1083,7 @@ __device__ __forceinline__ void attend(const AttendArgs &a, int block) {
   const v4f o = join_runs(s_m, s_den, s_o, col, wide, runs, dim, top, total);
   const int out_head = key_head * group + out_column / n;
   const size_t out_row = static_cast<size_t>(first + out_column % n) * c.n_heads + out_head;
-  if (a.parts == 1) {
+  if (whole) {
     const float factor = sink_factor(a.sinks, out_head, top, total);
     v4f y;
 #pragma unroll
@@ -1075,7 +1091,7 @@ __device__ __forceinline__ void attend(const AttendArgs &a, int block) {
     *reinterpret_cast<v4f *>(a.out + out_row * 64 + dim) = y;
     return;
   }
-  store_part(a, out_row * a.parts + a.first_part + part, dim, o, top, total);
+  store_part(a, out_row * a.parts + first_part + part, dim, o, top, total);
 }
 
 template <bool WIDE>
@@ -1086,11 +1102,27 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
 // ---- attention over a prefix that the batch shares ----------------------------------
 // The rows of a call see positions below `base` in the pages of one sequence, the
 // prefix, each row all of them, so all rows' queries of a key head are columns of the same
-// products, and the keys are read once for 64 columns at a time. What a row sees behind
-// `base` are its own sequence's positions (attend_kernel), and merge_kernel joins both:
-// with states (m_i, d_i, o_i) of disjoint keys, m = max m_i, o = sum 2^(m_i - m) o_i /
-// sum 2^(m_i - m) d_i.
+// products, and the keys are read once for 32 columns. What a row sees behind `base` are its
+// own sequence's positions (attend), and merge_kernel joins both: with states (m_i, d_i, o_i)
+// of disjoint keys, m = max m_i, o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) d_i.
 //
+// A wave takes 32 columns and 64 keys at a time, on the matrix instructions of 32 by 32.
+// Scores. Lane (l32, h) has column l32's query as two FP16 numbers an element, of 2^14 times the
+// power of two above the largest (to 2^-24 of an element, and 2^-39 of the largest at the
+// least); codes are FP16 numbers, so products are exact and their sums round as FP32's. Row m of
+// key tile t is position m % 4 + 4 (m / 8) of block 2 t + m / 4 % 2, so that lane (l32, h)
+// gets the scores of column l32 with the 16 keys of blocks h and 2 + h, a scale for each.
+// Weights. exp2(s - m) times the block's value scale is three BF16 numbers, as in consume, which
+// stand where the second product takes them; its other operand is the value codes of dim
+// l32 (and 32 + l32) as they stand, as BF16 numbers.
+//
+// Bound: the vector instructions, 605 for 64 keys, of which the codes' conversion is 176
+// and the weights' exponentials and parts 300, and the matrix instructions' 1,280 cycles, which
+// hide behind them in part only. 200 rows over 32,768 positions (8 key heads, 105 million
+// scores) take 94 us of the launch's 103; 512 columns' products alone are 27. The same with 16
+// columns a wave 108; with scores of one step more in flight, weights' parts by sums of two
+// products, or the scheduler told to mix both kinds it is no faster. Reading each sequence's
+// copy of the prefix would be 33 MB a sequence.
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 
@@ -1111,7 +1143,7 @@ __device__ __forceinline__ v8h halves_of(int first, int second) {
 
 // The sequence of each of a tile's rows row0 .. row0 + rows - 1 that one which takes part
 // has, by the threads of a workgroup or wave; `owner` begins at -1. False if none was found.
-__device__ __forceinline__ bool find_owners(const AttendArgs &a, int row0, int rows, int *owner, int thread, int threads) {
+__device__ __forceinline__ bool find_owners(const SharedArgs &a, int row0, int rows, int *owner, int thread, int threads) {
   const Cache &c = a.c;
   const int seq0 = c.row_start ? 0 : row0, seq_end = c.row_start ? c.n_seqs : row0 + rows;
   bool any = false;
@@ -1345,7 +1377,7 @@ struct Columns32 {
 // with these owners, and keys begin .. end - 1. `at`: the lane's column's number among
 // all rows and heads.
 template <bool WIDE>
-__device__ __forceinline__ void walk_prefix(const AttendArgs &a, Columns32 &state, int key_head, bool live, size_t at, int rows,
+__device__ __forceinline__ void walk_prefix(const SharedArgs &a, Columns32 &state, int key_head, bool live, size_t at, int rows,
                                             const int *owner, int begin, int end) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -1372,7 +1404,7 @@ __device__ __forceinline__ void walk_prefix(const AttendArgs &a, Columns32 &stat
 // Up to 64 columns: a workgroup for a part of the keys, its four waves side by side over
 // the columns (`beside` of them) and the part's runs.
 template <bool WIDE>
-__device__ __forceinline__ void attend_prefix_few(const AttendArgs &a) {
+__device__ __forceinline__ void attend_prefix_few(const SharedArgs &a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1429,7 +1461,7 @@ __device__ __forceinline__ void attend_prefix_few(const AttendArgs &a) {
 // number of columns leaves no wave idle. Waves follow one another by column, key head of
 // one value head, then part and value head, and each XCD has a stretch of them.
 template <bool WIDE>
-__device__ __forceinline__ void attend_prefix(const AttendArgs &a) {
+__device__ __forceinline__ void attend_prefix(const SharedArgs &a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1474,7 +1506,7 @@ __device__ __forceinline__ void attend_prefix(const AttendArgs &a) {
 // Both in one launch, the prefix's workgroups first: they take longer, and where their
 // vector instructions are the bound, the sequences' own keys come from memory meanwhile.
 template <bool WIDE, bool FEW>
-__global__ __launch_bounds__(256, 2) void shared_kernel(AttendArgs a) {
+__global__ __launch_bounds__(256, 2) void shared_kernel(SharedArgs a) {
   if (static_cast<int>(blockIdx.x) >= a.prefix_blocks)
     attend<WIDE>(a, blockIdx.x - a.prefix_blocks);
   else if constexpr (FEW)
@@ -1486,8 +1518,8 @@ __global__ __launch_bounds__(256, 2) void shared_kernel(AttendArgs a) {
 // The parts of a sequence's rows of one head: as many of the waves for each row as
 // there are, lane = element, eight parts of a wave in flight. Bound by the launch and
 // the trips to memory: 4.4 us for 7 parts of 25 rows, 5.3 for 57 parts of two.
-template <int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttendArgs a) {
+template <int WAVES, typename Args>
+__global__ __launch_bounds__(64 * WAVES) void merge_kernel(Args a) {
   const Cache &c = a.c;
   constexpr int BATCH = 8;
   const int head = blockIdx.x, seq = blockIdx.y;
@@ -1501,7 +1533,8 @@ __global__ __launch_bounds__(64 * WAVES) void merge_kernel(AttendArgs a) {
   if (!live) return;
   const int spread = n == 1 ? 1 : n == 2 ? 2 : n <= 4 ? 4 : 8;
   const int waves = spread < WAVES ? WAVES / spread : 1, own = wave % waves;
-  const int parts = a.first_part + (len + n - a.base - 1) / a.chunk + 1;
+  int parts = (len + n - 1) / a.chunk + 1;
+  if constexpr (kShared<Args>) parts = a.first_part + (len + n - a.base - 1) / a.chunk + 1;
   for (int r0 = 0; r0 < n; r0 += WAVES / waves) {
     const int r = r0 + wave / waves;
     const size_t row = static_cast<size_t>(first + (r < n ? r : 0)) * c.n_heads + head, at = row * a.parts;
@@ -1662,7 +1695,7 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
   FOCR_REQUIRE(q && out, FOCR_E_ARG, std::string(name) + ": null buffer");
   FOCR_REQUIRE(max_len > shared && max_len <= kv->seq_pages * kv->page, FOCR_E_SHAPE,
                std::string(name) + ": max_len is more than the shared positions, up to what a sequence's pages hold");
-  AttendArgs a = {};
+  SharedArgs a = {};
   a.c = cache_of(kv, rows, row_start, lens, n_seqs);
   a.q = q;
   a.sinks = sinks;
@@ -1718,26 +1751,32 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
     a.part_md = a.part_o + slots * 64;
   }
   const bool wide = kv->page >= 64;
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.prefix_blocks + grid)), dim3(256), 0, ctx->stream, a);
+  const AttendArgs &alone = a;
+  auto launch = [&](auto kernel, const auto &args) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(a.prefix_blocks + grid)), dim3(256), 0, ctx->stream, args);
   };
   if (shared == 0)
-    launch(wide ? attend_kernel<true> : attend_kernel<false>);
+    launch(wide ? attend_kernel<true> : attend_kernel<false>, alone);
   else if (few)
-    launch(wide ? shared_kernel<true, true> : shared_kernel<false, true>);
+    launch(wide ? shared_kernel<true, true> : shared_kernel<false, true>, a);
   else
-    launch(wide ? shared_kernel<true, false> : shared_kernel<false, false>);
+    launch(wide ? shared_kernel<true, false> : shared_kernel<false, false>, a);
   FOCR_HIP_CHECK(hipGetLastError());
   if (a.parts > 1) {
     const dim3 each(static_cast<unsigned>(kv->n_heads), static_cast<unsigned>(n_seqs));
     // Parts of all a sequence's rows (us a call with 4 / 16 waves: 26 parts of one row
     // 9.8 / 10.4, 3 of one in 64 sequences 112 / 120; 57 of two 34.8 / 32.8, 59 of
     // eight 33.3 / 20.3).
-    const bool four = shared > 0 ? n_seqs * kv->n_heads > 256 || a.parts * ((rows + n_seqs - 1) / n_seqs) <= 32 : a.parts * most <= 64;
-    if (four)
-      hipLaunchKernelGGL(merge_kernel<4>, each, dim3(256), 0, ctx->stream, a);
+    // Over a shared prefix by a sequence's mean rows, and 16 only for few sequences (17 parts of
+    // up to five rows in 8: 18.6 / 14.8; of one in 64 24.7 / 35.8; ten of five in 32 24.7 / 26.1).
+    const size_t mean = (rows + n_seqs - 1) / n_seqs;
+    const bool four = shared > 0 ? n_seqs * kv->n_heads > 256 || a.parts * mean <= 32 : a.parts * most <= 64;
+    const dim3 threads(four ? 256 : 1024);
+    auto merge = [&](auto kernel, const auto &args) { hipLaunchKernelGGL(kernel, each, threads, 0, ctx->stream, args); };
+    if (shared > 0)
+      merge(four ? merge_kernel<4, SharedArgs> : merge_kernel<16, SharedArgs>, a);
     else
-      hipLaunchKernelGGL(merge_kernel<16>, each, dim3(1024), 0, ctx->stream, a);
+      merge(four ? merge_kernel<4, AttendArgs> : merge_kernel<16, AttendArgs>, alone);
     FOCR_HIP_CHECK(hipGetLastError());
   }
   return FOCR_OK;
