@@ -1733,7 +1733,9 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
     a.beside = columns <= 32 ? 1 : 2;
     const size_t tiles = few ? 1 : (columns + 31) / 32, all = few ? 256 : 1024;
     const size_t each = kv->key_heads * tiles, parts = each >= all ? 1 : all / each;
-    const size_t prefix_chunk = std::max((shared + parts - 1) / parts, (shared + kMaxParts - 1) / kMaxParts);
+    // At most 4,096 keys a part up to a million, as their sums' roundings add up (3,648 keys: 6e-7
+    // of the result, 256: 2e-7).
+    const size_t prefix_chunk = std::max(std::min<size_t>((shared + parts - 1) / parts, 4096), (shared + kMaxParts - 1) / kMaxParts);
     a.prefix_chunk = static_cast<int>((prefix_chunk + 63) / 64 * 64);
     a.first_part = static_cast<int>((shared + a.prefix_chunk - 1) / a.prefix_chunk);
     a.prefix_tiles = static_cast<int>(tiles);

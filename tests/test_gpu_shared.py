@@ -100,6 +100,13 @@ def test_long_prefixes(fh, shared, page, sequences, rows):
     b.verify(host(b.shared_call()))
 
 
+def test_many_rows_over_a_long_prefix(fh):
+    # More columns than there are waves for: the prefix is still taken in parts of 4,096 keys.
+    n = 140
+    b = Batch(fh, 20480, [(7 * i) % 40 for i in range(n)], [8] * n, 128, seed=97)
+    b.verify(host(b.shared_call()), only=[0, 77, 139])
+
+
 def test_equals_attention_of_each_sequence(fh):
     # The same positions read by each sequence for itself: within the roundings of both.
     b = Batch(fh, 192, [5, 80, 0], [2, 1, 4], 32, seed=7)
@@ -151,6 +158,65 @@ def test_large_values_without_weight(fh, where, ratio):
     got = host(kv.attention_shared(to_dev(q), int32([shared + own - 1]), shared + own, shared))
     want, bound = accuracy.attention64(q, gk, gv, shared + own - 1)
     check(got, want, bound)
+
+
+@pytest.mark.parametrize("large", [1e4, 3e5])
+def test_a_large_query_element_that_meets_no_key(fh, large):
+    # Scores come from elements far below the largest one. A query's elements are off by 2^-24 of
+    # themselves, and 2^-39 of the largest (by 2^-30 of it among the sequence's own keys), times the key,
+    # and scores by the roundings of their own terms' sum and of the exponent.
+    shared, own, heads = 1024, 40, 2
+    kv = fh.KvPages(18, 64, 1, 18, heads, heads)
+    kv.map(0, 0, list(range(18)))
+    k, v, q = (gen.normal((n, heads, 64), 1.0, 91 + i) for i, n in enumerate((shared + own, shared + own, 1)))
+    k[:, :, 5] = 0
+    q[:, :, 5] = large
+    kv.append(to_dev(k), to_dev(v), int32([0]), row_start=int32([0, shared + own]))
+    gk, gv = (host(x).astype(np.float64) for x in kv.dequantize(shared + own, int32([0]), row_start=int32([0, shared + own])))
+    got = host(kv.attention_shared(to_dev(q), int32([shared + own - 1]), shared + own, shared)).astype(np.float64)
+    eps = 2.0 ** -24
+    for h in range(heads):
+        s = gk[:, h] @ q[0, h].astype(np.float64) / 8.0
+        w = np.exp(s - s.max())
+        w /= w.sum()
+        step = 2.0 ** -30 * large * np.abs(gk[:, h]).sum(axis=1).max() / 8
+        off = step + eps * (16 * (np.abs(gk[:, h]) @ np.abs(q[0, h])).max() / 8 + 8 * np.abs(s).max() + 16)
+        bound = w @ np.abs(gv[:, h]) * (2.2 * off + eps * (2 * 1024 + 112))
+        over = np.abs(got[0, h] - w @ gv[:, h]) / bound
+        assert (over <= 1).all(), f"head {h}: {over.max()} times what is allowed"
+
+
+@pytest.mark.parametrize("scale", [1e-34, 1e-20, 1e20, 1e35])
+def test_values_of_one_small_or_large_magnitude(fh, scale):
+    import test_gpu_pages_accuracy as accuracy
+
+    kv = fh.KvPages(6, 64, 1, 6, 2, 2)
+    kv.map(0, 0, [4, 2, 0, 1, 3, 5])
+    k, v, q = (gen.normal((n, 2, 64), 1.0, 101 + i) for i, n in enumerate((300, 300, 1)))
+    v *= F32(scale)
+    kv.append(to_dev(k), to_dev(v), int32([0]), row_start=int32([0, 300]))
+    gk, gv = (host(x) for x in kv.dequantize(300, int32([0]), row_start=int32([0, 300])))
+    got = host(kv.attention_shared(to_dev(q), int32([299]), 300, 256))
+    check(got, *accuracy.attention64(q, gk, gv, 299))
+
+
+@pytest.mark.parametrize("gap", [14.0, 20.0, 40.0])
+def test_a_first_key_that_takes_the_weight_and_has_no_value(fh, gap):
+    # Weights of e^-gap carry the whole result: half the dims' for a value of zeros there.
+    import test_gpu_pages_accuracy as accuracy
+
+    for half in (False, True):
+        kv = fh.KvPages(18, 64, 1, 18, 2, 2)
+        kv.map(0, 0, list(range(18)))
+        k, v, q = (gen.normal((n, 2, 64), 1.0, 111 + i) for i, n in enumerate((1100, 1100, 1)))
+        k[3] = accuracy.key_for(q, gap)
+        v[3] = 0
+        if half:
+            v[3, :, ::2] = 50.0
+        kv.append(to_dev(k), to_dev(v), int32([0]), row_start=int32([0, 1100]))
+        gk, gv = (host(x) for x in kv.dequantize(1100, int32([0]), row_start=int32([0, 1100])))
+        got = host(kv.attention_shared(to_dev(q), int32([1099]), 1100, 1024))
+        check(got, *accuracy.attention64(q, gk, gv, 1099))
 
 
 def test_non_finite_queries_keys_and_values(fh):
