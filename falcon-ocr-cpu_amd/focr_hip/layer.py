@@ -40,7 +40,8 @@ for Q8 records when ``options.exp`` is ExpMode.FAST, the exact one otherwise;
 fast mode's plan does (``PrefillAttention::Bf16`` / ``Bf16Static`` by
 ``options.softmax``). RoPE factors
 come from the caller ([rows][n_heads][32][2] cos/sin pairs), as
-``rotary_factors`` provides them to the reference's row kernels.
+``rotary_factors`` provides them to the reference's row kernels, or are formed
+on the device from positions with several axes (`Rotary.at`).
 
 Sessions that are decoded together keep their positions in a `KvPages` cache
 (one for each layer): `enter_pages` appends a prefilled prompt as one of its
@@ -49,7 +50,8 @@ sequences, and `decode_pages` runs one step of the whole batch::
     rms_norm(h) . qkv -> qkv                 the decode GEMV up to 8 rows in all (or 32, eight at a
                                              time, where the prompts' kernel is INT16's), else panels
     KvPages.qkv_rows -> q, codes             split, norm, rotation, append
-    KvPages.attention                        each sequence's rows over its pages
+    KvPages.attention                        each sequence's rows over its pages (attention_shared: over a
+                                             prompt that all have, read once, and then their own)
     wo, w13, w2                              as in `decode` or `prefill`
 
 `clock`, if given, is called with a stage name after each stage is
@@ -60,7 +62,7 @@ from __future__ import annotations
 from typing import Optional
 
 from . import (CompactKv, Context, Epilogue, ExpMode, FocrError, Geometry, KvPages, KvSplit, PrefillOptions, PrefillProjection,
-               Softmax, attention_decode_row, attention_prefill_bf16, attention_with, default_context,
+               RotaryRows, Softmax, attention_decode_row, attention_prefill_bf16, attention_with, default_context,
                default_fast_exp, qkv_rows,
                row_scales)
 
@@ -127,6 +129,14 @@ class DecoderLayer:
             self._work[name] = torch.empty(max(n, 2 * t.numel()), dtype=t.dtype, device=t.device)
         return self._buf(name, shape)
 
+    def _factors(self, rope, rows: int):
+        """The factors of `rows` rows, from their positions (`Rotary.at`) where `rope` has these."""
+        if type(rope) is not RotaryRows:
+            return rope
+        if rope.rotary.ctx is not self.ctx or rope.rotary.n_heads != self.n_heads:
+            raise FocrError(-2, "the frequencies are of other heads or another context")
+        return rope.rotary.factors(rope.positions, out=self._buf("rope", (rows, self.n_heads, 32, 2)))
+
     def kv(self, total: int) -> CompactKv:
         """The cache's first `total` positions as a CompactKv."""
         p = self.prefix_len
@@ -136,7 +146,7 @@ class DecoderLayer:
 
     def prefill(self, h, rope, image_start: int, image_end: int, clock=None):
         """The whole prompt (offset 0): updates `h` [rows][dim] in place and
-        fills the prefix cache."""
+        fills the prefix cache. `rope`: factors, or the rows' positions (`Rotary.at`)."""
         rows = h.shape[0]
         if self.len != 0:
             raise FocrError(-2, "a prefill forwards the whole prefix first")
@@ -146,6 +156,7 @@ class DecoderLayer:
             raise FocrError(-2, "attention image must be inside the prefix")
         ctx = self.ctx
         mark = clock or (lambda stage: None)
+        rope = self._factors(rope, rows)
         # The last prompt's sealed cache is gone; its buffers serve this one's.
         old, self.split = self.split, None
         if old is not None and (not old.handle or old.ctx is not ctx
@@ -206,7 +217,8 @@ class DecoderLayer:
 
     def decode(self, h, rope, clock=None):
         """1..=8 rows at positions len.. (a greedy step, or the last token plus
-        drafts): updates `h` [rows][dim] in place and appends to the cache."""
+        drafts): updates `h` [rows][dim] in place and appends to the cache. `rope`
+        as in `prefill`."""
         rows = h.shape[0]
         if not 1 <= rows <= 8:
             raise FocrError(-2, "decode takes 1..=8 rows")
@@ -214,6 +226,7 @@ class DecoderLayer:
             raise FocrError(-2, "KV context exhausted")
         ctx, p, pos = self.ctx, self.prefix_len, self.len
         mark = clock or (lambda stage: None)
+        rope = self._factors(rope, rows)
         qkv = self.qkv.linear_ex(h, rows, rms_norm=True, out=self._buf("dqkv", (rows, self.qkv.out_dim)))
         mark("qkv")
         total = pos + rows

@@ -91,6 +91,32 @@ def test_a_step_is_that_of_the_calls_it_replaces(fh, n):
     assert one.pages.refused() == two.pages.refused() == []
 
 
+def test_a_session_alone_takes_positions_too(fh):
+    # Prefill and decode of one session: positions in the place of factors, bitwise.
+    m, _ = matrices(fh)
+    rotary, got = fh.Rotary(frequencies()), []
+    p = gen.normal((40, 3), 20.0, 17)
+    for positions in (False, True):
+        for kv_bits in (32, 8):
+            layer = fh.DecoderLayer(m["qkv"], m["wo"], m["w13"], m["w2"], to_dev(gen.uniform((H,), -2.0, 2.0, 7)), 40, kv_bits=kv_bits)
+            of = (lambda x: rotary.at(to_dev(x))) if positions else (lambda x: rotary.factors(to_dev(x)))
+            paired = p.copy()
+            paired[:, 1:] = 0.0  # the sealed cache shares the temporal halves of paired heads
+            h = to_dev(gen.normal((34, DIM), 1.0, 19))
+            layer.prefill(h, of(paired[:34]), 0, 10)
+            step = to_dev(gen.normal((3, DIM), 1.0, 23))
+            layer.decode(step, of(paired[34:37]))
+            one = to_dev(gen.normal((1, DIM), 1.0, 29))
+            layer.decode(one, of(paired[37:38]))
+            got.append([host(x) for x in (h, step, one)])
+    for a, b in zip(got[:2], got[2:]):
+        for x, y in zip(a, b):
+            assert_bitwise(x, y)
+    with pytest.raises(fh.FocrError) as e:
+        layer.decode(to_dev(np.ones((1, DIM), F32)), fh.Rotary(np.ones((1, 4, 32), F32)).at(to_dev(np.ones((1, 1), F32))))
+    assert e.value.code == -2
+
+
 def test_a_captured_step_advances_itself(fh):
     import torch
 
