@@ -565,6 +565,7 @@ struct AttendArgs {
 // first_part of the parts; own_parts hold a sequence's own.
 struct SharedArgs : AttendArgs {
   int own_parts, first_part, base, prefix, prefix_chunk, prefix_tiles, prefix_blocks, beside;
+  int alone;  // a sequence's own by waves
 };
 template <typename Args>
 constexpr bool kShared = std::is_same<Args, SharedArgs>::value;
@@ -1099,6 +1100,66 @@ __global__ __launch_bounds__(256, 3) void attend_kernel(AttendArgs a) {
   attend<WIDE>(a, blockIdx.x);
 }
 
+// What attend does for a part of a sequence and a key head, by one wave, four columns at a
+// time: for many sequences of short lengths, as a launch over a shared prefix has room for two
+// workgroups a compute unit, and one for each of 64 sequences and 16 key heads would wait.
+template <bool WIDE>
+__device__ __forceinline__ void attend_alone(const SharedArgs &a, int block) {
+  const Cache &c = a.c;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int task = 4 * block + wave;
+  const int key_head = task % c.key_heads;
+  task /= c.key_heads;
+  const int part = task % a.own_parts, seq = task / a.own_parts;
+  if (seq >= c.n_seqs) return;
+  const int group = c.n_heads / c.key_heads;
+  int len, first, n;
+  bool bad;
+  const int start = start_of(c, seq);
+  if (!attend_span(a, seq, len, first, n, bad)) return;
+  const int limit = len + n, columns = group * n, begin = a.base + part * a.chunk;
+  const int end = begin + a.chunk < limit ? begin + a.chunk : limit;
+  if (begin >= end) return;
+  __shared__ __attribute__((aligned(16))) uint16_t turned[4][16 * kTurned];
+  __shared__ float s_m[16], s_den[16];
+  __shared__ __attribute__((aligned(16))) float s_o[16][68];
+  *reinterpret_cast<uint2 *>(turned[wave] + (12 + g) * kTurned + 4 * l16) = make_uint2(0, 0);
+  Reader<WIDE> reader(c, seq, key_head, limit);
+  for (int column0 = 0; column0 < columns; column0 += 4) {
+    Stage stage[2];
+    Found next = reader.find(begin);
+    float4 x[4];
+    const int wanted = column0 + l16 / 4, column = wanted < columns ? wanted : columns - 1;
+    const float *q = a.q + (static_cast<size_t>(first + column % n) * c.n_heads + key_head * group + column / n) * 64 + 16 * g;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = reinterpret_cast<const float4 *>(q)[i];
+    reader.load(next, begin, stage[0]);
+    next = reader.find(begin + 64);
+    Quad quad;
+    int power = -300;
+    quad.begin(x);
+    const int mine = column0 + g;
+    quad.visible = len + (mine < columns ? mine : columns - 1) % n + 1;
+    walk(reader, stage, next, begin, end,
+         [&](const Stage &now, int key0) { consume(quad, power, now, key0, reader.last_block, turned[wave]); });
+    if (column0 == 0) {
+      if (__any(reader.missing) && lane == 0) c.refused[seq] = 1;
+      if (overlaps(c, seq, first, start)) return;
+    }
+    quad.end(power, s_m + 4 * wave, s_den + 4 * wave, s_o + 4 * wave);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // Lane: a column and four dims.
+    const int at = column0 + g, dim = 4 * l16;
+    if (at < columns) {
+      const size_t row = static_cast<size_t>(first + at % n) * c.n_heads + key_head * group + at / n;
+      store_part(a, row * a.parts + a.first_part + part, dim, *reinterpret_cast<const v4f *>(&s_o[4 * wave + g][dim]), s_m[4 * wave + g],
+                 s_den[4 * wave + g]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
 // ---- attention over a prefix that the batch shares ----------------------------------
 // The rows of a call see positions below `base` in the pages of one sequence, the
 // prefix, each row all of them, so all rows' queries of a key head are columns of the same
@@ -1507,8 +1568,11 @@ __device__ __forceinline__ void attend_prefix(const SharedArgs &a) {
 // vector instructions are the bound, the sequences' own keys come from memory meanwhile.
 template <bool WIDE, bool FEW>
 __global__ __launch_bounds__(256, 2) void shared_kernel(SharedArgs a) {
-  if (static_cast<int>(blockIdx.x) >= a.prefix_blocks)
-    attend<WIDE>(a, blockIdx.x - a.prefix_blocks);
+  const int block = static_cast<int>(blockIdx.x) - a.prefix_blocks;
+  if (block >= 0 && a.alone)
+    attend_alone<WIDE>(a, block);
+  else if (block >= 0)
+    attend<WIDE>(a, block);
   else if constexpr (FEW)
     attend_prefix_few<WIDE>(a);
   else
@@ -1712,14 +1776,21 @@ int launch_attend(const char *name, Ctx *ctx, const Pages *kv, const float *q, s
   // up to 3,000 with up to 8 rows 17.6 / 15.4 / 15.9); more, of different lengths, want
   // parts to spare (20 of up to 9,000 49.0 / 47.1 / 44.7, 40 of up to 5,000 with up to 8
   // rows 84.7 / 84.8 / 63.7).
-  const size_t heads = n_seqs * kv->key_heads * a.tiles;
+  // Beside a prefix, many sequences of few columns and short lengths of their own have a wave a
+  // part (us a call with a workgroup / a wave: 64 of one row and up to 300 positions 25.5 / 21.8,
+  // 200 50.5 / 39.3, 32 19.7 / 14.6; of up to 1,000 64 26.5 / 24.5, of up to 4,000 48.9 / 55.7;
+  // with eight columns and 1,000 36.1 / 44.9; 16 sequences as they were), 1,024 waves (2,048:
+  // 25.6 for the first, 38.4, 14.4).
+  const size_t units = n_seqs * kv->key_heads;
+  a.alone = shared > 0 && units > 256 && rows * group <= 4 * n_seqs && own <= 1024;
+  const size_t tasks = a.alone ? units : units * a.tiles;
   const size_t enough = n_seqs <= 2 ? 512 : n_seqs <= 8 || shared > 0 ? 1024 : 2048;
-  const size_t want = heads >= enough ? 1 : enough / heads;
+  const size_t want = tasks >= enough ? 1 : enough / tasks;
   const size_t chunk = std::max(std::min<size_t>((own + want - 1) / want, 4096), (own + kMaxParts - 1) / kMaxParts);
   a.chunk = static_cast<int>((chunk + 255) / 256 * 256);
   a.own_parts = static_cast<int>((own + a.chunk - 1) / a.chunk);
   const size_t share = kv->key_heads / kv->kv_heads;
-  const size_t grid = (heads * a.own_parts + 8 * share - 1) / (8 * share) * (8 * share);
+  const size_t grid = a.alone ? (tasks * a.own_parts + 3) / 4 : (tasks * a.own_parts + 8 * share - 1) / (8 * share) * (8 * share);
   FOCR_REQUIRE(grid < (size_t(1) << 31), FOCR_E_SHAPE, std::string(name) + ": too many sequences and heads");
   bool few = false;
   if (shared > 0) {

@@ -107,6 +107,24 @@ def test_many_rows_over_a_long_prefix(fh):
     b.verify(host(b.shared_call()), only=[0, 77, 139])
 
 
+@pytest.mark.parametrize("key_heads,own,page", [(8, 40, 16), (16, 40, 64), (16, 1000, 32), (8, 1100, 64)])
+def test_many_ragged_sequences(fh, key_heads, own, page):
+    # Many sequences, most of one row, some of several, idle, refused or missing a page; own positions
+    # from none on, in one part and in several.
+    n = 48
+    counts = [0 if i % 11 == 5 else 8 if i == 20 else 3 if i % 16 == 7 else 1 for i in range(n)]
+    owns = [0 if i == 2 else (own * (7 * i % n) // n if i else own) for i in range(n)]
+    b = Batch(fh, 64, owns, counts, page, 16, 8, key_heads, seed=own + key_heads)
+    b.before[9] = 63
+    at = (64 + owns[30] // 2) // page
+    b.kv.map(30, at, [-1])
+    got = host(b.shared_call(max_len=64 + own + 8))
+    assert b.kv.refused() == [9, 30]
+    first = np.concatenate([[0], np.cumsum(counts)])
+    assert np.isnan(got[first[9]:first[10]]).all() and np.isnan(got[first[30]:first[31]]).all()
+    b.verify(got, only=[i for i in range(n) if i not in (9, 30)])
+
+
 def test_equals_attention_of_each_sequence(fh):
     # The same positions read by each sequence for itself: within the roundings of both.
     b = Batch(fh, 192, [5, 80, 0], [2, 1, 4], 32, seed=7)
