@@ -120,11 +120,11 @@ struct List {
 // the first and the last of a row may be cut.
 //
 // Bound: the logits read, and written where they are kept. 256 rows of 131,072 with all
-// rules and their logits kept take 66 us, 274 MB at 4.1 TB/s (44 without rules, 6.1); pieces
+// rules and their logits kept take 72 us, 274 MB at 3.8 TB/s (44 without rules, 6.2); pieces
 // of 4,096 78, as every piece looks through the row's lists (16,384 with 512 threads 65, but
-// a row of 50,021 loses 10 %). 64 rows of 65,536 take 14.5 us, 6.1 without rules: the
+// a row of 50,021 loses 10 %). 64 rows of 65,536 take 15.9 us, 6.1 without rules: the
 // history (2 us a thousand fours a thread), three barriers, three atomics one after
-// another. One row 6.2 us, a launch, two trips to memory and these atomics.
+// another. One row 6.9 us, a launch, two trips to memory and these atomics.
 template <bool RULES>
 __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint32_t words[];
