@@ -198,7 +198,7 @@ __device__ __forceinline__ float row_lane(float v) {
 // lanes 4, 2 and 1 apart (elements 16, 8 and 4), then the lane's own (2 and 1), of both
 // halves of 32; the four sums of a row's 16 lanes meet in four of them, so that the
 // divisions and the root are done once for all 16 rows. A rotated pair is the lane's own.
-__device__ __forceinline__ void norm_rotate(v4f (&x)[4], const v4f (&f)[4]) {
+__device__ __forceinline__ float norm_scales(const v4f (&x)[4]) {
   float sums = 0.0f;
   const int l16 = threadIdx.x & 15;
   auto total = [&](const v4f &v) {
@@ -219,14 +219,20 @@ __device__ __forceinline__ void norm_rotate(v4f (&x)[4], const v4f (&f)[4]) {
     const float t = total(x[s]);
     sums = l16 == s ? t : sums;
   }
-  const float scales = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(sums, 64.0f) + 1.1920929e-7f));
-  const float scale[4] = {row_lane<0>(scales), row_lane<1>(scales), row_lane<2>(scales), row_lane<3>(scales)};
+  return __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(sums, 64.0f) + 1.1920929e-7f));
+}
+// Of row s: lane s of the 16 has it.
+__device__ __forceinline__ float norm_scale(float scales, int s) {
+  return s == 0 ? row_lane<0>(scales) : s == 1 ? row_lane<1>(scales) : s == 2 ? row_lane<2>(scales) : row_lane<3>(scales);
+}
+__device__ __forceinline__ v4f rotated(const v4f &x, float scale, const v4f &f) {
+  const v4f y = {x[0] * scale, x[1] * scale, x[2] * scale, x[3] * scale};
+  return v4f{y[0] * f[0] - y[1] * f[1], y[0] * f[1] + y[1] * f[0], y[2] * f[2] - y[3] * f[3], y[2] * f[3] + y[3] * f[2]};
+}
+__device__ __forceinline__ void norm_rotate(v4f (&x)[4], const v4f (&f)[4]) {
+  const float scales = norm_scales(x);
 #pragma unroll
-  for (int s = 0; s < 4; s++) {
-    const v4f y = {x[s][0] * scale[s], x[s][1] * scale[s], x[s][2] * scale[s], x[s][3] * scale[s]};
-    x[s] = v4f{y[0] * f[s][0] - y[1] * f[s][1], y[0] * f[s][1] + y[1] * f[s][0], y[2] * f[s][2] - y[3] * f[s][3],
-               y[2] * f[s][3] + y[3] * f[s][2]};
-  }
+  for (int s = 0; s < 4; s++) x[s] = rotated(x[s], norm_scale(scales, s), f[s]);
 }
 
 // Units of an append: the blocks of a sequence's rows, the first and the last two
@@ -418,11 +424,12 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 // it the key head that is turned by the same factors, or one value head. Lanes are as
 // in append_kernel; a lane forms the factors of its two pairs in its four rows, bitwise
 // those of focr_rotary_factors, while the rows are on their way. Bound: for prompts the vector
-// instructions, some 1,400 for a block and a head, 350 of them the factors': 15,243 rows of
-// four with three axes take 66 us (3.1 TB/s); for single rows trips one after another, 64
-// sequences 8.4 us.
+// instructions, some 1,400 for a block and a head, 350 of them the factors', and the trips to
+// memory that five waves on a SIMD leave uncovered: 15,243 rows of four with three axes
+// take 55 to 61 us (3.3 to 3.7 TB/s); for single rows trips one after another, 64 sequences
+// 7.9 us.
 template <int AXES>
-__global__ __launch_bounds__(256) void turn_kernel(AppendArgs a) {
+__global__ __launch_bounds__(256, 5) void turn_kernel(AppendArgs a) {
   const Cache &c = a.c;
   const int lane = threadIdx.x & 63, r4 = lane / 16 * 4, e4 = lane % 16 * 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -449,60 +456,69 @@ __global__ __launch_bounds__(256) void turn_kernel(AppendArgs a) {
   const size_t slot = (static_cast<size_t>(unit.seq) * stored + at_stored) * 2;
   const float *const key_source = a.qkv + (is_value ? c.n_heads + c.kv_heads + value_head : c.n_heads + key_head * c.kv_heads / c.key_heads) * 64;
   const int first_block = unit.len / kBlock, blocks = touched(unit.len, unit.n), last_block = first_block + blocks - 1;
-  float2 speed[AXES];
+  __shared__ float places[4][kBlock * kMaxAxes];  // a wave's: positions of its block's rows
+  __shared__ float2 speeds[4][AXES][16];  // and the frequencies of its pairs
+  if (!is_value)
 #pragma unroll
-  for (int x = 0; x < AXES; x++)
-    speed[x] = is_value ? make_float2(0.0f, 0.0f)
-                        : *reinterpret_cast<const float2 *>(a.frequencies + (static_cast<size_t>(x) * c.n_heads + query) * 32 + e4 / 2);
+    for (int x = 0; x < AXES; x++)
+      speeds[wave][x][e4 / 4] = *reinterpret_cast<const float2 *>(a.frequencies + (static_cast<size_t>(x) * c.n_heads + query) * 32 + e4 / 2);
 
   auto process = [&](int block) {
     const int row0 = block * kBlock - unit.len;  // the row of its first position
     const float *const open = c.open + (slot + block % 2) * kBlock * 64;
     v4f x[4], y[4];
-    float place[4][AXES];
+    float place = 0.0f;
+    if (!is_value && lane < kBlock * AXES) {
+      const int row = row0 + lane / AXES;
+      place = a.positions[(unit.first + static_cast<size_t>(row < 0 ? 0 : row < unit.n ? row : unit.n - 1)) * AXES + lane % AXES];
+    }
 #pragma unroll
     for (int s = 0; s < 4; s++) {
       const int row = row0 + r4 + s;
       const size_t at = unit.first + (row < 0 ? 0 : row < unit.n ? row : unit.n - 1);
       // Earlier positions from the FP32 block, new ones from the rows.
       if (is_value || has_key) x[s] = *reinterpret_cast<const v4f *>((row < 0 ? open + (r4 + s) * 64 : key_source + at * width) + e4);
-      if (!is_value) {
-        y[s] = *reinterpret_cast<const v4f *>(a.qkv + query * 64 + at * width + e4);
-#pragma unroll
-        for (int i = 0; i < AXES; i++) place[s][i] = a.positions[at * AXES + i];
-      }
+      if (!is_value) y[s] = *reinterpret_cast<const v4f *>(a.qkv + query * 64 + at * width + e4);
     }
     if (!is_value) {
-      v4f f[4];
+      places[wave][lane] = place;
+      // One pair of one row after another, positions and frequencies from LDS, so that few
+      // 64-bit numbers are held: all at once, at 115 registers, four waves fit on a SIMD and
+      // the same prompts take 66 us; bounded to 80 registers, which spill, they lose 40 %.
+      const float scales = norm_scales(y);
+      float key_scales = 0.0f;
+      if (has_key) key_scales = norm_scales(x);
 #pragma unroll
       for (int s = 0; s < 4; s++) {
         // A step of few rows leaves most places of a block without one.
         const int row = row0 + r4 + s;
-        f[s] = v4f{1.0f, 0.0f, 1.0f, 0.0f};
         if (unit.n < kBlock && !__any(row >= 0 && row < unit.n)) continue;
-        double angle[2];
+        __builtin_amdgcn_sched_barrier(0);
+        v4f f;
 #pragma unroll
-        for (int i = 0; i < AXES; i++) {
-          const double p = place[s][i];
-          angle[0] = i == 0 ? p * speed[i].x : __builtin_fma(p, static_cast<double>(speed[i].x), angle[0]);
-          angle[1] = i == 0 ? p * speed[i].y : __builtin_fma(p, static_cast<double>(speed[i].y), angle[1]);
+        for (int j = 0; j < 2; j++) {
+          double angle;
+#pragma unroll
+          for (int i = 0; i < AXES; i++) {
+            const double at = places[wave][(r4 + s) * AXES + i], speed = j == 0 ? speeds[wave][i][e4 / 4].x : speeds[wave][i][e4 / 4].y;
+            angle = i == 0 ? at * speed : __builtin_fma(at, speed, angle);
+          }
+          const float2 turn = cos_sin(angle);
+          f[2 * j] = turn.x;
+          f[2 * j + 1] = turn.y;
+          __builtin_amdgcn_sched_barrier(0);
         }
-        const float2 u = cos_sin(angle[0]), v = cos_sin(angle[1]);
-        f[s] = v4f{u.x, u.y, v.x, v.y};
-      }
-      norm_rotate(y, f);
-#pragma unroll
-      for (int s = 0; s < 4; s++) {
-        const int row = row0 + r4 + s;
+        asm volatile("" ::: "memory");  // read again for the next row, not held
+        const v4f turned = rotated(y[s], norm_scale(scales, s), f);
         if (row >= 0 && row < unit.n)
-          *reinterpret_cast<v4f *>(a.q + (static_cast<size_t>(unit.first + row) * c.n_heads + query) * 64 + e4) = y[s];
+          *reinterpret_cast<v4f *>(a.q + (static_cast<size_t>(unit.first + row) * c.n_heads + query) * 64 + e4) = turned;
+        if (has_key) {
+          const v4f key = rotated(x[s], norm_scale(key_scales, s), f);
+          if (row >= 0) x[s] = key;
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
       if (!has_key) return;
-      v4f turned[4] = {x[0], x[1], x[2], x[3]};
-      norm_rotate(turned, f);
-#pragma unroll
-      for (int s = 0; s < 4; s++)
-        if (row0 + r4 + s >= 0) x[s] = turned[s];
     }
     put_block(c, unit, !is_value, is_value ? c.kv_heads : c.key_heads, is_value ? value_head : key_head, slot, block, last_block, x);
   };
