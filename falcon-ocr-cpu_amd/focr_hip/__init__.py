@@ -606,8 +606,8 @@ class Rotary:
         self.frequencies = table.to(device=f"cuda:{self.ctx.device}", dtype=torch.float32, copy=True).contiguous()
         self.axes, self.n_heads = int(table.shape[0]), int(table.shape[1])
         self._table = self.frequencies.data_ptr()
-        if self.ctx.stream != torch.cuda.current_stream(self.ctx.device).cuda_stream:
-            torch.cuda.current_stream(self.ctx.device).synchronize()  # the table is there for the context's stream
+        # The table is there for every context's stream: a cache of another one than `ctx` may read it.
+        torch.cuda.current_stream(self.ctx.device).synchronize()
 
     def factors(self, positions, out=None):
         """cos and sin [rows][n_heads][32][2] of positions [rows][axes], as every row step takes them (`rope`)."""

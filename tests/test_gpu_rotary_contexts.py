@@ -1,0 +1,56 @@
+"""A `Rotary` of one context with a cache of another, on streams of their own: bitwise the same
+row step of one context."""
+import numpy as np
+import pytest
+
+import gen
+from gpu_util import F32, assert_bitwise, host, to_dev
+from test_gpu_rotary import int32, pages_of, table
+
+pytestmark = pytest.mark.gpu
+ROWS = [3, 1, 20]
+
+
+@pytest.fixture(scope="module")
+def fh():
+    import focr_hip
+
+    return focr_hip
+
+
+def step(kv, rope, qkv, q=None):
+    return kv.qkv_rows(qkv, rope, int32([0, 16, 5]), row_start=int32(np.concatenate([[0], np.cumsum(ROWS)])), q=q)
+
+
+def test_a_table_made_behind_queued_work(fh):
+    # The frequencies are computed on torch's stream, behind other work, and the cache's context is on a
+    # stream that does not wait for it.
+    import torch
+
+    total = sum(ROWS)
+    f, p, x = table(2, 16, 3), gen.normal((total, 2), 50.0, 5), gen.normal((total, 32 * 64), 1.0, 7)
+    alone = pages_of(fh, [0, 16, 5], ROWS, 16, 8, 8, 16, 11)
+    want = host(step(alone, fh.Rotary(f).at(to_dev(p)), to_dev(x)))
+    ctx, stream = fh.Context(0), torch.cuda.Stream()
+    kv = pages_of(fh, [0, 16, 5], ROWS, 16, 8, 8, 16, 11, ctx)
+    lens, row_start = int32([0, 16, 5]), int32(np.concatenate([[0], np.cumsum(ROWS)]))
+    positions, qkv, given = to_dev(p), to_dev(x), to_dev(f)
+    q, a = torch.zeros(total, 16, 64, device="cuda:0"), torch.ones(4096, 4096, device="cuda:0")
+    torch.cuda.synchronize()
+    ctx.use_stream(stream)
+    for _ in range(20):
+        a = a @ a * 2.0 ** -12
+    rotary = fh.Rotary(given * a[0, 0])  # of the default context, on torch's stream; a is ones
+    with torch.cuda.stream(stream):
+        kv.qkv_rows(qkv, rotary.at(positions), lens, row_start=row_start, q=q)
+    stream.synchronize()
+    assert_bitwise(host(q), want, "queries")
+    torch.cuda.synchronize()
+    ctx.use_stream(torch.cuda.current_stream())
+    for i, n in enumerate((0, 16, 5)):
+        one = [-1] * 3
+        one[i] = n
+        starts = int32([0] * (i + 1) + [ROWS[i]] * (3 - i))
+        for a_, b_ in zip(kv.dequantize(ROWS[i], int32(one), row_start=starts), alone.dequantize(ROWS[i], int32(one), row_start=starts)):
+            assert_bitwise(host(a_), host(b_), f"cache of sequence {i}")
+    assert kv.refused() == alone.refused() == []
