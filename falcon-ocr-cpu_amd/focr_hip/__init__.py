@@ -607,7 +607,19 @@ class Rotary:
         self.axes, self.n_heads = int(table.shape[0]), int(table.shape[1])
         self._table = self.frequencies.data_ptr()
         # The table is there for every context's stream: a cache of another one than `ctx` may read it.
-        torch.cuda.current_stream(self.ctx.device).synchronize()
+        stream = torch.cuda.current_stream(self.ctx.device)
+        stream.synchronize()
+        self._stream, self._readers = stream.cuda_stream, [self.ctx]
+
+    def __del__(self):
+        # The table's memory is torch's, which gives it away in the order of the table's own stream: what reads it on
+        # others ends before.
+        for ctx in getattr(self, "_readers", ()):
+            try:
+                if ctx.stream != self._stream:
+                    ctx.sync()
+            except Exception:
+                pass
 
     def factors(self, positions, out=None):
         """cos and sin [rows][n_heads][32][2] of positions [rows][axes], as every row step takes them (`rope`)."""
@@ -937,6 +949,8 @@ class KvPages:
         if angles:
             _check(lib().focr_kv_pages_qkv_rows_at(self.ctx.handle, self.handle, self._ptr(qkv), rows, self._ptr(positions),
                                                    rotary.axes, rotary._table, start, lens, seqs, to))
+            if self.ctx is not rotary.ctx and self.ctx not in rotary._readers:
+                rotary._readers.append(self.ctx)
             return q
         _check(lib().focr_kv_pages_qkv_rows(self.ctx.handle, self.handle, self._ptr(qkv), rows, self._ptr(rope),
                                             start, lens, seqs, to))

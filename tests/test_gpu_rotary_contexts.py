@@ -54,3 +54,33 @@ def test_a_table_made_behind_queued_work(fh):
         for a_, b_ in zip(kv.dequantize(ROWS[i], int32(one), row_start=starts), alone.dequantize(ROWS[i], int32(one), row_start=starts)):
             assert_bitwise(host(a_), host(b_), f"cache of sequence {i}")
     assert kv.refused() == alone.refused() == []
+
+
+@pytest.mark.parametrize("owner", ["rotary", "cache"])
+def test_a_rotary_that_is_dropped_while_its_table_is_read(fh, owner):
+    # The call is queued behind other work on its stream when the rotary goes; torch's stream gives the
+    # table's memory to other tensors at once.
+    import torch
+
+    total = sum(ROWS)
+    f, p, x = table(2, 16, 3), gen.normal((total, 2), 50.0, 5), gen.normal((total, 32 * 64), 1.0, 7)
+    alone = pages_of(fh, [0, 16, 5], ROWS, 16, 8, 8, 16, 11)
+    want = host(step(alone, fh.Rotary(f).at(to_dev(p)), to_dev(x)))
+    ctx, stream = fh.Context(0), torch.cuda.Stream()
+    kv = pages_of(fh, [0, 16, 5], ROWS, 16, 8, 8, 16, 11, ctx)
+    lens, row_start = int32([0, 16, 5]), int32(np.concatenate([[0], np.cumsum(ROWS)]))
+    positions, qkv = to_dev(p), to_dev(x)
+    q, a = torch.zeros(total, 16, 64, device="cuda:0"), torch.ones(4096, 4096, device="cuda:0")
+    torch.cuda.synchronize()
+    ctx.use_stream(stream)
+    rotary = fh.Rotary(f, ctx=ctx if owner == "rotary" else None)
+    with torch.cuda.stream(stream):
+        for _ in range(20):
+            a = a @ a * 2.0 ** -12
+        kv.qkv_rows(qkv, rotary.at(positions), lens, row_start=row_start, q=q)
+    del rotary
+    other = [torch.full((2, 16, 32), 3.0, device="cuda:0") for _ in range(40)]
+    torch.cuda.synchronize()
+    assert_bitwise(host(q), want)
+    assert len(other) == 40
+    ctx.use_stream(torch.cuda.current_stream())

@@ -5,6 +5,8 @@ import pytest
 import torch
 
 import focr_hip
+from test_binding_refusals import cuda
+from test_served_abi import pages
 
 
 class Table:
@@ -42,3 +44,29 @@ def test_the_table_is_complete_on_return(device, stream):
     # may be the first to read it.
     focr_hip.Rotary(Table(device), ctx=SimpleNamespace(handle=None, device=0, stream=stream))
     assert device == ["copy", "wait"]
+
+
+def context(device, stream, name="ctx"):
+    return SimpleNamespace(handle=None, device=0, stream=stream, sync=lambda: device.append(name))
+
+
+@pytest.mark.parametrize("stream,waits", [(7, []), (8, ["ctx"]), (None, ["ctx"])])
+def test_the_table_is_kept_until_other_streams_have_read_it(device, stream, waits):
+    # Its memory goes to the next tensor of torch's stream.
+    rotary = focr_hip.Rotary(Table(device), ctx=context(device, stream))
+    device.clear()
+    del rotary
+    assert device == waits
+
+
+@pytest.mark.parametrize("stream", [7, 9])
+def test_a_cache_of_another_context_is_waited_for(device, stream, monkeypatch):
+    monkeypatch.setattr(focr_hip, "lib", lambda: SimpleNamespace(focr_kv_pages_qkv_rows_at=lambda *_: 0))
+    kv, x = pages(), cuda(2, 32 * 64)
+    kv.ctx = context(device, stream, "cache")
+    rotary = focr_hip.Rotary(Table(device), ctx=context(device, 7))
+    for _ in range(2):
+        kv.qkv_rows(x, rotary.at(cuda(2, 2)), cuda(2, dtype=torch.int32), q=cuda(2, 16, 64))
+    device.clear()
+    del rotary
+    assert device == (["cache"] if stream != 7 else [])
