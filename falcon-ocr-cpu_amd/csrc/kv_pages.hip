@@ -1223,6 +1223,8 @@ __device__ __forceinline__ v8h halves_of(int first, int second) {
 
 // The sequence of each of a tile's rows row0 .. row0 + rows - 1 that one which takes part
 // has, by the threads of a workgroup or wave; `owner` begins at -1. False if none was found.
+// Of several it is the first: where one of them is accepted, those behind it overlap it and
+// are refused, and one before it would have had it refused.
 __device__ __forceinline__ bool find_owners(const SharedArgs &a, int row0, int rows, int *owner, int thread, int threads) {
   const Cache &c = a.c;
   const int seq0 = c.row_start ? 0 : row0, seq_end = c.row_start ? c.n_seqs : row0 + rows;
@@ -1232,7 +1234,7 @@ __device__ __forceinline__ bool find_owners(const SharedArgs &a, int row0, int r
     bool bad;
     if (!attend_span(a, seq, len, first, n, bad)) continue;
     for (int r = first > row0 ? first : row0; r < first + n && r < row0 + rows; r++) {
-      atomicMax(owner + (r - row0), seq);
+      atomicMin(reinterpret_cast<uint32_t *>(owner + (r - row0)), static_cast<uint32_t>(seq));  // -1 is the largest
       any = true;
     }
   }
