@@ -129,13 +129,13 @@ class DecoderLayer:
             self._work[name] = torch.empty(max(n, 2 * t.numel()), dtype=t.dtype, device=t.device)
         return self._buf(name, shape)
 
-    def _factors(self, rope, rows: int):
-        """The factors of `rows` rows, from their positions (`Rotary.at`) where `rope` has these."""
+    def _factors(self, rope, rows: int, name: str):
+        """The factors of `rows` rows, from their positions (`Rotary.at`) where `rope` has these, in the buffer `name`."""
         if type(rope) is not RotaryRows:
             return rope
         if rope.rotary.ctx is not self.ctx or rope.rotary.n_heads != self.n_heads:
             raise FocrError(-2, "the frequencies are of other heads or another context")
-        return rope.rotary.factors(rope.positions, out=self._buf("rope", (rows, self.n_heads, 32, 2)))
+        return rope.rotary.factors(rope.positions, out=self._buf(name, (rows, self.n_heads, 32, 2)))
 
     def kv(self, total: int) -> CompactKv:
         """The cache's first `total` positions as a CompactKv."""
@@ -156,7 +156,7 @@ class DecoderLayer:
             raise FocrError(-2, "attention image must be inside the prefix")
         ctx = self.ctx
         mark = clock or (lambda stage: None)
-        rope = self._factors(rope, rows)
+        rope = self._factors(rope, rows, "rope")
         # The last prompt's sealed cache is gone; its buffers serve this one's.
         old, self.split = self.split, None
         if old is not None and (not old.handle or old.ctx is not ctx
@@ -226,7 +226,7 @@ class DecoderLayer:
             raise FocrError(-2, "KV context exhausted")
         ctx, p, pos = self.ctx, self.prefix_len, self.len
         mark = clock or (lambda stage: None)
-        rope = self._factors(rope, rows)
+        rope = self._factors(rope, rows, "drope")
         qkv = self.qkv.linear_ex(h, rows, rms_norm=True, out=self._buf("dqkv", (rows, self.qkv.out_dim)))
         mark("qkv")
         total = pos + rows
