@@ -1187,9 +1187,10 @@ __device__ __forceinline__ void attend_alone(const SharedArgs &a, int block) {
 // of disjoint keys, m = max m_i, o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) d_i.
 //
 // A wave takes 32 columns and 64 keys at a time, on the matrix instructions of 32 by 32.
-// Scores. Lane (l32, h) has column l32's query as two FP16 numbers an element, of 2^14 times the
-// power of two above the largest (to 2^-24 of an element, and 2^-39 of the largest at the
-// least); codes are FP16 numbers, so products are exact and their sums round as FP32's. Row m of
+// Scores. Lane (l32, h) has column l32's query as two FP16 numbers an element, scaled so that the
+// largest is in [2^13, 2^14). The rest after the first has up to 12 bits and a sign where FP16
+// has 11, so an element is off by up to 2^-23 of itself, or half an FP16 subnormal step, 2^-38 of the
+// largest. Codes are FP16 numbers, so products are exact and their sums round as FP32's. Row m of
 // key tile t is position m % 4 + 4 (m / 8) of block 2 t + m / 4 % 2, so that lane (l32, h)
 // gets the scores of column l32 with the 16 keys of blocks h and 2 + h, a scale for each.
 // Weights. exp2(s - m) times the block's value scale is three BF16 numbers, as in consume, which

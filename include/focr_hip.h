@@ -558,7 +558,7 @@ int focr_kv_pages_attention(focr_ctx *ctx, const focr_kv_pages *kv, const float 
  * prefix has no page, all are. Other sequences than the prefix's, or none, go in calls of
  * their own, whose lens_dev say -1 for the rest. Within FP32 rounding of
  * focr_kv_pages_attention on the same positions; below shared_len a query's elements are
- * taken to 2^-24 of themselves, and 2^-39 of its largest. */
+ * taken to 2^-23 of themselves, and 2^-38 of its largest (2^-129 where that is below 2^-91). */
 int focr_kv_pages_attention_shared(focr_ctx *ctx, const focr_kv_pages *kv, const float *q_dev, size_t rows,
                                    const int32_t *row_start_dev, const int32_t *lens_dev, size_t n_seqs,
                                    size_t max_len, size_t prefix_seq, size_t shared_len, const float *sinks_dev,
