@@ -262,8 +262,6 @@ extern "C" {
         q_dev: *mut f32,
         out_dev: *mut f32,
     ) -> c_int;
-
-    // ---- A9: greedy selection
     pub fn focr_rotary_factors(
         ctx: *mut focr_ctx,
         positions_dev: *const f32,
@@ -273,6 +271,15 @@ extern "C" {
         n_heads: usize,
         head_dim: usize,
         out_dev: *mut f32,
+    ) -> c_int;
+
+    // ---- A9: greedy selection; rules on logits
+    pub fn focr_argmax(
+        ctx: *mut focr_ctx,
+        logits_dev: *const f32,
+        rows: usize,
+        vocab: usize,
+        tokens: *mut u32,
     ) -> c_int;
     pub fn focr_logits_select(
         ctx: *mut focr_ctx,
@@ -294,13 +301,6 @@ extern "C" {
         append: c_int,
         adjusted_dev: *mut f32,
         tokens_dev: *mut i32,
-    ) -> c_int;
-    pub fn focr_argmax(
-        ctx: *mut focr_ctx,
-        logits_dev: *const f32,
-        rows: usize,
-        vocab: usize,
-        tokens: *mut u32,
     ) -> c_int;
 
     // ---- sealed split KV cache (Kv::Q8 / Kv::Q16)
