@@ -34,10 +34,8 @@ def test_a_longer_prompt_between_a_captured_decode_and_its_replay(fh, rows):
     prompt(layer, 20, 11)
     layer.decode(h.clone(), rotary.at(positions))  # the buffers grow uncaptured
     prompt(layer, 20, 11)
-    side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph, stream=side):
+    with torch.cuda.graph(graph):
         ctx.use_stream(torch.cuda.current_stream())
         layer.decode(h, rotary.at(positions))
     ctx.use_stream(torch.cuda.current_stream())
