@@ -590,11 +590,15 @@ def argmax(logits, rows: int, vocab: int, ctx: Optional[Context] = None):
     return list(tokens)
 
 
+_kept_tables = []
+
+
 class Rotary:
     """Rotary positions with 1 to 4 axes (time, height, width, ..): the pair of elements
     2 p, 2 p + 1 of head h is turned by the sum over the axes of position times
     `frequencies` [axes][n_heads][32] (radians; 0 where an axis does not turn a pair).
-    Angles are formed in FP64, and cos and sin rounded to FP32 once."""
+    Angles are formed in FP64, and cos and sin rounded to FP32 once. A graph that was captured
+    of a call reads the table of its `Rotary`, which has to live as long."""
 
     def __init__(self, frequencies, ctx: Optional[Context] = None):
         torch = _torch()
@@ -613,11 +617,17 @@ class Rotary:
 
     def __del__(self):
         # The table's memory is torch's, which gives it away in the order of the table's own stream: what reads it on
-        # others ends before.
-        for ctx in getattr(self, "_readers", ()):
+        # others ends before. A capture cannot be waited in: there the table stays.
+        others = [ctx for ctx in getattr(self, "_readers", ()) if ctx.stream != self._stream]
+        try:
+            if others and _torch().cuda.is_current_stream_capturing():
+                _kept_tables.append(self.frequencies)
+                return
+        except Exception:
+            pass
+        for ctx in others:
             try:
-                if ctx.stream != self._stream:
-                    ctx.sync()
+                ctx.sync()
             except Exception:
                 pass
 

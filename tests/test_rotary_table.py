@@ -34,7 +34,8 @@ def device(monkeypatch):
     log = []
     stream = SimpleNamespace(cuda_stream=7, synchronize=lambda: log.append("wait"))
     monkeypatch.setattr(focr_hip, "_torch", lambda: SimpleNamespace(
-        as_tensor=lambda t: t, float32=torch.float32, cuda=SimpleNamespace(current_stream=lambda device: stream)))
+        as_tensor=lambda t: t, float32=torch.float32,
+        cuda=SimpleNamespace(current_stream=lambda device: stream, is_current_stream_capturing=lambda: "capture" in log)))
     return log
 
 
@@ -70,3 +71,14 @@ def test_a_cache_of_another_context_is_waited_for(device, stream, monkeypatch):
     device.clear()
     del rotary
     assert device == (["cache"] if stream != 7 else [])
+
+
+@pytest.mark.parametrize("stream", [7, 8])
+def test_a_capture_is_not_waited_in(device, stream, monkeypatch):
+    # The table stays instead, where another stream may read it.
+    monkeypatch.setattr(focr_hip, "_kept_tables", [])
+    table = Table(device)
+    rotary = focr_hip.Rotary(table, ctx=context(device, stream))
+    device[:] = ["capture"]
+    del rotary
+    assert device == ["capture"] and focr_hip._kept_tables == ([table] if stream == 8 else [])
