@@ -484,7 +484,7 @@ __global__ __launch_bounds__(256, 5) void turn_kernel(AppendArgs a) {
       places[wave][lane] = place;
       // One pair of one row after another, positions and frequencies from LDS, so that few
       // 64-bit numbers are held: all at once, at 115 registers, four waves fit on a SIMD and
-      // the same prompts take 66 us; bounded to 80 registers, which spill, they lose 40 %.
+      // the same prompts take 66 us; bounded to 80 registers, which spill, 78.
       const float scales = norm_scales(y);
       float key_scales = 0.0f;
       if (has_key) key_scales = norm_scales(x);

@@ -120,11 +120,14 @@ struct List {
 // the first and the last of a row may be cut.
 //
 // Bound: the logits read, and written where they are kept. 256 rows of 131,072 with all
-// rules and their logits kept take 72 us, 274 MB at 3.8 TB/s (44 without rules, 6.2); pieces
-// of 4,096 78, as every piece looks through the row's lists (16,384 with 512 threads 65, but
-// a row of 50,021 loses 10 %). 64 rows of 65,536 take 15.9 us, 6.1 without rules: the
-// history (2 us a thousand fours a thread), three barriers, three atomics one after
-// another. One row 6.9 us, a launch, two trips to memory and these atomics.
+// rules and their logits kept take 72 us, 274 MB at 3.8 TB/s; 55 without rules (5.0, a copy's
+// rate), 56 with the mask, 60 with penalties, 65 with 300 biases: every piece looks through
+// the row's lists, and no logits are on their way meanwhile. 64 rows of 65,536 take 16 us,
+// 8.0 without rules, 9.1 with the mask, 11.4 with 200 biases, 14.5 with penalties, of which
+// 5 are the histories of up to 8,192 (eight fours a thread; with tokens spread evenly the
+// same). One row 6.9 us, a launch, two trips to memory and three atomics one after another.
+// Pieces of 4,096 tokens: 85 and 15.3; of 16,384 with 512 threads 69 and 14.7, one row and
+// seven of 50,021 as they are.
 template <bool RULES>
 __global__ __launch_bounds__(kThreads) void select_kernel(SelectArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint32_t words[];

@@ -556,9 +556,11 @@ int focr_kv_pages_attention(focr_ctx *ctx, const focr_kv_pages *kv, const float 
  * shared_len on each has its own. shared_len: whole pages (0: focr_kv_pages_attention). A
  * sequence that stands before shared_len (lens_dev[i] below it) is refused; where the
  * prefix has no page, all are. Other sequences than the prefix's, or none, go in calls of
- * their own, whose lens_dev say -1 for the rest. Within FP32 rounding of
- * focr_kv_pages_attention on the same positions; below shared_len a query's elements are
- * taken to 2^-23 of themselves, and 2^-38 of its largest (2^-129 where that is below 2^-91). */
+ * their own, whose lens_dev say -1 for the rest; such a call works on all 32 columns (a
+ * row's query heads) of which one takes part, so rows of one prefix stand together where they
+ * can. Within FP32 rounding of focr_kv_pages_attention on the same positions; below shared_len a
+ * query's elements are taken to 2^-23 of themselves, and 2^-38 of its largest (2^-129 where that
+ * is below 2^-91). */
 int focr_kv_pages_attention_shared(focr_ctx *ctx, const focr_kv_pages *kv, const float *q_dev, size_t rows,
                                    const int32_t *row_start_dev, const int32_t *lens_dev, size_t n_seqs,
                                    size_t max_len, size_t prefix_seq, size_t shared_len, const float *sinks_dev,
